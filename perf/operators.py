@@ -214,9 +214,9 @@ def _codes(x, kind):
     x = x.to(F32)
     most = x.abs().amax(-1)
     fine = most > TINY
-    zero = torch.zeros_like(most)
-    y = x * torch.where(fine, TOP[kind] / most, zero)[..., None]
-    return (torch.round(y) if kind == "int8" else y).to(TYPES[kind]), torch.where(fine, most / TOP[kind], zero)
+    zero, top = torch.zeros_like(most), torch.full_like(most, TOP[kind])   # (a number / a tensor is two roundings)
+    y = x * torch.where(fine, top / most, zero)[..., None]
+    return (torch.round(y) if kind == "int8" else y).to(TYPES[kind]), torch.where(fine, most / top, zero)
 
 
 def _bits(t):
