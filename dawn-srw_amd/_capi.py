@@ -32,6 +32,8 @@ SRW_F32, SRW_BF16 = 0, 1
 SRW_GATE_V41, SRW_GATE_GELU_V401 = 0, 1
 # srw_stats_mode_t
 SRW_STATS_ONEPASS, SRW_STATS_CENTERED, SRW_STATS_GRAM = 0, 1, 2
+# srw_kv_kind_t
+SRW_KV_BF16, SRW_KV_INT8, SRW_KV_FP8 = 0, 1, 2
 # flags
 SRW_FLAG_DIAG = 0x1
 SRW_FLAG_EMULATE = 0x2
@@ -57,6 +59,7 @@ EXPORTED_SYMBOLS = (
     "srw_set_kernel_events", "srw_backward_workspace_size", "srw_backward",
     "srw_workspace_size_batch", "srw_forward_batch", "srw_forward_noalloc",
     "srw_diag_summary", "srw_cast_bf16", "srw_dawn_decode_step",
+    "srw_kv_write", "srw_kv_read", "srw_attention_workspace_size", "srw_attention",
 )
 
 # srw_diag_out_t: the result tuple's per-token values and scalars (SRW_DSUM_*)
@@ -124,6 +127,26 @@ class SrwDawnStep(ctypes.Structure):
            ("ws_qkv", ctypes.c_void_p), ("ws_qkv_bytes", ctypes.c_size_t),
            ("ws_know", ctypes.c_void_p), ("ws_know_bytes", ctypes.c_size_t),
            ("path_qkv", ctypes.POINTER(ctypes.c_char_p))])
+
+
+class SrwKv(ctypes.Structure):
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table", "lens", "cu")]
+        + [(n, ctypes.c_int64) for n in ("B", "T", "n_pages", "table_width", "table_stride")]
+        + [(n, ctypes.c_int32) for n in ("n_kv_heads", "head_dim", "page_size", "kind")])
+
+
+class SrwKvRows(ctypes.Structure):
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("k", "v")]
+        + [(n, ctypes.c_int64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")])
+
+
+class SrwAttention(ctypes.Structure):
+    _fields_ = (
+        [("kv", SrwKv), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+        + [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride")]
+        + [(n, ctypes.c_int32) for n in ("n_heads", "max_new", "window", "sinks")] + [("scale", ctypes.c_float)])
 
 
 class SrwError(RuntimeError):
@@ -201,6 +224,14 @@ def load_library() -> ctypes.CDLL:
             ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p]
         lib.srw_dawn_decode_step.restype = ctypes.c_int
         lib.srw_dawn_decode_step.argtypes = [ctypes.POINTER(SrwDawnStep), ctypes.c_void_p]
+        for name in ("srw_kv_write", "srw_kv_read"):
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name).argtypes = [ctypes.POINTER(SrwKv), ctypes.POINTER(SrwKvRows), ctypes.c_int32,
+                                           ctypes.c_void_p]
+        lib.srw_attention_workspace_size.restype = ctypes.c_int
+        lib.srw_attention_workspace_size.argtypes = [ctypes.POINTER(SrwAttention), ctypes.POINTER(ctypes.c_size_t)]
+        lib.srw_attention.restype = ctypes.c_int
+        lib.srw_attention.argtypes = [ctypes.POINTER(SrwAttention), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         got = lib.srw_abi_version()
         if got != ABI_VERSION:
             raise SrwLibraryError(f"libsrw_amd.so ABI {got} != binding ABI {ABI_VERSION}")

@@ -1,0 +1,316 @@
+"""The paged key/value cache and the attention over it: torch tensors in,
+torch tensors out, every computation in libsrw_amd.so's HIP kernels.
+
+A layer's pages (:class:`KvPages`) hold ``page_size`` positions of every
+key/value head, in bf16 or in 8 bits with a float32 scale for each token and
+head.  Sequences of any lengths share them: a call describes its sequences by
+
+* ``table`` [B, width] int32: the page of each run of ``page_size`` positions
+  (an entry that names no page, -1 say, holds nothing and is not seen);
+* ``lens`` [B] int32: the sequences' lengths, the call's new tokens included;
+* ``cu`` [B + 1] int32: sequence b's new tokens are the packed rows
+  [cu[b], cu[b + 1]) of T and lie at its last positions; None: one each.
+
+All three are device tensors that only the kernels read: no call waits for the
+GPU.  :func:`kv_write` stores new tokens, :func:`kv_read` reads tokens back,
+:func:`paged_attention` attends from new tokens to everything before them.
+:class:`PagedKvCache` keeps the pages of all layers of a model and hands them
+out to sequences.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _capi as C
+
+__all__ = ["KvPages", "PagedKvCache", "kv_write", "kv_read", "paged_attention"]
+
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+_KINDS = {torch.bfloat16: C.SRW_KV_BF16, torch.int8: C.SRW_KV_INT8, torch.float8_e4m3fn: C.SRW_KV_FP8}
+_DTYPES = {torch.float32: C.SRW_F32, torch.bfloat16: C.SRW_BF16}
+
+
+def _tensor(name, t, dev, dtype, shape):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+class KvPages:
+    """One layer's pages: ``k`` [n_pages, H, page_size, head_dim], ``v``
+    [n_pages, H, head_dim, page_size] (dimension by dimension, as the
+    attention's matrix products read it), both bfloat16, int8 or
+    float8_e4m3fn; 8-bit pages with ``k_scale`` and ``v_scale`` [n_pages, H,
+    page_size] float32.  Holds the tensors, which the calls read and write in
+    place."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "heads", "page_size", "head_dim", "kind", "device", "_at")
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        if not isinstance(k, torch.Tensor) or k.dim() != 4:
+            raise ValueError("k must be a tensor [n_pages, heads, page_size, head_dim]")
+        n, h, p, d = k.shape
+        dev = k.device
+        if dev.type != "cuda":
+            raise ValueError(f"the cache lives on a HIP device; got {dev}")
+        if k.dtype not in _KINDS:
+            raise TypeError(f"pages hold bfloat16, int8 or float8_e4m3fn; got {k.dtype}")
+        if not k.is_contiguous():
+            raise ValueError("k must be contiguous")
+        _tensor("v", v, dev, k.dtype, (n, h, d, p))
+        self.kind = _KINDS[k.dtype]
+        if self.kind == C.SRW_KV_BF16:
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("bfloat16 pages have no scales")
+            self._at = (k.data_ptr(), v.data_ptr(), None, None)
+        else:
+            _tensor("k_scale", k_scale, dev, F32, (n, h, p))
+            _tensor("v_scale", v_scale, dev, F32, (n, h, p))
+            self._at = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.heads, self.page_size, self.head_dim, self.device = n, h, p, d, dev
+
+
+def _address(pages, table, lens, cu, T):
+    """The C description of a call's sequences over these pages."""
+    dev = pages.device
+    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
+    if B < 0:
+        raise ValueError("lens must be a tensor [B]")
+    _tensor("lens", lens, dev, I32, (B,))
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[0] != B:
+        raise ValueError(f"table must be a tensor [{B}, width]")
+    if table.device != dev or table.dtype != I32:
+        raise TypeError(f"table must be int32 on {dev}; got {table.dtype} on {table.device}")
+    width, stride = table.shape[1], table.stride(0)
+    if width > 1 and table.stride(1) != 1 or B > 1 and stride < width:
+        raise ValueError("rows of table must be consecutive")
+    if cu is not None:
+        _tensor("cu", cu, dev, I32, (B + 1,))
+    elif T != B:
+        raise ValueError(f"{T} tokens of {B} sequences need cu")
+    return C.SrwKv(*pages._at, table.data_ptr(), lens.data_ptr(), None if cu is None else cu.data_ptr(), B, T,
+                   pages.n_pages, width, max(stride, width), pages.heads, pages.head_dim, pages.page_size, pages.kind)
+
+
+def _rows(name, t, pages, T, dtypes, unit):
+    """t [T, heads, head_dim] with consecutive dims; rows that the kernels
+    cannot take as they lie (other strides or alignment) are copied."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.shape[2] != pages.head_dim or t.shape[0] != T:
+        got = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t)
+        raise ValueError(f"{name} must be [{T}, heads, {pages.head_dim}]; got {got}")
+    if t.device != pages.device:
+        raise ValueError(f"{name} is on {t.device}, expected {pages.device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s0 % unit or s1 % unit or t.data_ptr() % (unit * t.element_size()):
+        t = t.contiguous()
+        if t.data_ptr() % (unit * t.element_size()):  # contiguous, but off its alignment
+            t = t.clone()
+    return t
+
+
+class _OnDevice:
+    """The device made current where it is not (launches go to the current
+    device's streams)."""
+
+    def __init__(self, dev):
+        self.ctx = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def kv_write(pages: KvPages, k, v, table, lens, cu=None) -> None:
+    """Store the new tokens' keys and values (``k``, ``v`` [T, heads,
+    head_dim], bfloat16 or float32, any token and head strides) into the pages,
+    rounded to bfloat16 or quantised: a row x of one token and head as codes of
+    x * (127 / m) (int8) or x * (448 / m) (fp8) with scale m / 127 or m / 448,
+    m its largest magnitude.  Rows of at most 2^-100 are held as zeros; a row
+    with an infinity or NaN reads back as NaN.  Tokens whose position has no
+    page are left out; all other slots keep what they hold."""
+    T = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() else -1
+    a = _address(pages, table, lens, cu, T)
+    k = _rows("k", k, pages, T, _DTYPES, 4)
+    v = _rows("v", v, pages, T, (k.dtype,), 4)
+    if k.shape[1] != pages.heads or v.shape[1] != pages.heads:
+        raise ValueError(f"k and v have {k.shape[1]} and {v.shape[1]} heads, the pages {pages.heads}")
+    r = C.SrwKvRows(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    with _OnDevice(pages.device):
+        C.check(C.load_library().srw_kv_write(ctypes.byref(a), ctypes.byref(r), _DTYPES[k.dtype],
+                                              torch.cuda.current_stream(pages.device).cuda_stream))
+
+
+def kv_read(pages: KvPages, table, lens, cu=None, *, total=None, dtype=BF16):
+    """(k, v) [T, heads, head_dim] in ``dtype`` (bfloat16 or float32) of the
+    tokens that (lens, cu) describe -- with cu from cumulated lens, whole
+    sequences.  ``total`` is T, which lies on the device (cu's last entry);
+    None where cu is None.  Positions without a page give zeros."""
+    if dtype not in _DTYPES:
+        raise TypeError(f"kv_read gives float32 or bfloat16, not {dtype}")
+    if cu is not None and total is None:
+        raise ValueError("total, the number of tokens, is needed with cu")
+    T = int(total) if total is not None else lens.shape[0]
+    a = _address(pages, table, lens, cu, T)
+    k, v = (torch.empty((T, pages.heads, pages.head_dim), dtype=dtype, device=pages.device) for _ in range(2))
+    r = C.SrwKvRows(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    with _OnDevice(pages.device):
+        C.check(C.load_library().srw_kv_read(ctypes.byref(a), ctypes.byref(r), _DTYPES[dtype],
+                                             torch.cuda.current_stream(pages.device).cuda_stream))
+    return k, v
+
+
+def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0, scale=None, window: int = 0,
+                    sinks: int = 0, out=None):
+    """Attention of the new tokens ``q`` [T, n_heads, head_dim] (bfloat16, any
+    token and head strides; n_heads a multiple of the pages' heads) over their
+    sequences' pages, which must hold the new tokens already: a token at
+    position i sees the positions j <= i, with ``window`` > 0 those with j > i
+    - window or j < ``sinks``.  ``scale`` multiplies the scores (default 1 /
+    sqrt(head_dim)).  ``max_new``: the most new tokens of one sequence, where
+    the caller knows it (it chooses the kernel, not the result).  Returns
+    ``out`` [T, n_heads, head_dim] bfloat16; a token that sees nothing gets
+    zeros.  The softmax weights are rounded to bfloat16 for the second product;
+    sums and statistics are float32."""
+    T = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else -1
+    kv = _address(pages, table, lens, cu, T)
+    q = _rows("q", q, pages, T, (BF16,), 8)
+    Hq = q.shape[1]
+    if Hq < 1 or Hq % pages.heads:
+        raise ValueError(f"{Hq} query heads are no multiple of the pages' {pages.heads}")
+    if window < 0 or sinks < 0 or (sinks and not window) or max_new < 0:
+        raise ValueError("window, sinks and max_new are not negative, and sinks need a window")
+    scale = 1.0 / math.sqrt(pages.head_dim) if scale is None else float(scale)
+    dev = pages.device
+    if out is None:
+        out = torch.empty((T, Hq, pages.head_dim), dtype=BF16, device=dev)
+    else:
+        _tensor("out", out, dev, BF16, (T, Hq, pages.head_dim))
+    a = C.SrwAttention(kv, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), Hq, max_new, window, sinks, scale)
+    lib = C.load_library()
+    need = ctypes.c_size_t(0)
+    with _OnDevice(dev):
+        C.check(lib.srw_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+        C.check(lib.srw_attention(ctypes.byref(a), None if ws is None else ws.data_ptr(), need.value,
+                                  torch.cuda.current_stream(dev).cuda_stream))
+    return out
+
+
+class PagedKvCache:
+    """Pages of all layers of a model and the sequences that hold them.
+
+    ``layer(i)`` is layer i's :class:`KvPages`; a page id names the same page
+    of every layer.  ``add()`` opens a sequence, ``extend(seqs, counts)``
+    makes room for that many new tokens of each and returns the call's
+    (table, lens, cu, max_new) on the device, ``free(seq)`` gives its pages
+    back.  With a sliding window, ``evict(seq, window, sinks)`` gives back
+    the pages that no later token sees."""
+
+    def __init__(self, n_layers: int, n_pages: int, n_heads: int, head_dim: int, *, page_size: int = 64, dtype=BF16,
+                 device="cuda:0"):
+        dev = torch.device(device)
+        if dtype not in _KINDS:
+            raise TypeError(f"pages hold bfloat16, int8 or float8_e4m3fn; got {dtype}")
+        if head_dim not in (64, 128) or page_size not in (16, 32, 64, 128, 256):
+            raise ValueError("head_dim is 64 or 128 and page_size 16, 32, 64, 128 or 256")
+        if min(n_layers, n_pages, n_heads) < 1:
+            raise ValueError("n_layers, n_pages and n_heads are at least 1")
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.page_size, self.n_pages, self.device, self.dtype = page_size, n_pages, dev, dtype
+        shape = (n_layers, n_pages, n_heads)
+        self.k = torch.empty(*shape, page_size, head_dim, dtype=dtype, device=dev)
+        self.v = torch.empty(*shape, head_dim, page_size, dtype=dtype, device=dev)
+        self.k_scale = self.v_scale = None
+        if dtype != BF16:
+            self.k_scale, self.v_scale = (torch.empty(*shape, page_size, device=dev) for _ in range(2))
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._pages, self._lens, self._next = {}, {}, 0
+
+    def layer(self, i: int) -> KvPages:
+        if self.dtype == BF16:
+            return KvPages(self.k[i], self.v[i])
+        return KvPages(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i])
+
+    def add(self) -> int:
+        seq, self._next = self._next, self._next + 1
+        self._pages[seq], self._lens[seq] = [], 0
+        return seq
+
+    def length(self, seq: int) -> int:
+        return self._lens[seq]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def extend(self, seqs, counts):
+        """Room for counts[i] (0 or more) further tokens of seqs[i]; (table, lens, cu,
+        max_new) of the call that writes and attends to them.  Raises
+        MemoryError, with nothing changed, where the free pages do not do."""
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs):
+            raise ValueError("one count for each of different sequences")
+        need = {}
+        for s, n in zip(seqs, counts):
+            if s not in self._lens:
+                raise KeyError(f"no sequence {s}")
+            if n < 0:
+                raise ValueError("counts are not negative")
+            need[s] = -(-(self._lens[s] + n) // self.page_size) - len(self._pages[s])
+        if sum(need.values()) > len(self._free):
+            raise MemoryError(f"{sum(need.values())} pages are needed, {len(self._free)} are free")
+        for s, n in zip(seqs, counts):
+            self._pages[s].extend(self._free.pop() for _ in range(need[s]))
+            self._lens[s] += n
+        width = max((len(self._pages[s]) for s in seqs), default=0)
+        # one copy to the device: the table's rows, then lens, then cu
+        host, at = [], 0
+        for s in seqs:
+            host += self._pages[s] + [-1] * (width - len(self._pages[s]))
+        host += [self._lens[s] for s in seqs] + [0]
+        for n in counts:
+            at += n
+            host.append(at)
+        B = len(seqs)
+        t = torch.tensor(host, dtype=I32).to(self.device)
+        table, lens, cu = t[:B * width].view(B, width), t[B * width:B * width + B], t[B * width + B:]
+        most = max(counts, default=0)
+        return table, lens, None if most == 1 and min(counts) == 1 else cu, most
+
+    def evict(self, seq: int, window: int, sinks: int = 0) -> int:
+        """Give back the pages that hold only positions which a token at
+        position length(seq) or later does not see under this window; returns
+        their number."""
+        if window < 1 or sinks < 0:
+            raise ValueError("evict needs a window, and sinks are not negative")
+        P, pages, n = self.page_size, self._pages[seq], 0
+        for i in range(-(-sinks // P), len(pages)):
+            if (i + 1) * P > self._lens[seq] - window + 1:
+                break
+            if pages[i] >= 0:
+                self._free.append(pages[i])
+                pages[i] = -1
+                n += 1
+        return n
+
+    def free(self, seq: int) -> None:
+        self._free.extend(p for p in reversed(self._pages.pop(seq)) if p >= 0)
+        del self._lens[seq]

@@ -429,6 +429,79 @@ srw_status_t srw_dawn_decode_step(const srw_dawn_step_t* step, void* stream);
 #define SRW_MAX_CAST 8
 srw_status_t srw_cast_bf16(int32_t n, const float* const* src, void* const* dst, const int64_t* count, void* stream);
 
+/* Paged key/value cache and the attention over it.  No counterpart in the
+ * reference, whose cache is one [L, B, H, max_seq, d_head] array with one
+ * length for all sequences (v41:1772-1957).
+ *
+ * A layer's pages are four arrays of the caller:
+ *   k [n_pages, n_kv_heads, page_size, head_dim]
+ *   v [n_pages, n_kv_heads, head_dim, page_size]   (dimension by dimension)
+ *   k_scale, v_scale [n_pages, n_kv_heads, page_size] float32, with 8-bit kinds
+ * Sequence b has lens[b] positions, the call's new tokens included: the last
+ * cu[b + 1] - cu[b] of them, whose packed rows are [cu[b], cu[b + 1]) of T
+ * (cu[0] = 0, cu[B] = T); cu NULL: one new token each, T = B.  Position p is
+ * slot p % page_size of page table[b * table_stride + p / page_size]; an entry
+ * outside [0, n_pages) names no page.  lens, cu and table are device arrays of
+ * int32 and are read by the kernels alone (no synchronisation): whatever they
+ * hold, nothing outside the described arrays is read or written.
+ *
+ * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; table_width *
+ * page_size below 2^31 - 2^16; else SRW_EUNSUPPORTED.  The arrays 16-byte
+ * aligned. */
+typedef enum srw_kv_kind {
+  SRW_KV_BF16 = 0,
+  SRW_KV_INT8 = 1, /* codes round(x 127 / m), m the row's largest magnitude; scale m / 127 */
+  SRW_KV_FP8 = 2   /* e4m3 codes of x 448 / m; scale m / 448 */
+} srw_kv_kind_t;
+typedef struct srw_kv {
+  void *k, *v;
+  float *k_scale, *v_scale;  /* NULL with SRW_KV_BF16 */
+  const int32_t *table, *lens, *cu;
+  int64_t B, T, n_pages, table_width, table_stride;
+  int32_t n_kv_heads, head_dim, page_size, kind; /* srw_kv_kind_t */
+} srw_kv_t;
+
+/* Rows of every new token and head: k at k + t * k_token_stride + h *
+ * k_head_stride (elements, multiples of 4; pointers aligned to 4 elements),
+ * head_dim consecutive elements of dtype SRW_F32 or SRW_BF16. */
+typedef struct srw_kv_rows {
+  void *k, *v;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} srw_kv_rows_t;
+
+/* Writes the new tokens' rows into their slots, rounded to bf16 or quantised
+ * with a scale for each token and head; other slots keep what they hold.  Rows
+ * of magnitude 2^-100 or less are held as zeros; a row with an infinity or NaN
+ * reads back as NaN.  Tokens whose position has no page are left out. */
+srw_status_t srw_kv_write(const srw_kv_t* cache, const srw_kv_rows_t* rows, int32_t dtype, void* stream);
+
+/* Reads them back into rows (code * scale, rounded once to dtype); positions
+ * without a page give zeros. */
+srw_status_t srw_kv_read(const srw_kv_t* cache, const srw_kv_rows_t* rows, int32_t dtype, void* stream);
+
+/* out[t, h] = sum_j softmax_j(scale q[t, h] . k[j]) v[j] over the positions j
+ * that the token at position i sees: j <= i, and with window > 0 also j > i -
+ * window or j < sinks.  Positions without a page are not seen; a token that
+ * sees nothing gets zeros.  n_heads a multiple of n_kv_heads (head h reads key
+ * head h / (n_heads / n_kv_heads)).  q rows at q + t * q_token_stride + h *
+ * q_head_stride (elements, multiples of 8; 16-byte aligned), out [T, n_heads,
+ * head_dim] contiguous, both bf16; float32 inside but for the softmax weights,
+ * which the matrix cores read as bf16.  The cache must hold the new tokens
+ * (srw_kv_write before, on the same stream). */
+typedef struct srw_attention {
+  srw_kv_t kv;
+  const void* q;
+  void* out;
+  int64_t q_token_stride, q_head_stride;
+  int32_t n_heads;
+  int32_t max_new;        /* the most new tokens of a sequence, 0: not known.  It chooses the kernel;
+                             results are right for any value */
+  int32_t window, sinks;  /* 0: every earlier position is seen; sinks need a window */
+  float scale;
+} srw_attention_t;
+srw_status_t srw_attention_workspace_size(const srw_attention_t* a, size_t* bytes);
+srw_status_t srw_attention(const srw_attention_t* a, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Name of the kernel family the last srw_forward on this thread used
  * ("generic", "mfma_bf16", "mfma_ss_bf16", ...), for tests and benchmarks. */
 const char* srw_last_path(void);
