@@ -226,12 +226,12 @@ def load_library() -> ctypes.CDLL:
         lib.srw_dawn_decode_step.argtypes = [ctypes.POINTER(SrwDawnStep), ctypes.c_void_p]
         for name in ("srw_kv_write", "srw_kv_read"):
             getattr(lib, name).restype = ctypes.c_int
-            getattr(lib, name).argtypes = [ctypes.POINTER(SrwKv), ctypes.POINTER(SrwKvRows), ctypes.c_int32,
-                                           ctypes.c_void_p]
+            # structures by reference or as packed bytes
+            getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
         lib.srw_attention_workspace_size.restype = ctypes.c_int
-        lib.srw_attention_workspace_size.argtypes = [ctypes.POINTER(SrwAttention), ctypes.POINTER(ctypes.c_size_t)]
+        lib.srw_attention_workspace_size.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]
         lib.srw_attention.restype = ctypes.c_int
-        lib.srw_attention.argtypes = [ctypes.POINTER(SrwAttention), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.srw_attention.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         got = lib.srw_abi_version()
         if got != ABI_VERSION:
             raise SrwLibraryError(f"libsrw_amd.so ABI {got} != binding ABI {ABI_VERSION}")

@@ -13,15 +13,20 @@
 // the eight k-slots of a lane are consecutive positions of the value page.
 // All heads of a group share one pass over their key head's pages.
 //
-// 8-bit pages: codes are bf16 numbers exactly, so the products run on the
-// codes; a key's scale multiplies its score and a value's its weight, both in
-// float32.  Weights are rounded to bf16 once (after their scale; the sum l
-// takes them unrounded), as the matrix cores read them; everything else is
-// float32.
+// 8-bit pages: the codes are bf16 numbers exactly, so both products run on the
+// codes.  A key's scale multiplies its score, a value's scale goes into the
+// exponent,
+//   w[j] = 2^(s[j] + log2 vs[j] - m),  l = sum_j w[j] / vs[j],
+// so that m follows the weights that the second product reads.  (l would lose
+// keys only where value scales of one row differ by more than 2^100.)
 //
-// m is raised only when a score passes it by more than 2^8: weights then stay
-// under 2^8 and their sum far inside float32, and the accumulators are
-// rescaled a few times a row instead of once a tile.
+// The matrix cores read weights in bf16.  The kernel for few rows, bound by
+// memory, gives them in two parts (bf16 of w and of what is left, 16 bits in
+// all), the one for many rows rounds them once; everything else is float32.
+//
+// m is raised only when an exponent passes it by more than 8: weights then stay
+// under 2^8 and their sum far inside float32, and the accumulators are rescaled
+// a few times a row instead of once a tile.
 //
 // What a token must not see is left out by selects, not by adding numbers;
 // positions without a page (a table entry that names none, as for positions
@@ -42,7 +47,8 @@ namespace {
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;
-constexpr float kLazy = 8.f;  // log2 of the largest weight before m is raised
+constexpr float kLazy = 8.f;       // log2 of the largest weight before m is raised
+constexpr float kLowest = -1e30f;  // m of a row that has seen nothing
 
 struct AttnArgs {
   KvView kv;
@@ -81,6 +87,89 @@ __device__ inline f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
 }
+// c + the sum of two bf16 numbers
+__device__ inline float add_bf16x2(uint32_t two, float c) {
+  const bf16x2_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), ones, c, false);
+}
+// The low n bits.
+__device__ inline uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+// The tile's keys (bit k: position key0 + k) that a token at position pos sees.
+__device__ inline uint64_t seen_of(int pos, int key0, int window, int sinks) {
+  const int rel = pos - key0;
+  uint64_t see = low_bits(rel + 1);
+  if (window > 0) see &= ~low_bits(rel - window + 1) | low_bits(sinks - key0);
+  return see;
+}
+// All ones where bit n of w is set, else zero; v there, else -inf.
+template <int N>
+__device__ inline uint32_t bit_mask(uint32_t w) {
+  return static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(w), N, 1));
+}
+template <int N>
+__device__ inline float only(uint32_t w, float v) {
+  const uint32_t m = bit_mask<N>(w);
+  return __uint_as_float((__float_as_uint(v) & m) | (0xff800000u & ~m));
+}
+// t[j] += (of in lane j of the lane's row of 16) * s[j], j = J0 .. J0 + 7, as
+// one instruction each: the compiler folds a row broadcast into a multiply or
+// a subtraction, but not into a multiply-add.  (Two wait states lie between a
+// register's write and its broadcast; one after a transcendental.)
+template <int J0>
+__device__ inline void fma_lanes8(float* t, float of, const float* s) {
+  asm volatile(
+      "s_nop 1\n\t"
+      "v_fmac_f32_dpp %0, %8, %9 row_newbcast:%c17 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %1, %8, %10 row_newbcast:%c18 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %2, %8, %11 row_newbcast:%c19 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %3, %8, %12 row_newbcast:%c20 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %4, %8, %13 row_newbcast:%c21 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %5, %8, %14 row_newbcast:%c22 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %6, %8, %15 row_newbcast:%c23 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %7, %8, %16 row_newbcast:%c24 row_mask:0xf bank_mask:0xf"
+      : "+v"(t[0]), "+v"(t[1]), "+v"(t[2]), "+v"(t[3]), "+v"(t[4]), "+v"(t[5]), "+v"(t[6]), "+v"(t[7])
+      : "v"(of), "v"(s[0]), "v"(s[1]), "v"(s[2]), "v"(s[3]), "v"(s[4]), "v"(s[5]), "v"(s[6]), "v"(s[7]), "n"(J0),
+        "n"(J0 + 1), "n"(J0 + 2), "n"(J0 + 3), "n"(J0 + 4), "n"(J0 + 5), "n"(J0 + 6), "n"(J0 + 7));
+}
+// l += (of in lane j of the lane's row of 16) * t[j], j = 0 .. 15.
+__device__ inline void sum_lanes16(float& l, float of, const float* t) {
+  asm volatile(
+      "s_nop 1\n\t"
+      "v_fmac_f32_dpp %0, %1, %2 row_newbcast:0 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %3 row_newbcast:1 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %4 row_newbcast:2 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %5 row_newbcast:3 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %6 row_newbcast:4 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %7 row_newbcast:5 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %8 row_newbcast:6 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %9 row_newbcast:7 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %10 row_newbcast:8 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %11 row_newbcast:9 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %12 row_newbcast:10 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %13 row_newbcast:11 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %14 row_newbcast:12 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %15 row_newbcast:13 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %16 row_newbcast:14 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %0, %1, %17 row_newbcast:15 row_mask:0xf bank_mask:0xf"
+      : "+v"(l)
+      : "v"(of), "v"(t[0]), "v"(t[1]), "v"(t[2]), "v"(t[3]), "v"(t[4]), "v"(t[5]), "v"(t[6]), "v"(t[7]), "v"(t[8]),
+        "v"(t[9]), "v"(t[10]), "v"(t[11]), "v"(t[12]), "v"(t[13]), "v"(t[14]), "v"(t[15]));
+}
+// Matrix accumulators that inline assembly reads next: the compiler does not
+// count the wait states of their last product (at most 18) for it.
+__device__ inline void settled(f32x16_t& a, f32x16_t& b) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a), "+v"(b)); }
+// A value's scale in the exponent: its log2 and its inverse.  A scale of zero
+// stands for values of zero and takes 2^-100; NaN stays.
+__device__ inline void in_exponent(float vs, float& lv, float& rv) {
+  const float x = vs <= 7.888609052210118e-31f ? 7.888609052210118e-31f : vs;
+  lv = __builtin_amdgcn_logf(x);
+  rv = __builtin_amdgcn_rcpf(x);
+}
+// m after a tile whose largest exponent over m (over 0 at first) is mt.
+__device__ inline float raised(float m, float mt) {
+  if (m == kLowest) return mt == -INFINITY ? kLowest : mt;
+  return mt > 0.f ? m + mt : m;
+}
 __device__ inline u32x4_t ld16(const void* p) { return *static_cast<const u32x4_t*>(p); }
 
 // The largest magnitude among bf16 pairs, as bits: 0x7f80 and above is not
@@ -114,17 +203,15 @@ __device__ inline void add_not_finite(const KvView& kv, int64_t b, int h, int he
                           (static_cast<int64_t>(pg) * kv.H + h) * head_dim * kv.P + ((key0 + k) & (kv.P - 1));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float x = bf16_to_f32(src[static_cast<int64_t>(dim(i)) * kv.P]);
+      // one address and one load after the other: their registers are the kernel's
+      int at = dim(i);
+      asm volatile("" : "+v"(at) : : "memory");
+      const float x = bf16_to_f32(src[static_cast<int64_t>(at) * kv.P]);
       if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) add(i, x);
     }
   }
 }
 
-// v times the value of lane J of v2's row of 16, for J = 0 .. 15 in turn.
-template <int J>
-__device__ inline float by_lane(float v, float of) {
-  return v * row_lane<J>(of);
-}
 template <class F, int... J>
 __device__ inline void each16(F f, std::integer_sequence<int, J...>) {
   (f(std::integral_constant<int, J>{}), ...);
@@ -180,7 +267,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
         const int d = ES == 2 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s & 1);
         q[x][s] = in ? ld16(src + d) : u32x4_t{0, 0, 0, 0};
       }
-      m[x] = -INFINITY;
+      m[x] = kLowest;
       l[x] = 0.f;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[x][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -204,10 +291,10 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int j = 0; j < NPC; ++j) kf[t][j] = ld16(ksrc + 4 * t * (DH * ES) + 64 * j);
-      float ksl = a.sc, vsl = 1.f;
+      float ksl = 0.f, lvl = 0.f, rvl = 0.f;
       if constexpr (KIND != SRW_KV_BF16) {
         ksl = a.kv.ks[hv * P + (kv & (P - 1)) + col] * a.sc;
-        vsl = a.kv.vs[hv * P + (kv & (P - 1)) + col];
+        in_exponent(a.kv.vs[hv * P + (kv & (P - 1)) + col], lvl, rvl);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d)
@@ -237,59 +324,71 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
       // every row sees every key of the tile?
       const bool whole = __all(have) && key0 + kTile - 1 <= p_lo &&
                          (a.window == 0 || key0 > p_hi - a.window || key0 + kTile <= a.sinks);
-      uint32_t seen = 0xffffu;  // bit 4 t + v: some row of the tile sees the lane's key
-      if (!whole) seen = 0;
-      u32x4_t pf[NQ][2];
+      uint32_t seen = 0;  // bit j: some row of the tile sees the lane's key kv + j
+      u32x4_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
-        float s[16];
+        uint32_t mine = 0xffffu;
+        if (!whole) {
+          mine = have ? static_cast<uint32_t>(seen_of(pos[x], key0, a.window, a.sinks) >> (16 * g)) & 0xffffu : 0u;
+          seen |= mine;
+        }
+        // exponents of the weights, over m (0 while the row has seen nothing)
+        float t[16];
+        const float mu = m[x] == kLowest ? 0.f : m[x];
         for16([&](auto jt) {
           constexpr int j = decltype(jt)::value;
-          s[j] = KIND == SRW_KV_BF16 ? acc[x][j >> 2][j & 3] * a.sc : by_lane<j>(acc[x][j >> 2][j & 3], ksl);
+          const float s = acc[x][j >> 2][j & 3];
+          t[j] = KIND == SRW_KV_BF16 ? fmaf(s, a.sc, -mu) : s * row_lane<j>(ksl) + (row_lane<j>(lvl) - mu);
         });
         if (!whole) {
-          const int rel = pos[x] - kv;  // key kv + j: j <= rel, j > rel - window or j < sinks - kv
-          const int below = a.window > 0 ? rel - a.window : -kTile - 1, first = a.sinks - kv;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const bool see = have && j <= rel && (j > below || j < first);
-            s[j] = see ? s[j] : -INFINITY;
-            seen |= see ? 1u << j : 0u;
-          }
+          for16([&](auto jt) {
+            constexpr int j = decltype(jt)::value;
+            t[j] = only<j>(mine, t[j]);
+          });
         }
-        float mt = s[0];
+        float mt = t[0];
 #pragma unroll
-        for (int j = 1; j < 16; ++j) mt = fmaxf(mt, s[j]);
-        if (__any(mt > m[x] + kLazy)) {
+        for (int j = 1; j < 16; ++j) mt = fmaxf(mt, t[j]);
+        if (__any(mt > (m[x] == kLowest ? -INFINITY : kLazy))) {
           auto mx = [](float u, float w) { return fmaxf(u, w); };
           mt = join32(join16(mt, mx), mx);
-          const float mn = fmaxf(m[x], mt);
-          const float w = m[x] == mn ? 1.f : __builtin_amdgcn_exp2f(m[x] - mn);
+          const float mn = raised(m[x], mt), back = (mn == kLowest ? 0.f : mn) - mu;
+          const float w = __builtin_amdgcn_exp2f(m[x] - mn);
           m[x] = mn;
           l[x] *= w;
 #pragma unroll
           for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int v = 0; v < 4; ++v) o[x][d][v] *= w;
-        }
-        const float ms = m[x] == -INFINITY ? 0.f : m[x];
-        float p[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          p[j] = __builtin_amdgcn_exp2f(s[j] - ms);
-          l[x] += p[j];
+          for (int j = 0; j < 16; ++j) t[j] -= back;
         }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) t[j] = __builtin_amdgcn_exp2f(t[j]);
         if constexpr (KIND != SRW_KV_BF16) {
-          for16([&](auto jt) {
-            constexpr int j = decltype(jt)::value;
-            const float w = by_lane<j>(p[j], vsl);
-            p[j] = whole || s[j] != -INFINITY ? w : 0.f;
-          });
+          if (whole) {
+            for16([&](auto jt) {
+              constexpr int j = decltype(jt)::value;
+              l[x] += t[j] * row_lane<j>(rvl);
+            });
+          } else {  // the scale of a key that is not seen may be anything
+            for16([&](auto jt) {
+              constexpr int j = decltype(jt)::value;
+              l[x] += __uint_as_float(__float_as_uint(t[j] * row_lane<j>(rvl)) & bit_mask<j>(mine));
+            });
+          }
         }
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) pf[x][st][u] = pack_bf16(p[8 * st + 2 * u], p[8 * st + 2 * u + 1]);
+          for (int u = 0; u < 4; ++u) {
+            const float p0 = t[8 * st + 2 * u], p1 = t[8 * st + 2 * u + 1];
+            const uint32_t hi = pack_bf16(p0, p1);
+            pf[x][st][u] = hi;
+            pl[x][st][u] = pack_bf16(p0 - lo_f32(hi), p1 - hi_f32(hi));
+            if constexpr (KIND == SRW_KV_BF16) l[x] += p0 + p1;
+          }
       }
       bool odd = false;  // a value is not finite
       if (!whole && KIND != SRW_KV_INT8) {
@@ -331,7 +430,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
           else
             vb = widen8<KIND>(vf[d][0][2 * st], vf[d][0][2 * st + 1]);
 #pragma unroll
-          for (int x = 0; x < NQ; ++x) o[x][d] = mfma16(vb, pf[x][st], o[x][d]);
+          for (int x = 0; x < NQ; ++x) o[x][d] = mfma16(vb, pl[x][st], mfma16(vb, pf[x][st], o[x][d]));
         }
       }
       if (KIND == SRW_KV_BF16 && odd) {
@@ -339,10 +438,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
         for (int x = 0; x < NQ; ++x)
           add_not_finite<4 * ND>(
               a.kv, b, h, DH, key0,
-              [&](int k) {
-                return key0 + k <= pos[x] &&
-                       (a.window == 0 || key0 + k > pos[x] - a.window || key0 + k < a.sinks);
-              },
+              [&](int k) { return seen_of(pos[x], key0, a.window, a.sinks) >> k & 1; },
               [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, [&](int i, float v) { o[x][i / 4][i % 4] += v; });
       }
     }
@@ -375,7 +471,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
         for (int d = 0; d < ND; ++d) ov[d] = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          // a wave without visible keys has m = -inf and l = 0
+          // (a wave without visible keys has l = 0)
           const float e = sm[w][r] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[w][r] - mm);
           ll += sl[w][r] * e;
 #pragma unroll
@@ -407,31 +503,62 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
   }
 }
 
-// Joins the splits: one wave a row, DH / 64 dims a lane.
+// Joins the splits: a workgroup a row, in groups of DH / 4 lanes that take the
+// splits in turn, each with all its loads in flight, and join in LDS.
 template <int DH>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float* part, const float2* ml, uint16_t* out,
                                                         int64_t rows, int S) {
-  constexpr int N = DH / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  float mm = -INFINITY;
-  for (int s = lane; s < S; s += 64) mm = fmaxf(mm, ml[s * rows + row].x);
-  mm = wave_max(mm);
-  float ll = 0.f, o[N] = {};
-  for (int s = 0; s < S; ++s) {
-    const float2 x = ml[s * rows + row];
-    if (x.y == 0.f) continue;  // no visible keys there, and no output written
-    const float e = x.x == mm ? 1.f : __builtin_amdgcn_exp2f(x.x - mm);
-    ll += x.y * e;
+  constexpr int L = DH / 4, N = 256 / L;  // lanes a group, groups
+  __shared__ float sm[N], sl[N];
+  __shared__ f32x4_t so[N][L];
+  const int grp = threadIdx.x / L, c = threadIdx.x % L;
+  const int64_t row = blockIdx.x;
+  float m = kLowest, l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;
+  for (int s0 = grp; s0 < S; s0 += N * U) {
+    float2 x[U];
+    f32x4_t v[U];
 #pragma unroll
-    for (int d = 0; d < N; ++d) o[d] += part[(s * rows + row) * DH + lane * N + d] * e;
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + N * u < S ? s0 + N * u : s0;
+      x[u] = ml[s * rows + row];
+      v[u] = *reinterpret_cast<const f32x4_t*>(part + (s * rows + row) * DH + 4 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // a split without visible keys wrote no output
+      if (s0 + N * u >= S || x[u].y == 0.f) continue;
+      const float mn = fmaxf(m, x[u].x);
+      const float e0 = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      const float e1 = x[u].x == mn ? 1.f : __builtin_amdgcn_exp2f(x[u].x - mn);
+      m = mn;
+      l = l * e0 + x[u].y * e1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = o[k] * e0 + v[u][k] * e1;
+    }
+  }
+  if (c == 0) {
+    sm[grp] = m;
+    sl[grp] = l;
+  }
+  so[grp][c] = o;
+  __syncthreads();
+  if (grp != 0) return;
+  float mm = sm[0], ll = 0.f;
+#pragma unroll
+  for (int g = 1; g < N; ++g) mm = fmaxf(mm, sm[g]);
+  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < N; ++g) {
+    const float e = sm[g] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[g] - mm);
+    ll += sl[g] * e;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] += so[g][c][k] * e;
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  if constexpr (N == 2)
-    *reinterpret_cast<uint32_t*>(out + row * DH + 2 * lane) = pack_bf16(o[0] * inv, o[1] * inv);
-  else
-    out[row * DH + lane] = f32_to_bf16_bits(o[0] * inv);
+  *reinterpret_cast<uint2*>(out + row * DH + 4 * c) =
+      make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
 // -- many rows: chunks of prompts ---------------------------------------------
@@ -497,13 +624,18 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) q[s] = in ? ld16(src + 16 * s) : u32x4_t{0, 0, 0, 0};
   }
-  float m = -INFINITY, l = 0.f;
+  float m = kLowest, l = 0.f;
   f32x16_t o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
 
+  // A tile's position in its pages: slot of its first key (pages of 64 and more
+  // hold whole tiles; smaller ones start with one), then the slot of key k.
+  const int64_t page_bytes = static_cast<int64_t>(a.kv.H) * P * DH * ES, head_at = static_cast<int64_t>(h) * P * DH * ES;
+  const char* kbase = a.kv.k + head_at;
+  const char* vbase = a.kv.v + head_at;
   // pages of tile i: lane c holds that of positions key0 + 16 (c & 3)
   auto pages_of = [&](int i) {
     const int at = sp.key0(i) + 16 * (lane & 3);
@@ -511,36 +643,39 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   };
   u32x4_t rk[Q8 ? NI / 2 : 1], rv[Q8 ? NI / 2 : 1];  // 8-bit tiles on their way
   auto fetch = [&](int i, int ids, int stage) {
-    const int key0 = sp.key0(i);
+    const int slot0 = sp.key0(i) & (P - 1);
     const int safe = ids < 0 ? 0 : ids;
     if constexpr (!Q8) {
+      // pieces n of a lane: keys of one group of 16 for the whole wave
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         const int first = (wave * NI + n) * 64;      // piece of lane 0
         const int row = (first + lane) / NP, pc = ((first + lane) % NP) ^ k_swz<DH>(row);
         const int64_t pg = __builtin_amdgcn_readlane(safe, (first / NP) >> 4);
-        g2lds16(a.kv.k + (((pg * a.kv.H + h) * P + ((key0 + row) & (P - 1))) * DH + 8 * pc) * ES, kl[stage] + 16 * first);
+        g2lds16(kbase + pg * page_bytes + slot0 * (DH * ES) + ((row & (P - 1)) * DH + 8 * pc) * ES, kl[stage] + 16 * first);
       }
+      // values: positions 8 pc .. of a dim, pc = (lane & 7) ^ (lane >> 4) ^ 4 (n & 1)
+      const int pe = (lane & 7) ^ (lane >> 4);
+      const int64_t pg[2] = {__shfl(safe, pe >> 1), __shfl(safe, (pe ^ 4) >> 1)};
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         const int first = (wave * NI + n) * 64;
-        const int row = (first + lane) / 8, pc = ((first + lane) % 8) ^ v_swz(row);
-        const int64_t pg = __shfl(safe, pc >> 1);
-        g2lds16(a.kv.v + (((pg * a.kv.H + h) * DH + row) * P + ((key0 + 8 * pc) & (P - 1))) * ES, vl[stage] + 16 * first);
+        const int row = (first + lane) / 8, pc = pe ^ (4 * (n & 1));
+        g2lds16(vbase + pg[n & 1] * page_bytes + (row * P + slot0 + ((8 * pc) & (P - 1))) * ES, vl[stage] + 16 * first);
       }
     } else {
-      // a thread's 16 codes: of keys, 16 dims of a position; of values, 16
-      // positions of a dim
+      // a thread's 16 codes: of keys, 16 dims of a position (the wave's
+      // positions in one group of 16); of values, 16 positions of a dim
 #pragma unroll
       for (int n = 0; n < NI / 2; ++n) {
         const int at = n * 256 + threadIdx.x;
         const int row = at / (NP / 2), pc = at % (NP / 2);
-        const int64_t pg = __shfl(safe, row >> 4);
-        rk[n] = ld16(a.kv.k + ((pg * a.kv.H + h) * P + ((key0 + row) & (P - 1))) * DH + 16 * pc);
-        const int vrow = at / 4, vpc = at % 4;
-        const int64_t vg = __shfl(safe, vpc);
-        rv[n] = ld16(a.kv.v + ((vg * a.kv.H + h) * DH + vrow) * P + ((key0 + 16 * vpc) & (P - 1)));
+        const int64_t pg = __builtin_amdgcn_readlane(safe, (n * 256 + wave * 64) / (NP / 2) >> 4);
+        rk[n] = ld16(kbase + pg * page_bytes + slot0 * DH + ((row & (P - 1)) * DH + 16 * pc));
       }
+      const char* vsrc = vbase + safe * page_bytes + slot0 + ((16 * (lane & 3)) & (P - 1));
+#pragma unroll
+      for (int n = 0; n < NI / 2; ++n) rv[n] = ld16(vsrc + (n * 64 + (threadIdx.x >> 2)) * P);
     }
   };
   auto settle = [&](int stage) {  // 8 bits: widen into LDS
@@ -549,11 +684,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
       for (int n = 0; n < NI / 2; ++n) {
         const int at = n * 256 + threadIdx.x;
         const int row = at / (NP / 2), pc = at % (NP / 2);
+        const int vrow = at / 4, vpc = at % 4;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           *reinterpret_cast<u32x4_t*>(kl[stage] + row * (DH * 2) + 16 * ((2 * pc + u) ^ k_swz<DH>(row))) =
               widen8<KIND>(rk[n][2 * u], rk[n][2 * u + 1]);
-          const int vrow = at / 4, vpc = at % 4;
           *reinterpret_cast<u32x4_t*>(vl[stage] + vrow * 128 + 16 * ((2 * vpc + u) ^ v_swz(vrow))) =
               widen8<KIND>(rv[n][2 * u], rv[n][2 * u + 1]);
         }
@@ -562,16 +697,17 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   };
   // scales of the lane's keys: of its 32 score registers (kb, v), register
   // kb of lane v of a row of 16 holds that of key 32 kb + 16 (v / 8) + 8 hf + v % 8
-  float ksl[2], vsl[2], ksn[2], vsn[2];
+  float ksl[2], lvl[2], rvl[2], ksn[2], vsn[2];
   auto scales = [&](int i, int ids) {
     if constexpr (Q8) {
-      const int key0 = sp.key0(i);
+      const int slot0 = sp.key0(i) & (P - 1);
+      const int safe = ids < 0 ? 0 : ids;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const int k = 32 * kb + 8 * (lane & 8 ? 2 : 0) + 8 * hf + (lane & 7);
-        const int64_t pg = __shfl(ids < 0 ? 0 : ids, k >> 4);
-        const int64_t at = (pg * a.kv.H + h) * P + ((key0 + k) & (P - 1));
-        ksn[kb] = a.kv.ks[at] * a.sc;
+        const int k = 32 * kb + 16 * (lane >> 3 & 1) + 8 * hf + (lane & 7);
+        const int64_t pg = lane & 8 ? __builtin_amdgcn_readlane(safe, 2 * kb + 1) : __builtin_amdgcn_readlane(safe, 2 * kb);
+        const int64_t at = (pg * a.kv.H + h) * P + slot0 + (k & (P - 1));
+        ksn[kb] = a.kv.ks[at];
         vsn[kb] = a.kv.vs[at];
       }
     }
@@ -589,10 +725,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     wait_vm0();
     __syncthreads();
     const int cur = ids;
+    if constexpr (Q8) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      ksl[kb] = ksn[kb];
-      vsl[kb] = vsn[kb];
+      for (int kb = 0; kb < 2; ++kb) {
+        ksl[kb] = ksn[kb] * a.sc;
+        in_exponent(vsn[kb], lvl[kb], rvl[kb]);
+      }
     }
     if (i + 1 < i1) {
       fetch(i + 1, idn, stage ^ 1);
@@ -614,80 +752,96 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) acc[kb] = mfma(ld16(src + 16 * ((2 * s + hf) ^ k_swz<DH>(row))), q[s], acc[kb]);
     }
-    // positions of the tile that some row of the workgroup can see
-    uint64_t keys = ~0ull;
+    // positions of the tile that some row of the workgroup sees
+    uint64_t keys = low_bits(sp.hi - key0);
     {
-      const uint64_t have = __ballot(cur >= 0);
-      if ((have & 15) != 15) {
-        keys = 0;
+      const uint64_t have = __ballot(cur >= 0) & 15;
+      if (have != 15) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) keys |= (have >> u & 1) ? 0xffffull << (16 * u) : 0ull;
+        for (int u = 0; u < 4; ++u)
+          if (!(have >> u & 1)) keys &= ~(0xffffull << (16 * u));
       }
-      if (sp.hi - key0 < kTile) keys &= (1ull << (sp.hi - key0)) - 1;  // hi > key0
-      if (key0 < sp.lo) {
-        const int below = sp.lo - key0, first = a.sinks - key0;
-        uint64_t drop = below >= kTile ? ~0ull : (1ull << below) - 1;
-        if (first > 0) drop &= first >= kTile ? 0ull : ~((1ull << first) - 1);
-        keys &= ~drop;
-      }
+      if (key0 < sp.lo) keys &= ~low_bits(sp.lo - key0) | low_bits(a.sinks - key0);
     }
     const bool whole = keys == ~0ull && key0 + kTile - 1 <= p_lo &&
                        (a.window == 0 || key0 > p_hi - a.window || key0 + kTile <= a.sinks);
-    float s[2][16];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-      for16([&](auto vt) {
-        constexpr int v = decltype(vt)::value;
-        s[kb][v] = Q8 ? by_lane<v>(acc[kb][v], ksl[kb]) : acc[kb][v] * a.sc;
-      });
+    // bits 32 kb + 16 (v / 8) + v % 8: the lane's row sees the key of its register (kb, v)
+    uint32_t mine[2] = {~0u, ~0u};
     if (!whole) {
-      const uint64_t mine = keys >> (8 * hf);
-      const int rel = pos - key0 - 8 * hf, below = a.window > 0 ? rel - a.window : -2 * kTile,
-                first = a.sinks - key0 - 8 * hf;
+      const uint64_t see = (seen_of(pos, key0, a.window, a.sinks) & keys) >> (8 * hf);
+      mine[0] = static_cast<uint32_t>(see);
+      mine[1] = static_cast<uint32_t>(see >> 32);
+    }
+    // exponents of the weights, over m (0 while the row has seen nothing)
+    float t[2][16];
+    const float mu = m == kLowest ? 0.f : m;
+    if constexpr (Q8) {
+      settled(acc[0], acc[1]);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        float s[16];
+        for16([&](auto vt) {
+          constexpr int v = decltype(vt)::value;
+          s[v] = acc[kb][v];
+          t[kb][v] = row_lane<v>(lvl[kb]) - mu;
+        });
+        fma_lanes8<0>(t[kb], ksl[kb], s);
+        fma_lanes8<8>(t[kb] + 8, ksl[kb], s + 8);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < 32; ++v) t[v >> 4][v & 15] = fmaf(acc[v >> 4][v & 15], a.sc, -mu);
+    }
+    if (!whole) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int k = 32 * kb + 16 * (v / 8) + v % 8;
-          const bool see = (mine >> k & 1) && k <= rel && (k > below || k < first);
-          s[kb][v] = see ? s[kb][v] : -INFINITY;
-        }
+        for16([&](auto vt) {
+          constexpr int v = decltype(vt)::value;
+          t[kb][v] = only<16 * (v / 8) + v % 8>(mine[kb], t[kb][v]);
+        });
     }
-    float mt = s[0][0];
+    float mt = t[0][0];
 #pragma unroll
-    for (int v = 1; v < 32; ++v) mt = fmaxf(mt, s[v >> 4][v & 15]);
-    if (__any(mt > m + kLazy)) {
+    for (int v = 1; v < 32; ++v) mt = fmaxf(mt, t[v >> 4][v & 15]);
+    if (__any(mt > (m == kLowest ? -INFINITY : kLazy))) {
       mt = join32(mt, [](float u, float w) { return fmaxf(u, w); });
-      const float mn = fmaxf(m, mt);
-      const float w = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      const float mn = raised(m, mt), back = (mn == kLowest ? 0.f : mn) - mu;
+      const float w = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= w;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[d][v] *= w;
+#pragma unroll
+      for (int v = 0; v < 32; ++v) t[v >> 4][v & 15] -= back;
     }
-    const float ms = m == -INFINITY ? 0.f : m;
     u32x4_t pf[4];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      float p[16];
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        p[v] = __builtin_amdgcn_exp2f(s[kb][v] - ms);
-        l += p[v];
-      }
+      for16([&](auto vt) {
+        constexpr int v = decltype(vt)::value;
+        t[kb][v] = __builtin_amdgcn_exp2f(t[kb][v]);
+      });
       if constexpr (Q8) {
-        for16([&](auto vt) {
-          constexpr int v = decltype(vt)::value;
-          const float w = by_lane<v>(p[v], vsl[kb]);
-          p[v] = whole || s[kb][v] != -INFINITY ? w : 0.f;
-        });
+        if (whole) {
+          sum_lanes16(l, rvl[kb], t[kb]);
+        } else {  // the scale of a key that is not seen may be anything
+          for16([&](auto vt) {
+            constexpr int v = decltype(vt)::value;
+            l += __uint_as_float(__float_as_uint(row_lane<v>(rvl[kb]) * t[kb][v]) &
+                                 bit_mask<16 * (v / 8) + v % 8>(mine[kb]));
+          });
+        }
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) pf[2 * kb + j][u] = pack_bf16(p[8 * j + 2 * u], p[8 * j + 2 * u + 1]);
+        for (int u = 0; u < 4; ++u) {
+          const float p0 = t[kb][8 * j + 2 * u], p1 = t[kb][8 * j + 2 * u + 1];
+          pf[2 * kb + j][u] = pack_bf16(p0, p1);
+          if constexpr (!Q8) l = add_bf16x2(pf[2 * kb + j][u], l);
+        }
     }
     bool odd = false;  // a value is not finite
     if (KIND == SRW_KV_BF16 && !whole) {
@@ -721,9 +875,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     if (KIND == SRW_KV_BF16 && odd)
       add_not_finite<16 * ND>(
           a.kv, b, h, DH, key0,
-          [&](int k) {
-            return key0 + k <= pos && (a.window == 0 || key0 + k > pos - a.window || key0 + k < a.sinks);
-          },
+          [&](int k) { return seen_of(pos, key0, a.window, a.sinks) >> k & 1; },
           [&](int i) { return 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * hf + i % 4; },
           [&](int i, float v) { o[i / 16][i % 16] += v; });
   }
@@ -803,8 +955,8 @@ hipError_t launch_attention(const srw_attention_t& a, const AttnPlan& pl, AttnAr
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || g.S == 1) return e;
   const int64_t rows = a.kv.T * a.n_heads;
-  hipLaunchKernelGGL(attn_join_kernel<DH>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, g.part, g.ml,
-                     g.out, rows, g.S);
+  hipLaunchKernelGGL(attn_join_kernel<DH>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, g.part, g.ml, g.out, rows,
+                     g.S);
   return hipGetLastError();
 }
 

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -33,18 +34,26 @@ BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 _KINDS = {torch.bfloat16: C.SRW_KV_BF16, torch.int8: C.SRW_KV_INT8, torch.float8_e4m3fn: C.SRW_KV_FP8}
 _DTYPES = {torch.float32: C.SRW_F32, torch.bfloat16: C.SRW_BF16}
 
+# srw_kv_t, srw_kv_rows_t and srw_attention_t as bytes: a call's description is
+# packed in a fraction of the time that a ctypes structure takes to fill, which
+# for single tokens would be half of the call
+_KV = struct.Struct("@7P5q4i")
+_ROWS = struct.Struct("@2P4q")
+_ATTENTION = struct.Struct("@7P5q4i2P2q4if4x")
+
 
 def _tensor(name, t, dev, dtype, shape):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous():
+        return t.data_ptr()
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, expected {dev}")
     if t.dtype != dtype:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
 
 
 class KvPages:
@@ -64,44 +73,46 @@ class KvPages:
         dev = k.device
         if dev.type != "cuda":
             raise ValueError(f"the cache lives on a HIP device; got {dev}")
-        if k.dtype not in _KINDS:
+        kind = _KINDS.get(k.dtype)
+        if kind is None:
             raise TypeError(f"pages hold bfloat16, int8 or float8_e4m3fn; got {k.dtype}")
         if not k.is_contiguous():
             raise ValueError("k must be contiguous")
-        _tensor("v", v, dev, k.dtype, (n, h, d, p))
-        self.kind = _KINDS[k.dtype]
-        if self.kind == C.SRW_KV_BF16:
+        at = _tensor("v", v, dev, k.dtype, (n, h, d, p))
+        if kind == C.SRW_KV_BF16:
             if k_scale is not None or v_scale is not None:
                 raise ValueError("bfloat16 pages have no scales")
-            self._at = (k.data_ptr(), v.data_ptr(), None, None)
+            self._at = (k.data_ptr(), at, 0, 0)
         else:
-            _tensor("k_scale", k_scale, dev, F32, (n, h, p))
-            _tensor("v_scale", v_scale, dev, F32, (n, h, p))
-            self._at = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+            self._at = (k.data_ptr(), at, _tensor("k_scale", k_scale, dev, F32, (n, h, p)),
+                        _tensor("v_scale", v_scale, dev, F32, (n, h, p)))
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_pages, self.heads, self.page_size, self.head_dim, self.device = n, h, p, d, dev
+        self.n_pages, self.heads, self.page_size, self.head_dim, self.kind, self.device = n, h, p, d, kind, dev
 
 
 def _address(pages, table, lens, cu, T):
-    """The C description of a call's sequences over these pages."""
+    """The fields of srw_kv_t: a call's sequences over these pages."""
     dev = pages.device
-    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
-    if B < 0:
+    if not isinstance(lens, torch.Tensor) or lens.dim() != 1:
         raise ValueError("lens must be a tensor [B]")
-    _tensor("lens", lens, dev, I32, (B,))
+    B = lens.shape[0]
+    lens_at = _tensor("lens", lens, dev, I32, (B,))
     if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[0] != B:
         raise ValueError(f"table must be a tensor [{B}, width]")
-    if table.device != dev or table.dtype != I32:
+    if table.dtype is not I32 or table.device != dev:
         raise TypeError(f"table must be int32 on {dev}; got {table.dtype} on {table.device}")
-    width, stride = table.shape[1], table.stride(0)
-    if width > 1 and table.stride(1) != 1 or B > 1 and stride < width:
+    width = table.shape[1]
+    stride, step = table.stride()
+    if step != 1 and width > 1 or stride < width and B > 1:
         raise ValueError("rows of table must be consecutive")
     if cu is not None:
-        _tensor("cu", cu, dev, I32, (B + 1,))
-    elif T != B:
+        cu_at = _tensor("cu", cu, dev, I32, (B + 1,))
+    elif T == B:
+        cu_at = 0
+    else:
         raise ValueError(f"{T} tokens of {B} sequences need cu")
-    return C.SrwKv(*pages._at, table.data_ptr(), lens.data_ptr(), None if cu is None else cu.data_ptr(), B, T,
-                   pages.n_pages, width, max(stride, width), pages.heads, pages.head_dim, pages.page_size, pages.kind)
+    return (*pages._at, table.data_ptr(), lens_at, cu_at, B, T, pages.n_pages, width, stride if stride > width else width,
+            pages.heads, pages.head_dim, pages.page_size, pages.kind)
 
 
 def _rows(name, t, pages, T, dtypes, unit):
@@ -122,20 +133,14 @@ def _rows(name, t, pages, T, dtypes, unit):
     return t
 
 
-class _OnDevice:
-    """The device made current where it is not (launches go to the current
-    device's streams)."""
-
-    def __init__(self, dev):
-        self.ctx = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _call(f, dev, *args):
+    """f's status with the current stream of dev as its last argument (launches
+    go to the current device's streams)."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if torch._C._cuda_getDevice() == dev.index:
+        return f(*args, stream)
+    with torch.cuda.device(dev):
+        return f(*args, stream)
 
 
 def kv_write(pages: KvPages, k, v, table, lens, cu=None) -> None:
@@ -152,10 +157,8 @@ def kv_write(pages: KvPages, k, v, table, lens, cu=None) -> None:
     v = _rows("v", v, pages, T, (k.dtype,), 4)
     if k.shape[1] != pages.heads or v.shape[1] != pages.heads:
         raise ValueError(f"k and v have {k.shape[1]} and {v.shape[1]} heads, the pages {pages.heads}")
-    r = C.SrwKvRows(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    with _OnDevice(pages.device):
-        C.check(C.load_library().srw_kv_write(ctypes.byref(a), ctypes.byref(r), _DTYPES[k.dtype],
-                                              torch.cuda.current_stream(pages.device).cuda_stream))
+    r = _ROWS.pack(k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2])
+    C.check(_call(C.load_library().srw_kv_write, pages.device, _KV.pack(*a), r, _DTYPES[k.dtype]))
 
 
 def kv_read(pages: KvPages, table, lens, cu=None, *, total=None, dtype=BF16):
@@ -169,11 +172,11 @@ def kv_read(pages: KvPages, table, lens, cu=None, *, total=None, dtype=BF16):
         raise ValueError("total, the number of tokens, is needed with cu")
     T = int(total) if total is not None else lens.shape[0]
     a = _address(pages, table, lens, cu, T)
-    k, v = (torch.empty((T, pages.heads, pages.head_dim), dtype=dtype, device=pages.device) for _ in range(2))
-    r = C.SrwKvRows(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    with _OnDevice(pages.device):
-        C.check(C.load_library().srw_kv_read(ctypes.byref(a), ctypes.byref(r), _DTYPES[dtype],
-                                             torch.cuda.current_stream(pages.device).cuda_stream))
+    H, d = pages.heads, pages.head_dim
+    k = torch.empty((T, H, d), dtype=dtype, device=pages.device)
+    v = torch.empty_like(k)
+    r = _ROWS.pack(k.data_ptr(), v.data_ptr(), H * d, d, H * d, d)
+    C.check(_call(C.load_library().srw_kv_read, pages.device, _KV.pack(*a), r, _DTYPES[dtype]))
     return k, v
 
 
@@ -203,14 +206,16 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
         out = torch.empty((T, Hq, pages.head_dim), dtype=BF16, device=dev)
     else:
         _tensor("out", out, dev, BF16, (T, Hq, pages.head_dim))
-    a = C.SrwAttention(kv, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), Hq, max_new, window, sinks, scale)
+    st = q.stride()
+    a = _ATTENTION.pack(*kv, q.data_ptr(), out.data_ptr(), st[0], st[1], Hq, max_new, window, sinks, scale)
     lib = C.load_library()
-    need = ctypes.c_size_t(0)
-    with _OnDevice(dev):
-        C.check(lib.srw_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        C.check(lib.srw_attention(ctypes.byref(a), None if ws is None else ws.data_ptr(), need.value,
-                                  torch.cuda.current_stream(dev).cuda_stream))
+    status = _call(lib.srw_attention, dev, a, None, 0)
+    if status == C.SRW_EWORKSPACE:  # splits to join, nothing launched yet
+        need = ctypes.c_size_t(0)
+        C.check(lib.srw_attention_workspace_size(a, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        status = _call(lib.srw_attention, dev, a, ws.data_ptr(), need.value)
+    C.check(status)
     return out
 
 

@@ -436,7 +436,8 @@ srw_status_t srw_cast_bf16(int32_t n, const float* const* src, void* const* dst,
  * A layer's pages are four arrays of the caller:
  *   k [n_pages, n_kv_heads, page_size, head_dim]
  *   v [n_pages, n_kv_heads, head_dim, page_size]   (dimension by dimension)
- *   k_scale, v_scale [n_pages, n_kv_heads, page_size] float32, with 8-bit kinds
+ *   k_scale, v_scale [n_pages, n_kv_heads, page_size] float32 (not negative), with 8-bit
+ *     kinds
  * Sequence b has lens[b] positions, the call's new tokens included: the last
  * cu[b + 1] - cu[b] of them, whose packed rows are [cu[b], cu[b + 1]) of T
  * (cu[0] = 0, cu[B] = T); cu NULL: one new token each, T = B.  Position p is
@@ -486,7 +487,7 @@ srw_status_t srw_kv_read(const srw_kv_t* cache, const srw_kv_rows_t* rows, int32
  * head h / (n_heads / n_kv_heads)).  q rows at q + t * q_token_stride + h *
  * q_head_stride (elements, multiples of 8; 16-byte aligned), out [T, n_heads,
  * head_dim] contiguous, both bf16; float32 inside but for the softmax weights,
- * which the matrix cores read as bf16.  The cache must hold the new tokens
+ * which the matrix cores read as bf16 (in calls of few rows as two parts).  The cache must hold the new tokens
  * (srw_kv_write before, on the same stream). */
 typedef struct srw_attention {
   srw_kv_t kv;

@@ -541,7 +541,7 @@ def test_refusals(pkg, dev):
     long = Cache(pkg, dev, "bf16", 1, 64, 64, [9000], seed=132)
     from dawn_srw_amd.kv import _address
     q1, out = torch.zeros(1, 1, 64, dtype=BF, device=dev), torch.zeros(1, 1, 64, dtype=BF, device=dev)
-    a = C.SrwAttention(_address(long.pages, long.table, long.len_t, None, 1), q1.data_ptr(), out.data_ptr(), 64, 64, 1, 1,
+    a = C.SrwAttention(C.SrwKv(*_address(long.pages, long.table, long.len_t, None, 1)), q1.data_ptr(), out.data_ptr(), 64, 64, 1, 1,
                        0, 0, 1.0)
     need = ctypes.c_size_t(0)
     assert lib.srw_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)) == C.SRW_OK and need.value > 0
