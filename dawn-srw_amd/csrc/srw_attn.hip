@@ -83,14 +83,38 @@ __device__ inline Span span_of(const AttnArgs& a, int p_lo, int p_hi) {
   return s;
 }
 
+// The sequence and the tile of R rows (token, head of the group) of workgroup
+// `at`.  start(b) = cu[b] G / R + b leaves room for a last, partial tile; a
+// sequence's last tiles, which see most, come first.
+struct Tile {
+  int64_t b;
+  KvSeq sq;
+  int r0, r1;  // r0 = -1: none
+};
+template <int R>
+__device__ inline Tile tile_of(const AttnArgs& a, int64_t at) {
+  Tile t;
+  int64_t rt;
+  if (a.kv.cu) {
+    auto start = [&](int64_t i) { return static_cast<int64_t>(a.kv.cu[i]) * a.G / R + i; };
+    t.b = kv_find(a.kv.B, at, start);
+    rt = at - start(t.b);
+  } else {
+    const int per = (a.G + R - 1) / R;
+    t.b = at / per;
+    rt = at % per;
+  }
+  t.b = __builtin_amdgcn_readfirstlane(static_cast<int>(t.b));
+  t.sq = kv_seq(a.kv, t.b);
+  const int rows = t.sq.n * a.G, rts = (rows + R - 1) / R;
+  t.r0 = rt < 0 || rt >= rts ? -1 : (rts - 1 - static_cast<int>(rt)) * R;
+  t.r1 = t.r0 + R < rows ? t.r0 + R : rows;
+  return t;
+}
+
 __device__ inline f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
-}
-// c + the sum of two bf16 numbers
-__device__ inline float add_bf16x2(uint32_t two, float c) {
-  const bf16x2_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), ones, c, false);
 }
 // The low n bits.
 __device__ inline uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
@@ -157,7 +181,9 @@ __device__ inline void sum_lanes16(float& l, float of, const float* t) {
 }
 // Matrix accumulators that inline assembly reads next: the compiler does not
 // count the wait states of their last product (at most 18) for it.
-__device__ inline void settled(f32x16_t& a, f32x16_t& b) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a), "+v"(b)); }
+__device__ inline void settled(f32x4_t (&a)[4]) {
+  asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
+}
 // A value's scale in the exponent: its log2 and its inverse.  A scale of zero
 // stands for values of zero and takes 2^-100; NaN stays.
 __device__ inline void in_exponent(float vs, float& lv, float& rv) {
@@ -221,6 +247,78 @@ __device__ inline void for16(F f) {
   each16(f, std::make_integer_sequence<int, 16>{});
 }
 
+// The scores of a tile become weights.  A lane holds 16 scores of one token (of
+// lane & 15), those of the keys 16 g + j, g = lane >> 4, as acc[j / 4][j % 4];
+// scales of the tile's key k lie in lane k.  whole: every token sees every
+// key, else bit j of `mine` says whether the lane's token sees key 16 g + j.
+// pf gets the weights rounded to bf16, with TWO pl what the rounding left.
+template <int KIND, int ND, bool TWO>
+__device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, float rvl, bool whole, uint32_t mine,
+                             float& m, float& l, f32x4_t (&o)[ND], u32x4_t (&pf)[2], u32x4_t (&pl)[2]) {
+  // exponents, over m (0 while the token has seen nothing)
+  float t[16];
+  const float mu = m == kLowest ? 0.f : m;
+  if constexpr (KIND == SRW_KV_BF16) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t[j] = fmaf(acc[j >> 2][j & 3], sc, -mu);
+  } else {
+    float s[16];
+    settled(acc);
+    for16([&](auto jt) {
+      constexpr int j = decltype(jt)::value;
+      s[j] = acc[j >> 2][j & 3];
+      t[j] = row_lane<j>(lvl) - mu;
+    });
+    fma_lanes8<0>(t, ksl, s);
+    fma_lanes8<8>(t + 8, ksl, s + 8);
+  }
+  if (!whole) {
+    for16([&](auto jt) {
+      constexpr int j = decltype(jt)::value;
+      t[j] = only<j>(mine, t[j]);
+    });
+  }
+  float mt = t[0];
+#pragma unroll
+  for (int j = 1; j < 16; ++j) mt = fmaxf(mt, t[j]);
+  if (__any(mt > (m == kLowest ? -INFINITY : kLazy))) {
+    auto mx = [](float u, float w) { return fmaxf(u, w); };
+    mt = join32(join16(mt, mx), mx);
+    const float mn = raised(m, mt), back = (mn == kLowest ? 0.f : mn) - mu;
+    const float w = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= w;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) o[d][v] *= w;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t[j] -= back;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) t[j] = __builtin_amdgcn_exp2f(t[j]);
+  if constexpr (KIND == SRW_KV_BF16) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) l += t[j];
+  } else if (whole) {
+    sum_lanes16(l, rvl, t);
+  } else {  // the scale of a key that is not seen may be anything
+    for16([&](auto jt) {
+      constexpr int j = decltype(jt)::value;
+      l += __uint_as_float(__float_as_uint(row_lane<j>(rvl) * t[j]) & bit_mask<j>(mine));
+    });
+  }
+#pragma unroll
+  for (int st = 0; st < 2; ++st)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float p0 = t[8 * st + 2 * u], p1 = t[8 * st + 2 * u + 1];
+      const uint32_t hi = pack_bf16(p0, p1);
+      pf[st][u] = hi;
+      if constexpr (TWO) pl[st][u] = pack_bf16(p0 - lo_f32(hi), p1 - hi_f32(hi));
+    }
+}
+
 // -- few rows: single tokens, short chunks -----------------------------------
 //
 // A workgroup takes up to 16 NQ rows (token, head of the group) of one
@@ -239,296 +337,243 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
   const int split = blockIdx.z, h = blockIdx.y;
-  const int64_t b = blockIdx.x;
-  const KvSeq sq = kv_seq(a.kv, b);
-  const int rows = sq.n * a.G;
+  const Tile tl = tile_of<16 * NQ>(a, blockIdx.x);
+  if (tl.r0 < 0) return;
+  const int64_t b = tl.b;
+  const KvSeq sq = tl.sq;
+  const int r0 = tl.r0, r1 = tl.r1;
   const int P = a.kv.P;
-  for (int r0 = 0; r0 < rows; r0 += 16 * NQ) {
-    const int r1 = r0 + 16 * NQ < rows ? r0 + 16 * NQ : rows;
-    const int p_lo = sq.len - sq.n + r0 / a.G, p_hi = sq.len - sq.n + (r1 - 1) / a.G;
-    const Span sp = span_of(a, p_lo, p_hi);
-    const int i0 = split * a.per;
-    const int i1 = i0 + a.per < sp.tiles ? i0 + a.per : sp.tiles;
+  const int p_lo = sq.len - sq.n + r0 / a.G, p_hi = sq.len - sq.n + (r1 - 1) / a.G;
+  const Span sp = span_of(a, p_lo, p_hi);
+  const int i0 = split * a.per;
+  const int i1 = i0 + a.per < sp.tiles ? i0 + a.per : sp.tiles;
 
-    u32x4_t q[NQ][NS];
-    int pos[NQ];
-    float m[NQ], l[NQ];
-    f32x4_t o[NQ][ND];
+  u32x4_t q[NQ][NS];
+  int pos[NQ];
+  float m[NQ], l[NQ];
+  f32x4_t o[NQ][ND];
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      const int fr = r0 + 16 * x + col;
-      const bool in = fr < r1;
-      const int tok = in ? fr / a.G : 0;
-      pos[x] = in ? sq.len - sq.n + tok : -1;
-      const uint16_t* src = a.q + (sq.row0 + tok) * a.q_token + (h * a.G + (in ? fr - tok * a.G : 0)) * a.q_head;
+  for (int x = 0; x < NQ; ++x) {
+    const int fr = r0 + 16 * x + col;
+    const bool in = fr < r1;
+    const int tok = in ? fr / a.G : 0;
+    pos[x] = in ? sq.len - sq.n + tok : -1;
+    const uint16_t* src = a.q + (sq.row0 + tok) * a.q_token + (h * a.G + (in ? fr - tok * a.G : 0)) * a.q_head;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        // the dims of this step's slots, as the key pieces below hold them
-        const int d = ES == 2 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s & 1);
-        q[x][s] = in ? ld16(src + d) : u32x4_t{0, 0, 0, 0};
-      }
-      m[x] = kLowest;
-      l[x] = 0.f;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[x][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < NS; ++s) {
+      // the dims of this step's slots, as the key pieces below hold them
+      const int d = ES == 2 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s & 1);
+      q[x][s] = in ? ld16(src + d) : u32x4_t{0, 0, 0, 0};
     }
+    m[x] = kLowest;
+    l[x] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[x][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
 
-    for (int i = i0 + wave; i < i1; i += 4) {
-      const int key0 = sp.key0(i);
-      // rows of the first product: row 4 u + v of its tile t is key 16 u + 4 t
-      // + v, so lane (col, g) loads keys of group col / 4 and its score
-      // registers, like its k-slots of the second product, are those of group g
-      const int kk = key0 + 16 * (col >> 2), kv = key0 + 16 * g;
-      int pk = kk < sp.hi ? kv_page(a.kv, b, kk) : -1, pv = kv < sp.hi ? kv_page(a.kv, b, kv) : -1;
-      const bool have = pv >= 0;
-      pk = pk < 0 ? 0 : pk;
-      pv = pv < 0 ? 0 : pv;
-      const int64_t hk = static_cast<int64_t>(pk) * a.kv.H + h, hv = static_cast<int64_t>(pv) * a.kv.H + h;
-      const char* ksrc = a.kv.k + (hk * P + (kk & (P - 1)) + (col & 3)) * (DH * ES) + 16 * g;
-      const char* vsrc = a.kv.v + ((hv * DH + col) * P + (kv & (P - 1))) * ES;
-      u32x4_t kf[4][NPC], vf[ND][ES];
+  for (int i = i0 + wave; i < i1; i += 4) {
+    const int key0 = sp.key0(i);
+    // rows of the first product: row 4 u + v of its tile t is key 16 u + 4 t
+    // + v, so lane (col, g) loads keys of group col / 4 and its score
+    // registers, like its k-slots of the second product, are those of group g
+    const int kk = key0 + 16 * (col >> 2), kv = key0 + 16 * g;
+    int pk = kk < sp.hi ? kv_page(a.kv, b, kk) : -1, pv = kv < sp.hi ? kv_page(a.kv, b, kv) : -1;
+    const bool have = pv >= 0;
+    pk = pk < 0 ? 0 : pk;
+    pv = pv < 0 ? 0 : pv;
+    const int64_t hk = static_cast<int64_t>(pk) * a.kv.H + h, hv = static_cast<int64_t>(pv) * a.kv.H + h;
+    const char* ksrc = a.kv.k + (hk * P + (kk & (P - 1)) + (col & 3)) * (DH * ES) + 16 * g;
+    const char* vsrc = a.kv.v + ((hv * DH + col) * P + (kv & (P - 1))) * ES;
+    u32x4_t kf[4][NPC], vf[ND][ES];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < NPC; ++j) kf[t][j] = ld16(ksrc + 4 * t * (DH * ES) + 64 * j);
-      float ksl = 0.f, lvl = 0.f, rvl = 0.f;
-      if constexpr (KIND != SRW_KV_BF16) {
-        ksl = a.kv.ks[hv * P + (kv & (P - 1)) + col] * a.sc;
-        in_exponent(a.kv.vs[hv * P + (kv & (P - 1)) + col], lvl, rvl);
-      }
+      for (int j = 0; j < NPC; ++j) kf[t][j] = ld16(ksrc + 4 * t * (DH * ES) + 64 * j);
+    float ksl = 0.f, lvl = 0.f, rvl = 0.f;
+    if constexpr (KIND != SRW_KV_BF16) {
+      ksl = a.kv.ks[hv * P + (kv & (P - 1)) + col] * a.sc;
+      in_exponent(a.kv.vs[hv * P + (kv & (P - 1)) + col], lvl, rvl);
+    }
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int j = 0; j < ES; ++j) vf[d][j] = ld16(vsrc + static_cast<int64_t>(16 * d) * P * ES + 16 * j);
+      for (int j = 0; j < ES; ++j) vf[d][j] = ld16(vsrc + static_cast<int64_t>(16 * d) * P * ES + 16 * j);
 
-      f32x4_t acc[NQ][4];
+    f32x4_t acc[NQ][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        u32x4_t kb[NS];
+    for (int t = 0; t < 4; ++t) {
+      u32x4_t kb[NS];
 #pragma unroll
-        for (int j = 0; j < NPC; ++j) {
-          if constexpr (KIND == SRW_KV_BF16) {
-            kb[j] = kf[t][j];
-          } else {
-            kb[2 * j] = widen8<KIND>(kf[t][j][0], kf[t][j][1]);
-            kb[2 * j + 1] = widen8<KIND>(kf[t][j][2], kf[t][j][3]);
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-          acc[x][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < NS; ++s) acc[x][t] = mfma16(kb[s], q[x][s], acc[x][t]);
+      for (int j = 0; j < NPC; ++j) {
+        if constexpr (KIND == SRW_KV_BF16) {
+          kb[j] = kf[t][j];
+        } else {
+          kb[2 * j] = widen8<KIND>(kf[t][j][0], kf[t][j][1]);
+          kb[2 * j + 1] = widen8<KIND>(kf[t][j][2], kf[t][j][3]);
         }
       }
-      // every row sees every key of the tile?
-      const bool whole = __all(have) && key0 + kTile - 1 <= p_lo &&
-                         (a.window == 0 || key0 > p_hi - a.window || key0 + kTile <= a.sinks);
-      uint32_t seen = 0;  // bit j: some row of the tile sees the lane's key kv + j
-      u32x4_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
-        uint32_t mine = 0xffffu;
-        if (!whole) {
-          mine = have ? static_cast<uint32_t>(seen_of(pos[x], key0, a.window, a.sinks) >> (16 * g)) & 0xffffu : 0u;
-          seen |= mine;
-        }
-        // exponents of the weights, over m (0 while the row has seen nothing)
-        float t[16];
-        const float mu = m[x] == kLowest ? 0.f : m[x];
-        for16([&](auto jt) {
-          constexpr int j = decltype(jt)::value;
-          const float s = acc[x][j >> 2][j & 3];
-          t[j] = KIND == SRW_KV_BF16 ? fmaf(s, a.sc, -mu) : s * row_lane<j>(ksl) + (row_lane<j>(lvl) - mu);
-        });
-        if (!whole) {
-          for16([&](auto jt) {
-            constexpr int j = decltype(jt)::value;
-            t[j] = only<j>(mine, t[j]);
-          });
-        }
-        float mt = t[0];
+        acc[x][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 1; j < 16; ++j) mt = fmaxf(mt, t[j]);
-        if (__any(mt > (m[x] == kLowest ? -INFINITY : kLazy))) {
-          auto mx = [](float u, float w) { return fmaxf(u, w); };
-          mt = join32(join16(mt, mx), mx);
-          const float mn = raised(m[x], mt), back = (mn == kLowest ? 0.f : mn) - mu;
-          const float w = __builtin_amdgcn_exp2f(m[x] - mn);
-          m[x] = mn;
-          l[x] *= w;
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) o[x][d][v] *= w;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) t[j] -= back;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) t[j] = __builtin_amdgcn_exp2f(t[j]);
-        if constexpr (KIND != SRW_KV_BF16) {
-          if (whole) {
-            for16([&](auto jt) {
-              constexpr int j = decltype(jt)::value;
-              l[x] += t[j] * row_lane<j>(rvl);
-            });
-          } else {  // the scale of a key that is not seen may be anything
-            for16([&](auto jt) {
-              constexpr int j = decltype(jt)::value;
-              l[x] += __uint_as_float(__float_as_uint(t[j] * row_lane<j>(rvl)) & bit_mask<j>(mine));
-            });
-          }
-        }
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float p0 = t[8 * st + 2 * u], p1 = t[8 * st + 2 * u + 1];
-            const uint32_t hi = pack_bf16(p0, p1);
-            pf[x][st][u] = hi;
-            pl[x][st][u] = pack_bf16(p0 - lo_f32(hi), p1 - hi_f32(hi));
-            if constexpr (KIND == SRW_KV_BF16) l[x] += p0 + p1;
-          }
-      }
-      bool odd = false;  // a value is not finite
-      if (!whole && KIND != SRW_KV_INT8) {
-        for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);  // over the columns: keys that some row sees
-        u16x2_t most = {0, 0};
-#pragma unroll
-        for (int u = 0; u < 4 * ES; ++u) {  // a dword's keys
-          uint32_t keep;
-          if constexpr (ES == 2) {
-            const uint32_t two = seen >> (2 * u);
-            keep = (two & 1 ? 0x0000ffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
-          } else {
-            keep = ((seen >> (4 * u) & 15u) * 0x00204081u & 0x01010101u) * 0xffu;
-          }
-#pragma unroll
-          for (int d = 0; d < ND; ++d) vf[d][u / 4][u % 4] &= keep;
-        }
-        if (KIND == SRW_KV_BF16 && p_lo != p_hi) {
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int j = 0; j < ES; ++j) most = most16(most, vf[d][j]);
-          odd = __any(not_finite(most));
-          if (odd) {
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-              for (int j = 0; j < ES; ++j) vf[d][j] = finite16(vf[d][j]);
-          }
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          u32x4_t vb;
-          if constexpr (KIND == SRW_KV_BF16)
-            vb = vf[d][st];
-          else
-            vb = widen8<KIND>(vf[d][0][2 * st], vf[d][0][2 * st + 1]);
-#pragma unroll
-          for (int x = 0; x < NQ; ++x) o[x][d] = mfma16(vb, pl[x][st], mfma16(vb, pf[x][st], o[x][d]));
-        }
-      }
-      if (KIND == SRW_KV_BF16 && odd) {
-#pragma unroll
-        for (int x = 0; x < NQ; ++x)
-          add_not_finite<4 * ND>(
-              a.kv, b, h, DH, key0,
-              [&](int k) { return seen_of(pos[x], key0, a.window, a.sinks) >> k & 1; },
-              [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, [&](int i, float v) { o[x][i / 4][i % 4] += v; });
+        for (int s = 0; s < NS; ++s) acc[x][t] = mfma16(kb[s], q[x][s], acc[x][t]);
       }
     }
-
-    // join the four waves
-    auto sum = [](float u, float w) { return u + w; };
+    // every row sees every key of the tile?
+    const bool whole = __all(have) && key0 + kTile - 1 <= p_lo &&
+                       (a.window == 0 || key0 > p_hi - a.window || key0 + kTile <= a.sinks);
+    uint32_t seen = 0;  // bit j: some row of the tile sees the lane's key kv + j
+    u32x4_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-      l[x] = join32(join16(l[x], sum), sum);
-      if (g == 0) {
-        sm[wave][16 * x + col] = m[x];
-        sl[wave][16 * x + col] = l[x];
+      uint32_t mine = 0xffffu;
+      if (!whole) {
+        mine = have ? static_cast<uint32_t>(seen_of(pos[x], key0, a.window, a.sinks) >> (16 * g)) & 0xffffu : 0u;
+        seen |= mine;
       }
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-        *reinterpret_cast<f32x4_t*>(&so[wave][16 * x + col][16 * d + 4 * g]) = o[x][d];
+      weigh<KIND, ND, true>(acc[x], a.sc, ksl, lvl, rvl, whole, mine, m[x], l[x], o[x], pf[x], pl[x]);
     }
-    __syncthreads();
-    // thread (r, c): DH / 16 consecutive dims of a row, 16 rows a pass
+    bool odd = false;  // a value is not finite
+    if (!whole && KIND != SRW_KV_INT8) {
+      for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);  // over the columns: keys that some row sees
+      u16x2_t most = {0, 0};
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      const int r = 16 * x + (threadIdx.x >> 4), c = (threadIdx.x & 15) * ND;
-      const int fr = r0 + r;
-      if (fr < r1) {
-        float mm = sm[0][r];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm[w][r]);
-        float ll = 0.f, ov[ND];
-#pragma unroll
-        for (int d = 0; d < ND; ++d) ov[d] = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          // (a wave without visible keys has l = 0)
-          const float e = sm[w][r] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[w][r] - mm);
-          ll += sl[w][r] * e;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) ov[d] += so[w][r][c + d] * e;
-        }
-        const int tok = fr / a.G;
-        const int64_t row = (sq.row0 + tok) * a.Hq + h * a.G + (fr - tok * a.G);
-        if (a.S == 1) {
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          uint32_t w[ND / 2];
-#pragma unroll
-          for (int d = 0; d < ND / 2; ++d) w[d] = pack_bf16(ov[2 * d] * inv, ov[2 * d + 1] * inv);
-          if constexpr (ND == 8)
-            *reinterpret_cast<uint4*>(a.out + row * DH + c) = make_uint4(w[0], w[1], w[2], w[3]);
-          else
-            *reinterpret_cast<uint2*>(a.out + row * DH + c) = make_uint2(w[0], w[1]);
+      for (int u = 0; u < 4 * ES; ++u) {  // a dword's keys
+        uint32_t keep;
+        if constexpr (ES == 2) {
+          const uint32_t two = seen >> (2 * u);
+          keep = (two & 1 ? 0x0000ffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
         } else {
-          const int64_t at = split * (a.kv.T * a.Hq) + row;
-          if (ll != 0.f) {
+          keep = ((seen >> (4 * u) & 15u) * 0x00204081u & 0x01010101u) * 0xffu;
+        }
 #pragma unroll
-            for (int d = 0; d < ND; d += 4)
-              *reinterpret_cast<f32x4_t*>(a.part + at * DH + c + d) = f32x4_t{ov[d], ov[d + 1], ov[d + 2], ov[d + 3]};
-          }
-          if (c == 0) a.ml[at] = make_float2(mm, ll);
+        for (int d = 0; d < ND; ++d) vf[d][u / 4][u % 4] &= keep;
+      }
+      if (KIND == SRW_KV_BF16 && p_lo != p_hi) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int j = 0; j < ES; ++j) most = most16(most, vf[d][j]);
+        odd = __any(not_finite(most));
+        if (odd) {
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int j = 0; j < ES; ++j) vf[d][j] = finite16(vf[d][j]);
         }
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        u32x4_t vb;
+        if constexpr (KIND == SRW_KV_BF16)
+          vb = vf[d][st];
+        else
+          vb = widen8<KIND>(vf[d][0][2 * st], vf[d][0][2 * st + 1]);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) o[x][d] = mfma16(vb, pl[x][st], mfma16(vb, pf[x][st], o[x][d]));
+      }
+    }
+    if (KIND == SRW_KV_BF16 && odd) {
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+        add_not_finite<4 * ND>(
+            a.kv, b, h, DH, key0,
+            [&](int k) { return seen_of(pos[x], key0, a.window, a.sinks) >> k & 1; },
+            [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, [&](int i, float v) { o[x][i / 4][i % 4] += v; });
+    }
+  }
+
+  // join the four waves
+  auto sum = [](float u, float w) { return u + w; };
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    l[x] = join32(join16(l[x], sum), sum);
+    if (g == 0) {
+      sm[wave][16 * x + col] = m[x];
+      sl[wave][16 * x + col] = l[x];
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *reinterpret_cast<f32x4_t*>(&so[wave][16 * x + col][16 * d + 4 * g]) = o[x][d];
+  }
+  __syncthreads();
+  // thread (r, c): DH / 16 consecutive dims of a row, 16 rows a pass
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int r = 16 * x + (threadIdx.x >> 4), c = (threadIdx.x & 15) * ND;
+    const int fr = r0 + r;
+    if (fr < r1) {
+      float mm = sm[0][r];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm[w][r]);
+      float ll = 0.f, ov[ND];
+#pragma unroll
+      for (int d = 0; d < ND; ++d) ov[d] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        // (a wave without visible keys has l = 0)
+        const float e = sm[w][r] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[w][r] - mm);
+        ll += sl[w][r] * e;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) ov[d] += so[w][r][c + d] * e;
+      }
+      const int tok = fr / a.G;
+      const int64_t row = (sq.row0 + tok) * a.Hq + h * a.G + (fr - tok * a.G);
+      if (a.S == 1) {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        uint32_t w[ND / 2];
+#pragma unroll
+        for (int d = 0; d < ND / 2; ++d) w[d] = pack_bf16(ov[2 * d] * inv, ov[2 * d + 1] * inv);
+        if constexpr (ND == 8)
+          *reinterpret_cast<uint4*>(a.out + row * DH + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        else
+          *reinterpret_cast<uint2*>(a.out + row * DH + c) = make_uint2(w[0], w[1]);
+      } else {
+        const int64_t at = split * (a.kv.T * a.Hq) + row;
+        if (ll != 0.f) {
+#pragma unroll
+          for (int d = 0; d < ND; d += 4)
+            *reinterpret_cast<f32x4_t*>(a.part + at * DH + c + d) = f32x4_t{ov[d], ov[d + 1], ov[d + 2], ov[d + 3]};
+        }
+        if (c == 0) a.ml[at] = make_float2(mm, ll);
+      }
+    }
   }
 }
 
-// Joins the splits: a workgroup a row, in groups of DH / 4 lanes that take the
-// splits in turn, each with all its loads in flight, and join in LDS.
-template <int DH>
+// Joins the splits.  Groups of DH / 4 lanes; W of them take a row's splits in
+// turn, each with four loads in flight, and join in LDS: W = 1 for few splits of
+// many rows (no LDS, 256 / (DH / 4) rows a workgroup), all groups of a workgroup
+// for the many splits of a few rows.
+template <int DH, bool ONE>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float* part, const float2* ml, uint16_t* out,
                                                         int64_t rows, int S) {
-  constexpr int L = DH / 4, N = 256 / L;  // lanes a group, groups
-  __shared__ float sm[N], sl[N];
-  __shared__ f32x4_t so[N][L];
+  constexpr int L = DH / 4, N = 256 / L, W = ONE ? 1 : N;  // lanes a group, groups, groups a row
   const int grp = threadIdx.x / L, c = threadIdx.x % L;
-  const int64_t row = blockIdx.x;
+  const int64_t row = ONE ? static_cast<int64_t>(blockIdx.x) * N + grp : blockIdx.x;
+  if (row >= rows) return;
   float m = kLowest, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   constexpr int U = 4;
-  for (int s0 = grp; s0 < S; s0 += N * U) {
+  for (int s0 = ONE ? 0 : grp; s0 < S; s0 += W * U) {
     float2 x[U];
     f32x4_t v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int s = s0 + N * u < S ? s0 + N * u : s0;
+      const int s = s0 + W * u < S ? s0 + W * u : s0;
       x[u] = ml[s * rows + row];
-      v[u] = *reinterpret_cast<const f32x4_t*>(part + (s * rows + row) * DH + 4 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // a split without visible keys wrote no output
+      const int s = s0 + W * u < S ? s0 + W * u : s0;
+      if (x[u].y != 0.f) v[u] = *reinterpret_cast<const f32x4_t*>(part + (s * rows + row) * DH + 4 * c);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      // a split without visible keys wrote no output
-      if (s0 + N * u >= S || x[u].y == 0.f) continue;
+      if (s0 + W * u >= S || x[u].y == 0.f) continue;
       const float mn = fmaxf(m, x[u].x);
       const float e0 = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       const float e1 = x[u].x == mn ? 1.f : __builtin_amdgcn_exp2f(x[u].x - mn);
@@ -538,377 +583,395 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* part, const
       for (int k = 0; k < 4; ++k) o[k] = o[k] * e0 + v[u][k] * e1;
     }
   }
-  if (c == 0) {
-    sm[grp] = m;
-    sl[grp] = l;
+  if constexpr (!ONE) {
+    __shared__ float sm[N], sl[N];
+    __shared__ f32x4_t so[N][L];
+    if (c == 0) {
+      sm[grp] = m;
+      sl[grp] = l;
+    }
+    so[grp][c] = o;
+    __syncthreads();
+    if (grp != 0) return;
+    m = sm[0];
+    l = 0.f;
+#pragma unroll
+    for (int g = 1; g < N; ++g) m = fmaxf(m, sm[g]);
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      const float e = sm[g] == m ? 1.f : __builtin_amdgcn_exp2f(sm[g] - m);
+      l += sl[g] * e;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += so[g][c][k] * e;
+    }
   }
-  so[grp][c] = o;
-  __syncthreads();
-  if (grp != 0) return;
-  float mm = sm[0], ll = 0.f;
-#pragma unroll
-  for (int g = 1; g < N; ++g) mm = fmaxf(mm, sm[g]);
-  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int g = 0; g < N; ++g) {
-    const float e = sm[g] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[g] - mm);
-    ll += sl[g] * e;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] += so[g][c][k] * e;
-  }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(out + row * DH + 4 * c) =
       make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
 // -- many rows: chunks of prompts ---------------------------------------------
 //
-// 128 rows a workgroup, 32 a wave; a tile's keys and values go through LDS
-// once for the four waves, two stages deep.  bf16 pages are copied there
-// directly (global_load_lds), 8-bit ones are widened on the way.  16-byte
-// pieces of a row are XOR-swizzled by the row so that 16 lanes' fragment
-// reads cover all banks.
-template <int DH> __device__ inline int k_swz(int row) { return DH == 64 ? (row >> 1) & 7 : row & 15; }
-__device__ inline int v_swz(int row) { return (row >> 1) & 7; }
+// 128 rows a workgroup, 16 to each of eight waves; a tile's keys and values go
+// through LDS once for all of them, two stages deep.  bf16 pages are copied
+// there directly (global_load_lds), 8-bit ones are widened on the way.  16-byte
+// pieces of a row are XOR-swizzled by the row so that the 16 lanes of a
+// fragment read cover all banks.
+//
+// Bound by the vector ALU: a score takes 4 (bf16) or 5 (8 bits) instructions
+// and an exponential, which costs 2.5 of them, against 4 head_dim products.  A
+// wave alone issues a vector instruction every 8 cycles, half the SIMD's rate,
+// and matrix instructions run beside other waves' vector ones; so what counts
+// is waves on a SIMD, and with 16 rows a wave (at most 128 registers) four
+// fit, where 32 rows (240 registers at head_dim 128) left two.
+template <int DH> __device__ inline int k_swz(int row) {
+  // a fragment's 16 rows are 16 u + 4 t + v, u, v = 0 .. 3
+  return DH == 64 ? (row >> 1 & 1) | (row >> 3 & 6) : (row & 3) | (row >> 2 & 12);
+}
+// (the lanes of one LDS access may be of two neighbouring g, columns 0-3 and
+// 12-15 of one and 4-11 of the other, whose pieces differ in bits 1 and 2: bit 0
+// tells those columns apart)
+__device__ inline int v_swz(int row) { return ((row >> 2 ^ row >> 3) & 1) | (row & 2) | (row >> 1 & 4); }
 
 template <int KIND, int DH>
-__global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
   constexpr int ES = kv_bytes<KIND>();
-  constexpr int NS = DH / 16, ND = DH / 32;
-  constexpr int NP = DH / 8;                     // pieces of a key row
-  constexpr int kStage = kTile * DH * 2;         // bytes of a tile's keys (or values) in LDS
-  constexpr int NI = kStage / 4096;              // 16-byte pieces a thread of either
+  constexpr int NS = DH / 32, ND = DH / 16;
+  constexpr int NP = DH / 8;               // pieces of a key row
+  constexpr int kStage = kTile * DH * 2;   // bytes of a tile's keys (or values) in LDS
+  constexpr int NI = kStage / 8192;        // 16-byte pieces a thread of either
   constexpr bool Q8 = KIND != SRW_KV_BF16;
+  constexpr int kBatch = DH == 64 ? 8 : 4;  // fragments read together
   __shared__ __align__(16) char kl[2][kStage];
   __shared__ __align__(16) char vl[2][kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, hf = lane >> 5;
+  const int col = lane & 15, g = lane >> 4;
   const int h = blockIdx.y, split = blockIdx.z;
   const int P = a.kv.P;
-
-  // sequence and row tile; the last tiles, which see most, come first
-  int64_t b = 0;
-  int rt = blockIdx.x;
-  if (a.kv.cu) {
-    auto start = [&](int64_t i) { return (static_cast<int64_t>(a.kv.cu[i]) * a.G >> 7) + i; };
-    b = kv_find(a.kv.B, blockIdx.x, start);
-    rt = static_cast<int>(blockIdx.x - start(b));
-  } else {
-    const int per = (a.G + 127) / 128;
-    b = blockIdx.x / per;
-    rt = blockIdx.x % per;
-  }
-  b = __builtin_amdgcn_readfirstlane(static_cast<int>(b));
-  const KvSeq sq = kv_seq(a.kv, b);
-  const int rows = sq.n * a.G;
-  const int rts = (rows + 127) / 128;
-  if (rt < 0 || rt >= rts) return;
-  rt = rts - 1 - rt;
-  const int r0 = rt * 128, r1 = r0 + 128 < rows ? r0 + 128 : rows;
+  const Tile tl = tile_of<128>(a, blockIdx.x);
+  if (tl.r0 < 0) return;
+  const int64_t b = tl.b;
+  const KvSeq sq = tl.sq;
+  const int r0 = tl.r0, r1 = tl.r1;
   const Span sp = span_of(a, sq.len - sq.n + r0 / a.G, sq.len - sq.n + (r1 - 1) / a.G);
   const int i0 = split * a.per;
   const int i1 = i0 + a.per < sp.tiles ? i0 + a.per : sp.tiles;
 
   // this wave's rows
-  const int w0 = r0 + 32 * wave, w1 = w0 + 32 < r1 ? w0 + 32 : r1;
+  const int w0 = r0 + 16 * wave, w1 = w0 + 16 < r1 ? w0 + 16 : r1;
   const bool active = w0 < r1;
   const int p_lo = sq.len - sq.n + w0 / a.G, p_hi = sq.len - sq.n + (w1 - 1) / a.G;
-  const int fr = w0 + col;
-  const bool in = fr < r1;
-  const int tok = in ? fr / a.G : 0;
-  const int head = h * a.G + (in ? fr - tok * a.G : 0);
-  const int pos = in ? sq.len - sq.n + tok : -1;
+  // (the loop has no registers to keep a row's place: it is worked out again
+  // where it is needed)
+  struct Place {
+    bool in;
+    int tok, head, pos;
+  };
+  auto place = [&] {
+    int c = threadIdx.x & 15;
+    asm volatile("" : "+v"(c));
+    Place p;
+    p.in = w0 + c < r1;
+    p.tok = p.in ? (w0 + c) / a.G : 0;
+    p.head = h * a.G + (p.in ? w0 + c - p.tok * a.G : 0);
+    p.pos = p.in ? sq.len - sq.n + p.tok : -1;
+    return p;
+  };
   u32x4_t q[NS];
   {
-    const uint16_t* src = a.q + (sq.row0 + tok) * a.q_token + head * a.q_head + 8 * hf;
+    const Place p = place();
+    const bool in = p.in;
+    const int tok = p.tok, head = p.head;
+    const uint16_t* src = a.q + (sq.row0 + tok) * a.q_token + head * a.q_head + 8 * g;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) q[s] = in ? ld16(src + 16 * s) : u32x4_t{0, 0, 0, 0};
+    for (int s = 0; s < NS; ++s) q[s] = in ? ld16(src + 32 * s) : u32x4_t{0, 0, 0, 0};
   }
   float m = kLowest, l = 0.f;
-  f32x16_t o[ND];
+  f32x4_t o[ND];
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+  for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  // A tile's position in its pages: slot of its first key (pages of 64 and more
-  // hold whole tiles; smaller ones start with one), then the slot of key k.
+  // Slots: pages of 64 and more hold whole tiles (one page each), at slot0 of
+  // theirs; smaller ones start with one.  Where tiles lie is worked out 16 at a
+  // time, a lane for each group of 16 positions: lane 4 n + u has the byte offset
+  // of the page of tile ib + n's positions 16 u .. (of page 0 where they have
+  // none), and bit 4 n + u of `have` says whether there is one.  (Done a tile at
+  // a time by every wave, on the scalar unit that the whole CU shares, it cost
+  // as much as the products.)
+  const bool one = P >= kTile;
   const int64_t page_bytes = static_cast<int64_t>(a.kv.H) * P * DH * ES, head_at = static_cast<int64_t>(h) * P * DH * ES;
   const char* kbase = a.kv.k + head_at;
   const char* vbase = a.kv.v + head_at;
-  // pages of tile i: lane c holds that of positions key0 + 16 (c & 3)
-  auto pages_of = [&](int i) {
-    const int at = sp.key0(i) + 16 * (lane & 3);
-    return at < sp.hi ? kv_page(a.kv, b, at) : -1;
+  int ib = i0, off_lo = 0, off_hi = 0;
+  uint64_t have = 0;
+  auto locate = [&] {
+    const int i = ib + (lane >> 2), at = sp.key0(i) + 16 * (lane & 3);
+    const int id = i < i1 && at < sp.hi ? kv_page(a.kv, b, at) : -1;
+    have = __ballot(id >= 0);
+    const int64_t off = (id < 0 ? 0 : id) * page_bytes;
+    off_lo = static_cast<int>(off);
+    off_hi = static_cast<int>(off >> 32);
   };
-  u32x4_t rk[Q8 ? NI / 2 : 1], rv[Q8 ? NI / 2 : 1];  // 8-bit tiles on their way
-  auto fetch = [&](int i, int ids, int stage) {
-    const int slot0 = sp.key0(i) & (P - 1);
-    const int safe = ids < 0 ? 0 : ids;
-    if constexpr (!Q8) {
-      // pieces n of a lane: keys of one group of 16 for the whole wave
+  if (i0 < i1) locate();
+  // At head_dim 128 the loop has no registers for addresses that it could keep:
+  // they are worked out from the lane again.
+  auto fresh = [](int x) {
+    if constexpr (DH == 128) asm volatile("" : "+v"(x));
+    return x;
+  };
+  u32x4_t rk, rv;               // 8-bit tiles on their way
+  float ksn = 0.f, vsn = 0.f;   // scales of key `lane`
+  int havn = 0;                 // bit u: positions 16 u .. have a page
+  // Where a thread's pieces lie in a page, from its first slot of the tile.
+  // 8 bits: 16 codes, of keys 16 dims of a position (the wave's positions in one
+  // group of 16), of values 16 positions of a dim; at head_dim 64 the first four
+  // waves take the keys, the others the values.  (bf16: a wave's second key
+  // pieces are four positions, and four rows of the same swizzle, behind its
+  // first.)
+  auto key_at = [&]() -> uint32_t {
+    const int tx = fresh(threadIdx.x);
+    if constexpr (Q8) return (tx / (NP / 2) & (P - 1)) * DH + 16 * (tx % (NP / 2));
+    const int row = (wave * NI * 64 + (tx & 63)) / NP;
+    return ((row & (P - 1)) * DH + 8 * ((tx & 63) % NP ^ k_swz<DH>(row))) * ES;
+  };
+  auto value_at = [&](int n) -> uint32_t {
+    const int tx = fresh(threadIdx.x);
+    if constexpr (Q8) return ((tx >> 2) - (DH == 64 && wave >= 4 ? 64 : 0)) * P + ((16 * (tx & 3)) & (P - 1));
+    const int row = ((wave * NI + n) * 64 + (tx & 63)) / 8;
+    return (row * P + ((8 * ((tx & 7) ^ v_swz(row))) & (P - 1))) * ES;
+  };
+  uint32_t kat0 = 0, vat0[NI];
+  if constexpr (DH == 64) {
+    kat0 = key_at();
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const int first = (wave * NI + n) * 64;      // piece of lane 0
-        const int row = (first + lane) / NP, pc = ((first + lane) % NP) ^ k_swz<DH>(row);
-        const int64_t pg = __builtin_amdgcn_readlane(safe, (first / NP) >> 4);
-        g2lds16(kbase + pg * page_bytes + slot0 * (DH * ES) + ((row & (P - 1)) * DH + 8 * pc) * ES, kl[stage] + 16 * first);
-      }
-      // values: positions 8 pc .. of a dim, pc = (lane & 7) ^ (lane >> 4) ^ 4 (n & 1)
-      const int pe = (lane & 7) ^ (lane >> 4);
-      const int64_t pg[2] = {__shfl(safe, pe >> 1), __shfl(safe, (pe ^ 4) >> 1)};
+    for (int n = 0; n < NI; ++n) vat0[n] = value_at(n);
+  }
+  auto fetch = [&](int i, int stage) {
+    uint32_t kat = kat0, vat[NI];
+    if constexpr (DH == 128) kat = key_at();
+#pragma unroll
+    for (int n = 0; n < NI; ++n) vat[n] = DH == 64 ? vat0[n] : value_at(n);
+    const int at = 4 * (i - ib), slot0 = sp.key0(i) & (P - 1);
+    havn = static_cast<int>(have >> at) & 15;
+    auto page = [&](int u) -> int64_t {  // of group u, the same for the whole wave
+      const uint32_t lo = __builtin_amdgcn_readlane(off_lo, at + u), hi = __builtin_amdgcn_readlane(off_hi, at + u);
+      return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    };
+    auto page_of_lane = [&](int u) -> int64_t {
+      const uint32_t lo = __shfl(off_lo, at + u), hi = __shfl(off_hi, at + u);
+      return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    };
+    const int64_t page0 = one ? page(0) : 0;
+    if constexpr (!Q8) {
+      const int ku = wave * NI * 64 / NP >> 4;  // (a wave's keys are of one group)
+      const char* src = kbase + (one ? page0 : page(ku)) + slot0 * (DH * ES);
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+        g2lds16(src + n * (64 / NP * DH * ES) + kat, kl[stage] + 16 * (wave * NI + n) * 64);
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         const int first = (wave * NI + n) * 64;
-        const int row = (first + lane) / 8, pc = pe ^ (4 * (n & 1));
-        g2lds16(vbase + pg[n & 1] * page_bytes + (row * P + slot0 + ((8 * pc) & (P - 1))) * ES, vl[stage] + 16 * first);
-      }
-    } else {
-      // a thread's 16 codes: of keys, 16 dims of a position (the wave's
-      // positions in one group of 16); of values, 16 positions of a dim
-#pragma unroll
-      for (int n = 0; n < NI / 2; ++n) {
-        const int at = n * 256 + threadIdx.x;
-        const int row = at / (NP / 2), pc = at % (NP / 2);
-        const int64_t pg = __builtin_amdgcn_readlane(safe, (n * 256 + wave * 64) / (NP / 2) >> 4);
-        rk[n] = ld16(kbase + pg * page_bytes + slot0 * DH + ((row & (P - 1)) * DH + 16 * pc));
-      }
-      const char* vsrc = vbase + safe * page_bytes + slot0 + ((16 * (lane & 3)) & (P - 1));
-#pragma unroll
-      for (int n = 0; n < NI / 2; ++n) rv[n] = ld16(vsrc + (n * 64 + (threadIdx.x >> 2)) * P);
-    }
-  };
-  auto settle = [&](int stage) {  // 8 bits: widen into LDS
-    if constexpr (Q8) {
-#pragma unroll
-      for (int n = 0; n < NI / 2; ++n) {
-        const int at = n * 256 + threadIdx.x;
-        const int row = at / (NP / 2), pc = at % (NP / 2);
-        const int vrow = at / 4, vpc = at % 4;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          *reinterpret_cast<u32x4_t*>(kl[stage] + row * (DH * 2) + 16 * ((2 * pc + u) ^ k_swz<DH>(row))) =
-              widen8<KIND>(rk[n][2 * u], rk[n][2 * u + 1]);
-          *reinterpret_cast<u32x4_t*>(vl[stage] + vrow * 128 + 16 * ((2 * vpc + u) ^ v_swz(vrow))) =
-              widen8<KIND>(rv[n][2 * u], rv[n][2 * u + 1]);
+        if (one) {
+          g2lds16(vbase + page0 + slot0 * ES + vat[n], vl[stage] + 16 * first);
+        } else {
+          const int group = ((lane & 7) ^ v_swz((first + lane) / 8)) >> 1;
+          g2lds16(vbase + page_of_lane(group) + vat[n], vl[stage] + 16 * first);
         }
       }
+    } else {
+      if (DH == 128 || wave < 4) {
+        const char* src = kbase + (one ? page0 : page(wave * 64 / (NP / 2) >> 4)) + slot0 * DH;
+        rk = ld16(src + kat);
+      }
+      if (DH == 128 || wave >= 4) {
+        if (one)
+          rv = ld16(vbase + page0 + slot0 + vat[0]);
+        else
+          rv = ld16(vbase + page_of_lane(lane & 3) + vat[0]);
+      }
+      if (one) {
+        const int64_t first = (page0 >> (DH == 64 ? 6 : 7)) + (h * P + slot0);
+        int at4 = 4 * (threadIdx.x & 63);
+        asm volatile("" : "+v"(at4));
+        ksn = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(a.kv.ks + first) + static_cast<uint32_t>(at4));
+        vsn = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(a.kv.vs + first) + static_cast<uint32_t>(at4));
+      } else {
+        const int64_t first = (page_of_lane(g) >> (DH == 64 ? 6 : 7)) + (h * P + (lane & (P - 1)));
+        ksn = a.kv.ks[first];
+        vsn = a.kv.vs[first];
+      }
     }
   };
-  // scales of the lane's keys: of its 32 score registers (kb, v), register
-  // kb of lane v of a row of 16 holds that of key 32 kb + 16 (v / 8) + 8 hf + v % 8
-  float ksl[2], lvl[2], rvl[2], ksn[2], vsn[2];
-  auto scales = [&](int i, int ids) {
-    if constexpr (Q8) {
-      const int slot0 = sp.key0(i) & (P - 1);
-      const int safe = ids < 0 ? 0 : ids;
+  // positions of the tile at key0 that some row of the workgroup sees; hav: its
+  // groups that have pages
+  auto seen_by_any = [&](int key0, int hav) {
+    uint64_t keys = low_bits(sp.hi - key0);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const int k = 32 * kb + 16 * (lane >> 3 & 1) + 8 * hf + (lane & 7);
-        const int64_t pg = lane & 8 ? __builtin_amdgcn_readlane(safe, 2 * kb + 1) : __builtin_amdgcn_readlane(safe, 2 * kb);
-        const int64_t at = (pg * a.kv.H + h) * P + slot0 + (k & (P - 1));
-        ksn[kb] = a.kv.ks[at];
-        vsn[kb] = a.kv.vs[at];
+    for (int u = 0; u < 4; ++u)
+      if (!(hav >> u & 1)) keys &= ~(0xffffull << (16 * u));
+    if (key0 < sp.lo) keys &= ~low_bits(sp.lo - key0) | low_bits(a.sinks - key0);
+    return keys;
+  };
+  auto settle = [&](int key0, int stage) {  // 8 bits: widen into LDS
+    if constexpr (Q8) {
+      const int tx = fresh(threadIdx.x);
+      if (DH == 128 || wave < 4) {
+        const int row = tx / (NP / 2), pc = tx % (NP / 2);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          *reinterpret_cast<u32x4_t*>(kl[stage] + row * (DH * 2) + 16 * ((2 * pc + u) ^ k_swz<DH>(row))) =
+              widen8<KIND>(rk[2 * u], rk[2 * u + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (DH == 128 || wave >= 4) {
+        const int row = (tx >> 2) - (DH == 64 ? 64 : 0), pc = tx & 3;
+        const bool late = row & 2;  // (its pieces meet those of row - 2 in other banks)
+        if (KIND == SRW_KV_FP8 && (havn != 15 || sp.hi - key0 < kTile || key0 < sp.lo)) {
+          // codes of positions that no row sees may be NaN's
+          const uint32_t bits = static_cast<uint32_t>(seen_by_any(key0, havn) >> (16 * pc));
+#pragma unroll
+          for (int u = 0; u < 4; ++u) rv[u] &= ((bits >> (4 * u) & 15u) * 0x00204081u & 0x01010101u) * 0xffu;
+        }
+        const u32x4_t x = late ? u32x4_t{rv[2], rv[3], rv[0], rv[1]} : rv;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          *reinterpret_cast<u32x4_t*>(vl[stage] + row * 128 + 16 * ((2 * pc + (u ^ (late ? 1 : 0))) ^ v_swz(row))) =
+              widen8<KIND>(x[2 * u], x[2 * u + 1]);
       }
     }
   };
 
-  int ids = i0 < i1 ? pages_of(i0) : -1, idn = -1;
-  if (i0 < i1) {
-    fetch(i0, ids, 0);
-    scales(i0, ids);
-    if (i0 + 1 < i1) idn = pages_of(i0 + 1);
-  }
+  if (i0 < i1) fetch(i0, 0);
   for (int i = i0; i < i1; ++i) {
     const int stage = (i - i0) & 1;
-    settle(stage);
+    const int key0 = sp.key0(i);
+    settle(key0, stage);
     wait_vm0();
     __syncthreads();
-    const int cur = ids;
+    const int hav = havn;
+    float ksl = 0.f, lvl = 0.f, rvl = 0.f;
     if constexpr (Q8) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        ksl[kb] = ksn[kb] * a.sc;
-        in_exponent(vsn[kb], lvl[kb], rvl[kb]);
-      }
+      ksl = ksn * a.sc;
+      in_exponent(vsn, lvl, rvl);
     }
     if (i + 1 < i1) {
-      fetch(i + 1, idn, stage ^ 1);
-      scales(i + 1, idn);
-      ids = idn;
-      if (i + 2 < i1) idn = pages_of(i + 2);
+      if (i + 1 - ib == 16) {
+        ib += 16;
+        locate();
+      }
+      fetch(i + 1, stage ^ 1);
     }
-    const int key0 = sp.key0(i);
     if (!active || key0 > p_hi) continue;
 
-    f32x16_t acc[2];
+    // fragments are read several at a time, so that products wait for LDS a few
+    // times and not for each of them
+    const int fl = lane, fc = fl & 15, fg = fl >> 4;
+    f32x4_t acc[4];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int t0 = 0; t0 < 4; t0 += kBatch / NS) {
+      u32x4_t kf[kBatch / NS][NS];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) acc[kb][v] = 0.f;
-      // row m = 16 j + 8 u + 4 w + x of the product holds key 16 j + 8 w + 4 u + x
-      const int row = 32 * kb + (col & 19) + ((col & 4) << 1) + ((col & 8) >> 1);
-      const char* src = kl[stage] + row * (DH * 2);
+      for (int t = 0; t < kBatch / NS; ++t) {
+        // row 4 u + v of product t0 + t holds key 16 u + 4 (t0 + t) + v
+        const int row = 16 * (fc >> 2) + 4 * (t0 + t) + (fc & 3);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) acc[kb] = mfma(ld16(src + 16 * ((2 * s + hf) ^ k_swz<DH>(row))), q[s], acc[kb]);
-    }
-    // positions of the tile that some row of the workgroup sees
-    uint64_t keys = low_bits(sp.hi - key0);
-    {
-      const uint64_t have = __ballot(cur >= 0) & 15;
-      if (have != 15) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (!(have >> u & 1)) keys &= ~(0xffffull << (16 * u));
+        for (int s = 0; s < NS; ++s) kf[t][s] = ld16(kl[stage] + row * (DH * 2) + 16 * ((4 * s + fg) ^ k_swz<DH>(row)));
       }
-      if (key0 < sp.lo) keys &= ~low_bits(sp.lo - key0) | low_bits(a.sinks - key0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < kBatch / NS; ++t) {
+        acc[t0 + t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) acc[t0 + t] = mfma16(kf[t][s], q[s], acc[t0 + t]);
+      }
     }
-    const bool whole = keys == ~0ull && key0 + kTile - 1 <= p_lo &&
+    const bool whole = hav == 15 && sp.hi - key0 >= kTile && key0 + kTile - 1 <= p_lo &&
                        (a.window == 0 || key0 > p_hi - a.window || key0 + kTile <= a.sinks);
-    // bits 32 kb + 16 (v / 8) + v % 8: the lane's row sees the key of its register (kb, v)
-    uint32_t mine[2] = {~0u, ~0u};
+    uint64_t keys = ~0ull;
+    uint32_t mine = 0xffffu;
     if (!whole) {
-      const uint64_t see = (seen_of(pos, key0, a.window, a.sinks) & keys) >> (8 * hf);
-      mine[0] = static_cast<uint32_t>(see);
-      mine[1] = static_cast<uint32_t>(see >> 32);
+      keys = seen_by_any(key0, hav);
+      mine = static_cast<uint32_t>((seen_of(place().pos, key0, a.window, a.sinks) & keys) >> (16 * g)) & 0xffffu;
     }
-    // exponents of the weights, over m (0 while the row has seen nothing)
-    float t[2][16];
-    const float mu = m == kLowest ? 0.f : m;
-    if constexpr (Q8) {
-      settled(acc[0], acc[1]);
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        float s[16];
-        for16([&](auto vt) {
-          constexpr int v = decltype(vt)::value;
-          s[v] = acc[kb][v];
-          t[kb][v] = row_lane<v>(lvl[kb]) - mu;
-        });
-        fma_lanes8<0>(t[kb], ksl[kb], s);
-        fma_lanes8<8>(t[kb] + 8, ksl[kb], s + 8);
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < 32; ++v) t[v >> 4][v & 15] = fmaf(acc[v >> 4][v & 15], a.sc, -mu);
-    }
-    if (!whole) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        for16([&](auto vt) {
-          constexpr int v = decltype(vt)::value;
-          t[kb][v] = only<16 * (v / 8) + v % 8>(mine[kb], t[kb][v]);
-        });
-    }
-    float mt = t[0][0];
-#pragma unroll
-    for (int v = 1; v < 32; ++v) mt = fmaxf(mt, t[v >> 4][v & 15]);
-    if (__any(mt > (m == kLowest ? -INFINITY : kLazy))) {
-      mt = join32(mt, [](float u, float w) { return fmaxf(u, w); });
-      const float mn = raised(m, mt), back = (mn == kLowest ? 0.f : mn) - mu;
-      const float w = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= w;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[d][v] *= w;
-#pragma unroll
-      for (int v = 0; v < 32; ++v) t[v >> 4][v & 15] -= back;
-    }
-    u32x4_t pf[4];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      for16([&](auto vt) {
-        constexpr int v = decltype(vt)::value;
-        t[kb][v] = __builtin_amdgcn_exp2f(t[kb][v]);
-      });
-      if constexpr (Q8) {
-        if (whole) {
-          sum_lanes16(l, rvl[kb], t[kb]);
-        } else {  // the scale of a key that is not seen may be anything
-          for16([&](auto vt) {
-            constexpr int v = decltype(vt)::value;
-            l += __uint_as_float(__float_as_uint(row_lane<v>(rvl[kb]) * t[kb][v]) &
-                                 bit_mask<16 * (v / 8) + v % 8>(mine[kb]));
-          });
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float p0 = t[kb][8 * j + 2 * u], p1 = t[kb][8 * j + 2 * u + 1];
-          pf[2 * kb + j][u] = pack_bf16(p0, p1);
-          if constexpr (!Q8) l = add_bf16x2(pf[2 * kb + j][u], l);
-        }
-    }
+    u32x4_t pf[2], pl[2];
+    weigh<KIND, ND, false>(acc, a.sc, ksl, lvl, rvl, whole, mine, m, l, o, pf, pl);
     bool odd = false;  // a value is not finite
     if (KIND == SRW_KV_BF16 && !whole) {
       u16x2_t most = {0, 0};
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = 32 * d + col;
-          most = most16(most, ld16(vl[stage] + row * 128 + 16 * ((2 * j + hf) ^ v_swz(row))));
-        }
+      for (int d = 0; d < ND; ++d) {
+        const char* src = vl[stage] + (16 * d + fc) * 128;
+        most = most16(most16(most, ld16(src + 16 * ((2 * fg) ^ v_swz(fc)))), ld16(src + 16 * ((2 * fg + 1) ^ v_swz(fc))));
+        if (d % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+      }
       odd = __any(not_finite(most));
     }
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      const int row = 32 * d + col;
-      const char* src = vl[stage] + row * 128;
+    for (int d0 = 0; d0 < ND; d0 += kBatch / 2) {
+      u32x4_t vf[kBatch / 2][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u32x4_t vb = ld16(src + 16 * ((2 * j + hf) ^ v_swz(row)));
-        if (KIND != SRW_KV_INT8 && keys != ~0ull) {
-          const uint32_t bits = static_cast<uint32_t>(keys >> (16 * j + 8 * hf)) & 0xffu;
+      for (int d = 0; d < kBatch / 2; ++d)
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            vb[u] &= (bits >> (2 * u) & 1 ? 0x0000ffffu : 0u) | (bits >> (2 * u + 1) & 1 ? 0xffff0000u : 0u);
+        for (int st = 0; st < 2; ++st)
+          vf[d][st] = ld16(vl[stage] + (16 * (d0 + d) + fc) * 128 + 16 * ((2 * fg + st) ^ v_swz(fc)));
+      __builtin_amdgcn_sched_barrier(0);
+      if (KIND == SRW_KV_BF16 && (keys != ~0ull || odd)) {
+        // values that no row sees cleared, values that are not finite kept apart
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const uint32_t bits = static_cast<uint32_t>(keys >> (16 * g + 8 * st)) & 0xffu;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t keep = (bits >> (2 * u) & 1 ? 0x0000ffffu : 0u) | (bits >> (2 * u + 1) & 1 ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int d = 0; d < kBatch / 2; ++d) vf[d][st][u] &= keep;
+          }
+#pragma unroll
+          for (int d = 0; d < kBatch / 2; ++d) {
+            vf[d][st] = finite16(vf[d][st]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
-        if (KIND == SRW_KV_BF16 && odd) vb = finite16(vb);
-        o[d] = mfma(vb, pf[j], o[d]);
       }
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < kBatch / 2; ++d) o[d0 + d] = mfma16(vf[d][st], pf[st], o[d0 + d]);
     }
-    if (KIND == SRW_KV_BF16 && odd)
-      add_not_finite<16 * ND>(
-          a.kv, b, h, DH, key0,
-          [&](int k) { return seen_of(pos, key0, a.window, a.sinks) >> k & 1; },
-          [&](int i) { return 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * hf + i % 4; },
-          [&](int i, float v) { o[i / 16][i % 16] += v; });
+    if (KIND == SRW_KV_BF16 && odd) {
+      const int pos = place().pos;
+      add_not_finite<4 * ND>(
+          a.kv, b, h, DH, key0, [&](int k) { return seen_of(pos, key0, a.window, a.sinks) >> k & 1; },
+          [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, [&](int i, float v) { o[i / 4][i % 4] += v; });
+    }
   }
   if (!active) return;
-  l = join32(l, [](float u, float w) { return u + w; });
-  if (!in) return;
-  const int64_t row = (sq.row0 + tok) * a.Hq + head;
+  auto sum = [](float u, float w) { return u + w; };
+  l = join32(join16(l, sum), sum);
+  const Place p = place();
+  if (!p.in) return;
+  const int64_t row = (sq.row0 + p.tok) * a.Hq + p.head;
   if (a.S == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int v = 0; v < 16; v += 4)
-        *reinterpret_cast<uint2*>(a.out + row * DH + 32 * d + 2 * v + 4 * hf) =
-            make_uint2(pack_bf16(o[d][v] * inv, o[d][v + 1] * inv), pack_bf16(o[d][v + 2] * inv, o[d][v + 3] * inv));
+    *reinterpret_cast<uint2*>(a.out + row * DH + 16 * d + 4 * g) =
+        make_uint2(pack_bf16(o[d][0] * inv, o[d][1] * inv), pack_bf16(o[d][2] * inv, o[d][3] * inv));
   } else {
     const int64_t at = split * (a.kv.T * a.Hq) + row;
     if (l != 0.f) {
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int v = 0; v < 16; v += 4)
-          *reinterpret_cast<f32x4_t*>(a.part + at * DH + 32 * d + 2 * v + 4 * hf) =
-              f32x4_t{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(a.part + at * DH + 16 * d + 4 * g) = o[d];
     }
-    if (hf == 0) a.ml[at] = make_float2(m, l);
+    if (g == 0) a.ml[at] = make_float2(m, l);
   }
 }
 
 // How a call runs: the kernel, and in how many splits a sequence's tiles.
 struct AttnPlan {
-  int rows;       // rows a workgroup: 16, 32 (attn_rows_kernel) or 128
-  int64_t groups; // workgroups of one split
+  int rows;      // rows a workgroup: 16, 32 (attn_rows_kernel) or 128
+  int64_t tiles; // row tiles of a key head, at most
   int S, per;
 };
 
@@ -916,47 +979,51 @@ AttnPlan plan_of(const srw_attention_t& a) {
   AttnPlan p{};
   const int64_t G = a.n_heads / a.kv.n_kv_heads, B = a.kv.B, T = a.kv.T, H = a.kv.n_kv_heads;
   const int64_t most = !a.kv.cu ? 1 : a.max_new > 0 ? a.max_new : T;
-  p.rows = most * G <= 16 ? 16 : most * G <= 32 ? 32 : 128;
-  int64_t tiles = a.kv.table_width * a.kv.page_size / kTile + 1;  // of a row, at most
+  int64_t keys = (a.kv.table_width * a.kv.page_size + kTile - 1) / kTile;  // key tiles of a row, at most
   if (a.window > 0) {
     const int64_t w = (a.window + most + kTile - 1) / kTile + 1 + (a.sinks + kTile - 1) / kTile;
-    tiles = w < tiles ? w : tiles;
+    keys = w < keys ? w : keys;
   }
-  if (p.rows < 128) {
-    p.groups = B * H;
-    // about 2048 workgroups in all, of four tiles (one a wave) at least
-    int64_t per = (tiles * p.groups + 2047) / 2048;
-    per = per < 16 ? 16 : (per + 3) / 4 * 4;
-    p.per = static_cast<int>(per < tiles ? per : tiles);
-  } else {
-    p.groups = (!a.kv.cu ? B * ((G + 127) / 128) : T * G / 128 + B) * H;
-    int64_t per = (tiles * p.groups + 511) / 512;
-    per = per < 8 ? 8 : per;
-    p.per = static_cast<int>(per < tiles ? per : tiles);
-  }
+  // 32 rows a workgroup also where more would leave the GPU idle: 512 tokens of 6
+  // heads in 9.8 us against 12.2 of the kernel for many rows, four times as many
+  // in 13.5 against 13.0, 8 x 64 tokens over 2 000 positions in 40 against 25
+  p.rows = most * G <= 16 ? 16 : most * G <= 32 || T * G * H * keys <= 65536 ? 32 : 128;
+  p.tiles = !a.kv.cu ? B * ((G + p.rows - 1) / p.rows) : T * G / p.rows + B;
+  const int64_t groups = p.tiles * H;
+  // Splits where workgroups are too few for the GPU, of a few tiles at least: a
+  // second launch joins them.  (Few rows: 2 x 100 000 positions of 8 heads in 85
+  // us with about 1024 workgroups, 97 with 2048; one of 2 000 in 8.8 us with 4
+  // tiles a split, 13.5 with 16; 64 x 512, 9 tiles, in 8.8 us whole, 10.2 in two.
+  // Many rows: 512 tokens over 4 000 positions in 75 us with about 768, 92 with
+  // 1536.)
+  const int64_t want = p.rows < 128 ? 1024 : 768, least = p.rows < 128 ? 4 : 8;
+  int64_t S = groups >= want / 2 || keys <= 12 ? 1 : want / groups;
+  if (S > keys / least) S = keys / least > 1 ? keys / least : 1;
+  const int64_t per = (keys + S - 1) / S;
+  p.per = static_cast<int>(per < keys ? per : keys);
   if (p.per < 1) p.per = 1;
-  p.S = static_cast<int>((tiles + p.per - 1) / p.per);
+  p.S = static_cast<int>((keys + p.per - 1) / p.per);
   return p;
 }
 
 template <int KIND, int DH>
 hipError_t launch_attention(const srw_attention_t& a, const AttnPlan& pl, AttnArgs& g, hipStream_t s) {
-  if (pl.rows < 128) {
-    const dim3 grid(static_cast<unsigned>(a.kv.B), static_cast<unsigned>(g.kv.H), static_cast<unsigned>(g.S));
-    if (pl.rows == 16)
-      hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 1>), grid, dim3(256), 0, s, g);
-    else
-      hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 2>), grid, dim3(256), 0, s, g);
-  } else {
-    const dim3 grid(static_cast<unsigned>(pl.groups / g.kv.H), static_cast<unsigned>(g.kv.H),
-                    static_cast<unsigned>(g.S));
-    hipLaunchKernelGGL((attn_tile_kernel<KIND, DH>), grid, dim3(256), 0, s, g);
-  }
+  const dim3 grid(static_cast<unsigned>(pl.tiles), static_cast<unsigned>(g.kv.H), static_cast<unsigned>(g.S));
+  if (pl.rows == 16)
+    hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 1>), grid, dim3(256), 0, s, g);
+  else if (pl.rows == 32)
+    hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 2>), grid, dim3(256), 0, s, g);
+  else
+    hipLaunchKernelGGL((attn_tile_kernel<KIND, DH>), grid, dim3(512), 0, s, g);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || g.S == 1) return e;
   const int64_t rows = a.kv.T * a.n_heads;
-  hipLaunchKernelGGL(attn_join_kernel<DH>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, g.part, g.ml, g.out, rows,
-                     g.S);
+  if (g.S <= 8)
+    hipLaunchKernelGGL((attn_join_kernel<DH, true>), dim3(static_cast<unsigned>((rows + 1024 / DH - 1) / (1024 / DH))),
+                     dim3(256), 0, s, g.part, g.ml, g.out, rows, g.S);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<DH, false>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, g.part, g.ml,
+                     g.out, rows, g.S);
   return hipGetLastError();
 }
 

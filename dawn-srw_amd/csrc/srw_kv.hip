@@ -103,16 +103,21 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvView p, KvRows r) {
   if (page < 0) return;
   const int64_t ph = static_cast<int64_t>(page) * p.H + k.head;
   const int slot = (k.base & (p.P - 1)) + k.key0;
+  float xs[2][KPL][4];  // both tensors' rows are requested before either is used
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const T* src = static_cast<const T*>(which ? r.v : r.k) + k.head * (which ? r.v_head : r.k_head) + 4 * k.c;
     const int64_t ts = which ? r.v_token : r.k_token;
-    float x[KPL][4];
 #pragma unroll
     for (int i = 0; i < KPL; ++i) {
-      x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-      if (k.key0 + i >= k.first && k.key0 + i < k.last) load4(src + (k.row + k.key0 + i) * ts, x[i]);
+      // (rows that are not in the call load one that is)
+      const int at = k.key0 + i < k.first ? k.first : k.key0 + i >= k.last ? k.last - 1 : k.key0 + i;
+      load4(src + (k.row + at) * ts, xs[which][i]);
     }
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float(&x)[KPL][4] = xs[which];
     if constexpr (KIND != SRW_KV_BF16) {
 #pragma unroll
       for (int i = 0; i < KPL; ++i) {
