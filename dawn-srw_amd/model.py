@@ -11,7 +11,9 @@ Every SRW call (the QK pool with its Q and K routes paired over one x.R^T,
 the V pool, the Know pool) runs in libsrw_amd.so's HIP kernels.  The glue --
 embeddings, LayerNorm (eps 1e-6, :321-324), the router Dense layers, causal
 softmax attention, expand_O, the tied lm_head -- is plain float32 PyTorch, as
-the reference computes it in float32.  Parameters use the reference's Flax
+the reference computes it in float32.  ``DawnModel.extend`` serves sequences of
+different lengths from a paged key/value cache (kv.py; no counterpart in the
+reference, whose cache has one length).  Parameters use the reference's Flax
 tree names (``params['neuron_pool']['know_emb']``,
 ``params['router']['proj_attn']['kernel']``, ``params['block_3']['norm1']
 ['scale']`` ...), so a checkpoint's tree maps onto them one to one.
@@ -27,6 +29,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _capi as C
+from .kv import PagedKvCache, kv_write, paged_attention
 from .layer import GateConfig, SrwBatchPlan, SrwPlan
 from .srw import chunk_plan
 
@@ -178,6 +181,7 @@ class DawnModel:
         # the bf16 casts the SRW layer applies to the pool (v41:423-430), once
         self.pool_bf = {k: v.to(BF16).contiguous() for k, v in pool.items() if not k.endswith("_scale")}
         self.scale = {k: pool[f"{k}_scale"] for k in ("qk", "v", "know")}
+        self._qk_scale = None  # extend: the scale as a number, read once
         self._calls = {}
 
     # -- pieces -------------------------------------------------------------
@@ -210,9 +214,9 @@ class DawnModel:
     def _dense(x, prm):
         return torch.addmm(prm["bias"], x, prm["kernel"])
 
-    def _srw_qkv(self, normed, stats):
-        """Q, K, V of one layer (v41:1018-1053): router, paired QK call, V call,
-        the pool scales applied after den (outside the SRW function)."""
+    def _qkv_raw(self, normed, stats):
+        """Q and K [T, 2, D] and V [T, 1, D] of one layer as the pools give them
+        (v41:1018-1053): router, paired QK call, V call."""
         cfg, rt = self.cfg, self.p["router"]
         T, dr = normed.shape[0], cfg.d_route
         h_all = self._dense(normed, rt["proj_attn"])                    # :1018
@@ -221,10 +225,13 @@ class DawnModel:
         v_args = (normed, h_all[:, 2 * dr:].reshape(T, 1, dr), tau_all[:, 2:3])
         if 2 * T <= 128:
             # decode-sized: both calls in one srw_forward_batch
-            qk, v = self._qkv_batch(T, stats)(qk_args, v_args)
-        else:
-            qk = self._pool("qk", T, 2, stats)(*qk_args)
-            v = self._pool("v", T, 1, stats)(*v_args)
+            return self._qkv_batch(T, stats)(qk_args, v_args)
+        return self._pool("qk", T, 2, stats)(*qk_args), self._pool("v", T, 1, stats)(*v_args)
+
+    def _srw_qkv(self, normed, stats):
+        """Q, K, V of one layer, the pool scales applied after den (outside the
+        SRW function)."""
+        qk, v = self._qkv_raw(normed, stats)
         q = qk[:, 0].float() * self.scale["qk"]                         # :1044-1045
         k = qk[:, 1].float() * self.scale["qk"]
         v = v[:, 0].float() * self.scale["v"]                           # :1053
@@ -390,3 +397,67 @@ class DawnModel:
             x = x + self._know(self._ln(x, bp["norm2"]), "centered")
         x = self._ln(x, self.p["norm"])
         return x @ self.p["token_emb"]["embedding"].T, cache_K, cache_V, cache_len + 1
+
+    # -- serving sequences of different lengths --------------------------------
+    def new_cache(self, n_pages: int, *, page_size: int = 64, dtype=BF16) -> PagedKvCache:
+        """Pages for the keys and values of all layers (d_head 64 or 128), shared
+        by any number of sequences; ``dtype`` bfloat16 holds what the pools
+        give exactly, int8 and float8_e4m3fn half of the bytes."""
+        cfg = self.cfg
+        return PagedKvCache(cfg.n_layers, n_pages, cfg.n_heads, cfg.d_model // cfg.n_heads, page_size=page_size,
+                            dtype=dtype, device=self.device)
+
+    @torch.no_grad()
+    def extend(self, ids, cache: PagedKvCache, seqs, counts, *, window: int = 0, sinks: int = 0,
+               last_only: bool = False):
+        """counts[i] new tokens of each sequence seqs[i] of the cache -- chunks
+        of prompts and single generated tokens in one batch: ``ids`` [sum of
+        counts] holds them one sequence after the other.  Logits [T, vocab] of
+        the new tokens, or with ``last_only`` [len(seqs), vocab] of each
+        sequence's last (every count at least 1).  A token at position i
+        attends to positions j <= i of its sequence, with ``window`` to those
+        with j > i - window or j < ``sinks``.  Same model as :meth:`prefill` and
+        :meth:`decode_step` (the SRW layer as ``_srw_inference`` in bf16): the
+        cache holds the pools' outputs, the pool scales go into the attention's
+        scale and its result."""
+        cfg = self.cfg
+        D, H = cfg.d_model, cfg.n_heads
+        ids = ids.reshape(-1).to(self.device)
+        counts = [int(n) for n in counts]
+        T = sum(counts)
+        if ids.shape[0] != T:
+            raise ValueError(f"{ids.shape[0]} ids, but the counts make {T}")
+        if last_only and min(counts, default=1) < 1:
+            raise ValueError("last_only needs a new token of every sequence")
+        if T == 0:
+            raise ValueError("no new tokens")
+        for q, n in zip(seqs, counts):
+            if cache.length(q) + n > cfg.max_seq_len:
+                raise ValueError("Sequence length exceeds max_seq_len")
+        place = [cache.length(q) + i for q, n in zip(seqs, counts) for i in range(n)]
+        table, lens, cu, most = cache.extend(seqs, counts)
+        # rows up to one of a few token counts: the pools' plans are kept by it
+        Tp = -(-T // 16) * 16 if T <= 128 else -(-T // 128) * 128
+        x = torch.zeros(Tp, D, device=self.device)
+        place = torch.tensor(place, device=self.device)
+        x[:T] = self.p["token_emb"]["embedding"][ids] + self.p["pos_emb"]["embedding"][place]
+        if self._qk_scale is None:
+            self._qk_scale = float(self.scale["qk"])
+        scale = self._qk_scale ** 2 / math.sqrt(D // H)
+        a = torch.zeros(Tp, H, D // H, dtype=BF16, device=self.device)
+        for i in range(cfg.n_layers):
+            bp, pages = self.p[f"block_{i}"], cache.layer(i)
+            qk, v = self._qkv_raw(self._ln(x, bp["norm1"]), "centered")
+            q, k, v = (t[:T].view(T, H, -1) for t in (qk[:, 0], qk[:, 1], v[:, 0]))
+            kv_write(pages, k, v, table, lens, cu)
+            paged_attention(q, pages, table, lens, cu, max_new=most, scale=scale, window=window, sinks=sinks, out=a[:T])
+            x = x + (a.view(Tp, D).float() * self.scale["v"]) @ bp["attn"]["expand_O"]["kernel"]
+            x = x + self._know(self._ln(x, bp["norm2"]), "centered")
+        x = x[:T]
+        if last_only:
+            at, last = 0, []
+            for n in counts:
+                at += n
+                last.append(at - 1)
+            x = x[torch.tensor(last, device=self.device)]
+        return self._ln(x, self.p["norm"]) @ self.p["token_emb"]["embedding"].T
