@@ -21,7 +21,9 @@ out to sequences.
 from __future__ import annotations
 
 import ctypes
-import math
+import importlib.machinery
+import importlib.util
+import os
 import struct
 
 import torch
@@ -34,12 +36,33 @@ BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 _KINDS = {torch.bfloat16: C.SRW_KV_BF16, torch.int8: C.SRW_KV_INT8, torch.float8_e4m3fn: C.SRW_KV_FP8}
 _DTYPES = {torch.float32: C.SRW_F32, torch.bfloat16: C.SRW_BF16}
 
-# srw_kv_t, srw_kv_rows_t and srw_attention_t as bytes: a call's description is
-# packed in a fraction of the time that a ctypes structure takes to fill, which
-# for single tokens would be half of the call
+# srw_kv_t, srw_kv_rows_t and srw_attention_t as bytes (packed in a fraction of the
+# time that a ctypes structure takes to fill)
 _KV = struct.Struct("@7P5q4i")
 _ROWS = struct.Struct("@2P4q")
 _ATTENTION = struct.Struct("@7P5q4i2P2q4if4x")
+
+
+_host = None
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _native():
+    """The calls' native host side (csrc/srw_host.cpp), which takes calls whose
+    tensors are as the C entry points take them and answers None for any other:
+    those go through the checks and copies here.  (64 single tokens of 6 heads:
+    the kernel takes 10 us, the call from Python took 12, through this 5.)"""
+    global _host
+    if _host is None:
+        C.load_library()
+        path = os.path.join(os.path.dirname(C.LIB_PATH), "_srw_host.so")
+        if not os.path.exists(path):
+            raise C.SrwLibraryError(f"{path} is not built; run __graft_entry__.build() first")
+        spec = importlib.util.spec_from_file_location(
+            "_srw_host", path, loader=importlib.machinery.ExtensionFileLoader("_srw_host", path))
+        _host = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_host)
+    return _host
 
 
 def _tensor(name, t, dev, dtype, shape):
@@ -67,27 +90,33 @@ class KvPages:
     __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "heads", "page_size", "head_dim", "kind", "device", "_at")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
+        # (k, v, k_scale, v_scale addresses, n_pages, heads, page_size, head_dim, kind, device)
+        at = (_host or _native()).pages(k, v, k_scale, v_scale)
+        if at is None:
+            at = self._checked(k, v, k_scale, v_scale)
+        self._at = at
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        _, _, _, _, self.n_pages, self.heads, self.page_size, self.head_dim, self.kind, _ = at
+        self.device = k.device
+
+    @staticmethod
+    def _checked(k, v, k_scale, v_scale):
         if not isinstance(k, torch.Tensor) or k.dim() != 4:
             raise ValueError("k must be a tensor [n_pages, heads, page_size, head_dim]")
         n, h, p, d = k.shape
         dev = k.device
         if dev.type != "cuda":
             raise ValueError(f"the cache lives on a HIP device; got {dev}")
-        kind = _KINDS.get(k.dtype)
-        if kind is None:
+        if k.dtype not in _KINDS:
             raise TypeError(f"pages hold bfloat16, int8 or float8_e4m3fn; got {k.dtype}")
         if not k.is_contiguous():
             raise ValueError("k must be contiguous")
-        at = _tensor("v", v, dev, k.dtype, (n, h, d, p))
-        if kind == C.SRW_KV_BF16:
-            if k_scale is not None or v_scale is not None:
-                raise ValueError("bfloat16 pages have no scales")
-            self._at = (k.data_ptr(), at, 0, 0)
-        else:
-            self._at = (k.data_ptr(), at, _tensor("k_scale", k_scale, dev, F32, (n, h, p)),
-                        _tensor("v_scale", v_scale, dev, F32, (n, h, p)))
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_pages, self.heads, self.page_size, self.head_dim, self.kind, self.device = n, h, p, d, kind, dev
+        kind, v_at, scales = _KINDS[k.dtype], _tensor("v", v, dev, k.dtype, (n, h, d, p)), (0, 0)
+        if kind != C.SRW_KV_BF16:
+            scales = (_tensor("k_scale", k_scale, dev, F32, (n, h, p)), _tensor("v_scale", v_scale, dev, F32, (n, h, p)))
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("bfloat16 pages have no scales")
+        return (k.data_ptr(), v_at, *scales, n, h, p, d, kind, dev.index)
 
 
 def _address(pages, table, lens, cu, T):
@@ -111,7 +140,7 @@ def _address(pages, table, lens, cu, T):
         cu_at = 0
     else:
         raise ValueError(f"{T} tokens of {B} sequences need cu")
-    return (*pages._at, table.data_ptr(), lens_at, cu_at, B, T, pages.n_pages, width, stride if stride > width else width,
+    return (*pages._at[:4], table.data_ptr(), lens_at, cu_at, B, T, pages.n_pages, width, stride if stride > width else width,
             pages.heads, pages.head_dim, pages.page_size, pages.kind)
 
 
@@ -136,8 +165,8 @@ def _rows(name, t, pages, T, dtypes, unit):
 def _call(f, dev, *args):
     """f's status with the current stream of dev as its last argument (launches
     go to the current device's streams)."""
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if torch._C._cuda_getDevice() == dev.index:
+    stream = _raw_stream(dev.index)
+    if _current_device() == dev.index:
         return f(*args, stream)
     with torch.cuda.device(dev):
         return f(*args, stream)
@@ -151,6 +180,11 @@ def kv_write(pages: KvPages, k, v, table, lens, cu=None) -> None:
     m its largest magnitude.  Rows of at most 2^-100 are held as zeros; a row
     with an infinity or NaN reads back as NaN.  Tokens whose position has no
     page are left out; all other slots keep what they hold."""
+    at = pages._at
+    if _current_device() == at[9]:
+        status = (_host or _native()).write(at, k, v, table, lens, cu, _raw_stream(at[9]))
+        if status is not None:
+            return C.check(status)
     T = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() else -1
     a = _address(pages, table, lens, cu, T)
     k = _rows("k", k, pages, T, _DTYPES, 4)
@@ -171,6 +205,11 @@ def kv_read(pages: KvPages, table, lens, cu=None, *, total=None, dtype=BF16):
     if cu is not None and total is None:
         raise ValueError("total, the number of tokens, is needed with cu")
     T = int(total) if total is not None else lens.shape[0]
+    at = pages._at
+    if _current_device() == at[9]:
+        got = (_host or _native()).read(at, table, lens, cu, T, dtype is F32, _raw_stream(at[9]))
+        if got is not None:
+            return got
     a = _address(pages, table, lens, cu, T)
     H, d = pages.heads, pages.head_dim
     k = torch.empty((T, H, d), dtype=dtype, device=pages.device)
@@ -192,6 +231,12 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
     ``out`` [T, n_heads, head_dim] bfloat16; a token that sees nothing gets
     zeros.  The softmax weights are rounded to bfloat16 for the second product;
     sums and statistics are float32."""
+    at = pages._at
+    scale = pages.head_dim ** -0.5 if scale is None else float(scale)
+    if out is None and _current_device() == at[9]:
+        got = (_host or _native()).attention(at, q, table, lens, cu, max_new, scale, window, sinks, _raw_stream(at[9]))
+        if got is not None:
+            return got
     T = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else -1
     kv = _address(pages, table, lens, cu, T)
     q = _rows("q", q, pages, T, (BF16,), 8)
@@ -200,7 +245,6 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
         raise ValueError(f"{Hq} query heads are no multiple of the pages' {pages.heads}")
     if window < 0 or sinks < 0 or (sinks and not window) or max_new < 0:
         raise ValueError("window, sinks and max_new are not negative, and sinks need a window")
-    scale = 1.0 / math.sqrt(pages.head_dim) if scale is None else float(scale)
     dev = pages.device
     if out is None:
         out = torch.empty((T, Hq, pages.head_dim), dtype=BF16, device=dev)

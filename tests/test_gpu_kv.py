@@ -549,3 +549,32 @@ def test_refusals(pkg, dev):
     ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
     assert lib.srw_attention(ctypes.byref(a), ws.data_ptr(), need.value - 1, None) == C.SRW_EWORKSPACE
     torch.cuda.synchronize()
+
+
+def test_calls_without_the_native_host_side(pkg, dev, monkeypatch):
+    """The general path, which the native host side hands calls to that it does
+    not take, makes the same calls."""
+    from dawn_srw_amd import kv
+    new, past = [3, 1, 70], [40, 200, 0]
+    c = Cache(pkg, dev, "int8", 2, 64, 32, [n + m for n, m in zip(new, past)], seed=141)
+    g = torch.Generator().manual_seed(142)
+    _fill(pkg, dev, c, g)
+    k, v = (torch.randn(74, 2, 64, generator=g).to(BF).to(dev) for _ in range(2))
+    q = torch.randn(74, 4, 64, generator=g).to(BF).to(dev)
+    cu = _cu(dev, new)
+
+    def calls():
+        pkg.kv_write(c.pages, k, v, c.table, c.len_t, cu)
+        return (*pkg.kv_read(c.pages, c.table, c.len_t, cu, total=74, dtype=F32),
+                pkg.paged_attention(q, c.pages, c.table, c.len_t, cu, max_new=70, window=50, sinks=3),
+                c.pages.k.clone(), c.pages.v.clone(), pkg.KvPages(c.pages.k, c.pages.v, c.pages.k_scale, c.pages.v_scale)._at)
+
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    print("[gpu] kv without the native host side", flush=True)
+    native = calls()
+    monkeypatch.setattr(kv, "_host", Nothing())
+    for a, b in zip(native, calls()):
+        assert a == b if isinstance(a, tuple) else torch.equal(a, b)
