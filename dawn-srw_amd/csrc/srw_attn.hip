@@ -59,7 +59,7 @@ struct AttnArgs {
   int64_t q_token, q_head;
   int Hq, G, window, sinks;
   float sc;       // scale log2 e
-  int S, per;     // splits of a sequence's tiles, tiles each
+  int S, least;   // splits of a row tile's key tiles, of so many at least
 };
 
 // The tiles that rows at positions [p_lo, p_hi] see: those of the first
@@ -81,6 +81,13 @@ __device__ inline Span span_of(const AttnArgs& a, int p_lo, int p_hi) {
   s.skip = t0 - s.sink_tiles;
   s.tiles = s.sink_tiles + (t1 > t0 ? t1 - t0 : 0);
   return s;
+}
+
+// Tiles of a split, of the row tile's own number: a table far wider than a
+// sequence leaves no long split behind.
+__device__ inline int per_split(const AttnArgs& a, int tiles) {
+  const int per = (tiles + a.S - 1) / a.S;
+  return per > a.least ? per : a.least;
 }
 
 // The sequence and the tile of R rows (token, head of the group) of workgroup
@@ -351,8 +358,9 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
   const int P = a.kv.P;
   const int p_lo = sq.len - sq.n + r0 / a.G, p_hi = sq.len - sq.n + (r1 - 1) / a.G;
   const Span sp = span_of(a, p_lo, p_hi);
-  const int i0 = split * a.per;
-  const int i1 = i0 + a.per < sp.tiles ? i0 + a.per : sp.tiles;
+  const int per = per_split(a, sp.tiles);
+  const int i0 = split * per;
+  const int i1 = i0 + per < sp.tiles ? i0 + per : sp.tiles;
 
   u32x4_t q[NQ][NS];
   int pos[NQ];
@@ -551,20 +559,22 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
 }
 
 // Joins the splits.  Groups of DH / 4 lanes; W of them take a row's splits in
-// turn, each with four loads in flight, and join in LDS: W = 1 for few splits of
-// many rows (no LDS, 256 / (DH / 4) rows a workgroup), all groups of a workgroup
-// of 1024 for the many splits of a few rows.
-template <int DH, bool ONE>
-__global__ __launch_bounds__(ONE ? 256 : 1024) void attn_join_kernel(const float* part, const float2* ml, uint16_t* out,
-                                                        int64_t rows, int S) {
-  constexpr int L = DH / 4, N = (ONE ? 256 : 1024) / L, W = ONE ? 1 : N;  // lanes a group, groups, groups a row
-  const int grp = threadIdx.x / L, c = threadIdx.x % L;
-  const int64_t row = ONE ? static_cast<int64_t>(blockIdx.x) * N + grp : blockIdx.x;
-  if (row >= rows) return;
+// turn, each with four loads in flight, and join in LDS: one for few splits (no
+// LDS), four for more, all of a workgroup of 1024 for the many splits of up to
+// 256 rows (6 rows of 160 splits: 23 us with the attention before it, 30 with
+// four groups; 360 of 35: 21, and 17 with four; 128 tokens of 6 heads over 4 000
+// positions in 8 splits: 14 with one group, 23 with all).
+template <int DH, int W, int TH>
+__global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const float2* ml, uint16_t* out, int64_t rows,
+                                                       int S) {
+  constexpr int L = DH / 4, N = TH / L;  // lanes a group, groups
+  const int c = threadIdx.x % L, first = threadIdx.x / L / W * W, grp = threadIdx.x / L - first;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (N / W) + first / W;
+  const int64_t row = at < rows ? at : rows - 1;
   float m = kLowest, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   constexpr int U = 4;
-  for (int s0 = ONE ? 0 : grp; s0 < S; s0 += W * U) {
+  for (int s0 = grp; s0 < S; s0 += W * U) {
     float2 x[U];
     f32x4_t v[U];
 #pragma unroll
@@ -589,29 +599,30 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void attn_join_kernel(const float
       for (int k = 0; k < 4; ++k) o[k] = o[k] * e0 + v[u][k] * e1;
     }
   }
-  if constexpr (!ONE) {
+  if constexpr (W > 1) {
     __shared__ float sm[N], sl[N];
     __shared__ f32x4_t so[N][L];
     if (c == 0) {
-      sm[grp] = m;
-      sl[grp] = l;
+      sm[first + grp] = m;
+      sl[first + grp] = l;
     }
-    so[grp][c] = o;
+    so[first + grp][c] = o;
     __syncthreads();
     if (grp != 0) return;
-    m = sm[0];
+    m = sm[first];
     l = 0.f;
 #pragma unroll
-    for (int g = 1; g < N; ++g) m = fmaxf(m, sm[g]);
+    for (int g = 1; g < W; ++g) m = fmaxf(m, sm[first + g]);
     o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int g = 0; g < N; ++g) {
-      const float e = sm[g] == m ? 1.f : __builtin_amdgcn_exp2f(sm[g] - m);
-      l += sl[g] * e;
+    for (int g = 0; g < W; ++g) {
+      const float e = sm[first + g] == m ? 1.f : __builtin_amdgcn_exp2f(sm[first + g] - m);
+      l += sl[first + g] * e;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] += so[g][c][k] * e;
+      for (int k = 0; k < 4; ++k) o[k] += so[first + g][c][k] * e;
     }
   }
+  if (at >= rows) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(out + row * DH + 4 * c) =
       make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
@@ -661,8 +672,9 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
   const KvSeq sq = tl.sq;
   const int r0 = tl.r0, r1 = tl.r1;
   const Span sp = span_of(a, sq.len - sq.n + r0 / a.G, sq.len - sq.n + (r1 - 1) / a.G);
-  const int i0 = split * a.per;
-  const int i1 = i0 + a.per < sp.tiles ? i0 + a.per : sp.tiles;
+  const int per = per_split(a, sp.tiles);
+  const int i0 = split * per;
+  const int i1 = i0 + per < sp.tiles ? i0 + per : sp.tiles;
 
   // this wave's rows
   const int w0 = r0 + 16 * wave, w1 = w0 + 16 < r1 ? w0 + 16 : r1;
@@ -978,7 +990,7 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
 struct AttnPlan {
   int rows;      // rows a workgroup: 16, 32 (attn_rows_kernel) or 128
   int64_t tiles; // row tiles of a key head, at most
-  int S, per;
+  int S, least;  // splits of a row tile's key tiles, at most; tiles each, at least
 };
 
 AttnPlan plan_of(const srw_attention_t& a) {
@@ -1000,15 +1012,14 @@ AttnPlan plan_of(const srw_attention_t& a) {
   // second launch joins them.  (Few rows: 2 x 100 000 positions of 8 heads in 85
   // us with about 1024 workgroups, 97 with 2048; one of 2 000 in 8.8 us with 4
   // tiles a split, 13.5 with 16; 64 x 512, 9 tiles, in 8.8 us whole, 10.2 in two.
-  // Many rows: 512 tokens over 4 000 positions in 75 us with about 768, 92 with
-  // 1536.)
-  const int64_t want = p.rows < 128 ? 1024 : 768, least = p.rows < 128 ? 4 : 8;
-  int64_t S = groups >= want / 2 || keys <= 12 ? 1 : want / groups;
-  if (S > keys / least) S = keys / least > 1 ? keys / least : 1;
-  const int64_t per = (keys + S - 1) / S;
-  p.per = static_cast<int>(per < keys ? per : keys);
-  if (p.per < 1) p.per = 1;
-  p.S = static_cast<int>((keys + p.per - 1) / p.per);
+  // Many rows: what the GPU holds at once, 512 workgroups, where a row tile gets
+  // six splits or more of it, else half as many again, since early row tiles end
+  // early: 512 tokens of 16 heads over 4 000 positions in 47.5 us with 448, 53
+  // with 640; two prompts of 2 048 of 6 heads in 29 with 576, 34 with 384.)
+  const int64_t want = p.rows < 128 ? 1024 : groups * 6 <= 512 ? 512 : 768;
+  p.least = p.rows < 128 ? 4 : 8;
+  const int64_t S = groups >= want / 2 || keys <= 12 ? 1 : want / groups, most_splits = keys / p.least;
+  p.S = static_cast<int>(S < most_splits ? S : most_splits > 1 ? most_splits : 1);
   return p;
 }
 
@@ -1024,12 +1035,18 @@ hipError_t launch_attention(const srw_attention_t& a, const AttnPlan& pl, AttnAr
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || g.S == 1) return e;
   const int64_t rows = a.kv.T * a.n_heads;
+  auto join = [&](auto w, auto th) {
+    constexpr int W = decltype(w)::value, TH = decltype(th)::value, R = TH / (DH / 4) / W;
+    hipLaunchKernelGGL((attn_join_kernel<DH, W, TH>), dim3(static_cast<unsigned>((rows + R - 1) / R)), dim3(TH), 0, s,
+                       g.part, g.ml, g.out, rows, g.S);
+  };
+  using std::integral_constant;
   if (g.S <= 8)
-    hipLaunchKernelGGL((attn_join_kernel<DH, true>), dim3(static_cast<unsigned>((rows + 1024 / DH - 1) / (1024 / DH))),
-                     dim3(256), 0, s, g.part, g.ml, g.out, rows, g.S);
+    join(integral_constant<int, 1>{}, integral_constant<int, 256>{});
+  else if (g.S <= 32 || rows > 256)
+    join(integral_constant<int, 4>{}, integral_constant<int, 256>{});
   else
-    hipLaunchKernelGGL((attn_join_kernel<DH, false>), dim3(static_cast<unsigned>(rows)), dim3(1024), 0, s, g.part, g.ml,
-                     g.out, rows, g.S);
+    join(integral_constant<int, 4096 / DH>{}, integral_constant<int, 1024>{});
   return hipGetLastError();
 }
 
@@ -1058,7 +1075,7 @@ hipError_t attention(const srw_attention_t& a, char* ws, hipStream_t s) {
   g.sinks = a.sinks;
   g.sc = a.scale * 1.4426950408889634f;
   g.S = p.S;
-  g.per = p.per;
+  g.least = p.least;
   if (p.S > 1) {
     g.ml = reinterpret_cast<float2*>(ws);
     g.part = reinterpret_cast<float*>(ws + align256(static_cast<size_t>(a.kv.T) * a.n_heads * p.S * sizeof(float2)));
