@@ -1013,12 +1013,15 @@ AttnPlan plan_of(const srw_attention_t& a) {
   // us with about 1024 workgroups, 97 with 2048; one of 2 000 in 8.8 us with 4
   // tiles a split, 13.5 with 16; 64 x 512, 9 tiles, in 8.8 us whole, 10.2 in two.
   // Many rows: what the GPU holds at once, 512 workgroups, where a row tile gets
-  // six splits or more of it, else half as many again, since early row tiles end
-  // early: 512 tokens of 16 heads over 4 000 positions in 47.5 us with 448, 53
-  // with 640; two prompts of 2 048 of 6 heads in 29 with 576, 34 with 384.)
-  const int64_t want = p.rows < 128 ? 1024 : groups * 6 <= 512 ? 512 : 768;
-  p.least = p.rows < 128 ? 4 : 8;
-  const int64_t S = groups >= want / 2 || keys <= 12 ? 1 : want / groups, most_splits = keys / p.least;
+  // six splits or more of it; else more, since row tiles end early and sequences
+  // differ: 512 tokens of 16 heads over 4 000 positions in 47.5 us with 448, 53
+  // with 640; four ragged batches of 24 chunks over up to 2 000 in 47 with about
+  // 1280, 50 with 768; a batch whose row tiles fill three quarters whole.)
+  const bool many = p.rows == 128, once = groups * 6 <= 512;
+  const int64_t want = !many ? 1024 : once ? 512 : 1280, least = many ? 8 : 4;
+  const int64_t S = groups >= (many ? 384 : 512) || keys <= 12 ? 1 : want / groups;
+  p.least = static_cast<int>(least);
+  const int64_t most_splits = keys / least;
   p.S = static_cast<int>(S < most_splits ? S : most_splits > 1 ? most_splits : 1);
   return p;
 }
