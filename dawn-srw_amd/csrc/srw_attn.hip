@@ -332,7 +332,9 @@ __device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, 
 // sequence and key head; its four waves take every fourth tile of its split,
 // each with its own m, l and O, and join in LDS at the end.  Bound by the
 // pages' bytes: a wave loads both operands' fragments straight into
-// registers, 16 bytes a lane, no barrier in the loop.
+// registers, 16 bytes a lane, no barrier in the loop.  Measured: 32 sequences
+// of 4 000 to 32 000 positions, 32 heads on 8 of 128, fp8, in 260 us, 4.7 TB/s (a
+// large copy's traffic: 4.9); 64 sequences of up to 512, 6 heads of 64, int8, in 9.
 //
 // Waves on a SIMD that its registers are kept for (32 sequences of 18 000
 // positions, fp8, head_dim 128: 276 us with three, 281 with two).
@@ -642,6 +644,10 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
 // and matrix instructions run beside other waves' vector ones; so what counts
 // is waves on a SIMD, and with 16 rows a wave (at most 128 registers) four
 // fit, where 32 rows (240 registers at head_dim 128) left two.
+//
+// Measured: 2 048 tokens of 32 heads over 30 011 positions of 8, int8, head_dim
+// 128, in 1 400 us, 0.74 PFLOP/s (32 rows a wave: 1 363, but calls of few tiles
+// twice as long); 8 prompts of 512 of 6 heads of 64, bf16, in 14 us (39 so).
 template <int DH> __device__ inline int k_swz(int row) {
   // a fragment's 16 rows are 16 u + 4 t + v, u, v = 0 .. 3
   return DH == 64 ? (row >> 1 & 1) | (row >> 3 & 6) : (row & 3) | (row >> 2 & 12);
