@@ -317,6 +317,41 @@ def test_chunk_split_over_a_long_axis(pkg, dev, kind):
     _check(pkg, dev, kind, 128, 1, 2, 32, [70], [5000], window=3000, sinks=5, seed=42)
 
 
+# tables far wider than the sequences: splits of what a row tile sees, more of
+# them than it has tiles, joined by one, four or all groups of a workgroup
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh,H,G,new,past,width", [
+    (64, 2, 1, [1, 1, 1], [2000, 0, 129], 2048),             # one token each, many splits of few rows
+    (128, 1, 8, [1] * 40, [40 * i for i in range(40)], 128),  # some splits of more rows
+    (64, 1, 1, [60, 1, 40], [333, 70, 0], 512),              # 32 rows a workgroup
+    (128, 2, 2, [300, 0, 129], [900, 5, 0], 300),            # 128 rows a workgroup
+    (64, 1, 1, [300, 2], [1500, 3000], 2048),                # the same, many splits of many rows
+])
+@pytest.mark.parametrize("window", [0, 700])
+def test_tables_wider_than_their_sequences(pkg, dev, kind, dh, H, G, new, past, width, window):
+    print(f"[gpu] attention wide table {kind} dh{dh} H{H} G{G} new {new[:3]} width {width} window {window}", flush=True)
+    sinks = 4 if window else 0
+    lens = [n + m for n, m in zip(new, past)]
+    c = Cache(pkg, dev, kind, H, dh, 64, lens, seed=81)
+    g = torch.Generator().manual_seed(82)
+    _fill(pkg, dev, c, g)
+    table = torch.full((len(new), width), -1, dtype=I32, device=dev)
+    table[:, :c.table.shape[1]] = c.table
+    q = torch.randn(sum(new), H * G, dh, generator=g).to(BF)
+    cu = None if max(new) == 1 else _cu(dev, new)
+    got = pkg.paged_attention(q.to(dev), c.pages, table, c.len_t, cu, max_new=max(new), window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    at = 0
+    for b, n in enumerate(new):
+        if n == 0:
+            continue
+        k, v = c.held(b)
+        want, mag = _attend64(q[at:at + n], k, v, past[b], 1 / math.sqrt(dh), window, sinks)
+        err = (got[at:at + n].cpu().to(F64) - want).abs()
+        assert (err <= BAR * mag + 1e-30).all(), (b, float((err / (BAR * mag + 1e-30)).max()))
+        at += n
+
+
 @pytest.mark.parametrize("max_new", [0, 1, 5, 1000])
 def test_max_new_is_a_hint(pkg, dev, max_new):
     print(f"[gpu] attention max_new {max_new}", flush=True)
