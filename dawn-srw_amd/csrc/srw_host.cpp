@@ -13,17 +13,23 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "srw_amd.h"
 
 namespace {
 
+constexpr int64_t kMost = 0x7fffffff;
+
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 bool plain(const at::Tensor* t, at::ScalarType type, int64_t dims, int device) {
   return t && t->scalar_type() == type && t->dim() == dims && t->is_cuda() && t->get_device() == device;
 }
+
+// The calls have no backward: kv.py refuses tensors that want one.
+bool wants_grad(const at::Tensor* t) { return t->requires_grad() && c10::GradMode::is_enabled(); }
 
 bool i64(PyObject* o, int64_t* v) {
   if (!PyLong_Check(o)) return false;
@@ -36,23 +42,43 @@ PyObject* none() {
   Py_RETURN_NONE;
 }
 
-// The pages of a KvPages: (k, v, k_scale, v_scale addresses, n_pages, heads,
-// page_size, head_dim, kind, device).
+// The pages of a KvPages: the tensors k, v, k_scale, v_scale, looked at anew in
+// every call (their memory can be another's by then).
 bool pages_of(PyObject* o, srw_kv_t* c, int* device) {
-  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 10) return false;
-  int64_t v[10];
-  for (int i = 0; i < 10; ++i)
-    if (!i64(PyTuple_GET_ITEM(o, i), &v[i])) return false;
-  c->k = reinterpret_cast<void*>(v[0]);
-  c->v = reinterpret_cast<void*>(v[1]);
-  c->k_scale = reinterpret_cast<float*>(v[2]);
-  c->v_scale = reinterpret_cast<float*>(v[3]);
-  c->n_pages = v[4];
-  c->n_kv_heads = static_cast<int32_t>(v[5]);
-  c->page_size = static_cast<int32_t>(v[6]);
-  c->head_dim = static_cast<int32_t>(v[7]);
-  c->kind = static_cast<int32_t>(v[8]);
-  *device = static_cast<int>(v[9]);
+  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  const at::Tensor *k = tensor(PyTuple_GET_ITEM(o, 0)), *v = tensor(PyTuple_GET_ITEM(o, 1));
+  if (!k || !v || k->dim() != 4 || v->dim() != 4 || !k->is_cuda()) return false;
+  *device = static_cast<int>(k->get_device());
+  const auto type = k->scalar_type();
+  const int kind = type == at::kBFloat16 ? SRW_KV_BF16 : type == at::kChar ? SRW_KV_INT8
+                   : type == at::kFloat8_e4m3fn                            ? SRW_KV_FP8
+                                                                           : -1;
+  const int64_t N = k->size(0), H = k->size(1), P = k->size(2), D = k->size(3);
+  if (kind < 0 || !plain(v, type, 4, *device) || v->size(0) != N || v->size(1) != H || v->size(2) != D ||
+      v->size(3) != P || !k->is_contiguous() || !v->is_contiguous() || H > kMost || P > kMost || D > kMost)
+    return false;
+  float* scale[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i) {
+    PyObject* so = PyTuple_GET_ITEM(o, 2 + i);
+    if (kind == SRW_KV_BF16) {
+      if (so != Py_None) return false;
+      continue;
+    }
+    const at::Tensor* s = tensor(so);
+    if (!plain(s, at::kFloat, 3, *device) || s->size(0) != N || s->size(1) != H || s->size(2) != P ||
+        !s->is_contiguous())
+      return false;
+    scale[i] = static_cast<float*>(s->data_ptr());
+  }
+  c->k = k->data_ptr();
+  c->v = v->data_ptr();
+  c->k_scale = scale[0];
+  c->v_scale = scale[1];
+  c->n_pages = N;
+  c->n_kv_heads = static_cast<int32_t>(H);
+  c->page_size = static_cast<int32_t>(P);
+  c->head_dim = static_cast<int32_t>(D);
+  c->kind = kind;
   return true;
 }
 
@@ -79,39 +105,17 @@ bool rows(const at::Tensor* t, int64_t unit, int32_t head_dim) {
          reinterpret_cast<uintptr_t>(t->data_ptr()) % (unit * t->element_size()) == 0;
 }
 
-// pages(k, v, k_scale, v_scale) -> the tuple of pages_of, or None
-PyObject* host_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 4) return none();
-  const at::Tensor *k = tensor(a[0]), *v = tensor(a[1]);
-  if (!k || !v || k->dim() != 4 || v->dim() != 4 || !k->is_cuda()) return none();
-  const int device = static_cast<int>(k->get_device());
-  const auto type = k->scalar_type();
-  const int kind = type == at::kBFloat16 ? SRW_KV_BF16 : type == at::kChar ? SRW_KV_INT8
-                   : type == at::kFloat8_e4m3fn                            ? SRW_KV_FP8
-                                                                           : -1;
-  const int64_t N = k->size(0), H = k->size(1), P = k->size(2), D = k->size(3);
-  if (kind < 0 || !plain(v, type, 4, device) || v->size(0) != N || v->size(1) != H || v->size(2) != D ||
-      v->size(3) != P || !k->is_contiguous() || !v->is_contiguous())
-    return none();
-  int64_t scale[2] = {0, 0};
-  for (int i = 0; i < 2; ++i) {
-    if (kind == SRW_KV_BF16) {
-      if (a[2 + i] != Py_None) return none();
-      continue;
-    }
-    const at::Tensor* s = tensor(a[2 + i]);
-    if (!plain(s, at::kFloat, 3, device) || s->size(0) != N || s->size(1) != H || s->size(2) != P || !s->is_contiguous())
-      return none();
-    scale[i] = reinterpret_cast<int64_t>(s->data_ptr());
-  }
-  return Py_BuildValue("(LLLLLLLLii)", reinterpret_cast<long long>(k->data_ptr()),
-                       reinterpret_cast<long long>(v->data_ptr()), static_cast<long long>(scale[0]),
-                       static_cast<long long>(scale[1]), static_cast<long long>(N), static_cast<long long>(H),
-                       static_cast<long long>(P), static_cast<long long>(D), kind, device);
+// pages((k, v, k_scale, v_scale)) -> (n_pages, heads, page_size, head_dim, kind, device), or None
+PyObject* host_pages(PyObject* const* a, Py_ssize_t n) {
+  srw_kv_t c{};
+  int device;
+  if (n != 1 || !pages_of(a[0], &c, &device)) return none();
+  return Py_BuildValue("(Liiiii)", static_cast<long long>(c.n_pages), c.n_kv_heads, c.page_size, c.head_dim, c.kind,
+                       device);
 }
 
 // write(pages, k, v, table, lens, cu, stream) -> status, or None
-PyObject* host_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* host_write(PyObject* const* a, Py_ssize_t n) {
   srw_kv_t c{};
   int device;
   int64_t stream;
@@ -119,7 +123,8 @@ PyObject* host_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor *k = tensor(a[1]), *v = tensor(a[2]);
   if (!k || !v || k->dim() != 3) return none();
   const auto type = k->scalar_type();
-  if ((type != at::kBFloat16 && type != at::kFloat) || !plain(k, type, 3, device) || !plain(v, type, 3, device))
+  if ((type != at::kBFloat16 && type != at::kFloat) || !plain(k, type, 3, device) || !plain(v, type, 3, device) ||
+      wants_grad(k) || wants_grad(v))
     return none();
   const int64_t T = k->size(0);
   if (v->size(0) != T || k->size(1) != c.n_kv_heads || v->size(1) != c.n_kv_heads || !rows(k, 4, c.head_dim) ||
@@ -130,31 +135,27 @@ PyObject* host_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // read(pages, table, lens, cu, T, float32, stream) -> (k, v), or None
-PyObject* host_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* host_read(PyObject* const* a, Py_ssize_t n) {
   srw_kv_t c{};
   int device;
   int64_t T, f32, stream;
   if (n != 7 || !pages_of(a[0], &c, &device) || !i64(a[4], &T) || !i64(a[5], &f32) || !i64(a[6], &stream)) return none();
   if (T < 0 || !sequences(a[1], a[2], a[3], T, device, &c)) return none();
-  try {
-    const auto opt = at::TensorOptions().dtype(f32 ? at::kFloat : at::kBFloat16).device(at::kCUDA, device);
-    const int64_t H = c.n_kv_heads, D = c.head_dim;
-    at::Tensor k = at::empty({T, H, D}, opt), v = at::empty({T, H, D}, opt);
-    const srw_kv_rows_t r{k.data_ptr(), v.data_ptr(), H * D, D, H * D, D};
-    const int status = srw_kv_read(&c, &r, f32 ? SRW_F32 : SRW_BF16, reinterpret_cast<void*>(stream));
-    if (status != SRW_OK) return none();  // (the general path says what is wrong)
-    PyObject* out = PyTuple_New(2);
-    if (!out) return nullptr;
-    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(k)));
-    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(v)));
-    return out;
-  } catch (...) {
-    return none();  // (out of memory: the general path's allocation says so)
-  }
+  const auto opt = at::TensorOptions().dtype(f32 ? at::kFloat : at::kBFloat16).device(at::kCUDA, device);
+  const int64_t H = c.n_kv_heads, D = c.head_dim;
+  at::Tensor k = at::empty({T, H, D}, opt), v = at::empty({T, H, D}, opt);
+  const srw_kv_rows_t r{k.data_ptr(), v.data_ptr(), H * D, D, H * D, D};
+  const int status = srw_kv_read(&c, &r, f32 ? SRW_F32 : SRW_BF16, reinterpret_cast<void*>(stream));
+  if (status != SRW_OK) return none();  // (the general path says what is wrong)
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(v)));
+  return out;
 }
 
 // attention(pages, q, table, lens, cu, max_new, scale, window, sinks, stream) -> out, or None
-PyObject* host_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* host_attention(PyObject* const* a, Py_ssize_t n) {
   srw_attention_t s{};
   int device;
   int64_t most, window, sinks, stream;
@@ -162,8 +163,7 @@ PyObject* host_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !i64(a[9], &stream) || !PyFloat_Check(a[6]))
     return none();
   const at::Tensor* q = tensor(a[1]);
-  if (!plain(q, at::kBFloat16, 3, device) || !rows(q, 8, s.kv.head_dim)) return none();
-  constexpr int64_t kMost = 0x7fffffff;
+  if (!plain(q, at::kBFloat16, 3, device) || wants_grad(q) || !rows(q, 8, s.kv.head_dim)) return none();
   if (most < 0 || most > kMost || window < 0 || window > kMost || sinks < 0 || sinks > kMost || q->size(1) > kMost)
     return none();
   const int64_t T = q->size(0);
@@ -178,23 +178,30 @@ PyObject* host_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.scale = static_cast<float>(PyFloat_AS_DOUBLE(a[6]));
   size_t need = 0;
   if (srw_attention_workspace_size(&s, &need) != SRW_OK) return none();
+  const auto opt = at::TensorOptions().device(at::kCUDA, device);
+  at::Tensor out = at::empty({T, q->size(1), s.kv.head_dim}, opt.dtype(at::kBFloat16)), ws;
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, opt.dtype(at::kByte));
+  s.out = out.data_ptr();
+  if (srw_attention(&s, need ? ws.data_ptr() : nullptr, need, reinterpret_cast<void*>(stream)) != SRW_OK) return none();
+  return THPVariable_Wrap(std::move(out));
+}
+
+// Nothing thrown leaves through Python's C frames: a tensor without memory of its
+// own, no memory for an output -- the general path meets it again and says so.
+template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
+PyObject* caught(PyObject*, PyObject* const* a, Py_ssize_t n) {
   try {
-    const auto opt = at::TensorOptions().device(at::kCUDA, device);
-    at::Tensor out = at::empty({T, q->size(1), s.kv.head_dim}, opt.dtype(at::kBFloat16)), ws;
-    if (need) ws = at::empty({static_cast<int64_t>(need)}, opt.dtype(at::kByte));
-    s.out = out.data_ptr();
-    if (srw_attention(&s, need ? ws.data_ptr() : nullptr, need, reinterpret_cast<void*>(stream)) != SRW_OK) return none();
-    return THPVariable_Wrap(std::move(out));
+    return F(a, n);
   } catch (...) {
-    return none();  // (out of memory: the general path's allocation says so)
+    return none();
   }
 }
 
 PyMethodDef methods[] = {
-    {"pages", reinterpret_cast<PyCFunction>(host_pages), METH_FASTCALL, nullptr},
-    {"write", reinterpret_cast<PyCFunction>(host_write), METH_FASTCALL, nullptr},
-    {"read", reinterpret_cast<PyCFunction>(host_read), METH_FASTCALL, nullptr},
-    {"attention", reinterpret_cast<PyCFunction>(host_attention), METH_FASTCALL, nullptr},
+    {"pages", reinterpret_cast<PyCFunction>(caught<host_pages>), METH_FASTCALL, nullptr},
+    {"write", reinterpret_cast<PyCFunction>(caught<host_write>), METH_FASTCALL, nullptr},
+    {"read", reinterpret_cast<PyCFunction>(caught<host_read>), METH_FASTCALL, nullptr},
+    {"attention", reinterpret_cast<PyCFunction>(caught<host_attention>), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_srw_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -87,20 +87,26 @@ class KvPages:
     page_size] float32.  Holds the tensors, which the calls read and write in
     place."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "heads", "page_size", "head_dim", "kind", "device", "_at")
+    __slots__ = ("_t", "n_pages", "heads", "page_size", "head_dim", "kind", "device")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        # (k, v, k_scale, v_scale addresses, n_pages, heads, page_size, head_dim, kind, device)
-        at = (_host or _native()).pages(k, v, k_scale, v_scale)
+        self._t = (k, v, k_scale, v_scale)
+        at = (_host or _native()).pages(self._t)
         if at is None:
-            at = self._checked(k, v, k_scale, v_scale)
-        self._at = at
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        _, _, _, _, self.n_pages, self.heads, self.page_size, self.head_dim, self.kind, _ = at
+            at = self._at[4:]
+        self.n_pages, self.heads, self.page_size, self.head_dim, self.kind, _ = at
         self.device = k.device
 
-    @staticmethod
-    def _checked(k, v, k_scale, v_scale):
+    k = property(lambda self: self._t[0])
+    v = property(lambda self: self._t[1])
+    k_scale = property(lambda self: self._t[2])
+    v_scale = property(lambda self: self._t[3])
+
+    @property
+    def _at(self):
+        """(k, v, k_scale, v_scale addresses, n_pages, heads, page_size, head_dim,
+        kind, device) of the tensors as they are now."""
+        k, v, k_scale, v_scale = self._t
         if not isinstance(k, torch.Tensor) or k.dim() != 4:
             raise ValueError("k must be a tensor [n_pages, heads, page_size, head_dim]")
         n, h, p, d = k.shape
@@ -140,8 +146,11 @@ def _address(pages, table, lens, cu, T):
         cu_at = 0
     else:
         raise ValueError(f"{T} tokens of {B} sequences need cu")
-    return (*pages._at[:4], table.data_ptr(), lens_at, cu_at, B, T, pages.n_pages, width, stride if stride > width else width,
-            pages.heads, pages.head_dim, pages.page_size, pages.kind)
+    at = pages._at
+    if at[4:9] != (pages.n_pages, pages.heads, pages.page_size, pages.head_dim, pages.kind) or at[9] != dev.index:
+        raise ValueError("the pages' tensors have changed since KvPages took them")
+    return (*at[:4], table.data_ptr(), lens_at, cu_at, B, T, pages.n_pages, width,
+            stride if stride > width else width, pages.heads, pages.head_dim, pages.page_size, pages.kind)
 
 
 def _rows(name, t, pages, T, dtypes, unit):
@@ -154,6 +163,8 @@ def _rows(name, t, pages, T, dtypes, unit):
         raise ValueError(f"{name} is on {t.device}, expected {pages.device}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{name} requires a gradient; the paged cache's calls have none (torch.no_grad())")
     s0, s1, s2 = t.stride()
     if s2 != 1 or s0 % unit or s1 % unit or t.data_ptr() % (unit * t.element_size()):
         t = t.contiguous()
@@ -180,9 +191,8 @@ def kv_write(pages: KvPages, k, v, table, lens, cu=None) -> None:
     m its largest magnitude.  Rows of at most 2^-100 are held as zeros; a row
     with an infinity or NaN reads back as NaN.  Tokens whose position has no
     page are left out; all other slots keep what they hold."""
-    at = pages._at
-    if _current_device() == at[9]:
-        status = (_host or _native()).write(at, k, v, table, lens, cu, _raw_stream(at[9]))
+    if _current_device() == pages.device.index:
+        status = (_host or _native()).write(pages._t, k, v, table, lens, cu, _raw_stream(pages.device.index))
         if status is not None:
             return C.check(status)
     T = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() else -1
@@ -205,9 +215,8 @@ def kv_read(pages: KvPages, table, lens, cu=None, *, total=None, dtype=BF16):
     if cu is not None and total is None:
         raise ValueError("total, the number of tokens, is needed with cu")
     T = int(total) if total is not None else lens.shape[0]
-    at = pages._at
-    if _current_device() == at[9]:
-        got = (_host or _native()).read(at, table, lens, cu, T, dtype is F32, _raw_stream(at[9]))
+    if _current_device() == pages.device.index:
+        got = (_host or _native()).read(pages._t, table, lens, cu, T, dtype is F32, _raw_stream(pages.device.index))
         if got is not None:
             return got
     a = _address(pages, table, lens, cu, T)
@@ -231,10 +240,10 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
     ``out`` [T, n_heads, head_dim] bfloat16; a token that sees nothing gets
     zeros.  The softmax weights are rounded to bfloat16 for the second product;
     sums and statistics are float32."""
-    at = pages._at
     scale = pages.head_dim ** -0.5 if scale is None else float(scale)
-    if out is None and _current_device() == at[9]:
-        got = (_host or _native()).attention(at, q, table, lens, cu, max_new, scale, window, sinks, _raw_stream(at[9]))
+    if out is None and _current_device() == pages.device.index:
+        got = (_host or _native()).attention(pages._t, q, table, lens, cu, max_new, scale, window, sinks,
+                                             _raw_stream(pages.device.index))
         if got is not None:
             return got
     T = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else -1

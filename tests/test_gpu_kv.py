@@ -613,3 +613,44 @@ def test_calls_without_the_native_host_side(pkg, dev, monkeypatch):
     monkeypatch.setattr(kv, "_host", Nothing())
     for a, b in zip(native, calls()):
         assert a == b if isinstance(a, tuple) else torch.equal(a, b)
+
+
+def test_pages_are_looked_at_in_every_call(pkg, dev):
+    """Tensors whose memory became another's, names that cannot be put on other
+    tensors, tensors whose shape no longer fits."""
+    print("[gpu] pages looked at anew", flush=True)
+    lens = torch.tensor([20], dtype=I32, device=dev)
+    table = torch.tensor([[1, 0]], dtype=I32, device=dev)
+    cu = _cu(dev, [20])
+    g = torch.Generator().manual_seed(91)
+    rows = torch.randn(20, 1, 64, generator=g).to(BF).to(dev)
+    pages = pkg.KvPages(torch.zeros(2, 1, 16, 64, dtype=BF, device=dev), torch.zeros(2, 1, 64, 16, dtype=BF, device=dev))
+    old, old_v = pages.k.data, pages.v.data
+    pages.k.data, pages.v.data = torch.zeros_like(old), torch.zeros_like(old_v)
+    pkg.kv_write(pages, rows, rows, table, lens, cu)
+    assert (old == 0).all() and (old_v == 0).all()
+    assert torch.equal(pages.k[1, 0], rows[:16, 0]) and torch.equal(pages.v[0, 0, :, :4].T, rows[16:, 0])
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(pages, name, old)
+    pages.v.data = torch.zeros(2, 1, 16, 64, dtype=BF, device=dev)
+    for call in (lambda: pkg.kv_write(pages, rows, rows, table, lens, cu),
+                 lambda: pkg.kv_read(pages, table, lens, cu, total=20),
+                 lambda: pkg.paged_attention(rows, pages, table, lens, cu)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_tensors_that_want_gradients_are_refused(pkg, dev):
+    print("[gpu] no gradients", flush=True)
+    lens, table = torch.tensor([1], dtype=I32, device=dev), torch.tensor([[0]], dtype=I32, device=dev)
+    pages = pkg.KvPages(torch.zeros(1, 1, 16, 64, dtype=BF, device=dev), torch.zeros(1, 1, 64, 16, dtype=BF, device=dev))
+    x = torch.ones(1, 1, 64, dtype=BF, device=dev)
+    w = x.clone().requires_grad_()
+    for call in (lambda: pkg.kv_write(pages, w, x, table, lens), lambda: pkg.kv_write(pages, x, w, table, lens),
+                 lambda: pkg.paged_attention(w, pages, table, lens)):
+        with pytest.raises(NotImplementedError):
+            call()
+    with torch.no_grad():
+        pkg.kv_write(pages, w, w, table, lens)
+        assert torch.equal(pkg.paged_attention(w, pages, table, lens), x)
