@@ -25,8 +25,8 @@ constexpr float kKvTiny = 7.888609052210118e-31f;  // 2^-100
 // prompt's writes of 16-position runs of value rows meet in L2, where the
 // workgroup's four waves (consecutive runs of one head) complete the lines.
 // Measured, 65 521 positions of 8 heads of 128, int8 pages, float32 rows: written
-// in 150 to 180 us, 3.8 to 4.5 TB/s, read back in 114, 5.9 (part of the pages from
-// cache); 64 sequences' single tokens of 6 heads of 64 in 5 us, a launch and one
+// in 130 to 160 us, 4.2 to 5.2 TB/s, read back in 100 to 120, about 6 (part of the
+// pages from cache); 64 sequences' single tokens of 6 heads of 64 in 5 us, a launch and one
 // chain of dependent loads.
 template <int DH>
 struct Block {
@@ -67,20 +67,27 @@ __device__ inline bool find_block(const KvView& p, Block<DH>& k) {
   return true;
 }
 
-template <typename T>
+// Rows of a call pass once, read by kv_write, written by kv_read: with ONCE, and in
+// store4, they are marked so that they do not push the pages out of the caches
+// (65 521 positions as above written and read back: 297 us, 356 unmarked).
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <bool ONCE, typename T>
 __device__ inline void load4(const T* p, float (&x)[4]) {
+  auto get = [](auto* at) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(at);
+    else return *at;
+  };
   if constexpr (sizeof(T) == 4) {
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    x[0] = q.x;
-    x[1] = q.y;
-    x[2] = q.z;
-    x[3] = q.w;
+    const f32x4_t q = get(reinterpret_cast<const f32x4_t*>(p));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = q[j];
   } else {
-    const uint2 q = *reinterpret_cast<const uint2*>(p);
-    x[0] = lo_f32(q.x);
-    x[1] = hi_f32(q.x);
-    x[2] = lo_f32(q.y);
-    x[3] = hi_f32(q.y);
+    const u32x2_t q = get(reinterpret_cast<const u32x2_t*>(p));
+    x[0] = lo_f32(q[0]);
+    x[1] = hi_f32(q[0]);
+    x[2] = lo_f32(q[1]);
+    x[3] = hi_f32(q[1]);
   }
 }
 
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvView p, KvRows r) {
     for (int i = 0; i < KPL; ++i) {
       // (rows that are not in the call load one that is)
       const int at = k.key0 + i < k.first ? k.first : k.key0 + i >= k.last ? k.last - 1 : k.key0 + i;
-      load4(src + (k.row + at) * ts, xs[which][i]);
+      load4<true>(src + (k.row + at) * ts, xs[which][i]);
     }
   }
 #pragma unroll
@@ -216,9 +223,9 @@ __device__ inline void values4(uint32_t w, float (&x)[4]) {
 template <typename T>
 __device__ inline void store4(T* p, const float (&x)[4]) {
   if constexpr (sizeof(T) == 4)
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    __builtin_nontemporal_store(f32x4_t{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4_t*>(p));
   else
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    __builtin_nontemporal_store(u32x2_t{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])}, reinterpret_cast<u32x2_t*>(p));
 }
 
 // The same blocks read back; positions without a page give zeros.
@@ -239,13 +246,13 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvView p, KvRows r) {
     const char* vsrc = p.v + (ph * DH + 4 * k.c) * p.P * ES + slot * ES;
     if constexpr (KIND == SRW_KV_BF16) {
 #pragma unroll
-      for (int i = 0; i < KPL; ++i) load4(reinterpret_cast<const uint16_t*>(src + i * (DH * ES)), x[0][i]);
+      for (int i = 0; i < KPL; ++i) load4<false>(reinterpret_cast<const uint16_t*>(src + i * (DH * ES)), x[0][i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < KPL; i += 4) {
           float t[4];
-          load4(reinterpret_cast<const uint16_t*>(vsrc + (static_cast<int64_t>(j) * p.P + i) * ES), t);
+          load4<false>(reinterpret_cast<const uint16_t*>(vsrc + (static_cast<int64_t>(j) * p.P + i) * ES), t);
 #pragma unroll
           for (int u = 0; u < 4; ++u) x[1][i + u][j] = t[u];
         }
