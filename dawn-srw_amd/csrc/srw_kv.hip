@@ -29,12 +29,11 @@ constexpr float kKvTiny = 7.888609052210118e-31f;  // 2^-100
 // pages from cache); 64 sequences' single tokens of 6 heads of 64 in 5 us, a launch and one
 // chain of dependent loads.
 template <int DH>
-struct Block {
+struct Block : KvRun {
   static constexpr int kLanes = DH / 4;      // lanes a row
   static constexpr int kKeys = DH / 16;      // positions a lane
-  int64_t b, row;                            // sequence; packed row of the first position
-  int head, base, first, last;               // positions base + [first, last) of the 16 are in the call
-  int c, key0;                               // the lane's dims / 4 and its first position
+  int64_t b;                                 // sequence
+  int head, c, key0;                         // the lane's dims / 4 and its first position
 };
 
 // Units of 16 positions of sequence b: start(b) = cu[b] / 16 + 2 b leaves room
@@ -48,19 +47,11 @@ __device__ inline bool find_block(const KvView& p, Block<DH>& k) {
     auto start = [&](int64_t b) { return (static_cast<int64_t>(p.cu[b]) >> 4) + 2 * b; };
     k.b = kv_find(p.B, unit, start);
     at = unit - start(k.b);
-    if (at < 0) return false;
   } else {
     if (unit >= p.B) return false;
     k.b = unit;
   }
-  const KvSeq s = kv_seq(p, k.b);
-  const int64_t from = static_cast<int64_t>(s.len) - s.n;   // may lie before position 0
-  const int64_t base = ((from >> 4) + at) * 16;
-  if (base >= s.len) return false;
-  k.base = static_cast<int>(base);
-  k.first = from > base ? static_cast<int>(from - base) : 0;
-  k.last = s.len - base < 16 ? static_cast<int>(s.len - base) : 16;
-  k.row = s.row0 + (base - from);
+  if (!kv_run(kv_seq(p, k.b), at, k)) return false;
   k.head = blockIdx.y;
   k.c = lane % Block<DH>::kLanes;
   k.key0 = lane / Block<DH>::kLanes * Block<DH>::kKeys;
@@ -122,8 +113,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvView p, KvRows r) {
 #pragma unroll
     for (int i = 0; i < KPL; ++i) {
       // (rows that are not in the call load one that is)
-      const int at = k.key0 + i < k.first ? k.first : k.key0 + i >= k.last ? k.last - 1 : k.key0 + i;
-      load4<true>(src + (k.row + at) * ts, xs[which][i]);
+      load4<true>(src + (k.row + kv_in_run(k, k.key0 + i)) * ts, xs[which][i]);
     }
   }
 #pragma unroll

@@ -72,6 +72,29 @@ __device__ inline KvSeq kv_seq(const KvView& p, int64_t b) {
   return KvSeq{r0, static_cast<int>(r1 - r0), len};
 }
 
+// The positions base + [first, last) of an aligned run of kKvGroup that are new tokens
+// of a sequence, at packed rows row + [first, last): those of the at-th run from its
+// first new token's on; false where there are none, as for a sequence without new
+// tokens, which owns no row that could be read.
+struct KvRun {
+  int64_t row;
+  int base, first, last;
+};
+__host__ __device__ inline bool kv_run(const KvSeq& s, int64_t at, KvRun& k) {
+  const int64_t from = static_cast<int64_t>(s.len) - s.n;   // may lie before position 0
+  const int64_t base = ((from >> 4) + at) * kKvGroup;
+  if (s.n <= 0 || at < 0 || base >= s.len) return false;
+  k.base = static_cast<int>(base);
+  k.first = from > base ? static_cast<int>(from - base) : 0;
+  k.last = s.len - base < kKvGroup ? static_cast<int>(s.len - base) : kKvGroup;
+  k.row = s.row0 + (base - from);
+  return true;
+}
+// i, or the nearest that is in the run.
+__host__ __device__ inline int kv_in_run(const KvRun& k, int i) {
+  return i < k.first ? k.first : i >= k.last ? k.last - 1 : i;
+}
+
 // The page of position pos of sequence b, or -1: past the table, or an entry
 // that names no page.
 __device__ inline int kv_page(const KvView& p, int64_t b, int pos) {
