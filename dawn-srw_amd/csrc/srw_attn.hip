@@ -31,11 +31,11 @@
 // What a token must not see is left out by selects, not by adding numbers;
 // positions without a page (a table entry that names none, as for positions
 // that a window has left behind) are not seen, and value bytes that no token
-// of a tile sees are cleared before the product, since 0 x NaN is NaN.  Where
-// the tokens of a tile see different keys, bf16 values that are not finite are
-// kept out of the product too and added to the tokens that see them
-// (8-bit values are finite; their scales, which may not be, multiply weights,
-// which are a token's own).  A token that sees nothing gets zeros.
+// of a tile sees are cleared before the product, since 0 x NaN is NaN.  bf16
+// values that are not finite are kept out of the product too, where the tokens of
+// a tile see different keys or weights come in two parts, and added to the tokens
+// that see them (8-bit values are finite; their scales, which may not be, multiply
+// weights, which are a token's own).  A token that sees nothing gets zeros.
 
 #include <math.h>
 
@@ -381,12 +381,22 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
       const int d = ES == 2 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s & 1);
       q[x][s] = in ? ld16(src + d) : u32x4_t{0, 0, 0, 0};
     }
+  }
+
+  // apart: bf16 values that are not finite are kept out of the products (an
+  // infinity times what is left of a weight, zero or negative, would be NaN, and
+  // so would zero times one that a row does not see) and added to the rows that
+  // see them.  They are rare and leave a sum that is not finite: only a wave that
+  // ends with one goes over its tiles so, once more.
+  bool apart = false;
+again:
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
     m[x] = kLowest;
     l[x] = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[x][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-
   for (int i = i0 + wave; i < i1; i += 4) {
     const int key0 = sp.key0(i);
     // rows of the first product: row 4 u + v of its tile t is key 16 u + 4 t
@@ -452,7 +462,6 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
     bool odd = false;  // a value is not finite
     if (!whole && KIND != SRW_KV_INT8) {
       for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);  // over the columns: keys that some row sees
-      u16x2_t most = {0, 0};
 #pragma unroll
       for (int u = 0; u < 4 * ES; ++u) {  // a dword's keys
         uint32_t keep;
@@ -465,18 +474,19 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
 #pragma unroll
         for (int d = 0; d < ND; ++d) vf[d][u / 4][u % 4] &= keep;
       }
-      if (KIND == SRW_KV_BF16 && p_lo != p_hi) {
+    }
+    if (KIND == SRW_KV_BF16 && apart) {
+      u16x2_t most = {0, 0};
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < ES; ++j) most = most16(most, vf[d][j]);
+      odd = __any(not_finite(most));
+      if (odd) {
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-          for (int j = 0; j < ES; ++j) most = most16(most, vf[d][j]);
-        odd = __any(not_finite(most));
-        if (odd) {
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int j = 0; j < ES; ++j) vf[d][j] = finite16(vf[d][j]);
-        }
+          for (int j = 0; j < ES; ++j) vf[d][j] = finite16(vf[d][j]);
       }
     }
 #pragma unroll
@@ -500,6 +510,18 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
             [&](int k) { return seen_of(pos[x], key0, a.window, a.sinks) >> k & 1; },
             [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, [&](int i, float v) { o[x][i / 4][i % 4] += v; });
     }
+  }
+
+  if (KIND == SRW_KV_BF16 && !apart) {
+    float none = 0.f;  // NaN once a sum is not finite
+#pragma unroll
+    for (int x = 0; x < NQ; ++x)
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) none = fmaf(o[x][d][v], 0.f, none);
+    apart = __any(none != none);
+    if (apart) goto again;
   }
 
   // join the four waves

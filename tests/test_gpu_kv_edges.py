@@ -3,10 +3,12 @@ implementations on the CPU (bounds as in test_gpu_kv.py)."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
-from tests.test_gpu_kv import BF, F32, I32, KINDS, Cache, _codes, _cu
+from tests.test_gpu_kv import BAR, BF, F32, F64, I32, KINDS, Cache, _attend64, _codes, _cu
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +42,33 @@ def test_write_beside_sequences_without_new_tokens(pkg, dev, kind, counts):
         assert torch.equal(got.cpu(), held(want))
     for want, got in zip(new, pkg.kv_read(c.pages, c.table, c.len_t, cu, total=sum(counts), dtype=F32)):
         assert torch.equal(got.cpu(), held(want))
+
+
+# -- attention -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dh,G", [(64, 1), (128, 2), (64, 24)])
+@pytest.mark.parametrize("n,past", [(1, 300), (1, 9001), (20, 300)], ids=str)
+def test_infinite_values(pkg, dev, dh, G, n, past):
+    """A value of infinity weighs more than nothing in every row that sees it: that
+    dim is the infinity, two of opposite signs make it NaN, and no other dim nor
+    any row before it changes."""
+    print(f"[gpu] attention infinite values dh{dh} G{G} n{n} past{past}", flush=True)
+    L = past + n
+    c = Cache(pkg, dev, "bf16", 1, dh, 64, [L], seed=211)
+    g = torch.Generator().manual_seed(212)
+    k, v = (torch.randn(L, 1, dh, generator=g).to(BF) for _ in range(2))
+    q = torch.randn(n, G, dh, generator=g).to(BF)
+    want, mag = _attend64(q, k.to(F64), v.to(F64), past, dh ** -0.5, 0, 0)
+    bad = v.clone()
+    bad[5, 0, 3] = bad[L - 1, 0, 21] = math.inf
+    bad[70, 0, 9] = bad[L - 2, 0, 22] = -math.inf
+    bad[130, 0, 11], bad[200, 0, 11] = math.inf, -math.inf
+    bad[131, 0, 12] = math.nan
+    want[..., 3], want[..., 9], want[..., 11], want[..., 12] = math.inf, -math.inf, math.nan, math.nan
+    want[n - 1, :, 21] = math.inf                             # the last token's, which only it sees
+    want[max(n - 2, 0):, :, 22] = -math.inf
+    pkg.kv_write(c.pages, k.to(dev), bad.to(dev), c.table, c.len_t, _cu(dev, [L]))
+    got = pkg.paged_attention(q.to(dev), c.pages, c.table, c.len_t, _cu(dev, [n]), max_new=n).cpu().to(F64)
+    fine = torch.isfinite(want)
+    assert ((got - want).abs() <= BAR * mag)[fine].all()
+    assert torch.equal(got[~fine].nan_to_num(7.0, 1e300, -1e300), want[~fine].nan_to_num(7.0, 1e300, -1e300))
