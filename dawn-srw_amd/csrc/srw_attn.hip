@@ -17,8 +17,9 @@
 // codes.  A key's scale multiplies its score, a value's scale goes into the
 // exponent,
 //   w[j] = 2^(s[j] + log2 vs[j] - m),  l = sum_j w[j] / vs[j],
-// so that m follows the weights that the second product reads.  (l would lose
-// keys only where value scales of one row differ by more than 2^100.)
+// so that m follows the weights that the second product reads.  (A weight under
+// 2^-126 is lost to l: one of a key whose value scale is 2^-d times that of the
+// key that m follows, and which so weighs less than 2^(d - 126) of it.)
 //
 // The matrix cores read weights in bf16.  The kernel for few rows, bound by
 // memory, gives them in two parts (bf16 of w and of what is left, 16 bits in
@@ -192,9 +193,12 @@ __device__ inline void settled(f32x4_t (&a)[4]) {
   asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
 }
 // A value's scale in the exponent: its log2 and its inverse.  A scale of zero
-// stands for values of zero and takes 2^-100; NaN stays.
+// stands for values of zero and takes 2^-100.  The smallest that kv_write gives
+// other values is 2^-100 / 448, above 2^-109: smaller ones are taken for that,
+// so that the inverses' sums stay in float32.  NaN stays.
 __device__ inline void in_exponent(float vs, float& lv, float& rv) {
-  const float x = vs <= 7.888609052210118e-31f ? 7.888609052210118e-31f : vs;
+  constexpr float least = 1.5407439555097887e-33f;  // 2^-109
+  const float x = vs == 0.f ? 7.888609052210118e-31f : vs < least ? least : vs;
   lv = __builtin_amdgcn_logf(x);
   rv = __builtin_amdgcn_rcpf(x);
 }

@@ -436,8 +436,9 @@ srw_status_t srw_cast_bf16(int32_t n, const float* const* src, void* const* dst,
  * A layer's pages are four arrays of the caller:
  *   k [n_pages, n_kv_heads, page_size, head_dim]
  *   v [n_pages, n_kv_heads, head_dim, page_size]   (dimension by dimension)
- *   k_scale, v_scale [n_pages, n_kv_heads, page_size] float32 (not negative), with 8-bit
- *     kinds
+ *   k_scale, v_scale [n_pages, n_kv_heads, page_size] float32 (not negative; a v_scale
+ *     between 0 and 2^-109, which srw_kv_write does not give, is read by srw_attention as
+ *     2^-109), with 8-bit kinds
  * Sequence b has lens[b] positions, the call's new tokens included: the last
  * cu[b + 1] - cu[b] of them, whose packed rows are [cu[b], cu[b + 1]) of T
  * (cu[0] = 0, cu[B] = T); cu NULL: one new token each, T = B.  Position p is

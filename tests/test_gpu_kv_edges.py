@@ -72,3 +72,43 @@ def test_infinite_values(pkg, dev, dh, G, n, past):
     fine = torch.isfinite(want)
     assert ((got - want).abs() <= BAR * mag)[fine].all()
     assert torch.equal(got[~fine].nan_to_num(7.0, 1e300, -1e300), want[~fine].nan_to_num(7.0, 1e300, -1e300))
+
+
+def _wide(c, width):
+    """The table with unused entries behind it: calls of few tokens then take the
+    kernel for many rows."""
+    t = torch.full((c.table.shape[0], width), -1, dtype=I32, device=c.table.device)
+    t[:, :c.table.shape[1]] = c.table
+    return t
+
+
+# single tokens, split over a long axis, 32 rows a workgroup, 128
+SHAPES = [(1, 300, 1, 0), (1, 9001, 2, 0), (20, 300, 1, 0), (200, 300, 2, 400)]
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("n,past,G,width", SHAPES, ids=str)
+@pytest.mark.parametrize("beside", [False, True], ids=["alone", "beside"])
+def test_smallest_value_rows(pkg, dev, kind, n, past, G, width, beside):
+    """Value rows from the smallest that is not held as zeros on, whose scales lie
+    under 2^-100: attention reads them as they are read back.  Their weights'
+    exponents are about 110, kept to 2^-18: within the bound's 3e-4."""
+    print(f"[gpu] attention smallest value rows {kind} n{n} past{past} {beside}", flush=True)
+    L = past + n
+    c = Cache(pkg, dev, kind, 1, 64, 64, [L], seed=221)
+    g = torch.Generator().manual_seed(222)
+    k, v = (torch.randn(L, 1, 64, generator=g) for _ in range(2))
+    v = v / v.abs().amax(-1, keepdim=True)
+    size = torch.tensor([1.001 * 2.0 ** -100, 2.0 ** -99, 2.0 ** -95, 2.0 ** -92, 0.0])[torch.arange(L) % 5]
+    if beside:
+        size[::7] = 1.0
+    v = v * size[:, None, None]
+    q = torch.randn(n, G, 64, generator=g).to(BF)
+    pkg.kv_write(c.pages, k.to(dev), v.to(dev), c.table, c.len_t, _cu(dev, [L]))
+    table = _wide(c, width) if width else c.table
+    got = pkg.paged_attention(q.to(dev), c.pages, table, c.len_t, _cu(dev, [n]), max_new=n).cpu().to(F64)
+    kk, vv = c.held(0)
+    want, mag = _attend64(q, kk, vv, past, 0.125, 0, 0)
+    assert (mag > 0).all()
+    err = ((got - want).abs() / mag).max()
+    assert err <= BAR, float(err)
