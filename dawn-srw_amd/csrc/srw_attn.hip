@@ -32,11 +32,12 @@
 // What a token must not see is left out by selects, not by adding numbers;
 // positions without a page (a table entry that names none, as for positions
 // that a window has left behind) are not seen, and value bytes that no token
-// of a tile sees are cleared before the product, since 0 x NaN is NaN.  bf16
-// values that are not finite are kept out of the product too, where the tokens of
-// a tile see different keys or weights come in two parts, and added to the tokens
-// that see them (8-bit values are finite; their scales, which may not be, multiply
-// weights, which are a token's own).  A token that sees nothing gets zeros.
+// of a tile sees are cleared before the product, since 0 x NaN is NaN.  A token
+// that sees nothing gets zeros.
+//
+// Scores beyond +-4096, whose last bits are no longer small beside 1, and values
+// that are not finite are rare, and the loops carry nothing for them: a wave that
+// ends with either goes over its tiles again (careful_rows).
 
 #include <math.h>
 
@@ -49,7 +50,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;
 constexpr float kLazy = 8.f;       // log2 of the largest weight before m is raised
-constexpr float kLowest = -1e30f;  // m of a row that has seen nothing
+constexpr float kLowest = -INFINITY;  // m of a row that has seen nothing, or scores of -inf only
+constexpr float kLarge = 4096.f;      // an m whose last bit, 2^-11, moves a weight by under 2e-4
 
 struct AttnArgs {
   KvView kv;
@@ -202,11 +204,8 @@ __device__ inline void in_exponent(float vs, float& lv, float& rv) {
   lv = __builtin_amdgcn_logf(x);
   rv = __builtin_amdgcn_rcpf(x);
 }
-// m after a tile whose largest exponent over m (over 0 at first) is mt.
-__device__ inline float raised(float m, float mt) {
-  if (m == kLowest) return mt == -INFINITY ? kLowest : mt;
-  return mt > 0.f ? m + mt : m;
-}
+// What sums under the maximum m are worth under mn, which is not lower.
+__device__ inline float lowered(float m, float mn) { return m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn); }
 __device__ inline u32x4_t ld16(const void* p) { return *static_cast<const u32x4_t*>(p); }
 
 // The largest magnitude among bf16 pairs, as bits: 0x7f80 and above is not
@@ -228,23 +227,28 @@ __device__ inline u32x4_t finite16(u32x4_t x) {
   }
   return x;
 }
-// Adds to o the values that are not finite of the tile's positions for which
-// see(k) holds; value(d) gives the dim of o[d].  Rare: one load each.
-template <int N, class See, class Dim, class Acc>
+// Adds the values that are not finite of the tile's positions for which see(k)
+// holds: add(i, value) of dim(i).  Rare: one load each.
+template <int KIND, int N, class See, class Dim, class Acc>
 __device__ inline void add_not_finite(const KvView& kv, int64_t b, int h, int head_dim, int key0, See see, Dim dim,
                                       Acc add) {
   for (int k = 0; k < kTile; ++k) {
     const int pg = kv_page(kv, b, key0 + k);
     if (pg < 0 || !see(k)) continue;
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(kv.v) +
-                          (static_cast<int64_t>(pg) * kv.H + h) * head_dim * kv.P + ((key0 + k) & (kv.P - 1));
+    const char* src = kv.v + ((static_cast<int64_t>(pg) * kv.H + h) * head_dim * kv.P + ((key0 + k) & (kv.P - 1))) *
+                                 kv_bytes<KIND>();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       // one address and one load after the other: their registers are the kernel's
       int at = dim(i);
       asm volatile("" : "+v"(at) : : "memory");
-      const float x = bf16_to_f32(src[static_cast<int64_t>(at) * kv.P]);
-      if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) add(i, x);
+      const char* p = src + static_cast<int64_t>(at) * kv.P * kv_bytes<KIND>();
+      if constexpr (KIND == SRW_KV_BF16) {
+        const float x = bf16_to_f32(*reinterpret_cast<const uint16_t*>(p));
+        if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) add(i, x);
+      } else {
+        if ((*p & 0x7f) == 0x7f) add(i, __uint_as_float(0x7fc00000u));
+      }
     }
   }
 }
@@ -258,53 +262,92 @@ __device__ inline void for16(F f) {
   each16(f, std::make_integer_sequence<int, 16>{});
 }
 
+template <int ND>
+__device__ inline void rescale(f32x4_t (&o)[ND], float w) {
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) o[d][v] *= w;
+}
+__device__ inline float largest16(const float (&t)[16]) {
+  float r = t[0];
+#pragma unroll
+  for (int j = 1; j < 16; ++j) r = fmaxf(r, t[j]);
+  return r;
+}
+
 // The scores of a tile become weights.  A lane holds 16 scores of one token (of
 // lane & 15), those of the keys 16 g + j, g = lane >> 4, as acc[j / 4][j % 4];
 // scales of the tile's key k lie in lane k.  whole: every token sees every
 // key, else bit j of `mine` says whether the lane's token sees key 16 g + j.
 // pf gets the weights rounded to bf16, with TWO pl what the rounding left.
-template <int KIND, int ND, bool TWO>
+// CAREFUL: for scores of any size (careful_again).  Scores are rounded, and
+// compared over m or the largest of them, before value scales come in.
+template <int KIND, int ND, bool TWO, bool CAREFUL = false>
 __device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, float rvl, bool whole, uint32_t mine,
                              float& m, float& l, f32x4_t (&o)[ND], u32x4_t (&pf)[2], u32x4_t (&pl)[2]) {
   // exponents, over m (0 while the token has seen nothing)
   float t[16];
-  const float mu = m == kLowest ? 0.f : m;
-  if constexpr (KIND == SRW_KV_BF16) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) t[j] = fmaf(acc[j >> 2][j & 3], sc, -mu);
-  } else {
-    float s[16];
-    settled(acc);
-    for16([&](auto jt) {
-      constexpr int j = decltype(jt)::value;
-      s[j] = acc[j >> 2][j & 3];
-      t[j] = row_lane<j>(lvl) - mu;
-    });
-    fma_lanes8<0>(t, ksl, s);
-    fma_lanes8<8>(t + 8, ksl, s + 8);
-  }
-  if (!whole) {
+  auto mx = [](float u, float w) { return fmaxf(u, w); };
+  auto mask = [&] {
+    if (whole) return;
     for16([&](auto jt) {
       constexpr int j = decltype(jt)::value;
       t[j] = only<j>(mine, t[j]);
     });
-  }
-  float mt = t[0];
-#pragma unroll
-  for (int j = 1; j < 16; ++j) mt = fmaxf(mt, t[j]);
-  if (__any(mt > (m == kLowest ? -INFINITY : kLazy))) {
-    auto mx = [](float u, float w) { return fmaxf(u, w); };
-    mt = join32(join16(mt, mx), mx);
-    const float mn = raised(m, mt), back = (mn == kLowest ? 0.f : mn) - mu;
-    const float w = __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
+  };
+  const float mu = m == kLowest ? 0.f : m;
+  if constexpr (CAREFUL) {
+    for16([&](auto jt) {
+      constexpr int j = decltype(jt)::value;
+      t[j] = acc[j >> 2][j & 3] * (KIND == SRW_KV_BF16 ? sc : row_lane<j>(ksl));
+    });
+    mask();
+    float mt = join32(join16(largest16(t), mx), mx);
+    const float r = fabsf(m) <= kLarge ? m : fmaxf(m, mt), rz = r == kLowest ? 0.f : r;
+    for16([&](auto jt) {
+      constexpr int j = decltype(jt)::value;
+      t[j] -= rz;
+      if constexpr (KIND != SRW_KV_BF16) t[j] += row_lane<j>(lvl);
+    });
+    mask();
+    mt = join32(join16(largest16(t), mx), mx);
+    // (a large r does not resolve what value scales add)
+    const float up = !(fabsf(r) <= kLarge) ? 0.f : m == kLowest ? mt : fmaxf(mt, 0.f);
+    const float w = __builtin_amdgcn_exp2f((m == r ? 0.f : m - r) - up);
+    m = r + up;
     l *= w;
+    rescale(o, w);
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int j = 0; j < 16; ++j) t[j] -= up;
+  } else {
+    if constexpr (KIND == SRW_KV_BF16) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) o[d][v] *= w;
+      for (int j = 0; j < 16; ++j) t[j] = fmaf(acc[j >> 2][j & 3], sc, -mu);
+    } else {
+      float s[16];
+      settled(acc);
+      for16([&](auto jt) {
+        constexpr int j = decltype(jt)::value;
+        s[j] = acc[j >> 2][j & 3];
+        t[j] = row_lane<j>(lvl) - mu;
+      });
+      fma_lanes8<0>(t, ksl, s);
+      fma_lanes8<8>(t + 8, ksl, s + 8);
+    }
+    mask();
+    float mt = largest16(t);
+    if (__any(mt > (m == kLowest ? -INFINITY : kLazy))) {
+      mt = join32(join16(mt, mx), mx);
+      const bool none = mt == -INFINITY;
+      const float up = m == kLowest ? (none ? 0.f : mt) : fmaxf(mt, 0.f);
+      m = m == kLowest && none ? kLowest : mu + up;
+      const float w = __builtin_amdgcn_exp2f(-fmaxf(up, 0.f));  // (nothing yet: of zeros)
+      l *= w;
+      rescale(o, w);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) t[j] -= back;
+      for (int j = 0; j < 16; ++j) t[j] -= up;
+    }
   }
 #pragma unroll
   for (int j = 0; j < 16; ++j) t[j] = __builtin_amdgcn_exp2f(t[j]);
@@ -328,6 +371,114 @@ __device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, 
       pf[st][u] = hi;
       if constexpr (TWO) pl[st][u] = pack_bf16(p0 - lo_f32(hi), p1 - hi_f32(hi));
     }
+}
+
+// A wave's rows, up to 16 from r0 on, over the tiles first, first + step, ... < end
+// of a span, for scores and values of any size: straight from memory, a fragment
+// at a time.  Values that are not finite are kept out of the products and added
+// to the rows that see them.
+template <int KIND, int DH>
+__device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const Span& sp, int h, int r0, int r1, int first,
+                                    int end, int step, float& m, float& l, f32x4_t (&o)[DH / 16]) {
+  constexpr int ES = kv_bytes<KIND>();
+  constexpr int ND = DH / 16;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const KvSeq& sq = tl.sq;
+  const int P = a.kv.P, fr = r0 + col;
+  const bool in = fr < r1;
+  const int tok = in ? fr / a.G : 0, pos = in ? sq.len - sq.n + tok : -1;
+  const uint16_t* src = a.q + (sq.row0 + tok) * a.q_token + (h * a.G + (in ? fr - tok * a.G : 0)) * a.q_head;
+  m = kLowest;
+  l = 0.f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int i = first; i < end; i += step) {
+    const int key0 = sp.key0(i);
+    // (rows of the first product as in attn_rows_kernel)
+    const int kk = key0 + 16 * (col >> 2), kv = key0 + 16 * g;
+    int pk = kk < sp.hi ? kv_page(a.kv, tl.b, kk) : -1, pv = kv < sp.hi ? kv_page(a.kv, tl.b, kv) : -1;
+    const uint32_t mine =
+        pv < 0 ? 0u : static_cast<uint32_t>(seen_of(pos, key0, a.window, a.sinks) >> (16 * g)) & 0xffffu;
+    pk = pk < 0 ? 0 : pk;
+    pv = pv < 0 ? 0 : pv;
+    const int64_t hk = static_cast<int64_t>(pk) * a.kv.H + h, hv = static_cast<int64_t>(pv) * a.kv.H + h;
+    const char* ksrc = a.kv.k + (hk * P + (kk & (P - 1)) + (col & 3)) * (DH * ES) + 16 * g;
+    const char* vsrc = a.kv.v + ((hv * DH + col) * P + (kv & (P - 1))) * ES;
+    f32x4_t acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < DH * ES / 64; ++j) {
+        const u32x4_t k = ld16(ksrc + 4 * t * (DH * ES) + 64 * j);
+        if constexpr (KIND == SRW_KV_BF16) {
+          acc[t] = mfma16(k, in ? ld16(src + 32 * j + 8 * g) : u32x4_t{0, 0, 0, 0}, acc[t]);
+        } else {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            acc[t] = mfma16(widen8<KIND>(k[2 * s], k[2 * s + 1]),
+                            in ? ld16(src + 64 * j + 16 * g + 8 * s) : u32x4_t{0, 0, 0, 0}, acc[t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    float ksl = 0.f, lvl = 0.f, rvl = 0.f;
+    if constexpr (KIND != SRW_KV_BF16) {
+      ksl = a.kv.ks[hv * P + (kv & (P - 1)) + col] * a.sc;
+      in_exponent(a.kv.vs[hv * P + (kv & (P - 1)) + col], lvl, rvl);
+    }
+    u32x4_t pf[2], pl[2];
+    weigh<KIND, ND, true, true>(acc, a.sc, ksl, lvl, rvl, false, mine, m, l, o, pf, pl);
+    uint32_t seen = mine;  // bit j: some row sees the lane's key kv + j
+    for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);
+    u16x2_t most = {0, 0};
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const char* at = vsrc + static_cast<int64_t>(16 * d) * P * ES;
+      u32x4_t raw = ld16(at);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        u32x4_t v;
+        if constexpr (KIND == SRW_KV_BF16)
+          v = st ? ld16(at + 16) : raw;
+        else
+          v = widen8<KIND>(raw[2 * st], raw[2 * st + 1]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t two = seen >> (8 * st + 2 * u);
+          v[u] &= (two & 1 ? 0x0000ffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+        }
+        if constexpr (KIND != SRW_KV_INT8) {
+          most = most16(most, v);
+          v = finite16(v);
+        }
+        o[d] = mfma16(v, pl[st], mfma16(v, pf[st], o[d]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (KIND != SRW_KV_INT8) {
+      if (__any(not_finite(most)))
+        add_not_finite<KIND, 4 * ND>(
+            a.kv, tl.b, h, DH, key0, [&](int k) { return seen_of(pos, key0, a.window, a.sinks) >> k & 1; },
+            [&](int n) { return 16 * (n / 4) + 4 * g + n % 4; }, [&](int n, float v) { o[n / 4][n % 4] += v; });
+    }
+  }
+}
+
+// Whether a wave's rows have to be walked again, by careful_rows: m is so large
+// that a product (exact) and m (rounded) do not cancel, that 2^(product - m) could
+// be anything and log2 vs is lost beside m; or a sum is not finite, as such weights
+// or values leave it (an infinity times what is left of a weight, zero or negative,
+// is NaN, and so is zero times one that a row does not see).
+template <int ND>
+__device__ inline bool careful_again(float m, float l, const f32x4_t (&o)[ND]) {
+  f32x4_t none = {l * 0.f, 0.f, 0.f, 0.f};  // NaN once a sum is not finite
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) none[v] = fmaf(o[d][v], 0.f, none[v]);
+  const bool odd = none[0] + none[1] + none[2] + none[3] != 0.f;
+  return __any(odd || (fabsf(m) > kLarge && m != kLowest));
 }
 
 // -- few rows: single tokens, short chunks -----------------------------------
@@ -387,13 +538,6 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
     }
   }
 
-  // apart: bf16 values that are not finite are kept out of the products (an
-  // infinity times what is left of a weight, zero or negative, would be NaN, and
-  // so would zero times one that a row does not see) and added to the rows that
-  // see them.  They are rare and leave a sum that is not finite: only a wave that
-  // ends with one goes over its tiles so, once more.
-  bool apart = false;
-again:
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
     m[x] = kLowest;
@@ -463,7 +607,6 @@ again:
       }
       weigh<KIND, ND, true>(acc[x], a.sc, ksl, lvl, rvl, whole, mine, m[x], l[x], o[x], pf[x], pl[x]);
     }
-    bool odd = false;  // a value is not finite
     if (!whole && KIND != SRW_KV_INT8) {
       for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);  // over the columns: keys that some row sees
 #pragma unroll
@@ -479,20 +622,6 @@ again:
         for (int d = 0; d < ND; ++d) vf[d][u / 4][u % 4] &= keep;
       }
     }
-    if (KIND == SRW_KV_BF16 && apart) {
-      u16x2_t most = {0, 0};
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int j = 0; j < ES; ++j) most = most16(most, vf[d][j]);
-      odd = __any(not_finite(most));
-      if (odd) {
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int j = 0; j < ES; ++j) vf[d][j] = finite16(vf[d][j]);
-      }
-    }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
 #pragma unroll
@@ -506,27 +635,11 @@ again:
         for (int x = 0; x < NQ; ++x) o[x][d] = mfma16(vb, pl[x][st], mfma16(vb, pf[x][st], o[x][d]));
       }
     }
-    if (KIND == SRW_KV_BF16 && odd) {
-#pragma unroll
-      for (int x = 0; x < NQ; ++x)
-        add_not_finite<4 * ND>(
-            a.kv, b, h, DH, key0,
-            [&](int k) { return seen_of(pos[x], key0, a.window, a.sinks) >> k & 1; },
-            [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, [&](int i, float v) { o[x][i / 4][i % 4] += v; });
-    }
   }
 
-  if (KIND == SRW_KV_BF16 && !apart) {
-    float none = 0.f;  // NaN once a sum is not finite
 #pragma unroll
-    for (int x = 0; x < NQ; ++x)
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) none = fmaf(o[x][d][v], 0.f, none);
-    apart = __any(none != none);
-    if (apart) goto again;
-  }
+  for (int x = 0; x < NQ; ++x)
+    if (careful_again(m[x], l[x], o[x])) careful_rows<KIND, DH>(a, tl, sp, h, r0 + 16 * x, r1, i0 + wave, i1, 4, m[x], l[x], o[x]);
 
   // join the four waves
   auto sum = [](float u, float w) { return u + w; };
@@ -557,7 +670,7 @@ again:
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         // (a wave without visible keys has l = 0)
-        const float e = sm[w][r] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[w][r] - mm);
+        const float e = lowered(sm[w][r], mm);
         ll += sl[w][r] * e;
 #pragma unroll
         for (int d = 0; d < ND; ++d) ov[d] += so[w][r][c + d] * e;
@@ -619,8 +732,7 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
     for (int u = 0; u < U; ++u) {
       if (s0 + W * u >= S || x[u].y == 0.f) continue;
       const float mn = fmaxf(m, x[u].x);
-      const float e0 = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      const float e1 = x[u].x == mn ? 1.f : __builtin_amdgcn_exp2f(x[u].x - mn);
+      const float e0 = lowered(m, mn), e1 = lowered(x[u].x, mn);
       m = mn;
       l = l * e0 + x[u].y * e1;
 #pragma unroll
@@ -644,7 +756,7 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
     o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < W; ++g) {
-      const float e = sm[first + g] == m ? 1.f : __builtin_amdgcn_exp2f(sm[first + g] - m);
+      const float e = lowered(sm[first + g], m);
       l += sl[first + g] * e;
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[k] += so[first + g][c][k] * e;
@@ -946,17 +1058,6 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
     }
     u32x4_t pf[2], pl[2];
     weigh<KIND, ND, false>(acc, a.sc, ksl, lvl, rvl, whole, mine, m, l, o, pf, pl);
-    bool odd = false;  // a value is not finite
-    if (KIND == SRW_KV_BF16 && !whole) {
-      u16x2_t most = {0, 0};
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const char* src = vl[stage] + (16 * d + fc) * 128;
-        most = most16(most16(most, ld16(src + 16 * ((2 * fg) ^ v_swz(fc)))), ld16(src + 16 * ((2 * fg + 1) ^ v_swz(fc))));
-        if (d % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-      }
-      odd = __any(not_finite(most));
-    }
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += kBatch / 2) {
       u32x4_t vf[kBatch / 2][2];
@@ -966,8 +1067,7 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
         for (int st = 0; st < 2; ++st)
           vf[d][st] = ld16(vl[stage] + (16 * (d0 + d) + fc) * 128 + 16 * ((2 * fg + st) ^ v_swz(fc)));
       __builtin_amdgcn_sched_barrier(0);
-      if (KIND == SRW_KV_BF16 && (keys != ~0ull || odd)) {
-        // values that no row sees cleared, values that are not finite kept apart
+      if (KIND == SRW_KV_BF16 && keys != ~0ull) {  // values that no row sees
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const uint32_t bits = static_cast<uint32_t>(keys >> (16 * g + 8 * st)) & 0xffu;
@@ -977,26 +1077,16 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
             for (int d = 0; d < kBatch / 2; ++d) vf[d][st][u] &= keep;
           }
-#pragma unroll
-          for (int d = 0; d < kBatch / 2; ++d) {
-            vf[d][st] = finite16(vf[d][st]);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
+       }
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int d = 0; d < kBatch / 2; ++d) o[d0 + d] = mfma16(vf[d][st], pf[st], o[d0 + d]);
     }
-    if (KIND == SRW_KV_BF16 && odd) {
-      const int pos = place().pos;
-      add_not_finite<4 * ND>(
-          a.kv, b, h, DH, key0, [&](int k) { return seen_of(pos, key0, a.window, a.sinks) >> k & 1; },
-          [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, [&](int i, float v) { o[i / 4][i % 4] += v; });
-    }
   }
   if (!active) return;
+  if (careful_again(m, l, o)) careful_rows<KIND, DH>(a, tl, sp, h, w0, r1, i0, i1, 1, m, l, o);
   auto sum = [](float u, float w) { return u + w; };
   l = join32(join16(l, sum), sum);
   const Place p = place();

@@ -112,3 +112,53 @@ def test_smallest_value_rows(pkg, dev, kind, n, past, G, width, beside):
     assert (mag > 0).all()
     err = ((got - want).abs() / mag).max()
     assert err <= BAR, float(err)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,past,G,width", SHAPES, ids=str)
+@pytest.mark.parametrize("zero", [None, 0, 290], ids=str)
+def test_scores_far_below_zero(pkg, dev, kind, n, past, G, width, zero):
+    """Finite scores of -1.2e31 and -2.3e31 (in units of log2), alone and with one
+    of zero among them: equal keys weigh the same, the others nothing."""
+    print(f"[gpu] attention low scores {kind} n{n} past{past} {zero}", flush=True)
+    L = past + n
+    c = Cache(pkg, dev, kind, 1, 64, 64, [L], seed=231)
+    g = torch.Generator().manual_seed(232)
+    k = torch.full((L, 1, 64), 2.0 ** 50)
+    k[1::3] *= 2
+    if zero is not None:
+        k[zero] = 0
+    v = torch.randn(L, 1, 64, generator=g)
+    q = torch.full((n, G, 64), -2.0 ** 50).to(BF)
+    pkg.kv_write(c.pages, k.to(dev), v.to(dev), c.table, c.len_t, _cu(dev, [L]))
+    table = _wide(c, width) if width else c.table
+    got = pkg.paged_attention(q.to(dev), c.pages, table, c.len_t, _cu(dev, [n]), max_new=n).cpu().to(F64)
+    kk, vv = c.held(0)
+    kk = k.to(F64)                                           # 127 or 448 times a scale is off by a rounding, the same for all
+    want, mag = _attend64(q, kk, vv, past, 0.125, 0, 0)
+    assert ((got - want).abs() <= BAR * mag).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,past,G,width", SHAPES, ids=str)
+@pytest.mark.parametrize("size", [3, 4, 6, 9, 12, 16, 18, 30, 50])
+def test_equal_keys_weigh_the_same_at_any_size_of_scores(pkg, dev, kind, n, past, G, width, size):
+    """Two groups of equal keys, at scores of 22 x 4^size (in units of log2) of
+    either sign whose products take more bits than float32 holds: the larger
+    group's members share the weight, in every tile, split and wave alike."""
+    print(f"[gpu] attention scores of 22 x 4^{size} {kind} n{n} past{past}", flush=True)
+    L = past + n
+    c = Cache(pkg, dev, kind, 1, 64, 64, [L], seed=271)
+    g = torch.Generator().manual_seed(272)
+    k = torch.full((L, 1, 64), 1.5 * 2.0 ** size)
+    k[1::3] = 1.25 * 2.0 ** size
+    v = torch.randn(L, 1, 64, generator=g) * torch.exp(torch.randn(L, 1, 1, generator=g))
+    pkg.kv_write(c.pages, k.to(dev), v.to(dev), c.table, c.len_t, _cu(dev, [L]))
+    table = _wide(c, width) if width else c.table
+    _, vv = c.held(0)
+    for sign in (1, -1):
+        q = torch.full((n, G, 64), sign * 1.25 * 2.0 ** size).to(BF)
+        got = pkg.paged_attention(q.to(dev), c.pages, table, c.len_t, _cu(dev, [n]), max_new=n).cpu().to(F64)
+        want, mag = _attend64(q, k.to(F64), vv, past, 0.125, 0, 0)
+        err = ((got - want).abs() / mag).max()
+        assert err <= BAR, (sign, float(err))
