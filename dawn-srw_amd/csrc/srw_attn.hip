@@ -48,7 +48,6 @@ namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 64;
 constexpr float kLazy = 8.f;       // log2 of the largest weight before m is raised
 constexpr float kLowest = -INFINITY;  // m of a row that has seen nothing, or scores of -inf only
 constexpr float kLarge = 4096.f;      // an m whose last bit, 2^-11, moves a weight by under 2e-4
@@ -65,25 +64,8 @@ struct AttnArgs {
   int S, least;   // splits of a row tile's key tiles, of so many at least
 };
 
-// The tiles that rows at positions [p_lo, p_hi] see: those of the first
-// tokens, then those of the window.
-struct Span {
-  int lo, hi, sink_tiles, skip, tiles;  // window positions [lo, hi)
-  __device__ int key0(int i) const { return (i < sink_tiles ? i : i + skip) * kTile; }
-};
-__device__ inline Span span_of(const AttnArgs& a, int p_lo, int p_hi) {
-  Span s;
-  s.hi = p_hi + 1 < a.kv.cap ? p_hi + 1 : a.kv.cap;
-  if (s.hi < 0) s.hi = 0;
-  s.lo = a.window > 0 && p_lo - a.window + 1 > 0 ? p_lo - a.window + 1 : 0;
-  const int sinks = a.sinks < s.lo ? a.sinks : s.lo;
-  const int t1 = (s.hi + kTile - 1) / kTile;
-  s.sink_tiles = (sinks + kTile - 1) / kTile;
-  if (s.sink_tiles > t1) s.sink_tiles = t1;
-  const int t0 = s.lo / kTile > s.sink_tiles ? s.lo / kTile : s.sink_tiles;
-  s.skip = t0 - s.sink_tiles;
-  s.tiles = s.sink_tiles + (t1 > t0 ? t1 - t0 : 0);
-  return s;
+__device__ inline KvSpan span_of(const AttnArgs& a, int p_lo, int p_hi) {
+  return kv_span(a.kv.cap, a.window, a.sinks, p_lo, p_hi);
 }
 
 // Tiles of a split, of the row tile's own number: a table far wider than a
@@ -125,15 +107,6 @@ __device__ inline Tile tile_of(const AttnArgs& a, int64_t at) {
 __device__ inline f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
-}
-// The low n bits.
-__device__ inline uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
-// The tile's keys (bit k: position key0 + k) that a token at position pos sees.
-__device__ inline uint64_t seen_of(int pos, int key0, int window, int sinks) {
-  const int rel = pos - key0;
-  uint64_t see = low_bits(rel + 1);
-  if (window > 0) see &= ~low_bits(rel - window + 1) | low_bits(sinks - key0);
-  return see;
 }
 // All ones where bit n of w is set, else zero; v there, else -inf.
 template <int N>
@@ -378,7 +351,7 @@ __device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, 
 // at a time.  Values that are not finite are kept out of the products and added
 // to the rows that see them.
 template <int KIND, int DH>
-__device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const Span& sp, int h, int r0, int r1, int first,
+__device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvSpan& sp, int h, int r0, int r1, int first,
                                     int end, int step, float& m, float& l, f32x4_t (&o)[DH / 16]) {
   constexpr int ES = kv_bytes<KIND>();
   constexpr int ND = DH / 16;
@@ -398,7 +371,7 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const Spa
     const int kk = key0 + 16 * (col >> 2), kv = key0 + 16 * g;
     int pk = kk < sp.hi ? kv_page(a.kv, tl.b, kk) : -1, pv = kv < sp.hi ? kv_page(a.kv, tl.b, kv) : -1;
     const uint32_t mine =
-        pv < 0 ? 0u : static_cast<uint32_t>(seen_of(pos, key0, a.window, a.sinks) >> (16 * g)) & 0xffffu;
+        pv < 0 ? 0u : static_cast<uint32_t>(kv_seen(pos, key0, a.window, a.sinks) >> (16 * g)) & 0xffffu;
     pk = pk < 0 ? 0 : pk;
     pv = pv < 0 ? 0 : pv;
     const int64_t hk = static_cast<int64_t>(pk) * a.kv.H + h, hv = static_cast<int64_t>(pv) * a.kv.H + h;
@@ -459,7 +432,7 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const Spa
     if constexpr (KIND != SRW_KV_INT8) {
       if (__any(not_finite(most)))
         add_not_finite<KIND, 4 * ND>(
-            a.kv, tl.b, h, DH, key0, [&](int k) { return seen_of(pos, key0, a.window, a.sinks) >> k & 1; },
+            a.kv, tl.b, h, DH, key0, [&](int k) { return kv_seen(pos, key0, a.window, a.sinks) >> k & 1; },
             [&](int n) { return 16 * (n / 4) + 4 * g + n % 4; }, [&](int n, float v) { o[n / 4][n % 4] += v; });
     }
   }
@@ -514,7 +487,7 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
   const int r0 = tl.r0, r1 = tl.r1;
   const int P = a.kv.P;
   const int p_lo = sq.len - sq.n + r0 / a.G, p_hi = sq.len - sq.n + (r1 - 1) / a.G;
-  const Span sp = span_of(a, p_lo, p_hi);
+  const KvSpan sp = span_of(a, p_lo, p_hi);
   const int per = per_split(a, sp.tiles);
   const int i0 = split * per;
   const int i1 = i0 + per < sp.tiles ? i0 + per : sp.tiles;
@@ -602,7 +575,7 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
     for (int x = 0; x < NQ; ++x) {
       uint32_t mine = 0xffffu;
       if (!whole) {
-        mine = have ? static_cast<uint32_t>(seen_of(pos[x], key0, a.window, a.sinks) >> (16 * g)) & 0xffffu : 0u;
+        mine = have ? static_cast<uint32_t>(kv_seen(pos[x], key0, a.window, a.sinks) >> (16 * g)) & 0xffffu : 0u;
         seen |= mine;
       }
       weigh<KIND, ND, true>(acc[x], a.sc, ksl, lvl, rvl, whole, mine, m[x], l[x], o[x], pf[x], pl[x]);
@@ -815,7 +788,7 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
   const int64_t b = tl.b;
   const KvSeq sq = tl.sq;
   const int r0 = tl.r0, r1 = tl.r1;
-  const Span sp = span_of(a, sq.len - sq.n + r0 / a.G, sq.len - sq.n + (r1 - 1) / a.G);
+  const KvSpan sp = span_of(a, sq.len - sq.n + r0 / a.G, sq.len - sq.n + (r1 - 1) / a.G);
   const int per = per_split(a, sp.tiles);
   const int i0 = split * per;
   const int i1 = i0 + per < sp.tiles ? i0 + per : sp.tiles;
@@ -1054,7 +1027,7 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
     uint32_t mine = 0xffffu;
     if (!whole) {
       keys = seen_by_any(key0, hav);
-      mine = static_cast<uint32_t>((seen_of(place().pos, key0, a.window, a.sinks) & keys) >> (16 * g)) & 0xffffu;
+      mine = static_cast<uint32_t>((kv_seen(place().pos, key0, a.window, a.sinks) & keys) >> (16 * g)) & 0xffffu;
     }
     u32x4_t pf[2], pl[2];
     weigh<KIND, ND, false>(acc, a.sc, ksl, lvl, rvl, whole, mine, m, l, o, pf, pl);

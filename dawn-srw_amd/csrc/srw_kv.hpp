@@ -95,6 +95,41 @@ __host__ __device__ inline int kv_in_run(const KvRun& k, int i) {
   return i < k.first ? k.first : i >= k.last ? k.last - 1 : i;
 }
 
+constexpr int kTile = 64;  // positions that the attention takes at a time
+
+// The low n bits.
+__host__ __device__ inline uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
+// The tiles that rows at positions [p_lo, p_hi] see of cap positions: those of the
+// first tokens, then those of the window.
+struct KvSpan {
+  int lo, hi, sink_tiles, skip, tiles;  // window positions [lo, hi)
+  __host__ __device__ int key0(int i) const { return (i < sink_tiles ? i : i + skip) * kTile; }
+};
+__host__ __device__ inline KvSpan kv_span(int cap, int window, int first, int p_lo, int p_hi) {
+  KvSpan s;
+  s.hi = p_hi < cap ? p_hi + 1 : cap;
+  if (s.hi < 0) s.hi = 0;
+  // (p_lo may be far below 0, and window 2^31 - 1)
+  s.lo = window > 0 && p_lo >= window ? p_lo - window + 1 : 0;
+  const int sinks = first < s.lo ? first : s.lo;
+  const int t1 = (s.hi + kTile - 1) / kTile;
+  s.sink_tiles = (sinks + kTile - 1) / kTile;
+  if (s.sink_tiles > t1) s.sink_tiles = t1;
+  const int t0 = s.lo / kTile > s.sink_tiles ? s.lo / kTile : s.sink_tiles;
+  s.skip = t0 - s.sink_tiles;
+  s.tiles = s.sink_tiles + (t1 > t0 ? t1 - t0 : 0);
+  return s;
+}
+// The tile's keys (bit k: position key0 + k) that a token at position pos sees.
+__host__ __device__ inline uint64_t kv_seen(int pos, int key0, int window, int sinks) {
+  if (pos < key0) return 0;
+  const int rel = pos - key0;
+  uint64_t see = low_bits(rel + 1);
+  if (window > 0) see &= ~low_bits(rel - window + 1) | low_bits(sinks - key0);
+  return see;
+}
+
 // The page of position pos of sequence b, or -1: past the table, or an entry
 // that names no page.
 __device__ inline int kv_page(const KvView& p, int64_t b, int pos) {

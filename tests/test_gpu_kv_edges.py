@@ -162,3 +162,22 @@ def test_equal_keys_weigh_the_same_at_any_size_of_scores(pkg, dev, kind, n, past
         want, mag = _attend64(q, k.to(F64), vv, past, 0.125, 0, 0)
         err = ((got - want).abs() / mag).max()
         assert err <= BAR, (sign, float(err))
+
+
+@pytest.mark.parametrize("sinks", [0, 4])
+@pytest.mark.parametrize("width", [0, 2048])
+def test_the_largest_window_hides_nothing(pkg, dev, sinks, width):
+    """A window of 2^31 - 1, also for a call with rows before the first position."""
+    print(f"[gpu] attention largest window sinks {sinks} width {width}", flush=True)
+    n, L = 90, 80
+    c = Cache(pkg, dev, "bf16", 1, 64, 64, [L], seed=241)
+    g = torch.Generator().manual_seed(242)
+    k, v = (torch.randn(L, 1, 64, generator=g).to(BF) for _ in range(2))
+    q = torch.randn(n, 1, 64, generator=g).to(BF).to(dev)
+    pkg.kv_write(c.pages, k.to(dev), v.to(dev), c.table, c.len_t, _cu(dev, [L]))
+    table = _wide(c, width) if width else c.table
+    want = pkg.paged_attention(q, c.pages, table, c.len_t, _cu(dev, [n]), max_new=n)
+    assert (want[:10] == 0).all() and (want[10:] != 0).any(-1).all()
+    for window in (1 << 20, (1 << 31) - 1):
+        got = pkg.paged_attention(q, c.pages, table, c.len_t, _cu(dev, [n]), max_new=n, window=window, sinks=sinks)
+        assert torch.equal(got, want), window

@@ -20,7 +20,8 @@ def program(tmp_path_factory):
         pytest.skip("needs hipcc")
     exe = tmp_path_factory.mktemp("kv_ranges") / "kv_ranges"
     root = os.path.dirname(HERE)
-    build = subprocess.run([HIPCC, "--offload-host-only", "-O1", "-std=c++17", "-Wall", "-Wno-unused-function",
+    build = subprocess.run([HIPCC, "--offload-host-only", "-O1", "-std=c++17",
+                            "-Xarch_host", "-fsanitize=undefined", "-Xarch_host", "-fno-sanitize-recover=all", "-Wall", "-Wno-unused-function",
                             "-I", os.path.join(root, "include"), "-I", os.path.join(root, "dawn-srw_amd", "csrc"),
                             os.path.join(HERE, "kv_ranges", "kv_ranges.hip"), "-o", str(exe)],
                            capture_output=True, text=True)
@@ -39,3 +40,9 @@ def test_rows_of_units_are_rows_of_the_call(program):
     only: none of a sequence without new tokens, whose neighbours' rows may end
     or begin the tensor."""
     _run(program, "rows")
+
+
+def test_spans_hold_what_rows_see(program):
+    """Tiles and keys of rows against the definition, with windows and first tokens
+    up to 2^31 - 1 and rows before the first position."""
+    _run(program, "spans")
