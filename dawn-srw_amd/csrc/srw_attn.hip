@@ -1094,7 +1094,7 @@ AttnPlan plan_of(const srw_attention_t& a) {
   const int64_t most = !a.kv.cu ? 1 : a.max_new > 0 ? a.max_new : T;
   int64_t keys = (a.kv.table_width * a.kv.page_size + kTile - 1) / kTile;  // key tiles of a row, at most
   if (a.window > 0) {
-    const int64_t w = (a.window + most + kTile - 1) / kTile + 1 + (a.sinks + kTile - 1) / kTile;
+    const int64_t w = (a.window + most + kTile - 1) / kTile + 1 + (int64_t{a.sinks} + kTile - 1) / kTile;
     keys = w < keys ? w : keys;
   }
   // 32 rows a workgroup also where more would leave the GPU idle: 512 tokens of 6

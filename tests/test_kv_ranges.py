@@ -46,3 +46,19 @@ def test_spans_hold_what_rows_see(program):
     """Tiles and keys of rows against the definition, with windows and first tokens
     up to 2^31 - 1 and rows before the first position."""
     _run(program, "spans")
+
+
+@pytest.mark.skipif(shutil.which("make") is None or not os.path.exists(HIPCC), reason="needs make and hipcc")
+def test_entry_points_clean_under_asan_ubsan():
+    """Descriptions, workspace sizes and refusals over the whole range of a call's
+    fields (tests/kv_ranges/kv_sanitize.c)."""
+    folder = os.path.join(HERE, "kv_ranges")
+    build = subprocess.run(["make", "-C", folder, "-j4"], capture_output=True, text=True)
+    assert build.returncode == 0, build.stdout[-2000:] + build.stderr[-2000:]
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=0:abort_on_error=1:verify_asan_link_order=0",
+               UBSAN_OPTIONS="print_stacktrace=1:halt_on_error=1")
+    run = subprocess.run([os.path.join(folder, "_build", "kv_sanitize")], capture_output=True, text=True, env=env,
+                         timeout=300)
+    out = run.stdout + run.stderr
+    assert run.returncode == 0 and " 0 failures" in out, out[-4000:]
+    assert "runtime error" not in out and "AddressSanitizer" not in out
