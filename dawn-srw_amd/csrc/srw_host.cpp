@@ -99,9 +99,12 @@ bool sequences(PyObject* table, PyObject* lens, PyObject* cu, int64_t T, int dev
   return true;
 }
 
-// Rows [T, heads, head_dim] as the kernels read them, unit elements at a time.
-bool rows(const at::Tensor* t, int64_t unit, int32_t head_dim) {
-  return t->size(2) == head_dim && t->stride(2) == 1 && t->stride(0) % unit == 0 && t->stride(1) % unit == 0 &&
+// Rows [T, heads, head_dim] as the kernels read them, unit elements at a time, and
+// their strides (that of a single token or head is never used, and may be anything).
+bool rows(const at::Tensor* t, int64_t unit, int32_t head_dim, int64_t* token, int64_t* head) {
+  *head = t->size(1) == 1 ? head_dim : t->stride(1);
+  *token = t->size(0) == 1 ? t->size(1) * head_dim : t->stride(0);
+  return t->size(2) == head_dim && t->stride(2) == 1 && *token % unit == 0 && *head % unit == 0 &&
          reinterpret_cast<uintptr_t>(t->data_ptr()) % (unit * t->element_size()) == 0;
 }
 
@@ -127,10 +130,11 @@ PyObject* host_write(PyObject* const* a, Py_ssize_t n) {
       wants_grad(k) || wants_grad(v))
     return none();
   const int64_t T = k->size(0);
-  if (v->size(0) != T || k->size(1) != c.n_kv_heads || v->size(1) != c.n_kv_heads || !rows(k, 4, c.head_dim) ||
-      !rows(v, 4, c.head_dim) || !sequences(a[3], a[4], a[5], T, device, &c))
+  srw_kv_rows_t r{k->data_ptr(), v->data_ptr(), 0, 0, 0, 0};
+  if (v->size(0) != T || k->size(1) != c.n_kv_heads || v->size(1) != c.n_kv_heads ||
+      !rows(k, 4, c.head_dim, &r.k_token_stride, &r.k_head_stride) ||
+      !rows(v, 4, c.head_dim, &r.v_token_stride, &r.v_head_stride) || !sequences(a[3], a[4], a[5], T, device, &c))
     return none();
-  const srw_kv_rows_t r{k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1), v->stride(0), v->stride(1)};
   return PyLong_FromLong(srw_kv_write(&c, &r, type == at::kFloat ? SRW_F32 : SRW_BF16, reinterpret_cast<void*>(stream)));
 }
 
@@ -163,14 +167,14 @@ PyObject* host_attention(PyObject* const* a, Py_ssize_t n) {
       !i64(a[9], &stream) || !PyFloat_Check(a[6]))
     return none();
   const at::Tensor* q = tensor(a[1]);
-  if (!plain(q, at::kBFloat16, 3, device) || wants_grad(q) || !rows(q, 8, s.kv.head_dim)) return none();
+  if (!plain(q, at::kBFloat16, 3, device) || wants_grad(q) ||
+      !rows(q, 8, s.kv.head_dim, &s.q_token_stride, &s.q_head_stride))
+    return none();
   if (most < 0 || most > kMost || window < 0 || window > kMost || sinks < 0 || sinks > kMost || q->size(1) > kMost)
     return none();
   const int64_t T = q->size(0);
   if (T == 0 || !sequences(a[2], a[3], a[4], T, device, &s.kv)) return none();
   s.q = q->data_ptr();
-  s.q_token_stride = q->stride(0);
-  s.q_head_stride = q->stride(1);
   s.n_heads = static_cast<int32_t>(q->size(1));
   s.max_new = static_cast<int32_t>(most);
   s.window = static_cast<int32_t>(window);

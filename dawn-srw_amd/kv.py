@@ -154,8 +154,10 @@ def _address(pages, table, lens, cu, T):
 
 
 def _rows(name, t, pages, T, dtypes, unit):
-    """t [T, heads, head_dim] with consecutive dims; rows that the kernels
-    cannot take as they lie (other strides or alignment) are copied."""
+    """(t, token stride, head stride) of t [T, heads, head_dim] with consecutive
+    dims; rows that the kernels cannot take as they lie (other strides or
+    alignment) are copied.  (The stride of a single token or head is never used,
+    and may be anything.)"""
     if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.shape[2] != pages.head_dim or t.shape[0] != T:
         got = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t)
         raise ValueError(f"{name} must be [{T}, heads, {pages.head_dim}]; got {got}")
@@ -165,12 +167,12 @@ def _rows(name, t, pages, T, dtypes, unit):
         raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{name} requires a gradient; the paged cache's calls have none (torch.no_grad())")
+    H, d = t.shape[1:]
     s0, s1, s2 = t.stride()
+    s0, s1 = H * d if T == 1 else s0, d if H == 1 else s1
     if s2 != 1 or s0 % unit or s1 % unit or t.data_ptr() % (unit * t.element_size()):
-        t = t.contiguous()
-        if t.data_ptr() % (unit * t.element_size()):  # contiguous, but off its alignment
-            t = t.clone()
-    return t
+        t, s0, s1 = t.clone(memory_format=torch.contiguous_format), H * d, d
+    return t, s0, s1
 
 
 def _call(f, dev, *args):
@@ -197,11 +199,11 @@ def kv_write(pages: KvPages, k, v, table, lens, cu=None) -> None:
             return C.check(status)
     T = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() else -1
     a = _address(pages, table, lens, cu, T)
-    k = _rows("k", k, pages, T, _DTYPES, 4)
-    v = _rows("v", v, pages, T, (k.dtype,), 4)
+    k, *ks = _rows("k", k, pages, T, _DTYPES, 4)
+    v, *vs = _rows("v", v, pages, T, (k.dtype,), 4)
     if k.shape[1] != pages.heads or v.shape[1] != pages.heads:
         raise ValueError(f"k and v have {k.shape[1]} and {v.shape[1]} heads, the pages {pages.heads}")
-    r = _ROWS.pack(k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2])
+    r = _ROWS.pack(k.data_ptr(), v.data_ptr(), *ks, *vs)
     C.check(_call(C.load_library().srw_kv_write, pages.device, _KV.pack(*a), r, _DTYPES[k.dtype]))
 
 
@@ -248,7 +250,7 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
             return got
     T = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else -1
     kv = _address(pages, table, lens, cu, T)
-    q = _rows("q", q, pages, T, (BF16,), 8)
+    q, *qs = _rows("q", q, pages, T, (BF16,), 8)
     Hq = q.shape[1]
     if Hq < 1 or Hq % pages.heads:
         raise ValueError(f"{Hq} query heads are no multiple of the pages' {pages.heads}")
@@ -259,8 +261,7 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
         out = torch.empty((T, Hq, pages.head_dim), dtype=BF16, device=dev)
     else:
         _tensor("out", out, dev, BF16, (T, Hq, pages.head_dim))
-    st = q.stride()
-    a = _ATTENTION.pack(*kv, q.data_ptr(), out.data_ptr(), st[0], st[1], Hq, max_new, window, sinks, scale)
+    a = _ATTENTION.pack(*kv, q.data_ptr(), out.data_ptr(), *qs, Hq, max_new, window, sinks, scale)
     lib = C.load_library()
     status = _call(lib.srw_attention, dev, a, None, 0)
     if status == C.SRW_EWORKSPACE:  # splits to join, nothing launched yet

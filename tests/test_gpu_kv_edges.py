@@ -181,3 +181,34 @@ def test_the_largest_window_hides_nothing(pkg, dev, sinks, width):
     for window in (1 << 20, (1 << 31) - 1):
         got = pkg.paged_attention(q, c.pages, table, c.len_t, _cu(dev, [n]), max_new=n, window=window, sinks=sinks)
         assert torch.equal(got, want), window
+
+
+# -- what tensors the calls take ---------------------------------------------------
+
+class _Nothing:
+    """A native host side that takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "general"])
+@pytest.mark.parametrize("T,H", [(1, 1), (1, 3), (5, 1)])
+def test_odd_strides_of_single_tokens_and_heads(pkg, dev, monkeypatch, native, T, H):
+    """The stride of a dimension of one element is no stride: slices of tensors of
+    odd widths."""
+    from dawn_srw_amd import kv
+    print(f"[gpu] kv odd strides T{T} H{H}", flush=True)
+    c = Cache(pkg, dev, "bf16", H, 64, 16, [T], seed=251)
+    if not native:
+        monkeypatch.setattr(kv, "_host", _Nothing())
+    g = torch.Generator().manual_seed(252)
+    wide = torch.randn(T, 3 * H * 64 + 3, generator=g).to(BF).to(dev)
+    rows = [torch.as_strided(wide, (T, H, 64), (wide.stride(0), 64 if H > 1 else 67, 1), i * H * 64) for i in range(3)]
+    cu = _cu(dev, [T])
+    pkg.kv_write(c.pages, rows[0], rows[1], c.table, c.len_t, cu)
+    for got, want in zip(pkg.kv_read(c.pages, c.table, c.len_t, cu, total=T), rows):
+        assert torch.equal(got, want)
+    got = pkg.paged_attention(rows[2], c.pages, c.table, c.len_t, cu)
+    assert torch.equal(got, pkg.paged_attention(rows[2].clone(memory_format=torch.contiguous_format), c.pages, c.table,
+                                                c.len_t, cu))
