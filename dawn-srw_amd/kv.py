@@ -175,6 +175,14 @@ def _rows(name, t, pages, T, dtypes, unit):
     return t, s0, s1
 
 
+def _check_window(window, sinks):
+    for n in (window, sinks):
+        if not hasattr(n, "__index__"):
+            raise TypeError(f"window and sinks are whole numbers; got {n!r}")
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("window and sinks are not negative, and sinks need a window")
+
+
 def _call(f, dev, *args):
     """f's status with the current stream of dev as its last argument (launches
     go to the current device's streams)."""
@@ -254,8 +262,9 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
     Hq = q.shape[1]
     if Hq < 1 or Hq % pages.heads:
         raise ValueError(f"{Hq} query heads are no multiple of the pages' {pages.heads}")
-    if window < 0 or sinks < 0 or (sinks and not window) or max_new < 0:
-        raise ValueError("window, sinks and max_new are not negative, and sinks need a window")
+    _check_window(window, sinks)
+    if max_new < 0:
+        raise ValueError("max_new is not negative")
     dev = pages.device
     if out is None:
         out = torch.empty((T, Hq, pages.head_dim), dtype=BF16, device=dev)
@@ -323,8 +332,9 @@ class PagedKvCache:
 
     def extend(self, seqs, counts):
         """Room for counts[i] (0 or more) further tokens of seqs[i]; (table, lens, cu,
-        max_new) of the call that writes and attends to them.  Raises
-        MemoryError, with nothing changed, where the free pages do not do."""
+        max_new) of the call that writes and attends to them, copied to the device
+        (which waits for it).  Raises MemoryError where the free pages do not do;
+        whatever it raises, nothing has changed."""
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs):
             raise ValueError("one count for each of different sequences")
         need = {}
@@ -339,6 +349,13 @@ class PagedKvCache:
         for s, n in zip(seqs, counts):
             self._pages[s].extend(self._free.pop() for _ in range(need[s]))
             self._lens[s] += n
+        try:
+            return self._call_of(seqs, counts)
+        except BaseException:
+            self._take_back(seqs, counts)
+            raise
+
+    def _call_of(self, seqs, counts):
         width = max((len(self._pages[s]) for s in seqs), default=0)
         # one copy to the device: the table's rows, then lens, then cu
         host, at = [], 0
@@ -353,6 +370,14 @@ class PagedKvCache:
         table, lens, cu = t[:B * width].view(B, width), t[B * width:B * width + B], t[B * width + B:]
         most = max(counts, default=0)
         return table, lens, None if most == 1 and min(counts) == 1 else cu, most
+
+    def _take_back(self, seqs, counts):
+        """What extend did, undone for a call that failed after it."""
+        for s, n in reversed(list(zip(seqs, counts))):
+            self._lens[s] -= n
+            pages = self._pages[s]
+            while len(pages) > -(-self._lens[s] // self.page_size):
+                self._free.append(pages.pop())
 
     def evict(self, seq: int, window: int, sinks: int = 0) -> int:
         """Give back the pages that hold only positions which a token at

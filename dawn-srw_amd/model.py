@@ -29,7 +29,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _capi as C
-from .kv import PagedKvCache, kv_write, paged_attention
+from .kv import PagedKvCache, _check_window, kv_write, paged_attention
 from .layer import GateConfig, SrwBatchPlan, SrwPlan
 from .srw import chunk_plan
 
@@ -419,9 +419,10 @@ class DawnModel:
         with j > i - window or j < ``sinks``.  Same model as :meth:`prefill` and
         :meth:`decode_step` (the SRW layer as ``_srw_inference`` in bf16): the
         cache holds the pools' outputs, the pool scales go into the attention's
-        scale and its result."""
+        scale and its result.  Whatever it raises, the cache's sequences are as
+        before the call."""
         cfg = self.cfg
-        D, H = cfg.d_model, cfg.n_heads
+        _check_window(window, sinks)
         ids = ids.reshape(-1).to(self.device)
         counts = [int(n) for n in counts]
         T = sum(counts)
@@ -435,7 +436,18 @@ class DawnModel:
             if cache.length(q) + n > cfg.max_seq_len:
                 raise ValueError("Sequence length exceeds max_seq_len")
         place = [cache.length(q) + i for q, n in zip(seqs, counts) for i in range(n)]
-        table, lens, cu, most = cache.extend(seqs, counts)
+        call = cache.extend(seqs, counts)
+        try:
+            return self._extend(ids, place, cache, counts, call, window, sinks, last_only)
+        except BaseException:
+            cache._take_back(seqs, counts)
+            raise
+
+    def _extend(self, ids, place, cache, counts, call, window, sinks, last_only):
+        cfg = self.cfg
+        D, H = cfg.d_model, cfg.n_heads
+        T = len(place)
+        table, lens, cu, most = call
         # rows up to one of a few token counts: the pools' plans are kept by it
         Tp = -(-T // 16) * 16 if T <= 128 else -(-T // 128) * 128
         x = torch.zeros(Tp, D, device=self.device)

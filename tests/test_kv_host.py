@@ -180,3 +180,18 @@ def test_cache_refusals(pkg):
         c.layer(0)                     # the calls run on a HIP device
     with pytest.raises(ValueError):
         c.evict(c.add(), 0)
+
+
+def test_a_failed_extend_changes_nothing(pkg, monkeypatch):
+    """A copy to the device that fails (no memory) after pages were handed out."""
+    c = pkg.PagedKvCache(1, 8, 1, 64, page_size=16, device="cpu")
+    a, b = c.add(), c.add()
+    c.extend([a], [20])
+    before = (dict(c._lens), {s: list(p) for s, p in c._pages.items()}, list(c._free))
+    with monkeypatch.context() as m:
+        m.setattr(torch, "tensor", lambda *x, **kw: (_ for _ in ()).throw(RuntimeError("no memory")))
+        with pytest.raises(RuntimeError):
+            c.extend([a, b], [13, 40])
+    assert before == (c._lens, c._pages, c._free)
+    table, lens, _, _ = c.extend([a, b], [13, 40])
+    assert lens.tolist() == [33, 40] and len({p for p in table.flatten().tolist() if p >= 0}) == 6
