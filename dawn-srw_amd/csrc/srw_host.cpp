@@ -43,9 +43,10 @@ PyObject* none() {
 }
 
 // The pages of a KvPages: the tensors k, v, k_scale, v_scale, looked at anew in
-// every call (their memory can be another's by then).
+// every call (their memory can be another's by then), and, behind them, what
+// host_pages gave for them, which still has to be so (kv.py refuses others).
 bool pages_of(PyObject* o, srw_kv_t* c, int* device) {
-  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  if (!PyTuple_CheckExact(o) || (PyTuple_GET_SIZE(o) != 4 && PyTuple_GET_SIZE(o) != 10)) return false;
   const at::Tensor *k = tensor(PyTuple_GET_ITEM(o, 0)), *v = tensor(PyTuple_GET_ITEM(o, 1));
   if (!k || !v || k->dim() != 4 || v->dim() != 4 || !k->is_cuda()) return false;
   *device = static_cast<int>(k->get_device());
@@ -69,6 +70,13 @@ bool pages_of(PyObject* o, srw_kv_t* c, int* device) {
         !s->is_contiguous())
       return false;
     scale[i] = static_cast<float*>(s->data_ptr());
+  }
+  if (PyTuple_GET_SIZE(o) == 10) {
+    const int64_t now[6] = {N, H, P, D, kind, *device};
+    for (int i = 0; i < 6; ++i) {
+      int64_t then;
+      if (!i64(PyTuple_GET_ITEM(o, 4 + i), &then) || then != now[i]) return false;
+    }
   }
   c->k = k->data_ptr();
   c->v = v->data_ptr();

@@ -95,6 +95,7 @@ class KvPages:
         if at is None:
             at = self._at[4:]
         self.n_pages, self.heads, self.page_size, self.head_dim, self.kind, _ = at
+        self._t += tuple(at)  # as they were taken
         self.device = k.device
 
     k = property(lambda self: self._t[0])
@@ -106,7 +107,7 @@ class KvPages:
     def _at(self):
         """(k, v, k_scale, v_scale addresses, n_pages, heads, page_size, head_dim,
         kind, device) of the tensors as they are now."""
-        k, v, k_scale, v_scale = self._t
+        k, v, k_scale, v_scale = self._t[:4]
         if not isinstance(k, torch.Tensor) or k.dim() != 4:
             raise ValueError("k must be a tensor [n_pages, heads, page_size, head_dim]")
         n, h, p, d = k.shape
@@ -147,7 +148,7 @@ def _address(pages, table, lens, cu, T):
     else:
         raise ValueError(f"{T} tokens of {B} sequences need cu")
     at = pages._at
-    if at[4:9] != (pages.n_pages, pages.heads, pages.page_size, pages.head_dim, pages.kind) or at[9] != dev.index:
+    if at[4:] != pages._t[4:]:
         raise ValueError("the pages' tensors have changed since KvPages took them")
     return (*at[:4], table.data_ptr(), lens_at, cu_at, B, T, pages.n_pages, width,
             stride if stride > width else width, pages.heads, pages.head_dim, pages.page_size, pages.kind)

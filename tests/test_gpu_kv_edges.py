@@ -212,3 +212,21 @@ def test_odd_strides_of_single_tokens_and_heads(pkg, dev, monkeypatch, native, T
     got = pkg.paged_attention(rows[2], c.pages, c.table, c.len_t, cu)
     assert torch.equal(got, pkg.paged_attention(rows[2].clone(memory_format=torch.contiguous_format), c.pages, c.table,
                                                 c.len_t, cu))
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "general"])
+def test_pages_of_another_shape_are_refused(pkg, dev, monkeypatch, native):
+    """Tensors that got another shape after KvPages took them."""
+    from dawn_srw_amd import kv
+    print("[gpu] kv pages of another shape", flush=True)
+    lens, table = torch.tensor([1], dtype=I32, device=dev), torch.tensor([[0]], dtype=I32, device=dev)
+    for dh, P in ((128, 16), (64, 32)):
+        pages = pkg.KvPages(torch.zeros(1, 1, 16, 64, dtype=BF, device=dev), torch.zeros(1, 1, 64, 16, dtype=BF, device=dev))
+        pages.k.data, pages.v.data = (torch.zeros(s, dtype=BF, device=dev) for s in ((1, 1, P, dh), (1, 1, dh, P)))
+        x = torch.ones(1, 1, dh, dtype=BF, device=dev)
+        if not native:
+            monkeypatch.setattr(kv, "_host", _Nothing())
+        for call in (lambda: pkg.kv_write(pages, x, x, table, lens), lambda: pkg.kv_read(pages, table, lens),
+                     lambda: pkg.paged_attention(x, pages, table, lens)):
+            with pytest.raises(ValueError):
+                call()
