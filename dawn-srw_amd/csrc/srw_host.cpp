@@ -28,8 +28,10 @@ bool plain(const at::Tensor* t, at::ScalarType type, int64_t dims, int device) {
   return t && t->scalar_type() == type && t->dim() == dims && t->is_cuda() && t->get_device() == device;
 }
 
-// The calls have no backward: kv.py refuses tensors that want one.
-bool wants_grad(const at::Tensor* t) { return t->requires_grad() && c10::GradMode::is_enabled(); }
+// The calls have no derivatives: kv.py refuses tensors that want them, of either mode.
+bool wants_grad(const at::Tensor* t) {
+  return (t->requires_grad() && c10::GradMode::is_enabled()) || t->_fw_grad(/*level=*/0).defined();
+}
 
 bool i64(PyObject* o, int64_t* v) {
   if (!PyLong_Check(o)) return false;
@@ -56,7 +58,8 @@ bool pages_of(PyObject* o, srw_kv_t* c, int* device) {
                                                                            : -1;
   const int64_t N = k->size(0), H = k->size(1), P = k->size(2), D = k->size(3);
   if (kind < 0 || !plain(v, type, 4, *device) || v->size(0) != N || v->size(1) != H || v->size(2) != D ||
-      v->size(3) != P || !k->is_contiguous() || !v->is_contiguous() || H > kMost || P > kMost || D > kMost)
+      v->size(3) != P || !k->is_contiguous() || !v->is_contiguous() || H > kMost || P > kMost || D > kMost ||
+      wants_grad(k) || wants_grad(v))
     return false;
   float* scale[2] = {nullptr, nullptr};
   for (int i = 0; i < 2; ++i) {
@@ -67,7 +70,7 @@ bool pages_of(PyObject* o, srw_kv_t* c, int* device) {
     }
     const at::Tensor* s = tensor(so);
     if (!plain(s, at::kFloat, 3, *device) || s->size(0) != N || s->size(1) != H || s->size(2) != P ||
-        !s->is_contiguous())
+        !s->is_contiguous() || wants_grad(s))
       return false;
     scale[i] = static_cast<float*>(s->data_ptr());
   }

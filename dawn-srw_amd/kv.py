@@ -27,6 +27,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi as C
 
@@ -126,6 +127,11 @@ class KvPages:
         return (k.data_ptr(), v_at, *scales, n, h, p, d, kind, dev.index)
 
 
+def _no_grad(name, t):
+    if t.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} requires a gradient; the paged cache's calls have none (torch.no_grad())")
+
+
 def _address(pages, table, lens, cu, T):
     """The fields of srw_kv_t: a call's sequences over these pages."""
     dev = pages.device
@@ -150,6 +156,9 @@ def _address(pages, table, lens, cu, T):
     at = pages._at
     if at[4:] != pages._t[4:]:
         raise ValueError("the pages' tensors have changed since KvPages took them")
+    for name, t in zip(("k", "v", "k_scale", "v_scale"), pages._t):
+        if t is not None:
+            _no_grad("the pages' " + name, t)
     return (*at[:4], table.data_ptr(), lens_at, cu_at, B, T, pages.n_pages, width,
             stride if stride > width else width, pages.heads, pages.head_dim, pages.page_size, pages.kind)
 
@@ -166,8 +175,7 @@ def _rows(name, t, pages, T, dtypes, unit):
         raise ValueError(f"{name} is on {t.device}, expected {pages.device}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError(f"{name} requires a gradient; the paged cache's calls have none (torch.no_grad())")
+    _no_grad(name, t)
     H, d = t.shape[1:]
     s0, s1, s2 = t.stride()
     s0, s1 = H * d if T == 1 else s0, d if H == 1 else s1

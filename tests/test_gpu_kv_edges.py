@@ -230,3 +230,32 @@ def test_pages_of_another_shape_are_refused(pkg, dev, monkeypatch, native):
                      lambda: pkg.paged_attention(x, pages, table, lens)):
             with pytest.raises(ValueError):
                 call()
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "general"])
+def test_pages_and_tangents_that_want_gradients(pkg, dev, monkeypatch, native):
+    """No gradient is dropped silently: neither of pages nor of forward mode."""
+    from torch.autograd import forward_ad
+    from dawn_srw_amd import kv
+    print("[gpu] kv pages and tangents", flush=True)
+    lens, table = torch.tensor([1], dtype=I32, device=dev), torch.tensor([[0]], dtype=I32, device=dev)
+    k, v = (torch.zeros(s, dtype=BF, device=dev) for s in ((1, 1, 16, 64), (1, 1, 64, 16)))
+    pages, x = pkg.KvPages(k, v), torch.ones(1, 1, 64, dtype=BF, device=dev)
+    if not native:
+        monkeypatch.setattr(kv, "_host", _Nothing())
+
+    def refused(*calls):
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call()
+
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        refused(lambda: pkg.kv_write(pages, d, x, table, lens), lambda: pkg.kv_write(pages, x, d, table, lens),
+                lambda: pkg.paged_attention(d, pages, table, lens))
+    pkg.kv_write(pages, x, x, table, lens)
+    v.requires_grad_()
+    refused(lambda: pkg.kv_write(pages, x, x, table, lens), lambda: pkg.kv_read(pages, table, lens),
+            lambda: pkg.paged_attention(x, pages, table, lens))
+    with torch.no_grad():
+        assert torch.equal(pkg.paged_attention(x, pages, table, lens), x)
