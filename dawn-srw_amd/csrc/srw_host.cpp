@@ -146,7 +146,12 @@ PyObject* host_write(PyObject* const* a, Py_ssize_t n) {
       !rows(k, 4, c.head_dim, &r.k_token_stride, &r.k_head_stride) ||
       !rows(v, 4, c.head_dim, &r.v_token_stride, &r.v_head_stride) || !sequences(a[3], a[4], a[5], T, device, &c))
     return none();
-  return PyLong_FromLong(srw_kv_write(&c, &r, type == at::kFloat ? SRW_F32 : SRW_BF16, reinterpret_cast<void*>(stream)));
+  const int status = srw_kv_write(&c, &r, type == at::kFloat ? SRW_F32 : SRW_BF16, reinterpret_cast<void*>(stream));
+  for (int i = 0; i < 4; ++i) {  // written in place
+    const at::Tensor* t = tensor(PyTuple_GET_ITEM(a[0], i));
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
+  return PyLong_FromLong(status);
 }
 
 // read(pages, table, lens, cu, T, float32, stream) -> (k, v), or None

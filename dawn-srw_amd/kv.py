@@ -132,6 +132,13 @@ def _no_grad(name, t):
         raise NotImplementedError(f"{name} requires a gradient; the paged cache's calls have none (torch.no_grad())")
 
 
+def _written(*tensors):
+    """Counts the tensors as changed in place."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _address(pages, table, lens, cu, T):
     """The fields of srw_kv_t: a call's sequences over these pages."""
     dev = pages.device
@@ -222,6 +229,7 @@ def kv_write(pages: KvPages, k, v, table, lens, cu=None) -> None:
         raise ValueError(f"k and v have {k.shape[1]} and {v.shape[1]} heads, the pages {pages.heads}")
     r = _ROWS.pack(k.data_ptr(), v.data_ptr(), *ks, *vs)
     C.check(_call(C.load_library().srw_kv_write, pages.device, _KV.pack(*a), r, _DTYPES[k.dtype]))
+    _written(*pages._t[:4])
 
 
 def kv_read(pages: KvPages, table, lens, cu=None, *, total=None, dtype=BF16):
@@ -275,10 +283,12 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
     if max_new < 0:
         raise ValueError("max_new is not negative")
     dev = pages.device
-    if out is None:
-        out = torch.empty((T, Hq, pages.head_dim), dtype=BF16, device=dev)
-    else:
+    given = out is not None
+    if given:
         _tensor("out", out, dev, BF16, (T, Hq, pages.head_dim))
+        _no_grad("out", out)
+    else:
+        out = torch.empty((T, Hq, pages.head_dim), dtype=BF16, device=dev)
     a = _ATTENTION.pack(*kv, q.data_ptr(), out.data_ptr(), *qs, Hq, max_new, window, sinks, scale)
     lib = C.load_library()
     status = _call(lib.srw_attention, dev, a, None, 0)
@@ -288,6 +298,8 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
         status = _call(lib.srw_attention, dev, a, ws.data_ptr(), need.value)
     C.check(status)
+    if given:
+        _written(out)
     return out
 
 

@@ -259,3 +259,34 @@ def test_pages_and_tangents_that_want_gradients(pkg, dev, monkeypatch, native):
             lambda: pkg.paged_attention(x, pages, table, lens))
     with torch.no_grad():
         assert torch.equal(pkg.paged_attention(x, pages, table, lens), x)
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "general"])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_written_tensors_tell_their_version(pkg, dev, monkeypatch, native, kind):
+    """What a call writes in place counts as changed: a gradient that was to use
+    the old values is refused."""
+    from dawn_srw_amd import kv
+    print(f"[gpu] kv versions {kind}", flush=True)
+    c = Cache(pkg, dev, kind, 1, 64, 16, [1], seed=261)
+    if not native:
+        monkeypatch.setattr(kv, "_host", _Nothing())
+    x = torch.ones(1, 1, 64, dtype=BF, device=dev)
+    held = [t for t in (c.pages.k, c.pages.v, c.pages.k_scale, c.pages.v_scale) if t is not None]
+    before = [t._version for t in held]
+    pkg.kv_write(c.pages, x, x, c.table, c.len_t)
+    assert all(t._version > b for t, b in zip(held, before))
+    out = torch.zeros(1, 1, 64, dtype=BF, device=dev)
+    pkg.kv_read(c.pages, c.table, c.len_t)
+    before = [t._version for t in (*held, out)]
+    pkg.paged_attention(x, c.pages, c.table, c.len_t, out=out)
+    assert [t._version for t in held] == before[:-1] and out._version > before[-1]
+    w = torch.ones(1, 1, 64, device=dev, requires_grad=True)
+    y = (w * out.float()).sum() + (w * out).sum()
+    pkg.paged_attention(x, c.pages, c.table, c.len_t, out=out)
+    with pytest.raises(RuntimeError):
+        y.backward()
+    with torch.inference_mode():                              # which keeps no versions
+        other = pkg.KvPages(*(None if t is None else t.clone() for t in (c.pages.k, c.pages.v, c.pages.k_scale, c.pages.v_scale)))
+        pkg.kv_write(other, x, x, c.table, c.len_t)
+        pkg.paged_attention(x, other, c.table, c.len_t, out=torch.zeros_like(x))
