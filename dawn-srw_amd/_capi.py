@@ -59,7 +59,7 @@ EXPORTED_SYMBOLS = (
     "srw_set_kernel_events", "srw_backward_workspace_size", "srw_backward",
     "srw_workspace_size_batch", "srw_forward_batch", "srw_forward_noalloc",
     "srw_diag_summary", "srw_cast_bf16", "srw_dawn_decode_step",
-    "srw_kv_write", "srw_kv_read", "srw_attention_workspace_size", "srw_attention",
+    "srw_kv_write", "srw_kv_read", "srw_attention_workspace_size", "srw_attention", "srw_attention_plan",
 )
 
 # srw_diag_out_t: the result tuple's per-token values and scalars (SRW_DSUM_*)
@@ -230,6 +230,8 @@ def load_library() -> ctypes.CDLL:
             getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
         lib.srw_attention_workspace_size.restype = ctypes.c_int
         lib.srw_attention_workspace_size.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]
+        lib.srw_attention_plan.restype = ctypes.c_int
+        lib.srw_attention_plan.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]
         lib.srw_attention.restype = ctypes.c_int
         lib.srw_attention.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         got = lib.srw_abi_version()

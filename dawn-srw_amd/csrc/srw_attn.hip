@@ -1159,6 +1159,12 @@ size_t attention_workspace_bytes(const srw_attention_t& a) {
   return align256(rows * sizeof(float2)) + align256(rows * a.kv.head_dim * sizeof(float));
 }
 
+void attention_plan(const srw_attention_t& a, int32_t* rows, int32_t* splits) {
+  const AttnPlan p = plan_of(a);
+  *rows = p.rows;
+  *splits = p.S;
+}
+
 hipError_t attention(const srw_attention_t& a, char* ws, hipStream_t s) {
   const AttnPlan p = plan_of(a);
   AttnArgs g{};

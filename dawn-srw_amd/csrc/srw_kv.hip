@@ -405,6 +405,15 @@ srw_status_t srw_attention_workspace_size(const srw_attention_t* a, size_t* byte
   return SRW_OK;
 }
 
+srw_status_t srw_attention_plan(const srw_attention_t* a, int32_t* rows, int32_t* splits) {
+  const srw_status_t st = srw::check_attention(a);
+  if (st != SRW_OK) return st;
+  if (!rows || !splits) return SRW_EINVAL;
+  *rows = *splits = 0;
+  if (a->kv.T > 0) srw::attention_plan(*a, rows, splits);
+  return SRW_OK;
+}
+
 srw_status_t srw_attention(const srw_attention_t* a, void* workspace, size_t workspace_bytes, void* stream) {
   const srw_status_t st = srw::check_attention(a);
   if (st != SRW_OK) return st;

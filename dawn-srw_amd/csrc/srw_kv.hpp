@@ -212,6 +212,7 @@ struct KvRows {
 hipError_t kv_write(const srw_kv_t& c, const KvRows& r, bool f32, hipStream_t s);
 hipError_t kv_read(const srw_kv_t& c, const KvRows& r, bool f32, hipStream_t s);
 size_t attention_workspace_bytes(const srw_attention_t& a);
+void attention_plan(const srw_attention_t& a, int32_t* rows, int32_t* splits);
 hipError_t attention(const srw_attention_t& a, char* ws, hipStream_t s);
 
 }  // namespace srw

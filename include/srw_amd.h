@@ -504,6 +504,11 @@ typedef struct srw_attention {
 srw_status_t srw_attention_workspace_size(const srw_attention_t* a, size_t* bytes);
 srw_status_t srw_attention(const srw_attention_t* a, void* workspace, size_t workspace_bytes, void* stream);
 
+/* How such a call runs, for tests and benchmarks: rows (tokens x heads of a key
+ * head's group) a workgroup takes, 16, 32 or 128, and splits of their positions
+ * (more than one: joined by a second launch).  0 and 0 without tokens. */
+srw_status_t srw_attention_plan(const srw_attention_t* a, int32_t* rows, int32_t* splits);
+
 /* Name of the kernel family the last srw_forward on this thread used
  * ("generic", "mfma_bf16", "mfma_ss_bf16", ...), for tests and benchmarks. */
 const char* srw_last_path(void);

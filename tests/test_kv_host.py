@@ -195,3 +195,30 @@ def test_a_failed_extend_changes_nothing(pkg, monkeypatch):
     assert before == (c._lens, c._pages, c._free)
     table, lens, _, _ = c.extend([a, b], [13, 40])
     assert lens.tolist() == [33, 40] and len({p for p in table.flatten().tolist() if p >= 0}) == 6
+
+
+def test_plans_of_calls(C):
+    """Rows a workgroup and splits: single tokens, short and long chunks."""
+    lib = C.load_library()
+
+    def plan(max_new, window=0, sinks=0, **kw):
+        f = dict(kind=C.SRW_KV_BF16, page_size=64, B=1)
+        f.update(kw)
+        f["table_stride"] = f["table_width"]
+        a = C.SrwAttention(_kv(C, **f), 4096, 4096, 256, 64, 4, max_new, window, sinks, 1.0)
+        rows, splits = ctypes.c_int32(-1), ctypes.c_int32(-1)
+        assert lib.srw_attention_plan(ctypes.byref(a), ctypes.byref(rows), ctypes.byref(splits)) == C.SRW_OK
+        return rows.value, splits.value
+
+    assert plan(0, T=0, table_width=8) == (0, 0)
+    assert plan(1, T=1, cu=None, table_width=8) == (16, 1)
+    assert plan(1, T=1, cu=None, table_width=1000)[0] == 16 and plan(1, T=1, cu=None, table_width=1000)[1] > 1
+    assert plan(16, T=16, table_width=8) == (32, 1)
+    assert plan(300, T=300, table_width=8) == (32, 1)              # 1 200 rows of 8 tiles: too few for 128 each
+    assert plan(4000, T=4000, table_width=12) == (128, 1)
+    assert plan(300, T=300, table_width=1000)[0] == 128 and plan(300, T=300, table_width=1000)[1] > 1
+    assert plan(300, T=300, table_width=1000, window=100) == (32, 1)
+    a = C.SrwAttention(_kv(C), 4096, 4096, 256, 64, 4, 0, 0, 0, 1.0)
+    n = ctypes.c_int32(0)
+    assert lib.srw_attention_plan(ctypes.byref(a), ctypes.byref(n), None) == C.SRW_EINVAL
+    assert lib.srw_attention_plan(None, ctypes.byref(n), ctypes.byref(n)) == C.SRW_EINVAL
