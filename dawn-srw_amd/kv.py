@@ -128,7 +128,9 @@ class KvPages:
 
 
 def _no_grad(name, t):
-    if t.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(t).tangent is not None:
+    # (tangents are of a level: outside of one there are none to look for)
+    if (t.requires_grad and torch.is_grad_enabled()
+            or forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None):
         raise NotImplementedError(f"{name} requires a gradient; the paged cache's calls have none (torch.no_grad())")
 
 
@@ -192,9 +194,8 @@ def _rows(name, t, pages, T, dtypes, unit):
 
 
 def _check_window(window, sinks):
-    for n in (window, sinks):
-        if not hasattr(n, "__index__"):
-            raise TypeError(f"window and sinks are whole numbers; got {n!r}")
+    if not (type(window) is int is type(sinks) or hasattr(window, "__index__") and hasattr(sinks, "__index__")):
+        raise TypeError(f"window and sinks are whole numbers; got {window!r} and {sinks!r}")
     if window < 0 or sinks < 0 or (sinks and not window):
         raise ValueError("window and sinks are not negative, and sinks need a window")
 
