@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
+import operator
 import os
 import struct
 
@@ -359,6 +360,7 @@ class PagedKvCache:
         whatever it raises, nothing has changed."""
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs):
             raise ValueError("one count for each of different sequences")
+        counts = [operator.index(n) for n in counts]
         need = {}
         for s, n in zip(seqs, counts):
             if s not in self._lens:

@@ -222,3 +222,16 @@ def test_plans_of_calls(C):
     n = ctypes.c_int32(0)
     assert lib.srw_attention_plan(ctypes.byref(a), ctypes.byref(n), None) == C.SRW_EINVAL
     assert lib.srw_attention_plan(None, ctypes.byref(n), ctypes.byref(n)) == C.SRW_EINVAL
+
+
+def test_counts_are_whole_numbers(pkg):
+    """A count of another type is refused before any sequence has its pages."""
+    import numpy as np
+    c = pkg.PagedKvCache(1, 8, 1, 64, page_size=16, device="cpu")
+    a, b = c.add(), c.add()
+    before = (dict(c._lens), {s: list(p) for s, p in c._pages.items()}, list(c._free))
+    for bad in (1.0, "1", None):
+        with pytest.raises(TypeError):
+            c.extend([a, b], [20, bad])
+        assert before == (c._lens, c._pages, c._free)
+    assert c.extend([a, b], [np.int64(20), 1])[1].tolist() == [20, 1]
