@@ -749,12 +749,14 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
 // pieces of a row are XOR-swizzled by the row so that the 16 lanes of a
 // fragment read cover all banks.
 //
-// Bound by the vector ALU: a score takes 4 (bf16) or 5 (8 bits) instructions
-// and an exponential, which costs 2.5 of them, against 4 head_dim products.  A
-// wave alone issues a vector instruction every 8 cycles, half the SIMD's rate,
-// and matrix instructions run beside other waves' vector ones; so what counts
-// is waves on a SIMD, and with 16 rows a wave (at most 128 registers) four
-// fit, where 32 rows (240 registers at head_dim 128) left two.
+// Vector work fills it most: a score takes 4 (bf16) or 5 (8 bits) instructions
+// and an exponential, which costs 2.5 of them, against 4 head_dim products.  Of a
+// long chunk's SIMD cycles the vector ALU is active for 70%, the matrix cores for
+// 30%; the LDS, whose every fragment feeds one product, is for 44% of a CU's.  None
+// is full: a wave alone issues a vector instruction every 8 cycles, half the SIMD's
+// rate, and matrix instructions run beside other waves' vector ones; so what counts
+// is waves on a SIMD, and with 16 rows a wave (at most 128 registers) four fit,
+// where 32 rows (240 registers at head_dim 128) left two.
 //
 // Measured: 2 048 tokens of 32 heads over 30 011 positions of 8, int8, head_dim
 // 128, in 1 400 us, 0.74 PFLOP/s (32 rows a wave: 1 363, but calls of few tiles
@@ -1069,13 +1071,13 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
-    *reinterpret_cast<uint2*>(a.out + row * DH + 16 * d + 4 * g) =
-        make_uint2(pack_bf16(o[d][0] * inv, o[d][1] * inv), pack_bf16(o[d][2] * inv, o[d][3] * inv));
+      *reinterpret_cast<uint2*>(a.out + row * DH + 16 * d + 4 * g) =
+          make_uint2(pack_bf16(o[d][0] * inv, o[d][1] * inv), pack_bf16(o[d][2] * inv, o[d][3] * inv));
   } else {
     const int64_t at = split * (a.kv.T * a.Hq) + row;
     if (l != 0.f) {
 #pragma unroll
-    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(a.part + at * DH + 16 * d + 4 * g) = o[d];
+      for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(a.part + at * DH + 16 * d + 4 * g) = o[d];
     }
     if (g == 0) a.ml[at] = make_float2(m, l);
   }

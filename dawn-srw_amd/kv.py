@@ -10,12 +10,15 @@ head.  Sequences of any lengths share them: a call describes its sequences by
 * ``lens`` [B] int32: the sequences' lengths, the call's new tokens included;
 * ``cu`` [B + 1] int32: sequence b's new tokens are the packed rows
   [cu[b], cu[b + 1]) of T and lie at its last positions; None: one each.
+  cu[0] is 0 and cu[B] is T: rows of an output that no sequence names are not
+  written.
 
-All three are device tensors that only the kernels read: no call waits for the
-GPU.  :func:`kv_write` stores new tokens, :func:`kv_read` reads tokens back,
-:func:`paged_attention` attends from new tokens to everything before them.
-:class:`PagedKvCache` keeps the pages of all layers of a model and hands them
-out to sequences.
+All three are device tensors that only the kernels read: the functions wait for
+nothing on the GPU.  :func:`kv_write` stores new tokens, :func:`kv_read` reads
+tokens back, :func:`paged_attention` attends from new tokens to everything
+before them.  :class:`PagedKvCache` keeps the pages of all layers of a model and
+hands them out to sequences; its ``extend`` copies a call's table to the device,
+which waits.
 """
 
 from __future__ import annotations
@@ -265,10 +268,14 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
     position i sees the positions j <= i, with ``window`` > 0 those with j > i
     - window or j < ``sinks``.  ``scale`` multiplies the scores (default 1 /
     sqrt(head_dim)).  ``max_new``: the most new tokens of one sequence, where
-    the caller knows it (it chooses the kernel, not the result).  Returns
-    ``out`` [T, n_heads, head_dim] bfloat16; a token that sees nothing gets
-    zeros.  The softmax weights are rounded to bfloat16 for the second product;
-    sums and statistics are float32."""
+    the caller knows it.  Returns ``out`` [T, n_heads, head_dim] bfloat16; a
+    token that sees nothing gets zeros.
+
+    Sums and statistics are float32.  The softmax weights enter the second
+    product as one bfloat16 in calls of many rows, as two (16 bits) in calls of
+    few.  Which kernel and how many splits a call gets goes by ``max_new``, its
+    rows, heads and the table's width: a sequence's outputs are the same bit for
+    bit in calls that agree in these, and within these roundings in any."""
     scale = pages.head_dim ** -0.5 if scale is None else float(scale)
     if out is None and _current_device() == pages.device.index:
         got = (_host or _native()).attention(pages._t, q, table, lens, cu, max_new, scale, window, sinks,

@@ -488,16 +488,17 @@ srw_status_t srw_kv_read(const srw_kv_t* cache, const srw_kv_rows_t* rows, int32
  * head h / (n_heads / n_kv_heads)).  q rows at q + t * q_token_stride + h *
  * q_head_stride (elements, multiples of 8; 16-byte aligned), out [T, n_heads,
  * head_dim] contiguous, both bf16; float32 inside but for the softmax weights,
- * which the matrix cores read as bf16 (in calls of few rows as two parts).  The cache must hold the new tokens
- * (srw_kv_write before, on the same stream). */
+ * which the matrix cores read as bf16 (in calls of few rows as two parts).  Rows
+ * of out that no sequence names (cu[B] < T) are not written.  The cache must hold
+ * the new tokens (srw_kv_write before, on the same stream). */
 typedef struct srw_attention {
   srw_kv_t kv;
   const void* q;
   void* out;
   int64_t q_token_stride, q_head_stride;
   int32_t n_heads;
-  int32_t max_new;        /* the most new tokens of a sequence, 0: not known.  It chooses the kernel;
-                             results are right for any value */
+  int32_t max_new;        /* the most new tokens of a sequence, 0: not known.  It chooses kernel and
+                             splits, and so roundings; results are right for any value */
   int32_t window, sinks;  /* 0: every earlier position is seen; sinks need a window */
   float scale;
 } srw_attention_t;
