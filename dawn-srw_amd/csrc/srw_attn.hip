@@ -39,6 +39,7 @@
 // that are not finite are rare, and the loops carry nothing for them: a wave that
 // ends with either goes over its tiles again (careful_rows).
 
+#include <float.h>
 #include <math.h>
 
 #include "srw_kv.hpp"
@@ -49,7 +50,7 @@ namespace {
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLazy = 8.f;       // log2 of the largest weight before m is raised
-constexpr float kLowest = -INFINITY;  // m of a row that has seen nothing, or scores of -inf only
+constexpr float kLowest = -FLT_MAX;  // m of a row that has seen nothing, or scores of -inf only
 constexpr float kLarge = 4096.f;      // an m whose last bit, 2^-11, moves a weight by under 2e-4
 
 struct AttnArgs {
@@ -200,30 +201,10 @@ __device__ inline u32x4_t finite16(u32x4_t x) {
   }
   return x;
 }
-// Adds the values that are not finite of the tile's positions for which see(k)
-// holds: add(i, value) of dim(i).  Rare: one load each.
-template <int KIND, int N, class See, class Dim, class Acc>
-__device__ inline void add_not_finite(const KvView& kv, int64_t b, int h, int head_dim, int key0, See see, Dim dim,
-                                      Acc add) {
-  for (int k = 0; k < kTile; ++k) {
-    const int pg = kv_page(kv, b, key0 + k);
-    if (pg < 0 || !see(k)) continue;
-    const char* src = kv.v + ((static_cast<int64_t>(pg) * kv.H + h) * head_dim * kv.P + ((key0 + k) & (kv.P - 1))) *
-                                 kv_bytes<KIND>();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      // one address and one load after the other: their registers are the kernel's
-      int at = dim(i);
-      asm volatile("" : "+v"(at) : : "memory");
-      const char* p = src + static_cast<int64_t>(at) * kv.P * kv_bytes<KIND>();
-      if constexpr (KIND == SRW_KV_BF16) {
-        const float x = bf16_to_f32(*reinterpret_cast<const uint16_t*>(p));
-        if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) add(i, x);
-      } else {
-        if ((*p & 0x7f) == 0x7f) add(i, __uint_as_float(0x7fc00000u));
-      }
-    }
-  }
+// 1 for each of two bf16 numbers that a test of its bits holds for, else 0.
+template <class Test>
+__device__ inline uint32_t ones16(uint32_t w, Test test) {
+  return (test(w & 0xffffu) ? 0x3f80u : 0u) | (test(w >> 16) ? 0x3f800000u : 0u);
 }
 
 template <class F, int... J>
@@ -310,12 +291,11 @@ __device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, 
     }
     mask();
     float mt = largest16(t);
-    if (__any(mt > (m == kLowest ? -INFINITY : kLazy))) {
+    if (__any(mt > (m == kLowest ? kLowest : kLazy))) {
       mt = join32(join16(mt, mx), mx);
-      const bool none = mt == -INFINITY;
-      const float up = m == kLowest ? (none ? 0.f : mt) : fmaxf(mt, 0.f);
-      m = m == kLowest && none ? kLowest : mu + up;
-      const float w = __builtin_amdgcn_exp2f(-fmaxf(up, 0.f));  // (nothing yet: of zeros)
+      const float mn = fmaxf(mu + mt, m), up = mn - mu;
+      const float w = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
       l *= w;
       rescale(o, w);
 #pragma unroll
@@ -348,35 +328,64 @@ __device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, 
 
 // A wave's rows, up to 16 from r0 on, over the tiles first, first + step, ... < end
 // of a span, for scores and values of any size: straight from memory, a fragment
-// at a time.  Values that are not finite are kept out of the products and added
-// to the rows that see them.
+// at a time.  Values that are not finite are kept out of the products; where there
+// are any, a second pass adds them to the rows that see them.
 template <int KIND, int DH>
 __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvSpan& sp, int h, int r0, int r1, int first,
                                     int end, int step, float& m, float& l, f32x4_t (&o)[DH / 16]) {
   constexpr int ES = kv_bytes<KIND>();
   constexpr int ND = DH / 16;
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // nothing here is worked out before it is needed
+  const int col = lane & 15, g = lane >> 4;
   const KvSeq& sq = tl.sq;
   const int P = a.kv.P, fr = r0 + col;
   const bool in = fr < r1;
   const int tok = in ? fr / a.G : 0, pos = in ? sq.len - sq.n + tok : -1;
   const uint16_t* src = a.q + (sq.row0 + tok) * a.q_token + (h * a.G + (in ? fr - tok * a.G : 0)) * a.q_head;
+  // the keys of lane group g in the tile at key0: which the lane's token sees (bit j:
+  // key 16 g + j), which any row does, and their values
+  uint32_t mine, seen;
+  const char* vsrc;
+  auto values_of = [&](int key0) {
+    const int kv = key0 + 16 * g;
+    const int pv = kv < sp.hi ? kv_page(a.kv, tl.b, kv) : -1;
+    mine = pv < 0 ? 0u : static_cast<uint32_t>(kv_seen(pos, key0, a.window, a.sinks) >> (16 * g)) & 0xffffu;
+    seen = mine;
+    for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);
+    const int64_t hv = static_cast<int64_t>(pv < 0 ? 0 : pv) * a.kv.H + h;
+    vsrc = a.kv.v + ((hv * DH + col) * P + (kv & (P - 1))) * ES;
+    return hv * P + (kv & (P - 1)) + col;  // (of the scales)
+  };
+  auto value = [&](int d, int st) {  // of the keys that some row sees
+    const char* at = vsrc + static_cast<int64_t>(16 * d) * P * ES;
+    u32x4_t v;
+    if constexpr (KIND == SRW_KV_BF16) {
+      v = ld16(at + 16 * st);
+    } else {
+      const uint2 raw = *reinterpret_cast<const uint2*>(at + 8 * st);
+      v = widen8<KIND>(raw.x, raw.y);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t two = seen >> (8 * st + 2 * u);
+      v[u] &= (two & 1 ? 0x0000ffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+    }
+    return v;
+  };
   m = kLowest;
   l = 0.f;
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  u16x2_t most = {0, 0};
   for (int i = first; i < end; i += step) {
     const int key0 = sp.key0(i);
     // (rows of the first product as in attn_rows_kernel)
-    const int kk = key0 + 16 * (col >> 2), kv = key0 + 16 * g;
-    int pk = kk < sp.hi ? kv_page(a.kv, tl.b, kk) : -1, pv = kv < sp.hi ? kv_page(a.kv, tl.b, kv) : -1;
-    const uint32_t mine =
-        pv < 0 ? 0u : static_cast<uint32_t>(kv_seen(pos, key0, a.window, a.sinks) >> (16 * g)) & 0xffffu;
+    const int kk = key0 + 16 * (col >> 2);
+    int pk = kk < sp.hi ? kv_page(a.kv, tl.b, kk) : -1;
     pk = pk < 0 ? 0 : pk;
-    pv = pv < 0 ? 0 : pv;
-    const int64_t hk = static_cast<int64_t>(pk) * a.kv.H + h, hv = static_cast<int64_t>(pv) * a.kv.H + h;
+    const int64_t hk = static_cast<int64_t>(pk) * a.kv.H + h;
     const char* ksrc = a.kv.k + (hk * P + (kk & (P - 1)) + (col & 3)) * (DH * ES) + 16 * g;
-    const char* vsrc = a.kv.v + ((hv * DH + col) * P + (kv & (P - 1))) * ES;
     f32x4_t acc[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -395,32 +404,19 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvS
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    const int64_t scale_at = values_of(key0);
     float ksl = 0.f, lvl = 0.f, rvl = 0.f;
     if constexpr (KIND != SRW_KV_BF16) {
-      ksl = a.kv.ks[hv * P + (kv & (P - 1)) + col] * a.sc;
-      in_exponent(a.kv.vs[hv * P + (kv & (P - 1)) + col], lvl, rvl);
+      ksl = a.kv.ks[scale_at] * a.sc;
+      in_exponent(a.kv.vs[scale_at], lvl, rvl);
     }
     u32x4_t pf[2], pl[2];
     weigh<KIND, ND, true, true>(acc, a.sc, ksl, lvl, rvl, false, mine, m, l, o, pf, pl);
-    uint32_t seen = mine;  // bit j: some row sees the lane's key kv + j
-    for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);
-    u16x2_t most = {0, 0};
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      const char* at = vsrc + static_cast<int64_t>(16 * d) * P * ES;
-      u32x4_t raw = ld16(at);
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        u32x4_t v;
-        if constexpr (KIND == SRW_KV_BF16)
-          v = st ? ld16(at + 16) : raw;
-        else
-          v = widen8<KIND>(raw[2 * st], raw[2 * st + 1]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t two = seen >> (8 * st + 2 * u);
-          v[u] &= (two & 1 ? 0x0000ffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
-        }
+        u32x4_t v = value(d, st);
         if constexpr (KIND != SRW_KV_INT8) {
           most = most16(most, v);
           v = finite16(v);
@@ -428,13 +424,35 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvS
         o[d] = mfma16(v, pl[st], mfma16(v, pf[st], o[d]));
         __builtin_amdgcn_sched_barrier(0);
       }
-    }
-    if constexpr (KIND != SRW_KV_INT8) {
-      if (__any(not_finite(most)))
-        add_not_finite<KIND, 4 * ND>(
-            a.kv, tl.b, h, DH, key0, [&](int k) { return kv_seen(pos, key0, a.window, a.sinks) >> k & 1; },
-            [&](int n) { return 16 * (n / 4) + 4 * g + n % 4; }, [&](int n, float v) { o[n / 4][n % 4] += v; });
-    }
+  }
+  if (KIND == SRW_KV_INT8 || !__any(not_finite(most))) return;
+  for (int i = first; i < end; i += step) {
+    values_of(sp.key0(i));
+    // a row gets each kind of number that is not finite which it sees: how many there
+    // are is a product of zeros and ones
+    auto add = [&](auto test, float x) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        f32x4_t n = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          u32x4_t is = value(d, st), sees;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            is[u] = ones16(is[u], test);
+            const uint32_t two = mine >> (8 * st + 2 * u);
+            sees[u] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
+          }
+          n = mfma16(is, sees, n);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[d][r] += n[r] > 0.f ? x : 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    add([](uint32_t b) { return b == 0x7f80u; }, INFINITY);
+    add([](uint32_t b) { return b == 0xff80u; }, -INFINITY);
+    add([](uint32_t b) { return (b & 0x7fffu) > 0x7f80u; }, __uint_as_float(0x7fc00000u));
   }
 }
 
@@ -829,6 +847,13 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
+  // At head_dim 128 the loop has no registers for addresses that it could keep:
+  // they are worked out from the lane again (one that was spilled cost a wait for
+  // the tile's loads in flight: a tenth of a call over small pages).
+  auto fresh = [](int x) {
+    if constexpr (DH == 128) asm volatile("" : "+v"(x));
+    return x;
+  };
   // Slots: pages of 64 and more hold whole tiles (one page each), at slot0 of
   // theirs; smaller ones start with one.  Where tiles lie is worked out 16 at a
   // time, a lane for each group of 16 positions: lane 4 n + u has the byte offset
@@ -843,7 +868,9 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
   int ib = i0, off_lo = 0, off_hi = 0;
   uint64_t have = 0;
   auto locate = [&] {
-    const int i = ib + (lane >> 2), at = sp.key0(i) + 16 * (lane & 3);
+    int ln = lane;  // (once in 16 tiles: not worth a register either)
+    asm volatile("" : "+v"(ln));
+    const int i = ib + (ln >> 2), at = sp.key0(i) + 16 * (ln & 3);
     const int id = i < i1 && at < sp.hi ? kv_page(a.kv, b, at) : -1;
     have = __ballot(id >= 0);
     const int64_t off = (id < 0 ? 0 : id) * page_bytes;
@@ -851,12 +878,6 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
     off_hi = static_cast<int>(off >> 32);
   };
   if (i0 < i1) locate();
-  // At head_dim 128 the loop has no registers for addresses that it could keep:
-  // they are worked out from the lane again.
-  auto fresh = [](int x) {
-    if constexpr (DH == 128) asm volatile("" : "+v"(x));
-    return x;
-  };
   u32x4_t rk, rv;               // 8-bit tiles on their way
   float ksn = 0.f, vsn = 0.f;   // scales of key `lane`
   int havn = 0;                 // bit u: positions 16 u .. have a page
@@ -912,7 +933,7 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
         if (one) {
           g2lds16(vbase + page0 + slot0 * ES + vat[n], vl[stage] + 16 * first);
         } else {
-          const int group = ((lane & 7) ^ v_swz((first + lane) / 8)) >> 1;
+          const int ln = fresh(lane), group = ((ln & 7) ^ v_swz((first + ln) / 8)) >> 1;
           g2lds16(vbase + page_of_lane(group) + vat[n], vl[stage] + 16 * first);
         }
       }
@@ -1052,7 +1073,7 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
             for (int d = 0; d < kBatch / 2; ++d) vf[d][st][u] &= keep;
           }
-       }
+        }
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st)
