@@ -770,14 +770,14 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
 // Vector work fills it most: a score takes 4 (bf16) or 5 (8 bits) instructions
 // and an exponential, which costs 2.5 of them, against 4 head_dim products.  Of a
 // long chunk's SIMD cycles the vector ALU is active for 70%, the matrix cores for
-// 30%; the LDS, whose every fragment feeds one product, is for 44% of a CU's.  None
+// 29%; the LDS, whose every fragment feeds one product, is for 44% of a CU's.  None
 // is full: a wave alone issues a vector instruction every 8 cycles, half the SIMD's
 // rate, and matrix instructions run beside other waves' vector ones; so what counts
 // is waves on a SIMD, and with 16 rows a wave (at most 128 registers) four fit,
 // where 32 rows (240 registers at head_dim 128) left two.
 //
 // Measured: 2 048 tokens of 32 heads over 30 011 positions of 8, int8, head_dim
-// 128, in 1 400 us, 0.74 PFLOP/s (32 rows a wave: 1 363, but calls of few tiles
+// 128, in 1 400 to 1 430 us, 0.73 PFLOP/s (32 rows a wave: 1 363, but calls of few tiles
 // twice as long); 8 prompts of 512 of 6 heads of 64, bf16, in 14 us (39 so).
 template <int DH> __device__ inline int k_swz(int row) {
   // a fragment's 16 rows are 16 u + 4 t + v, u, v = 0 .. 3
