@@ -698,7 +698,7 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
 // positions in 8 splits: 14 with one group, 23 with all).
 template <int DH, int W, int TH>
 __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const float2* ml, uint16_t* out, int64_t rows,
-                                                       int S) {
+                                                       int S, const int32_t* cu, int64_t B, int Hq) {
   constexpr int L = DH / 4, N = TH / L;  // lanes a group, groups
   const int c = threadIdx.x % L, first = threadIdx.x / L / W * W, grp = threadIdx.x / L - first;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (N / W) + first / W;
@@ -754,6 +754,9 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
     }
   }
   if (at >= rows) return;
+  // (no split wrote rows that no sequence names, and neither is written here)
+  const int64_t t = row / Hq;
+  if (cu && (t < cu[0] || t >= cu[B])) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(out + row * DH + 4 * c) =
       make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
@@ -1159,7 +1162,7 @@ hipError_t launch_attention(const srw_attention_t& a, const AttnPlan& pl, AttnAr
   auto join = [&](auto w, auto th) {
     constexpr int W = decltype(w)::value, TH = decltype(th)::value, R = TH / (DH / 4) / W;
     hipLaunchKernelGGL((attn_join_kernel<DH, W, TH>), dim3(static_cast<unsigned>((rows + R - 1) / R)), dim3(TH), 0, s,
-                       g.part, g.ml, g.out, rows, g.S);
+                       g.part, g.ml, g.out, rows, g.S, g.kv.cu, g.kv.B, g.Hq);
   };
   using std::integral_constant;
   if (g.S <= 8)
