@@ -15,7 +15,9 @@ from ._capi import SrwError, SrwLibraryError, load_library  # noqa: F401
 from .layer import GateConfig, SrwBackwardPlan, SrwBatchPlan, SrwPlan, srw_backward, srw_forward  # noqa: F401
 from .srw import (chunk_plan, make_sharded_srw, make_sharded_srw_paired, make_sharded_srw_v401,  # noqa: F401
                   make_sharded_srw_paired_v401, srw_inference, srw_inference_with_gates)
-from .kv import KvPages, PagedKvCache, kv_read, kv_write, paged_attention  # noqa: F401
+from .kv import (KvIndex, KvPages, PagedKvCache, kv_copy, kv_index, kv_read, kv_select, kv_write,  # noqa: F401
+                 paged_attention)
+from .sampling import sample  # noqa: F401
 from . import checkpoint, data, inputs, model  # noqa: F401
 from .model import DawnConfig, DawnModel, init_params  # noqa: F401
 
@@ -23,5 +25,6 @@ __all__ = ["SrwError", "SrwLibraryError", "load_library", "GateConfig",
            "SrwPlan", "SrwBatchPlan", "SrwBackwardPlan", "srw_forward", "srw_backward", "chunk_plan",
            "make_sharded_srw", "make_sharded_srw_paired", "make_sharded_srw_v401",
            "make_sharded_srw_paired_v401", "srw_inference", "srw_inference_with_gates",
-           "KvPages", "PagedKvCache", "kv_write", "kv_read", "paged_attention",
+           "KvPages", "KvIndex", "PagedKvCache", "kv_write", "kv_read", "kv_copy", "kv_index", "kv_select",
+           "paged_attention", "sample",
            "inputs", "model", "checkpoint", "data", "DawnConfig", "DawnModel", "init_params"]

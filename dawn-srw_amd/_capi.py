@@ -60,6 +60,8 @@ EXPORTED_SYMBOLS = (
     "srw_workspace_size_batch", "srw_forward_batch", "srw_forward_noalloc",
     "srw_diag_summary", "srw_cast_bf16", "srw_dawn_decode_step",
     "srw_kv_write", "srw_kv_read", "srw_attention_workspace_size", "srw_attention", "srw_attention_plan",
+    "srw_kv_copy", "srw_kv_index", "srw_kv_select", "srw_attention_kept_workspace_size", "srw_attention_kept",
+    "srw_sample",
 )
 
 # srw_diag_out_t: the result tuple's per-token values and scalars (SRW_DSUM_*)
@@ -149,6 +151,38 @@ class SrwAttention(ctypes.Structure):
         + [(n, ctypes.c_int32) for n in ("n_heads", "max_new", "window", "sinks")] + [("scale", ctypes.c_float)])
 
 
+COPY_TENSORS = 8       # SRW_KV_COPY_TENSORS
+
+
+class SrwKvCopy(ctypes.Structure):
+    _fields_ = (
+        [(n, ctypes.c_void_p * COPY_TENSORS) for n in ("src", "dst")]
+        + [(n, ctypes.c_int64 * COPY_TENSORS) for n in ("page_bytes", "src_layer_stride", "dst_layer_stride")]
+        + [(n, ctypes.c_int64) for n in ("n_layers", "n_src_pages", "n_dst_pages", "n_pairs")]
+        + [(n, ctypes.c_void_p) for n in ("src_page", "dst_page")]
+        + [(n, ctypes.c_int32) for n in ("n_tensors", "reserved")])
+
+
+class SrwKvIndex(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scale")]
+
+
+class SrwKvSelect(ctypes.Structure):
+    _fields_ = (
+        [("kv", SrwKv), ("index", SrwKvIndex), ("q", ctypes.c_void_p), ("keep", ctypes.c_void_p)]
+        + [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride")]
+        + [(n, ctypes.c_int32) for n in ("n_heads", "n", "first", "last")])
+
+
+class SrwSample(ctypes.Structure):
+    _fields_ = (
+        [("logits", ctypes.c_void_p)]
+        + [(n, ctypes.c_int64) for n in ("row_stride", "B", "V")]
+        + [(n, ctypes.c_void_p) for n in ("u", "temperature", "top_p", "min_p", "top_k", "token", "logprob")]
+        + [(n, ctypes.c_float) for n in ("temperature_all", "top_p_all", "min_p_all")]
+        + [(n, ctypes.c_int32) for n in ("top_k_all", "dtype", "reserved")])
+
+
 class SrwError(RuntimeError):
     """A non-OK status returned by libsrw_amd.so."""
 
@@ -234,6 +268,16 @@ def load_library() -> ctypes.CDLL:
         lib.srw_attention_plan.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]
         lib.srw_attention.restype = ctypes.c_int
         lib.srw_attention.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        for name in ("srw_kv_copy", "srw_kv_select", "srw_sample"):
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        lib.srw_kv_index.restype = ctypes.c_int
+        lib.srw_kv_index.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+        lib.srw_attention_kept_workspace_size.restype = ctypes.c_int
+        lib.srw_attention_kept_workspace_size.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]
+        lib.srw_attention_kept.restype = ctypes.c_int
+        lib.srw_attention_kept.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                           ctypes.c_size_t, ctypes.c_void_p]
         got = lib.srw_abi_version()
         if got != ABI_VERSION:
             raise SrwLibraryError(f"libsrw_amd.so ABI {got} != binding ABI {ABI_VERSION}")

@@ -65,6 +65,28 @@ struct AttnArgs {
   int S, least;   // splits of a row tile's key tiles, of so many at least
 };
 
+// Attention to kept pages alone: the lists' places of the pages, in the order of a
+// token's and key head's list, stand for its positions.
+struct KeptArgs : AttnArgs {
+  const int32_t* keep;  // [T][H][n]
+  int n;
+};
+
+// The 16 positions at 16 u of a list's tile i: their page (-1: none) and first position.
+struct Group {
+  int page, at;
+};
+__device__ inline Group kept_group(const KeptArgs& a, int64_t b, const int32_t* list, int i, int u) {
+  const int v = kTile * i + kKvGroup * u, e = v >> a.kv.logP;
+  if (e >= a.n) return {-1, 0};
+  const int place = list[e], before = e > 0 ? list[e - 1] : -1;
+  if (place <= before || place < 0 || place >= a.kv.cap >> a.kv.logP) return {-1, 0};
+  const int at = (place << a.kv.logP) + (v & (a.kv.P - 1));
+  return {kv_page(a.kv, b, at), at};
+}
+// Bit j: a token at position pos sees at + j.
+__device__ inline uint32_t seen16(int pos, int at) { return pos < at ? 0u : static_cast<uint32_t>(low_bits(pos - at + 1)) & 0xffffu; }
+
 __device__ inline KvSpan span_of(const AttnArgs& a, int p_lo, int p_hi) {
   return kv_span(a.kv.cap, a.window, a.sinks, p_lo, p_hi);
 }
@@ -105,6 +127,20 @@ __device__ inline Tile tile_of(const AttnArgs& a, int64_t at) {
   return t;
 }
 
+// The 16 rows from 16 `part` on of token t's heads of a group; r0 = -1: the token is
+// no sequence's.
+__device__ inline Tile token_tile(const AttnArgs& a, int64_t t, int part) {
+  Tile tl;
+  tl.b = a.kv.cu ? kv_find(a.kv.B, t, [&](int64_t i) { return static_cast<int64_t>(a.kv.cu[i]); }) : t;
+  tl.b = __builtin_amdgcn_readfirstlane(static_cast<int>(tl.b));
+  tl.sq = kv_seq(a.kv, tl.b);
+  const int64_t tok = t - tl.sq.row0;
+  const bool in = tok >= 0 && tok < tl.sq.n;
+  const int first = in ? static_cast<int>(tok) * a.G : 0;
+  tl.r0 = in ? first + 16 * part : -1;
+  tl.r1 = first + 16 * part + 16 < first + a.G ? first + 16 * part + 16 : first + a.G;
+  return tl;
+}
 __device__ inline f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
@@ -330,9 +366,11 @@ __device__ inline void weigh(f32x4_t (&acc)[4], float sc, float ksl, float lvl, 
 // of a span, for scores and values of any size: straight from memory, a fragment
 // at a time.  Values that are not finite are kept out of the products; where there
 // are any, a second pass adds them to the rows that see them.
-template <int KIND, int DH>
-__device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvSpan& sp, int h, int r0, int r1, int first,
-                                    int end, int step, float& m, float& l, f32x4_t (&o)[DH / 16]) {
+// (Of KeptArgs: of the list.)
+template <int KIND, int DH, class Args>
+__device__ inline void careful_rows(const Args& a, const Tile& tl, const KvSpan& sp, const int32_t* list, int h, int r0,
+                                    int r1, int first, int end, int step, float& m, float& l, f32x4_t (&o)[DH / 16]) {
+  constexpr bool KEPT = std::is_same<Args, KeptArgs>::value;
   constexpr int ES = kv_bytes<KIND>();
   constexpr int ND = DH / 16;
   int lane = threadIdx.x & 63;
@@ -347,10 +385,18 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvS
   // key 16 g + j), which any row does, and their values
   uint32_t mine, seen;
   const char* vsrc;
-  auto values_of = [&](int key0) {
-    const int kv = key0 + 16 * g;
-    const int pv = kv < sp.hi ? kv_page(a.kv, tl.b, kv) : -1;
-    mine = pv < 0 ? 0u : static_cast<uint32_t>(kv_seen(pos, key0, a.window, a.sinks) >> (16 * g)) & 0xffffu;
+  auto values_of = [&](int i) {
+    const int key0 = sp.key0(i);
+    int kv = key0 + 16 * g, pv;
+    if constexpr (KEPT) {
+      const Group gr = kept_group(a, tl.b, list, i, g);
+      kv = gr.at;
+      pv = gr.page;
+      mine = pv < 0 ? 0u : seen16(pos, kv);
+    } else {
+      pv = kv < sp.hi ? kv_page(a.kv, tl.b, kv) : -1;
+      mine = pv < 0 ? 0u : static_cast<uint32_t>(kv_seen(pos, key0, a.window, a.sinks) >> (16 * g)) & 0xffffu;
+    }
     seen = mine;
     for (int w = 1; w < 16; w <<= 1) seen |= __shfl_xor(seen, w);
     const int64_t hv = static_cast<int64_t>(pv < 0 ? 0 : pv) * a.kv.H + h;
@@ -381,8 +427,14 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvS
   for (int i = first; i < end; i += step) {
     const int key0 = sp.key0(i);
     // (rows of the first product as in attn_rows_kernel)
-    const int kk = key0 + 16 * (col >> 2);
-    int pk = kk < sp.hi ? kv_page(a.kv, tl.b, kk) : -1;
+    int kk = key0 + 16 * (col >> 2), pk;
+    if constexpr (KEPT) {
+      const Group gr = kept_group(a, tl.b, list, i, col >> 2);
+      kk = gr.at;
+      pk = gr.page;
+    } else {
+      pk = kk < sp.hi ? kv_page(a.kv, tl.b, kk) : -1;
+    }
     pk = pk < 0 ? 0 : pk;
     const int64_t hk = static_cast<int64_t>(pk) * a.kv.H + h;
     const char* ksrc = a.kv.k + (hk * P + (kk & (P - 1)) + (col & 3)) * (DH * ES) + 16 * g;
@@ -404,7 +456,7 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvS
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    const int64_t scale_at = values_of(key0);
+    const int64_t scale_at = values_of(i);
     float ksl = 0.f, lvl = 0.f, rvl = 0.f;
     if constexpr (KIND != SRW_KV_BF16) {
       ksl = a.kv.ks[scale_at] * a.sc;
@@ -427,7 +479,7 @@ __device__ inline void careful_rows(const AttnArgs& a, const Tile& tl, const KvS
   }
   if (KIND == SRW_KV_INT8 || !__any(not_finite(most))) return;
   for (int i = first; i < end; i += step) {
-    values_of(sp.key0(i));
+    values_of(i);
     // a row gets each kind of number that is not finite which it sees: how many there
     // are is a product of zeros and ones
     auto add = [&](auto test, float x) {
@@ -487,8 +539,13 @@ __device__ inline bool careful_again(float m, float l, const f32x4_t (&o)[ND]) {
 template <int KIND, int DH, int NQ> constexpr int rows_waves() {
   return NQ > 1 ? 1 : DH == 64 ? 4 : KIND == SRW_KV_BF16 ? 2 : 3;
 }
-template <int KIND, int DH, int NQ>
-__global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_kernel(AttnArgs a) {
+//
+// Of KeptArgs: a workgroup takes up to 16 heads of one token; where the tiles of its
+// list lie is worked out 16 tiles of a wave at a time, a lane for each group of 16
+// positions, so that the chain of list, table and page is waited for once.
+template <int KIND, int DH, int NQ, class Args>
+__global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_kernel(Args a) {
+  constexpr bool KEPT = std::is_same<Args, KeptArgs>::value;
   constexpr int ES = kv_bytes<KIND>();
   constexpr int NPC = DH * ES / 64;  // 16-byte pieces of a key a lane
   constexpr int NS = DH / 32;        // k-steps of the first product
@@ -498,14 +555,28 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
   const int split = blockIdx.z, h = blockIdx.y;
-  const Tile tl = tile_of<16 * NQ>(a, blockIdx.x);
-  if (tl.r0 < 0) return;
+  Tile tl;
+  const int32_t* list = nullptr;
+  if constexpr (KEPT) {
+    const int per = (a.G + 15) / 16;
+    const int64_t t = blockIdx.x / per;
+    tl = token_tile(a, t, static_cast<int>(blockIdx.x % per));
+    if (tl.r0 < 0) return;
+    list = a.keep + (t * a.kv.H + h) * a.n;
+  } else {
+    tl = tile_of<16 * NQ>(a, blockIdx.x);
+    if (tl.r0 < 0) return;
+  }
   const int64_t b = tl.b;
   const KvSeq sq = tl.sq;
   const int r0 = tl.r0, r1 = tl.r1;
   const int P = a.kv.P;
   const int p_lo = sq.len - sq.n + r0 / a.G, p_hi = sq.len - sq.n + (r1 - 1) / a.G;
-  const KvSpan sp = span_of(a, p_lo, p_hi);
+  KvSpan sp{};
+  if constexpr (KEPT)
+    sp.tiles = p_lo < 0 ? 0 : static_cast<int>((static_cast<int64_t>(a.n) * P + kTile - 1) / kTile);
+  else
+    sp = span_of(a, p_lo, p_hi);
   const int per = per_split(a, sp.tiles);
   const int i0 = split * per;
   const int i1 = i0 + per < sp.tiles ? i0 + per : sp.tiles;
@@ -536,13 +607,29 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[x][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+  Group gr{-1, 0};  // of the list's tile i0 + wave + 4 (16 n + lane / 4)
   for (int i = i0 + wave; i < i1; i += 4) {
     const int key0 = sp.key0(i);
     // rows of the first product: row 4 u + v of its tile t is key 16 u + 4 t
     // + v, so lane (col, g) loads keys of group col / 4 and its score
     // registers, like its k-slots of the second product, are those of group g
-    const int kk = key0 + 16 * (col >> 2), kv = key0 + 16 * g;
-    int pk = kk < sp.hi ? kv_page(a.kv, b, kk) : -1, pv = kv < sp.hi ? kv_page(a.kv, b, kv) : -1;
+    int kk = key0 + 16 * (col >> 2), kv = key0 + 16 * g, pk, pv;
+    if constexpr (KEPT) {
+      const int n = (i - i0) >> 2 & 15;
+      if (n == 0) {
+        const int to = i + 4 * (lane >> 2);
+        gr = to < i1 ? kept_group(a, b, list, to, lane & 3) : Group{-1, 0};
+        if (gr.at > p_lo) gr.page = -1;
+      }
+      if (!(__ballot(gr.page >= 0) >> (4 * n) & 15)) continue;  // nothing that the token sees
+      pk = __shfl(gr.page, 4 * n + (col >> 2));
+      kk = __shfl(gr.at, 4 * n + (col >> 2));
+      pv = __shfl(gr.page, 4 * n + g);
+      kv = __shfl(gr.at, 4 * n + g);
+    } else {
+      pk = kk < sp.hi ? kv_page(a.kv, b, kk) : -1;
+      pv = kv < sp.hi ? kv_page(a.kv, b, kv) : -1;
+    }
     const bool have = pv >= 0;
     pk = pk < 0 ? 0 : pk;
     pv = pv < 0 ? 0 : pv;
@@ -585,15 +672,22 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
       }
     }
     // every row sees every key of the tile?
-    const bool whole = __all(have) && key0 + kTile - 1 <= p_lo &&
-                       (a.window == 0 || key0 > p_hi - a.window || key0 + kTile <= a.sinks);
+    bool whole;
+    if constexpr (KEPT)
+      whole = __all(have && kv + kKvGroup - 1 <= p_lo);
+    else
+      whole = __all(have) && key0 + kTile - 1 <= p_lo &&
+              (a.window == 0 || key0 > p_hi - a.window || key0 + kTile <= a.sinks);
     uint32_t seen = 0;  // bit j: some row of the tile sees the lane's key kv + j
     u32x4_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       uint32_t mine = 0xffffu;
       if (!whole) {
-        mine = have ? static_cast<uint32_t>(kv_seen(pos[x], key0, a.window, a.sinks) >> (16 * g)) & 0xffffu : 0u;
+        if constexpr (KEPT)
+          mine = have ? seen16(pos[x], kv) : 0u;
+        else
+          mine = have ? static_cast<uint32_t>(kv_seen(pos[x], key0, a.window, a.sinks) >> (16 * g)) & 0xffffu : 0u;
         seen |= mine;
       }
       weigh<KIND, ND, true>(acc[x], a.sc, ksl, lvl, rvl, whole, mine, m[x], l[x], o[x], pf[x], pl[x]);
@@ -630,7 +724,7 @@ __global__ __launch_bounds__(256, (rows_waves<KIND, DH, NQ>())) void attn_rows_k
 
 #pragma unroll
   for (int x = 0; x < NQ; ++x)
-    if (careful_again(m[x], l[x], o[x])) careful_rows<KIND, DH>(a, tl, sp, h, r0 + 16 * x, r1, i0 + wave, i1, 4, m[x], l[x], o[x]);
+    if (careful_again(m[x], l[x], o[x])) careful_rows<KIND, DH>(a, tl, sp, list, h, r0 + 16 * x, r1, i0 + wave, i1, 4, m[x], l[x], o[x]);
 
   // join the four waves
   auto sum = [](float u, float w) { return u + w; };
@@ -1085,7 +1179,7 @@ __global__ __launch_bounds__(512, 4) void attn_tile_kernel(AttnArgs a) {
     }
   }
   if (!active) return;
-  if (careful_again(m, l, o)) careful_rows<KIND, DH>(a, tl, sp, h, w0, r1, i0, i1, 1, m, l, o);
+  if (careful_again(m, l, o)) careful_rows<KIND, DH>(a, tl, sp, nullptr, h, w0, r1, i0, i1, 1, m, l, o);
   auto sum = [](float u, float w) { return u + w; };
   l = join32(join16(l, sum), sum);
   const Place p = place();
@@ -1147,18 +1241,9 @@ AttnPlan plan_of(const srw_attention_t& a) {
   return p;
 }
 
-template <int KIND, int DH>
-hipError_t launch_attention(const srw_attention_t& a, const AttnPlan& pl, AttnArgs& g, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(pl.tiles), static_cast<unsigned>(g.kv.H), static_cast<unsigned>(g.S));
-  if (pl.rows == 16)
-    hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 1>), grid, dim3(256), 0, s, g);
-  else if (pl.rows == 32)
-    hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 2>), grid, dim3(256), 0, s, g);
-  else
-    hipLaunchKernelGGL((attn_tile_kernel<KIND, DH>), grid, dim3(512), 0, s, g);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || g.S == 1) return e;
-  const int64_t rows = a.kv.T * a.n_heads;
+template <int DH>
+hipError_t launch_join(const AttnArgs& g, hipStream_t s) {
+  const int64_t rows = g.kv.T * g.Hq;
   auto join = [&](auto w, auto th) {
     constexpr int W = decltype(w)::value, TH = decltype(th)::value, R = TH / (DH / 4) / W;
     hipLaunchKernelGGL((attn_join_kernel<DH, W, TH>), dim3(static_cast<unsigned>((rows + R - 1) / R)), dim3(TH), 0, s,
@@ -1174,26 +1259,52 @@ hipError_t launch_attention(const srw_attention_t& a, const AttnPlan& pl, AttnAr
   return hipGetLastError();
 }
 
+template <int KIND, int DH>
+hipError_t launch_attention(const AttnPlan& pl, const AttnArgs& g, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(pl.tiles), static_cast<unsigned>(g.kv.H), static_cast<unsigned>(g.S));
+  if (pl.rows == 16)
+    hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 1, AttnArgs>), grid, dim3(256), 0, s, g);
+  else if (pl.rows == 32)
+    hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 2, AttnArgs>), grid, dim3(256), 0, s, g);
+  else
+    hipLaunchKernelGGL((attn_tile_kernel<KIND, DH>), grid, dim3(512), 0, s, g);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || g.S == 1 ? e : launch_join<DH>(g, s);
+}
+
+template <int KIND, int DH>
+hipError_t launch_attention(const AttnPlan& pl, const KeptArgs& g, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(pl.tiles), static_cast<unsigned>(g.kv.H), static_cast<unsigned>(g.S));
+  hipLaunchKernelGGL((attn_rows_kernel<KIND, DH, 1, KeptArgs>), grid, dim3(256), 0, s, g);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || g.S == 1 ? e : launch_join<DH>(g, s);
+}
+
+// A call over lists of n pages: every token's tiles are as many, so splits are only for
+// calls of too few workgroups.
+AttnPlan kept_plan(const srw_attention_t& a, int64_t n) {
+  AttnPlan p{};
+  const int64_t G = a.n_heads / a.kv.n_kv_heads, H = a.kv.n_kv_heads;
+  p.rows = 16;
+  p.tiles = a.kv.T * ((G + 15) / 16);
+  p.least = 4;
+  const int64_t tiles = (n * a.kv.page_size + kTile - 1) / kTile, groups = p.tiles * H;
+  const int64_t S = groups >= 512 || tiles <= 12 ? 1 : 1024 / groups, most = tiles / p.least;
+  p.S = static_cast<int>(S < most ? S : most > 1 ? most : 1);
+  return p;
+}
+
 size_t align256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
 
-}  // namespace
-
-size_t attention_workspace_bytes(const srw_attention_t& a) {
-  const AttnPlan p = plan_of(a);
-  if (p.S == 1) return 0;
-  const size_t rows = static_cast<size_t>(a.kv.T) * a.n_heads * p.S;
+// Partial results of S splits: (m, l), then outputs.
+size_t split_bytes(const srw_attention_t& a, int S) {
+  if (S == 1) return 0;
+  const size_t rows = static_cast<size_t>(a.kv.T) * a.n_heads * S;
   return align256(rows * sizeof(float2)) + align256(rows * a.kv.head_dim * sizeof(float));
 }
 
-void attention_plan(const srw_attention_t& a, int32_t* rows, int32_t* splits) {
-  const AttnPlan p = plan_of(a);
-  *rows = p.rows;
-  *splits = p.S;
-}
-
-hipError_t attention(const srw_attention_t& a, char* ws, hipStream_t s) {
-  const AttnPlan p = plan_of(a);
-  AttnArgs g{};
+template <class Args>
+hipError_t run(const srw_attention_t& a, const AttnPlan& p, Args& g, char* ws, hipStream_t s) {
   g.kv = kv_view(a.kv);
   g.q = static_cast<const uint16_t*>(a.q);
   g.out = static_cast<uint16_t*>(a.out);
@@ -1212,13 +1323,36 @@ hipError_t attention(const srw_attention_t& a, char* ws, hipStream_t s) {
   }
   auto by = [&](auto kind) {
     constexpr int K = decltype(kind)::value;
-    return a.kv.head_dim == 64 ? launch_attention<K, 64>(a, p, g, s) : launch_attention<K, 128>(a, p, g, s);
+    return a.kv.head_dim == 64 ? launch_attention<K, 64>(p, g, s) : launch_attention<K, 128>(p, g, s);
   };
   switch (a.kv.kind) {
     case SRW_KV_BF16: return by(std::integral_constant<int, SRW_KV_BF16>{});
     case SRW_KV_INT8: return by(std::integral_constant<int, SRW_KV_INT8>{});
     default: return by(std::integral_constant<int, SRW_KV_FP8>{});
   }
+}
+
+}  // namespace
+
+size_t attention_workspace_bytes(const srw_attention_t& a) { return split_bytes(a, plan_of(a).S); }
+size_t attention_kept_workspace_bytes(const srw_attention_t& a, int64_t n_keep) { return split_bytes(a, kept_plan(a, n_keep).S); }
+
+void attention_plan(const srw_attention_t& a, int32_t* rows, int32_t* splits) {
+  const AttnPlan p = plan_of(a);
+  *rows = p.rows;
+  *splits = p.S;
+}
+
+hipError_t attention(const srw_attention_t& a, char* ws, hipStream_t s) {
+  AttnArgs g{};
+  return run(a, plan_of(a), g, ws, s);
+}
+
+hipError_t attention_kept(const srw_attention_t& a, const int32_t* keep, int64_t n_keep, char* ws, hipStream_t s) {
+  KeptArgs g{};
+  g.keep = keep;
+  g.n = static_cast<int>(n_keep);
+  return run(a, kept_plan(a, n_keep), g, ws, s);
 }
 
 }  // namespace srw

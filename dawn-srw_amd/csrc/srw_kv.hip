@@ -313,6 +313,8 @@ hipError_t rows_by_kind(const srw_kv_t& c, const KvRows& r, hipStream_t s) {
 
 bool aligned(const void* q, size_t a) { return q && !(reinterpret_cast<uintptr_t>(q) & (a - 1)); }
 
+}  // namespace
+
 srw_status_t check_kv(const srw_kv_t* c) {
   if (!c) return SRW_EINVAL;
   if (c->B < 0 || c->T < 0 || c->n_pages < 0 || c->table_width < 0 || c->n_kv_heads < 1) return SRW_EINVAL;
@@ -335,6 +337,8 @@ srw_status_t check_kv(const srw_kv_t* c) {
   return SRW_OK;
 }
 
+namespace {
+
 // Rows of dtype at these strides, read or written four elements at a time.
 srw_status_t check_rows(const srw_kv_t& c, const KvRows& r, int32_t dtype) {
   if (dtype != SRW_F32 && dtype != SRW_BF16) return SRW_EINVAL;
@@ -355,6 +359,23 @@ srw_status_t check_attention(const srw_attention_t* a) {
   if (!isfinite(a->scale)) return SRW_EINVAL;
   // rows of a call: tokens x heads
   if (a->kv.T > 0 && a->n_heads > 0x7fffffff / a->kv.T) return SRW_EUNSUPPORTED;
+  return SRW_OK;
+}
+
+// q rows are read 16 bytes at a time, out is written 8
+srw_status_t check_queries(const srw_attention_t& a) {
+  if (!aligned(a.q, 16) || !aligned(a.out, 16)) return SRW_EINVAL;
+  if (a.q_token_stride < 0 || a.q_head_stride < 0 || a.q_token_stride % 8 || a.q_head_stride % 8) return SRW_EINVAL;
+  return SRW_OK;
+}
+
+srw_status_t check_kept(const srw_attention_t* a, int64_t n_keep) {
+  const srw_status_t st = check_attention(a);
+  if (st != SRW_OK) return st;
+  if (n_keep < 1 || a->window != 0) return SRW_EINVAL;
+  // positions of a list are counted in 32 bits; a launch has under 2^32 threads
+  if (n_keep > 0x7fff0000 / a->kv.page_size) return SRW_EUNSUPPORTED;
+  if (a->kv.T * ((a->n_heads / a->kv.n_kv_heads + 15) / 16) >= (1 << 24)) return SRW_EUNSUPPORTED;
   return SRW_OK;
 }
 
@@ -418,14 +439,37 @@ srw_status_t srw_attention(const srw_attention_t* a, void* workspace, size_t wor
   const srw_status_t st = srw::check_attention(a);
   if (st != SRW_OK) return st;
   if (a->kv.T == 0) return SRW_OK;
-  // q rows are read 16 bytes at a time, out is written 8
-  if (!srw::aligned(a->q, 16) || !srw::aligned(a->out, 16)) return SRW_EINVAL;
-  if (a->q_token_stride < 0 || a->q_head_stride < 0 || a->q_token_stride % 8 || a->q_head_stride % 8) return SRW_EINVAL;
+  const srw_status_t q = srw::check_queries(*a);
+  if (q != SRW_OK) return q;
   const size_t need = srw::attention_workspace_bytes(*a);
   if (need > 0 && (!srw::aligned(workspace, 16) || workspace_bytes < need)) return SRW_EWORKSPACE;
   (void)hipGetLastError();
   return srw::attention(*a, static_cast<char*>(workspace), static_cast<hipStream_t>(stream)) == hipSuccess ? SRW_OK
                                                                                                          : SRW_EHIP;
+}
+
+srw_status_t srw_attention_kept_workspace_size(const srw_attention_t* a, int64_t n_keep, size_t* bytes) {
+  const srw_status_t st = srw::check_kept(a, n_keep);
+  if (st != SRW_OK) return st;
+  if (!bytes) return SRW_EINVAL;
+  *bytes = a->kv.T == 0 ? 0 : srw::attention_kept_workspace_bytes(*a, n_keep);
+  return SRW_OK;
+}
+
+srw_status_t srw_attention_kept(const srw_attention_t* a, const int32_t* keep, int64_t n_keep, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  srw_status_t st = srw::check_kept(a, n_keep);
+  if (st != SRW_OK) return st;
+  if (a->kv.T == 0) return SRW_OK;
+  st = srw::check_queries(*a);
+  if (st != SRW_OK) return st;
+  if (!srw::aligned(keep, 4)) return SRW_EINVAL;
+  const size_t need = srw::attention_kept_workspace_bytes(*a, n_keep);
+  if (need > 0 && (!srw::aligned(workspace, 16) || workspace_bytes < need)) return SRW_EWORKSPACE;
+  (void)hipGetLastError();
+  return srw::attention_kept(*a, keep, n_keep, static_cast<char*>(workspace), static_cast<hipStream_t>(stream)) == hipSuccess
+             ? SRW_OK
+             : SRW_EHIP;
 }
 
 }  // extern "C"

@@ -211,8 +211,11 @@ struct KvRows {
 };
 hipError_t kv_write(const srw_kv_t& c, const KvRows& r, bool f32, hipStream_t s);
 hipError_t kv_read(const srw_kv_t& c, const KvRows& r, bool f32, hipStream_t s);
+srw_status_t check_kv(const srw_kv_t* c);
 size_t attention_workspace_bytes(const srw_attention_t& a);
 void attention_plan(const srw_attention_t& a, int32_t* rows, int32_t* splits);
 hipError_t attention(const srw_attention_t& a, char* ws, hipStream_t s);
+size_t attention_kept_workspace_bytes(const srw_attention_t& a, int64_t n_keep);
+hipError_t attention_kept(const srw_attention_t& a, const int32_t* keep, int64_t n_keep, char* ws, hipStream_t s);
 
 }  // namespace srw

@@ -1,0 +1,617 @@
+// srw_pages.hip -- the paged cache's pages: copies of them, an index of what their
+// keys are about, and the choice of pages by it.
+
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "srw_kv.hpp"
+
+namespace srw {
+namespace {
+
+bool aligned(const void* q, size_t a) { return q && !(reinterpret_cast<uintptr_t>(q) & (a - 1)); }
+
+// -- copies -------------------------------------------------------------------------
+//
+// A workgroup copies up to kPiece bytes of one page of one layer of one tensor, every
+// lane four 16-byte loads in flight.  The pairs travel as kernel arguments, so a call
+// copies nothing to the device first and waits for nothing.
+constexpr int kPiece = 16384, kPairs = 256, kCopyThreads = 256;
+
+struct CopyArgs {
+  const char* src[SRW_KV_COPY_TENSORS];
+  char* dst[SRW_KV_COPY_TENSORS];
+  int64_t page[SRW_KV_COPY_TENSORS];                                // bytes
+  int64_t src_layer[SRW_KV_COPY_TENSORS], dst_layer[SRW_KV_COPY_TENSORS];
+  int32_t begin[SRW_KV_COPY_TENSORS + 1];                           // of each tensor's pieces
+  int32_t n, wide;                                                  // tensors; bit i: tensor i in units of 16 bytes
+  int32_t from[kPairs], to[kPairs];
+};
+
+template <typename U>
+__device__ inline void copy_piece(const char* src, char* dst, int bytes) {
+  constexpr int K = kPiece / kCopyThreads / sizeof(U), N = K < 4 ? K : 4;
+  const U* s = reinterpret_cast<const U*>(src);
+  U* d = reinterpret_cast<U*>(dst);
+  const int n = bytes / static_cast<int>(sizeof(U));
+  for (int i = threadIdx.x; i < n; i += N * kCopyThreads) {
+    U x[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (i + k * kCopyThreads < n) x[k] = __builtin_nontemporal_load(s + i + k * kCopyThreads);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (i + k * kCopyThreads < n) __builtin_nontemporal_store(x[k], d + i + k * kCopyThreads);
+  }
+}
+
+__global__ __launch_bounds__(kCopyThreads) void kv_copy_kernel(CopyArgs a) {
+  int t = 0;
+  const int at = blockIdx.x;
+  while (t + 1 < a.n && at >= a.begin[t + 1]) ++t;
+  const int64_t page = a.page[t], off = static_cast<int64_t>(at - a.begin[t]) * kPiece;
+  const char* src = a.src[t] + blockIdx.z * a.src_layer[t] + a.from[blockIdx.y] * page + off;
+  char* dst = a.dst[t] + blockIdx.z * a.dst_layer[t] + a.to[blockIdx.y] * page + off;
+  const int bytes = static_cast<int>(page - off < kPiece ? page - off : kPiece);
+  if (a.wide >> t & 1)
+    copy_piece<u32x4_t>(src, dst, bytes);
+  else
+    copy_piece<uint32_t>(src, dst, bytes);
+}
+
+// Whether [a, a + m) and [b, b + n) meet.
+bool meet(const void* a, int64_t m, const void* b, int64_t n) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + static_cast<uintptr_t>(n) && y < x + static_cast<uintptr_t>(m);
+}
+
+srw_status_t check_copy(const srw_kv_copy_t* c) {
+  if (!c || c->n_tensors < 0 || c->n_tensors > SRW_KV_COPY_TENSORS) return SRW_EINVAL;
+  if (c->n_layers < 0 || c->n_src_pages < 0 || c->n_dst_pages < 0 || c->n_pairs < 0) return SRW_EINVAL;
+  if (c->n_layers > 65535 || c->n_src_pages > 0x7fffffff || c->n_dst_pages > 0x7fffffff) return SRW_EUNSUPPORTED;
+  if (c->n_pairs > c->n_dst_pages) return SRW_EINVAL;  // (some page is written twice)
+  if (c->n_pairs == 0 || c->n_layers == 0 || c->n_tensors == 0) return SRW_OK;
+  if (!aligned(c->src_page, 4) || !aligned(c->dst_page, 4)) return SRW_EINVAL;
+  int64_t src_bytes[SRW_KV_COPY_TENSORS], dst_bytes[SRW_KV_COPY_TENSORS];
+  bool inside = false;  // tensors copied within themselves
+  for (int i = 0; i < c->n_tensors; ++i) {
+    if (c->page_bytes[i] < 1 || c->page_bytes[i] % 4) return SRW_EINVAL;
+    if (c->page_bytes[i] > (int64_t{1} << 30)) return SRW_EUNSUPPORTED;
+    if (!aligned(c->src[i], 4) || !aligned(c->dst[i], 4)) return SRW_EINVAL;
+    auto span = [&](int64_t stride, int64_t pages, int64_t* bytes) {
+      const int64_t block = pages * c->page_bytes[i];  // below 2^61
+      if (c->n_layers > 1 && (stride < block || stride % 4 || stride > (int64_t{1} << 46))) return false;
+      *bytes = block + (c->n_layers - 1) * (c->n_layers > 1 ? stride : 0);
+      return true;
+    };
+    if (!span(c->src_layer_stride[i], c->n_src_pages, &src_bytes[i]) ||
+        !span(c->dst_layer_stride[i], c->n_dst_pages, &dst_bytes[i]))
+      return SRW_EINVAL;
+  }
+  for (int i = 0; i < c->n_tensors; ++i)
+    for (int j = 0; j < c->n_tensors; ++j) {
+      if (i < j && meet(c->dst[i], dst_bytes[i], c->dst[j], dst_bytes[j])) return SRW_EINVAL;
+      if (!meet(c->src[i], src_bytes[i], c->dst[j], dst_bytes[j])) continue;
+      if (i != j || c->src[i] != c->dst[i] || c->n_src_pages != c->n_dst_pages ||
+          (c->n_layers > 1 && c->src_layer_stride[i] != c->dst_layer_stride[i]))
+        return SRW_EINVAL;
+      inside = true;
+    }
+  for (int64_t j = 0; j < c->n_pairs; ++j)
+    if (c->src_page[j] < 0 || c->src_page[j] >= c->n_src_pages || c->dst_page[j] < 0 || c->dst_page[j] >= c->n_dst_pages)
+      return SRW_EINVAL;
+  if (c->n_pairs <= 16) {
+    for (int64_t j = 0; j < c->n_pairs; ++j)
+      for (int64_t k = 0; k < c->n_pairs; ++k)
+        if ((k != j && c->dst_page[j] == c->dst_page[k]) || (inside && c->src_page[j] == c->dst_page[k])) return SRW_EINVAL;
+    return SRW_OK;
+  }
+  try {
+    std::vector<uint64_t> written(static_cast<size_t>(c->n_dst_pages / 64 + 1));
+    for (int64_t j = 0; j < c->n_pairs; ++j) {
+      uint64_t& w = written[c->dst_page[j] >> 6];
+      const uint64_t bit = uint64_t{1} << (c->dst_page[j] & 63);
+      if (w & bit) return SRW_EINVAL;
+      w |= bit;
+    }
+    if (inside)
+      for (int64_t j = 0; j < c->n_pairs; ++j)
+        if (written[c->src_page[j] >> 6] >> (c->src_page[j] & 63) & 1) return SRW_EINVAL;
+  } catch (...) {  // no memory for the bits
+    return SRW_EHIP;
+  }
+  return SRW_OK;
+}
+
+hipError_t kv_copy(const srw_kv_copy_t& c, hipStream_t s) {
+  CopyArgs a{};
+  a.n = c.n_tensors;
+  for (int i = 0; i < c.n_tensors; ++i) {
+    a.src[i] = static_cast<const char*>(c.src[i]);
+    a.dst[i] = static_cast<char*>(c.dst[i]);
+    a.page[i] = c.page_bytes[i];
+    a.src_layer[i] = c.n_layers > 1 ? c.src_layer_stride[i] : 0;
+    a.dst_layer[i] = c.n_layers > 1 ? c.dst_layer_stride[i] : 0;
+    a.begin[i + 1] = a.begin[i] + static_cast<int32_t>((c.page_bytes[i] + kPiece - 1) / kPiece);
+    if (aligned(c.src[i], 16) && aligned(c.dst[i], 16) && (a.page[i] | a.src_layer[i] | a.dst_layer[i]) % 16 == 0)
+      a.wide |= 1 << i;
+  }
+  for (int64_t at = 0; at < c.n_pairs; at += kPairs) {
+    const int n = static_cast<int>(c.n_pairs - at < kPairs ? c.n_pairs - at : kPairs);
+    for (int j = 0; j < n; ++j) {
+      a.from[j] = c.src_page[at + j];
+      a.to[j] = c.dst_page[at + j];
+    }
+    hipLaunchKernelGGL(kv_copy_kernel,
+                       dim3(static_cast<unsigned>(a.begin[a.n]), static_cast<unsigned>(n), static_cast<unsigned>(c.n_layers)),
+                       dim3(kCopyThreads), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+// -- the index ------------------------------------------------------------------------
+
+constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
+
+// Codes of numbers whose largest magnitude has the bits `most`: x * inv to the nearest;
+// inv 0 for zeros and where a number is not finite.
+__device__ inline bool not_finite(uint32_t most) { return most >= 0x7f800000u; }
+__device__ inline float code_factor(uint32_t most) {
+  const float m = __uint_as_float(most);
+  return not_finite(most) || m <= kTiny ? 0.f : 127.f / m;
+}
+__device__ inline uint32_t code_of(float x, float inv) {
+  return static_cast<uint32_t>(static_cast<int>(rintf(inv == 0.f ? 0.f : x * inv))) & 0xffu;
+}
+
+// One wave: a page and head.  A lane holds 16 bytes' dims of every (64 / lanes a
+// key)th key and sums them in 64 bits, where sums of up to 256 keys of any 8-bit or
+// bf16 page are exact but for rare exponents far apart, so that the codes do not go by
+// the order of adding.  Bound by the keys' bytes.
+template <int KIND, int DH>
+__global__ __launch_bounds__(256) void kv_index_kernel(KvView p, int8_t* codes, float* scale) {
+  constexpr int ES = kv_bytes<KIND>(), N = 16 / ES;     // dims a lane
+  constexpr int kLanes = DH / N, kKeys = 64 / kLanes;   // lanes a key, keys a step
+  constexpr int U = 4;                                  // steps in flight
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, head = blockIdx.y;
+  // units of a page of sequence b: start(b) = cu[b] / P + 2 b leaves room for both
+  // partial ends
+  int64_t b = unit, at = 0;
+  if (p.cu) {
+    auto start = [&](int64_t i) { return (static_cast<int64_t>(p.cu[i]) >> p.logP) + 2 * i; };
+    b = kv_find(p.B, unit, start);
+    at = unit - start(b);
+  } else if (unit >= p.B) {
+    return;
+  }
+  const KvSeq sq = kv_seq(p, b);
+  if (sq.n <= 0 || at < 0) return;
+  const int first = sq.len > sq.n ? (sq.len - sq.n) >> p.logP : 0;  // the first page with a new token
+  const int64_t base = (first + at) << p.logP;
+  if (base >= sq.len) return;
+  const int page = kv_page(p, b, static_cast<int>(base));
+  if (page < 0) return;
+  const int have = sq.len - base < p.P ? static_cast<int>(sq.len - base) : p.P;
+  const int64_t ph = static_cast<int64_t>(page) * p.H + head;
+  const char* src = p.k + ph * p.P * (DH * ES) + 16 * lane;
+  double sum[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) sum[j] = 0.0;
+  const int mine = lane / kLanes;
+  for (int k0 = 0; k0 < have; k0 += kKeys * U) {
+    u32x4_t w[U];
+    float ks[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = k0 + u * kKeys + mine;
+      w[u] = u32x4_t{0, 0, 0, 0};
+      ks[u] = 0.f;
+      if (key < have) {
+        w[u] = *reinterpret_cast<const u32x4_t*>(src + static_cast<int64_t>(k0 + u * kKeys) * (DH * ES));
+        if constexpr (KIND != SRW_KV_BF16) ks[u] = p.ks[ph * p.P + key];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if constexpr (KIND == SRW_KV_BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum[2 * j] += static_cast<double>(lo_f32(w[u][j]));
+          sum[2 * j + 1] += static_cast<double>(hi_f32(w[u][j]));
+        }
+      } else {
+        const double s = ks[u];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x[4];
+          if constexpr (KIND == SRW_KV_FP8) {
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[u][j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[u][j], true);
+            x[0] = lo[0];
+            x[1] = lo[1];
+            x[2] = hi[0];
+            x[3] = hi[1];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(static_cast<int8_t>(w[u][j] >> (8 * i)));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[4 * j + i] = fma(static_cast<double>(x[i]), s, sum[4 * j + i]);
+        }
+      }
+    }
+  }
+  float mean[N];
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+#pragma unroll
+    for (int w = kLanes; w < 64; w <<= 1) sum[j] += __shfl_xor(sum[j], w);
+    mean[j] = static_cast<float>(sum[j] / have);
+    const uint32_t m = __float_as_uint(mean[j]) & 0x7fffffffu;
+    most = m > most ? m : most;
+  }
+#pragma unroll
+  for (int w = 1; w < kLanes; w <<= 1) {
+    const uint32_t o = __shfl_xor(most, w);
+    most = o > most ? o : most;
+  }
+  if (lane >= kLanes) return;
+  const float inv = code_factor(most), m = __uint_as_float(most);
+  uint32_t c[N / 4];
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j)
+    c[j] = code_of(mean[4 * j], inv) | code_of(mean[4 * j + 1], inv) << 8 | code_of(mean[4 * j + 2], inv) << 16 |
+           code_of(mean[4 * j + 3], inv) << 24;
+  char* dst = reinterpret_cast<char*>(codes) + ph * DH + lane * N;
+  if constexpr (N == 8)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
+  else
+    *reinterpret_cast<uint4*>(dst) = make_uint4(c[0], c[1], c[2], c[3]);
+  if (lane == 0) scale[ph] = not_finite(most) ? __uint_as_float(0x7fc00000u) : inv == 0.f ? 0.f : m / 127.f;
+}
+
+// -- the choice of pages ----------------------------------------------------------------
+//
+// A workgroup takes R tokens of a sequence and one key head; the threads score pages
+// (whole numbers by dot products of four codes, one page a thread and step), as keys
+// that order like the scores, into LDS; 256 / R threads then find each row's border by
+// digits of the keys and write the places that lie before it.  Tables of more pages
+// than LDS holds keys are scored again for each digit.
+
+struct SelectArgs {
+  KvView kv;
+  const int8_t* codes;
+  const float* scale;
+  const uint16_t* q;
+  int32_t* keep;
+  int64_t q_token, q_head;
+  int G, n, first, last, hold;  // hold: keys of a row in LDS, a multiple of 64
+};
+
+// A score's place among all; 0 is no page's.
+constexpr uint32_t kAlways = 0xffffffffu;
+__device__ inline uint32_t key_of(float score) {
+  if (score != score) return kAlways - 1;
+  const uint32_t b = __float_as_uint(score + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+template <int DH, int R>
+__global__ __launch_bounds__(256) void kv_select_kernel(SelectArgs a) {
+  constexpr int kRow = 256 / R;  // threads of a row
+  extern __shared__ uint32_t keys[];  // [R][hold]
+  __shared__ __align__(16) uint32_t qc[R][DH / 4];
+  __shared__ uint32_t most[R], hist[R][256], found[R][2];  // found: the digit, what lies before it
+  __shared__ uint64_t above[R][kRow / 64], equal[R][kRow / 64];
+  const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
+  const KvView& p = a.kv;
+  int64_t b, at;
+  if (p.cu) {
+    auto start = [&](int64_t i) { return static_cast<int64_t>(p.cu[i]) / R + i; };
+    b = kv_find(p.B, blockIdx.x, start);
+    at = blockIdx.x - start(b);
+  } else {
+    b = blockIdx.x;
+    at = 0;
+  }
+  b = __builtin_amdgcn_readfirstlane(static_cast<int>(b));
+  const KvSeq sq = kv_seq(p, b);
+  const int tok0 = static_cast<int>(at) * R;
+  if (at < 0 || at * R >= sq.n) return;
+  const int toks = sq.n - tok0 < R ? sq.n - tok0 : R;
+
+  // the rows' codes
+  if (tid < R) most[tid] = 0;
+  __syncthreads();
+  constexpr int kEach = R * DH / 4 > 256 ? R * DH / 4 / 256 : 1;  // times four dims a thread
+  float x[kEach][4];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + 256 * e, r = i / (DH / 4), c = i % (DH / 4);
+    if (r < toks) {
+      double s[4] = {0.0, 0.0, 0.0, 0.0};
+      const uint16_t* src = a.q + (sq.row0 + tok0 + r) * a.q_token + static_cast<int64_t>(head) * a.G * a.q_head + 4 * c;
+      for (int g = 0; g < a.G; ++g) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src + g * a.q_head);
+        s[0] += static_cast<double>(lo_f32(w.x));
+        s[1] += static_cast<double>(hi_f32(w.x));
+        s[2] += static_cast<double>(lo_f32(w.y));
+        s[3] += static_cast<double>(hi_f32(w.y));
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[e][j] = static_cast<float>(s[j]);
+        const uint32_t v = __float_as_uint(x[e][j]) & 0x7fffffffu;
+        m = v > m ? v : m;
+      }
+      atomicMax(&most[r], m);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + 256 * e, r = i / (DH / 4), c = i % (DH / 4);
+    if (r < toks) {
+      const float inv = code_factor(most[r]);
+      qc[r][c] = code_of(x[e][0], inv) | code_of(x[e][1], inv) << 8 | code_of(x[e][2], inv) << 16 | code_of(x[e][3], inv) << 24;
+    } else if (r < R) {
+      qc[r][c] = 0;
+    }
+  }
+  __syncthreads();
+
+  // pages that a row sees: [0, own]
+  auto own_of = [&](int r) {
+    const int pos = sq.len - sq.n + tok0 + r;
+    const int most_pages = p.cap >> p.logP;
+    if (r >= toks || pos < 0 || most_pages == 0) return -1;
+    return pos >> p.logP < most_pages ? pos >> p.logP : most_pages - 1;
+  };
+  const int pages = own_of(toks - 1) + 1;
+  auto score = [&](int from) {  // keys of places [from, from + hold)
+    const int to = pages - from < a.hold ? pages - from : a.hold;
+    for (int i = tid; i < ((to + 63) & ~63); i += 256) {
+      const int j = from + i;
+      const int page = i < to ? kv_page(p, b, j << p.logP) : -1;
+      int dot[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) dot[r] = 0;
+      float sc = 0.f;
+      if (page >= 0) {
+        const int64_t ph = static_cast<int64_t>(page) * p.H + head;
+        const u32x4_t* src = reinterpret_cast<const u32x4_t*>(a.codes + ph * DH);
+        u32x4_t w[DH / 16];
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) w[c] = src[c];
+        sc = a.scale[ph];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < DH / 16; ++c) {
+            const u32x4_t y = *reinterpret_cast<const u32x4_t*>(&qc[r][4 * c]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              dot[r] = __builtin_amdgcn_sdot4(static_cast<int>(w[c][e]), static_cast<int>(y[e]), dot[r], false);
+          }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int own = own_of(r);
+        uint32_t key = 0;
+        if (page >= 0 && j <= own)
+          key = j < a.first || j > own - a.last ? kAlways : key_of(static_cast<float>(dot[r]) * sc);
+        keys[r * a.hold + i] = key;
+      }
+    }
+  };
+
+  const int r = tid / kRow, t = tid % kRow;
+  const uint32_t* row = keys + r * a.hold;
+  // the border: keys above K, and as many equal to it as are left
+  uint32_t K = 0, left = a.n;
+  const bool held = pages <= a.hold;
+  if (held) score(0);
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = t; i < 256; i += kRow) hist[r][i] = 0;
+    __syncthreads();
+    for (int from = 0; from < pages; from += a.hold) {
+      if (!held) {
+        score(from);
+        __syncthreads();
+      }
+      const int to = pages - from < a.hold ? pages - from : a.hold;
+      for (int i = t; i < to; i += kRow) {
+        const uint32_t key = row[i];
+        if (shift == 24 || key >> (shift + 8) == K >> (shift + 8)) atomicAdd(&hist[r][255 - (key >> shift & 255)], 1u);
+      }
+      __syncthreads();
+    }
+    if (t < 64) {
+      uint32_t c[4], s = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        c[k] = hist[r][4 * lane + k];
+        s += c[k];
+      }
+      uint32_t run = s;
+#pragma unroll
+      for (int w = 1; w < 64; w <<= 1) {
+        const uint32_t o = __shfl_up(run, w);
+        if (lane >= w) run += o;
+      }
+      if (lane == 63 && run < left) {  // fewer than that: all
+        found[r][0] = 255;
+        found[r][1] = run - c[3];
+      }
+      uint32_t before = run - s;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (before < left && before + c[k] >= left) {
+          found[r][0] = 4 * lane + k;
+          found[r][1] = before;
+        }
+        before += c[k];
+      }
+    }
+    __syncthreads();
+    K |= (255 - found[r][0]) << shift;
+    left -= found[r][1];
+  }
+  // write: runs of places in order
+  const int tok = tok0 + r;
+  int32_t* out = a.keep + ((sq.row0 + (r < toks ? tok : 0)) * p.H + head) * a.n;
+  int written = 0;
+  const bool mine = r < toks;
+  for (int from = 0; from < pages; from += a.hold) {
+    if (!held) {
+      __syncthreads();
+      score(from);
+      __syncthreads();
+    }
+    const int to = pages - from < a.hold ? pages - from : a.hold;
+    for (int i0 = 0; i0 < to; i0 += kRow) {
+      const uint32_t key = i0 + t < to ? row[i0 + t] : 0;
+      const uint64_t ab = __ballot(key > K), eq = __ballot(key != 0 && key == K);
+      if constexpr (kRow > 64) {
+        if (lane == 0) {
+          above[r][t >> 6] = ab;
+          equal[r][t >> 6] = eq;
+        }
+        __syncthreads();
+      }
+      int base = written;
+      uint32_t l = left;
+      uint64_t keep = 0;
+#pragma unroll
+      for (int w = 0; w < kRow / 64; ++w) {
+        const uint64_t wa = kRow > 64 ? above[r][w] : ab, we = kRow > 64 ? equal[r][w] : eq;
+        const uint32_t e = static_cast<uint32_t>(__popcll(we));
+        uint64_t k = wa;
+        if (e <= l) {
+          k |= we;
+          l -= e;
+        } else {
+          uint64_t rest = we;
+          for (; l > 0; --l) {
+            k |= rest & -rest;
+            rest &= rest - 1;
+          }
+        }
+        if (w == t >> 6) {
+          keep = k;
+          base = written;
+        }
+        written += __popcll(k);
+      }
+      left = l;
+      if (mine && (keep >> lane & 1)) {
+        const int o = base + __popcll(keep & ((1ull << lane) - 1));
+        if (o < a.n) out[o] = from + i0 + t;
+      }
+      if constexpr (kRow > 64) __syncthreads();
+    }
+  }
+  if (mine)
+    for (int o = written + t; o < a.n; o += kRow) out[o] = -1;
+}
+
+template <int DH>
+hipError_t launch_select(const srw_kv_select_t& c, hipStream_t s) {
+  SelectArgs a{};
+  a.kv = kv_view(c.kv);
+  a.codes = c.index.codes;
+  a.scale = c.index.scale;
+  a.q = static_cast<const uint16_t*>(c.q);
+  a.keep = c.keep;
+  a.q_token = c.q_token_stride;
+  a.q_head = c.q_head_stride;
+  a.G = c.n_heads / c.kv.n_kv_heads;
+  a.n = c.n;
+  a.first = c.first;
+  a.last = c.last;
+  const int R = c.kv.cu ? 4 : 1;
+  const int64_t most = 12288 / R, width = (c.kv.table_width + 63) / 64 * 64;
+  a.hold = static_cast<int>(width < 64 ? 64 : width < most ? width : most);
+  const int64_t tiles = c.kv.cu ? c.kv.T / R + c.kv.B : c.kv.B;
+  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(c.kv.n_kv_heads));
+  const unsigned lds = static_cast<unsigned>(a.hold) * R * 4;
+  if (R == 1)
+    hipLaunchKernelGGL((kv_select_kernel<DH, 1>), grid, dim3(256), lds, s, a);
+  else
+    hipLaunchKernelGGL((kv_select_kernel<DH, 4>), grid, dim3(256), lds, s, a);
+  return hipGetLastError();
+}
+
+srw_status_t check_index(const srw_kv_t& c, const srw_kv_index_t& i) {
+  if (c.T > 0 && c.n_pages > 0 && (!aligned(i.codes, 16) || !aligned(i.scale, 4))) return SRW_EINVAL;
+  return SRW_OK;
+}
+
+template <int KIND>
+hipError_t launch_index(const srw_kv_t& c, const srw_kv_index_t& x, hipStream_t s) {
+  const KvView p = kv_view(c);
+  const int64_t units = c.cu ? (c.T >> p.logP) + 2 * c.B : c.B;
+  const dim3 grid(static_cast<unsigned>((units + 3) / 4), static_cast<unsigned>(c.n_kv_heads));
+  if (c.head_dim == 64)
+    hipLaunchKernelGGL((kv_index_kernel<KIND, 64>), grid, dim3(256), 0, s, p, x.codes, x.scale);
+  else
+    hipLaunchKernelGGL((kv_index_kernel<KIND, 128>), grid, dim3(256), 0, s, p, x.codes, x.scale);
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace srw
+
+extern "C" {
+
+srw_status_t srw_kv_copy(const srw_kv_copy_t* c, void* stream) {
+  const srw_status_t st = srw::check_copy(c);
+  if (st != SRW_OK) return st;
+  if (c->n_pairs == 0 || c->n_layers == 0 || c->n_tensors == 0) return SRW_OK;
+  (void)hipGetLastError();
+  return srw::kv_copy(*c, static_cast<hipStream_t>(stream)) == hipSuccess ? SRW_OK : SRW_EHIP;
+}
+
+srw_status_t srw_kv_index(const srw_kv_t* cache, const srw_kv_index_t* index, void* stream) {
+  srw_status_t st = srw::check_kv(cache);
+  if (st != SRW_OK) return st;
+  if (!index) return SRW_EINVAL;
+  st = srw::check_index(*cache, *index);
+  if (st != SRW_OK) return st;
+  if (cache->T == 0 || cache->n_pages == 0) return SRW_OK;
+  if (cache->T > (1 << 29)) return SRW_EUNSUPPORTED;  // (a launch has under 2^32 threads)
+  (void)hipGetLastError();
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipError_t e = cache->kind == SRW_KV_BF16   ? srw::launch_index<SRW_KV_BF16>(*cache, *index, s)
+                       : cache->kind == SRW_KV_INT8 ? srw::launch_index<SRW_KV_INT8>(*cache, *index, s)
+                                                    : srw::launch_index<SRW_KV_FP8>(*cache, *index, s);
+  return e == hipSuccess ? SRW_OK : SRW_EHIP;
+}
+
+srw_status_t srw_kv_select(const srw_kv_select_t* c, void* stream) {
+  if (!c) return SRW_EINVAL;
+  srw_status_t st = srw::check_kv(&c->kv);
+  if (st != SRW_OK) return st;
+  st = srw::check_index(c->kv, c->index);
+  if (st != SRW_OK) return st;
+  if (c->n_heads < 1 || c->n_heads % c->kv.n_kv_heads || c->n < 1 || c->first < 0 || c->last < 1 ||
+      static_cast<int64_t>(c->first) + c->last > c->n)
+    return SRW_EINVAL;
+  if (c->kv.T == 0) return SRW_OK;
+  if (c->kv.T > (1 << 25)) return SRW_EUNSUPPORTED;  // (a launch has under 2^32 threads)
+  if (!srw::aligned(c->q, 8) || !srw::aligned(c->keep, 4) || c->q_token_stride < 0 || c->q_head_stride < 0 ||
+      c->q_token_stride % 4 || c->q_head_stride % 4)
+    return SRW_EINVAL;
+  (void)hipGetLastError();
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipError_t e = c->kv.head_dim == 64 ? srw::launch_select<64>(*c, s) : srw::launch_select<128>(*c, s);
+  return e == hipSuccess ? SRW_OK : SRW_EHIP;
+}
+
+}  // extern "C"

@@ -1,0 +1,84 @@
+"""Choosing tokens from logits: one HIP kernel (csrc/srw_sample.hip), torch tensors
+in and out.  :func:`sample` takes its random numbers from the caller, so a program
+that keeps them can repeat a run; it waits for nothing and can be captured in a
+graph."""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _capi as C
+from .kv import _call, _no_grad, _tensor
+
+__all__ = ["sample"]
+
+F32, I32, I64 = torch.float32, torch.int32, torch.int64
+_DTYPES = {torch.float32: C.SRW_F32, torch.bfloat16: C.SRW_BF16}
+_SAMPLE = struct.Struct("@P3q7P3f3i")
+
+
+def _parameter(name, x, dev, dtype, B):
+    """(address, 0) of a tensor [B], (None, number) of a number."""
+    if isinstance(x, torch.Tensor):
+        _no_grad(name, x)
+        return _tensor(name, x, dev, dtype, (B,)), 0
+    if dtype is I32:
+        if not hasattr(x, "__index__"):
+            raise TypeError(f"{name} is a whole number or a tensor; got {x!r}")
+        if not 0 <= x <= 0x7fffffff:
+            raise ValueError(f"{name} is not negative; got {x!r}")
+        return 0, x
+    x = float(x)
+    if not (x >= 0 and (name == "temperature" or x <= 1)):
+        raise ValueError(f"{name} is not negative{'' if name == 'temperature' else ' and at most 1'}; got {x!r}")
+    return 0, x
+
+
+def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(tokens [B] int64, logprobs [B] float32): one token of every row of ``logits``
+    [B, vocab] (float32 or bfloat16, any row stride) from the random numbers ``u`` [B]
+    float32 in [0, 1).
+
+    A logit l of a row with largest M weighs exp((l - M) / temperature).  In the order
+    of the logits, the largest first, equal ones by index, ``top_k`` (0: off) keeps the
+    first k, ``top_p`` (1: off) of these the shortest run whose weights reach p times
+    their sum, ``min_p`` (0: off) what weighs min_p or more.  The token is the first, by
+    index, at which the kept weights' running sum passes u times their sum; its logprob
+    is the logarithm of its share.  Temperature 0 takes the first in the order, with
+    logprob 0.  NaN counts as -infinity, several infinite logits weigh the same; a row
+    of -infinity gives token -1 and logprob -infinity.
+
+    Each parameter is a number or a tensor [B] of the logits' device (float32; ``top_k``
+    int32), whose entries are read on the device: there a temperature that is not above
+    0 counts as 0, a top_k below 1, a top_p that is not below 1 and a min_p that is not
+    above 0 as off, a min_p above 1 as 1.  u outside of [0, 1) counts as the nearest
+    number inside (NaN as 0).
+
+    Weights are summed as whole numbers in units of 2^-51 or, of large vocabularies,
+    2^62 / vocab: a row's token goes by its own numbers alone, not by the batch."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        raise ValueError("logits must be a tensor [B, vocab]")
+    dev = logits.device
+    if dev.type != "cuda":
+        raise ValueError(f"logits live on a HIP device; got {dev}")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"logits has dtype {logits.dtype}, expected float32 or bfloat16")
+    B, V = logits.shape
+    if V < 1:
+        raise ValueError("logits has no vocabulary")
+    _no_grad("logits", logits)
+    if isinstance(u, torch.Tensor):
+        _no_grad("u", u)
+    u = _tensor("u", u, dev, F32, (B,))
+    given = [_parameter(n, x, dev, t, B) for n, x, t in (("temperature", temperature, F32), ("top_p", top_p, F32),
+                                                        ("min_p", min_p, F32), ("top_k", top_k, I32))]
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    token = torch.empty(B, dtype=I64, device=dev)
+    logprob = torch.empty(B, dtype=F32, device=dev)
+    d = _SAMPLE.pack(logits.data_ptr(), logits.stride(0), B, V, u, *(a for a, _ in given), token.data_ptr(),
+                     logprob.data_ptr(), *(x for _, x in given), _DTYPES[logits.dtype], 0)
+    C.check(_call(C.load_library().srw_sample, dev, d))
+    return token, logprob

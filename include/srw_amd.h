@@ -510,6 +510,97 @@ srw_status_t srw_attention(const srw_attention_t* a, void* workspace, size_t wor
  * (more than one: joined by a second launch).  0 and 0 without tokens. */
 srw_status_t srw_attention_plan(const srw_attention_t* a, int32_t* rows, int32_t* splits);
 
+/* Pages of a cache's tensors copied onto other pages, in all layers: tensor i has
+ * n_layers blocks layer_stride[i] bytes apart, of n_pages pages of page_bytes[i]
+ * bytes each (multiples of 4).  Page dst_page[j] of every layer of dst gets what page
+ * src_page[j] of that layer of src holds; src[i] == dst[i]: within a tensor.  src_page
+ * and dst_page are host arrays, read before the call returns.  A page that is named
+ * twice in dst_page, or that is both read and written, and tensors that overlap in
+ * any other way are SRW_EINVAL. */
+#define SRW_KV_COPY_TENSORS 8
+typedef struct srw_kv_copy {
+  const void* src[SRW_KV_COPY_TENSORS];
+  void* dst[SRW_KV_COPY_TENSORS];
+  int64_t page_bytes[SRW_KV_COPY_TENSORS];
+  int64_t src_layer_stride[SRW_KV_COPY_TENSORS], dst_layer_stride[SRW_KV_COPY_TENSORS];
+  int64_t n_layers, n_src_pages, n_dst_pages, n_pairs;
+  const int32_t *src_page, *dst_page;
+  int32_t n_tensors, reserved;
+} srw_kv_copy_t;
+srw_status_t srw_kv_copy(const srw_kv_copy_t* c, void* stream);
+
+/* An index over a cache's pages: of each page and key/value head the mean of the
+ * keys, m its largest magnitude, as codes round(mean * (127 / m)) [n_pages,
+ * n_kv_heads, head_dim] and scale m / 127 [n_pages, n_kv_heads] (magnitudes of 2^-100
+ * or less: zeros; an infinity or NaN among the keys: scale NaN).  16-byte aligned. */
+typedef struct srw_kv_index {
+  int8_t* codes;
+  float* scale;
+} srw_kv_index_t;
+
+/* Brings the entries of the pages that hold the call's new tokens up to date, from
+ * what the cache holds of them (srw_kv_write before, on the same stream): the mean of
+ * a page's positions before lens[b].  Other entries keep what they hold. */
+srw_status_t srw_kv_index(const srw_kv_t* cache, const srw_kv_index_t* index, void* stream);
+
+/* For every new token and key/value head the places in its sequence's table of the
+ * pages to attend to, keep [T, n_kv_heads, n] ascending, -1 behind the last.  A token
+ * at position i sees the pages of positions up to i; with n of them or fewer it keeps
+ * all, else the first `first`, the last `last` (its own among them, first + last <= n,
+ * last >= 1) and of the others those with the largest scores, equal ones from the
+ * front.  A page scores scale * (c . codes), c the codes of the sum of the queries of
+ * the heads that read the key head (rounded once to float32, codes as a mean's): whole
+ * numbers, rounded once in the product with the scale.  A page whose scale is NaN
+ * comes before all scores.  Places without a page are not kept, rows of keep that no
+ * sequence names are not written.  q as in srw_attention. */
+typedef struct srw_kv_select {
+  srw_kv_t kv;
+  srw_kv_index_t index;
+  const void* q;
+  int32_t* keep;
+  int64_t q_token_stride, q_head_stride;
+  int32_t n_heads, n, first, last;
+} srw_kv_select_t;
+srw_status_t srw_kv_select(const srw_kv_select_t* s, void* stream);
+
+/* srw_attention over kept pages alone: a token sees, for the heads that read key head
+ * h, the positions j <= i of the pages at keep[t, h] (int32 [T, n_kv_heads, n_keep],
+ * device; each list ascending; entries outside the table, and those that are not
+ * larger than the one before, name nothing).  window and sinks have to be 0, max_new is
+ * not looked at.  Whatever keep holds, nothing outside the cache is read. */
+srw_status_t srw_attention_kept_workspace_size(const srw_attention_t* a, int64_t n_keep, size_t* bytes);
+srw_status_t srw_attention_kept(const srw_attention_t* a, const int32_t* keep, int64_t n_keep, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* One token of every row of logits [B, V] (dtype SRW_F32 or SRW_BF16, rows row_stride
+ * elements apart) from random numbers u [B] in [0, 1).  With temperature t > 0 and M a
+ * row's largest logit, token i weighs w_i = exp((logit_i - M) / t).  In the order of
+ * the logits, the largest first, equal ones by index, top_k (0: off) keeps the first k,
+ * top_p (1: off) the shortest run of those whose weights reach p times the sum of
+ * theirs, min_p (0: off) what weighs min_p or more.  The token is the first, by index,
+ * at which the kept weights' running sum passes u times their sum; logprob (NULL: not
+ * wanted) the logarithm of its weight's share of that sum.  t = 0: the first in the
+ * order, logprob 0.  NaN counts as -infinity; of infinite logits each weighs the same;
+ * a row of -infinity gives token -1 and logprob -infinity.
+ *
+ * Parameters are device arrays of B or, where the array is NULL, the number beside it,
+ * which is checked.  In arrays a temperature that is not above 0 counts as 0, a top_k
+ * below 1 as off, a top_p that is not below 1 as off, a min_p that is not above 0 as
+ * off and one above 1 as 1; u is taken into [0, 1).  Sums are of whole numbers (weights
+ * in units of 2^-q, q = min(51, 62 - log2 V)): results do not go by the batch or the
+ * order of adding.  V up to 2^24, B up to 2^21. */
+typedef struct srw_sample {
+  const void* logits;
+  int64_t row_stride, B, V;
+  const float *u, *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  int64_t* token;
+  float* logprob;
+  float temperature_all, top_p_all, min_p_all;
+  int32_t top_k_all, dtype, reserved;
+} srw_sample_t;
+srw_status_t srw_sample(const srw_sample_t* s, void* stream);
+
 /* Name of the kernel family the last srw_forward on this thread used
  * ("generic", "mfma_bf16", "mfma_ss_bf16", ...), for tests and benchmarks. */
 const char* srw_last_path(void);
