@@ -12,13 +12,12 @@
 // border is where 64 bits put it.  What rounds to zero cannot be drawn and takes
 // no part.
 //
-// Nothing is sorted.  One pass finds M, a second one counts (and, for top-p,
-// sums) tokens by how far they lie under M, in 2 048 steps of equal width: the
-// border of top-k or top-p lies in the first step at which the running count or
-// sum reaches it.  The tokens down to that step, if there are no more than kList,
-// become a list in LDS, on which the rest is done: the border's place within its
-// step by digits of the logits' bits, and the draw by digits of the index.  Rows
-// that keep more are walked again instead.
+// Nothing is sorted.  One pass finds M.  A threshold that the border of top-k or
+// top-p cannot lie above comes from counts or sums of tokens by how far they lie
+// under M, in steps of 2^(1/64); the tokens down to it, if there are no more than
+// kList, become a list that a workgroup holds in registers, and the rest is done on
+// them: the border by digits of the logits' bits, the draw by digits of the index.
+// Rows that keep more are walked again instead.
 
 #include <math.h>
 
@@ -28,9 +27,9 @@
 namespace srw {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kSteps = 2048;   // of the distance under M
-constexpr int kList = 4096;    // tokens that LDS holds
+constexpr int kSteps = 2048;   // of 2^(1/64) under M
+constexpr int kList = 4096;    // tokens that a workgroup's registers hold
+constexpr int kDigit = 9;      // bits of a select's pass
 
 struct SampleArgs {
   const char* logits;
@@ -54,47 +53,51 @@ __device__ inline uint32_t key_of(float l) {
 __device__ inline float of_key(uint32_t k) {
   return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+__device__ inline float float_under(double x) {  // the largest float that is not above x
+  const float f = static_cast<float>(x);
+  if (!(static_cast<double>(f) > x)) return f;
+  return of_key(key_of(f) - 1);
+}
 
-// What a row's weights go by.
+// What a row's weights go by: log2 w = (l - M) c, c = log2 e / t.
 struct Weights {
-  double M, c;  // largest logit, log2 e / t
-  bool inf;     // M is infinite: its tokens weigh 1, all others nothing
+  double c, M, lowest, unit;  // lowest: what weighs less rounds to zero; unit 2^(52 - q)
   int q;
-  // log2 of the weight
-  __device__ double log2w(float l) const {
-    if (inf) return l == INFINITY ? 0.0 : -INFINITY;
-    return (static_cast<double>(l) - M) * c;
-  }
-  __device__ bool some(double y) const { return y > -(q + 1.0); }  // (false for NaN)
-  // 2^y for y in (-q - 1, 0]: the exponential's series over half a unit of the
-  // exponent, (ln 2 / 2)^12 / 12! = 6e-15 short at most
-  __device__ static double weight(double y) {
-    const double n = rint(y), r = y - n;
-    double p = 4.4455382718708115e-10;
-    p = fma(p, r, 7.0549116208011233e-09);
-    p = fma(p, r, 1.0178086009239699e-07);
-    p = fma(p, r, 1.3215486790144309e-06);
-    p = fma(p, r, 1.5252733804059841e-05);
-    p = fma(p, r, 1.5403530393381609e-04);
-    p = fma(p, r, 1.3333558146428443e-03);
-    p = fma(p, r, 9.6181291076284772e-03);
-    p = fma(p, r, 5.5504108664821580e-02);
-    p = fma(p, r, 2.4022650695910072e-01);
-    p = fma(p, r, 6.9314718055994531e-01);
+  const double* tab;                // 2^(j / 64)
+  __device__ double log2w(float l) const { return (static_cast<double>(l) - M) * c; }
+  // 64 log2 w to the nearest, in the low bits of a sum (of log2 w above -2^25)
+  static constexpr double kMagic = 0x1.8p46;
+  // round(2^q w): 2^(n / 64) from the table, the rest of the exponent, at most 1 / 128,
+  // by a polynomial that is 1 at 0 and elsewhere 5e-15 off at most.  Garbage below
+  // `lowest`.
+  __device__ uint64_t whole(double y) const {
+    const double t = y + kMagic;
+    const int n = static_cast<int>(__double_as_longlong(t));
+    const double r = y - (t - kMagic);
+    double p = 0x1.3b2acb2c36b23p-7;
+    p = fma(p, r, 0x1.c6b0b9214b9aep-5);
+    p = fma(p, r, 0x1.ebfbdff82bb76p-3);
+    p = fma(p, r, 0x1.62e42fefa2417p-1);
     p = fma(p, r, 1.0);
-    return ldexp(p, static_cast<int>(n));
+    p *= tab[n & 63];
+    p = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
+    // the low bits of a sum whose last place is 2^-q
+    return static_cast<uint64_t>(__double_as_longlong(p + unit)) & 0xfffffffffffffull;
   }
-  // round(2^q w), w <= 1: the low bits of a sum whose last place is 2^-q
-  __device__ uint64_t whole(double w) const {
-    return static_cast<uint64_t>(__double_as_longlong(w + ldexp(1.0, 52 - q))) & 0xfffffffffffffull;
-  }
-  __device__ uint64_t of(float l) const {
+  // What a token adds to sums, down to the log2 weight `least` (false for NaN).
+  __device__ uint64_t of(float l, double least) const {
     const double y = log2w(l);
-    return some(y) ? whole(weight(y)) : 0;
+    const uint64_t w = whole(y);
+    return y >= least ? w : 0;
+  }
+  // steps of 2^(1/64) under M
+  __device__ int step(double y) const {
+    const int n = -static_cast<int>(__double_as_longlong(fmax(y, -40.0) + kMagic));
+    return n < 0 ? 0 : n < kSteps ? n : kSteps - 1;
   }
 };
 
-template <typename T> struct Row {
+template <typename T, int NT> struct Row {
   static constexpr int E = 16 / sizeof(T);  // logits of a vector
   const T* p;
   int V, off, n;  // the row begins off logits behind a 16-byte border; its vectors
@@ -103,6 +106,12 @@ template <typename T> struct Row {
     V = a.V;
     off = static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
     n = (off + V + E - 1) / E;
+  }
+  __device__ float one(int i) const {
+    if constexpr (E == 4)
+      return p[i];
+    else
+      return __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
   }
   // Vector v: logits E v - off ...; those outside the row as NaN.
   __device__ void get(int v, float (&x)[E]) const {
@@ -122,127 +131,132 @@ template <typename T> struct Row {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         x[j] = __uint_as_float(0x7fc00000u);
-        if (i + j >= 0 && i + j < V) {
-          if constexpr (E == 4)
-            x[j] = p[i + j];
-          else
-            x[j] = __uint_as_float(static_cast<uint32_t>(p[i + j]) << 16);
-        }
+        if (i + j >= 0 && i + j < V) x[j] = one(i + j);
       }
     }
   }
-  // f(index, logit) of the vectors [v0, v1), one a lane, by the whole wave
+  // f(index of the first, logits) of the vectors [v0, v1), one a lane, by the whole wave
   template <class F>
   __device__ void walk(int v0, int v1, F f) const {
     constexpr int U = 4;  // loads in flight
-    for (int v = v0 + (threadIdx.x & 63); v < v1; v += 64 * U) {
+    int v = v0 + (threadIdx.x & 63);
+    for (; v + 64 * (U - 1) < v1; v += 64 * U) {
       float x[U][E];
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (v + 64 * k < v1) get(v + 64 * k, x[k]);
+      for (int k = 0; k < U; ++k) get(v + 64 * k, x[k]);
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (v + 64 * k < v1)
-#pragma unroll
-          for (int j = 0; j < E; ++j) f((v + 64 * k) * E - off + j, x[k][j]);
+      for (int k = 0; k < U; ++k) f((v + 64 * k) * E - off, x[k]);
+    }
+    for (; v < v1; v += 64) {
+      float x[E];
+      get(v, x);
+      f(v * E - off, x);
     }
   }
   // the part of the row that is this wave's
   template <class F>
   __device__ void mine(F f) const {
+    constexpr int kWaves = NT / 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int per = (n + kWaves - 1) / kWaves;
     walk(wave * per, (wave + 1) * per < n ? (wave + 1) * per : n, f);
   }
 };
 
-template <class T, class Op>
-__device__ inline T wave_all(T v, Op op) {
+// v of the lane that DPP control C names, 0 where there is none or MASK leaves the
+// row of 16 out.
+template <int C, int MASK>
+__device__ inline uint32_t moved(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), C, MASK, 0xf, false));
+}
+template <int C, int MASK>
+__device__ inline uint64_t moved(uint64_t v) {
+  return static_cast<uint64_t>(moved<C, MASK>(static_cast<uint32_t>(v >> 32))) << 32 |
+         moved<C, MASK>(static_cast<uint32_t>(v));
+}
+// Sums over this lane and those before it: within rows of 16, then the rows.
+template <class N>
+__device__ inline N wave_scan(N v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+__device__ inline uint32_t last_lane(uint32_t v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ inline uint64_t last_lane(uint64_t v) {
+  return static_cast<uint64_t>(last_lane(static_cast<uint32_t>(v >> 32))) << 32 | last_lane(static_cast<uint32_t>(v));
+}
+template <class N>
+__device__ inline N wave_sum(N v) {
+  return last_lane(wave_scan(v));
+}
+template <class N, class Op>
+__device__ inline N wave_all(N v, Op op) {
 #pragma unroll
   for (int w = 1; w < 64; w <<= 1) v = op(v, __shfl_xor(v, w));
   return v;
 }
-// Sums over this lane and those before it.
-template <class T>
-__device__ inline T wave_scan(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) {
-    const T o = __shfl_up(v, w);
-    if (lane >= w) v += o;
-  }
-  return v;
-}
 
 struct Shared {
-  uint32_t count[kSteps];
+  double tab[64];
   unsigned long long mass[kSteps];
+  uint32_t count[kSteps];
   unsigned long long list[kList];  // key << 32 | index
-  unsigned long long wave_mass[kWaves];
-  uint32_t wave_count[kWaves];
-  float wave_max[kWaves];
-  // a crossing: the bin, what lies before it and in it
+  unsigned long long wave_m[16];
+  uint32_t wave_n[16];
+  float wave_max[16];
+  // a crossing: the bin (-1: none), what lies before it and in it
   int bin;
   uint32_t before_n, in_n, listed, lo, hi;
   unsigned long long before_m, in_m;
 };
 
+template <int NT>
 __device__ inline uint64_t block_sum(Shared& s, uint64_t v) {
-  const int wave = threadIdx.x >> 6;
-  v = wave_all(v, [](uint64_t a, uint64_t b) { return a + b; });
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.wave_mass[wave] = v;
+  v = wave_sum(v);
+  if ((threadIdx.x & 63) == 0) s.wave_m[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) v += s.wave_mass[w];
+  for (int w = 0; w < NT / 64; ++w) v += s.wave_m[w];
   __syncthreads();
   return v;
 }
 
-// The first of n = 256 or kSteps bins (of s.count and, with BY_MASS, s.mass) at
-// which the running count (or mass) reaches target; nothing is written where it
-// never does (s.bin = -1 before).  All threads; s is read after a barrier.
-template <bool BY_MASS>
-__device__ inline void crossing(Shared& s, int n, uint64_t target, uint32_t before_n, uint64_t before_m) {
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  constexpr int per = kSteps / kThreads;  // bins a thread
-  uint32_t c[per], cs = 0;
-  uint64_t m[per], ms = 0;
+// The first of kSteps bins (of s.count, or BY_MASS of s.mass) at which the running
+// count (or mass) reaches what target(total) says.
+template <int NT, bool BY_MASS, class Target>
+__device__ inline void crossing(Shared& s, Target target) {
+  const int tid = threadIdx.x, wave = tid >> 6;
+  constexpr int per = kSteps / NT;  // bins a thread
+  uint64_t x[per], sum = 0;
 #pragma unroll
   for (int k = 0; k < per; ++k) {
-    const int i = tid * per + k;
-    c[k] = i < n ? s.count[i] : 0;
-    m[k] = BY_MASS && i < n ? s.mass[i] : 0;
-    cs += c[k];
-    ms += m[k];
+    x[k] = BY_MASS ? s.mass[tid * per + k] : s.count[tid * per + k];
+    sum += x[k];
   }
-  uint32_t cr = wave_scan(cs);
-  uint64_t mr = BY_MASS ? wave_scan(ms) : 0;
-  if (lane == 63) {
-    s.wave_count[wave] = cr;
-    if constexpr (BY_MASS) s.wave_mass[wave] = mr;
-  }
+  uint64_t run = wave_scan(sum);
+  if ((tid & 63) == 63) s.wave_m[wave] = run;
   if (tid == 0) s.bin = -1;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    before_n += s.wave_count[w];
-    if constexpr (BY_MASS) before_m += s.wave_mass[w];
+  uint64_t total = 0;
+  run -= sum;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    run += w < wave ? s.wave_m[w] : 0;
+    total += s.wave_m[w];
   }
-  before_n += cr - cs;
-  before_m += mr - ms;
+  const uint64_t t = target(total);
 #pragma unroll
   for (int k = 0; k < per; ++k) {
-    const uint64_t was = BY_MASS ? before_m : before_n, is = BY_MASS ? before_m + m[k] : before_n + c[k];
-    if (was < target && is >= target) {
+    if (run < t && run + x[k] >= t) {
       s.bin = tid * per + k;
-      s.before_n = before_n;
-      s.before_m = before_m;
-      s.in_n = c[k];
-      s.in_m = m[k];
+      s.before_m = run;
     }
-    before_n += c[k];
-    before_m += m[k];
+    run += x[k];
   }
   __syncthreads();
 }
@@ -252,32 +266,54 @@ __device__ inline void crossing(Shared& s, int n, uint64_t target, uint32_t befo
 // in it.  each(f) calls f(rank, mass) for every candidate of this thread.  There
 // must be such a rank.
 struct Found {
-  uint32_t rank, before_n, in_n;
-  uint64_t before_m, in_m;
+  uint32_t rank, in_n;
+  uint64_t before, in_m;
 };
-template <bool BY_MASS, class Each>
+template <int NT, bool BY_MASS, class Each>
 __device__ inline Found select(Shared& s, int bits, uint64_t target, Each each) {
-  Found f{0, 0, 0, 0, 0};
+  constexpr int kBins = 1 << kDigit, kEach = kBins / 64;
+  auto place = [](int i) { return i + i / kEach; };  // (a lane's run of bins, over all banks)
+  Found f{0, 0, 0, 0};
   int left = bits;
   while (left > 0) {
-    const int d = left < 8 ? left : 8, shift = left - d;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += kThreads) {
+    const int d = left < kDigit ? left : kDigit, shift = left - d, last = (1 << d) - 1;
+    for (int i = threadIdx.x; i < kBins + 64; i += NT) {
       s.count[i] = 0;
-      s.mass[i] = 0;
+      if constexpr (BY_MASS) s.mass[i] = 0;
     }
     __syncthreads();
     each([&](uint32_t rank, uint64_t m) {
       if (left < 32 && rank >> left != f.rank) return;
-      const int bin = (1 << d) - 1 - static_cast<int>(rank >> shift & ((1u << d) - 1));  // the largest first
+      const int bin = place(last - static_cast<int>(rank >> shift & static_cast<uint32_t>(last)));  // the largest first
       atomicAdd(&s.count[bin], 1u);
       if constexpr (BY_MASS) atomicAdd(&s.mass[bin], static_cast<unsigned long long>(m));
     });
     __syncthreads();
-    crossing<BY_MASS>(s, 1 << d, target, f.before_n, f.before_m);
-    f.rank = f.rank << d | static_cast<uint32_t>((1 << d) - 1 - s.bin);
-    f.before_n = s.before_n;
-    f.before_m = s.before_m;
+    if (threadIdx.x < 64) {
+      uint32_t c[kEach];
+      uint64_t m[kEach], sum = 0;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const int i = place(threadIdx.x * kEach + k);
+        c[k] = s.count[i];
+        m[k] = BY_MASS ? s.mass[i] : c[k];
+        sum += m[k];
+      }
+      uint64_t run = f.before + wave_scan(sum) - sum;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        if (run < target && run + m[k] >= target) {
+          s.bin = threadIdx.x * kEach + k;
+          s.before_m = run;
+          s.in_n = c[k];
+          s.in_m = m[k];
+        }
+        run += m[k];
+      }
+    }
+    __syncthreads();
+    f.rank = f.rank << d | static_cast<uint32_t>(last - s.bin);
+    f.before = s.before_m;
     f.in_n = s.in_n;
     f.in_m = s.in_m;
     left = shift;
@@ -294,13 +330,16 @@ struct Cut {
   __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= index); }
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
+  constexpr int kWaves = NT / 64, kEach = kList / NT;  // kEach: a thread's tokens of a list
+  constexpr bool kWhole = NT == 256;                   // every row is its own list
+  using R = Row<T, NT>;
+  constexpr int E = R::E;
   __shared__ Shared s;
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const Row<T> row(a, b);
-  constexpr int E = Row<T>::E;
+  const R row(a, b);
   const float t = a.temperature ? a.temperature[b] : a.temperature_all;
   const int k = a.top_k ? a.top_k[b] : a.top_k_all;
   const float p = a.top_p ? a.top_p[b] : a.top_p_all;
@@ -308,22 +347,30 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   least = least > 0.f ? (least < 1.f ? least : 1.f) : 0.f;
   const float u = a.u[b];
 
-  float m = -INFINITY;
-  row.mine([&](int, float l) { m = fmaxf(m, l); });
-  m = wave_all(m, [](float x, float y) { return fmaxf(x, y); });
-  if (lane == 0) s.wave_max[wave] = m;
+  if (tid < 64) s.tab[tid] = exp2(tid / 64.0);
   if (tid == 0) {
     s.listed = 0;
     s.lo = 0xffffffffu;
     s.hi = 0;
   }
-  for (int i = tid; i < kSteps; i += kThreads) {
-    s.count[i] = 0;
-    s.mass[i] = 0;
-  }
-  __syncthreads();
+  auto clear = [&] {
+    for (int i = tid; i < kSteps; i += NT) {
+      s.count[i] = 0;
+      s.mass[i] = 0;
+    }
+  };
+  clear();
+  float mine = -INFINITY;  // the thread's largest
+  row.mine([&](int, const float(&x)[E]) {
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s.wave_max[w]);
+    for (int j = 0; j < E; ++j) mine = fmaxf(mine, x[j]);
+  });
+  const float wm = wave_all(mine, [](float x, float y) { return fmaxf(x, y); });
+  if (lane == 0) s.wave_max[wave] = wm;
+  __syncthreads();
+  float m = s.wave_max[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s.wave_max[w]);
   if (m == -INFINITY) {  // nothing to draw
     if (tid == 0) {
       a.token[b] = -1;
@@ -331,11 +378,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     }
     return;
   }
-  const bool greedy = !(t > 0.f);
-  if (greedy || (k == 1)) {
-    row.mine([&](int i, float l) {
-      if (l == m) atomicMin(&s.lo, static_cast<uint32_t>(i));
-    });
+  if (!(t > 0.f) || k == 1) {  // the first of the largest
+    uint32_t first = 0xffffffffu;
+    if (mine == m)
+      row.mine([&](int i, const float(&x)[E]) {
+#pragma unroll
+        for (int j = E - 1; j >= 0; --j)
+          if (x[j] == m && static_cast<uint32_t>(i + j) < first) first = i + j;
+      });
+    if (first != 0xffffffffu) atomicMin(&s.lo, first);
     __syncthreads();
     if (tid == 0) {
       a.token[b] = s.lo;
@@ -344,215 +395,314 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     return;
   }
 
-  Weights wt;
-  wt.M = m;
-  wt.c = 1.4426950408889634 / static_cast<double>(t);
-  wt.inf = m == INFINITY;
-  wt.q = a.q;
-  const bool by_k = k > 0 && k < a.V, by_p = p < 1.f;
-  // steps under M: any way that never puts a smaller logit before a larger one does
-  float scale = (kSteps - 1) / (static_cast<float>(a.q + 1) * 0.6931472f * t);
-  scale = scale < 3e38f ? scale : 3e38f;
-  auto step = [&](float l) {
-    const float x = (m - l) * scale;
-    return x < kSteps - 1 ? static_cast<int>(x) : kSteps - 1;
-  };
-
-  Cut cut{0, 0xffffffffu};  // all
-  bool listed = false;      // the tokens of the cut, and some behind it, are a list
-  // f(key, index, logit) of the list's tokens, or the row's, that weigh anything
-  auto each_listed = [&](auto f) {
-    for (uint32_t i = tid; i < s.listed; i += kThreads) {
-      const uint64_t e = s.list[i];
-      f(static_cast<uint32_t>(e >> 32), static_cast<uint32_t>(e), of_key(static_cast<uint32_t>(e >> 32)));
-    }
-  };
-  auto each_in_row = [&](auto f) {
-    row.mine([&](int i, float l) {
-      if (wt.some(wt.log2w(l))) f(key_of(l), static_cast<uint32_t>(i), l);
-    });
-  };
-  // the cut at which the running count or mass of the tokens with keys in [lo, hi] (of
-  // the present cut) reaches target
-  auto narrow = [&](auto by_mass, uint32_t lo, uint32_t hi, uint64_t target) {
-    constexpr bool M = decltype(by_mass)::value;
-    auto among = [&](auto each) {
-      const Found f = select<M>(s, bits_of(hi - lo), target, [&](auto g) {
-        each([&](uint32_t key, uint32_t i, float l) {
-          if (key >= lo && key <= hi && cut.keeps(key, i)) g(key - lo, M ? wt.of(l) : 0);
-        });
+  // The first token, by index, at which the running sum of f(index, logit) passes
+  // at(total): its index goes to done.  Every wave sums a part of the row, then of the
+  // part in which that is, until one wave holds the rest.
+  auto draw_in_row = [&](auto f, auto at_of, auto done) {
+    int v0 = 0, v1 = row.n;
+    uint64_t total = 0, at = 0;
+    for (bool first = true; first || v1 - v0 > 64; first = false) {
+      const int per = (v1 - v0 + kWaves - 1) / kWaves;
+      const int w0 = v0 + wave * per, w1 = w0 + per < v1 ? w0 + per : v1;
+      uint64_t sum = 0;
+      row.walk(w0, w1, [&](int i, const float(&x)[E]) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum += f(i + j, x[j]);
       });
-      const uint32_t key = lo + f.rank;
-      // equal ones: as many as it takes
-      uint64_t n = target - (M ? f.before_m : f.before_n);
-      if constexpr (M) {
-        const uint64_t one = f.in_m / f.in_n;
-        n = (n + one - 1) / one;
-      }
-      uint32_t index = cut.key == key ? cut.index : 0xffffffffu;
-      if (n < f.in_n) {
-        const uint32_t last = a.V - 1;
-        const Found g = select<false>(s, bits_of(last), n, [&](auto h) {
-          each([&](uint32_t ky, uint32_t i, float) {
-            if (ky == key && cut.keeps(ky, i)) h(last - i, 0);
-          });
-        });
-        index = last - g.rank;
-      }
-      cut = Cut{key, index};
-    };
-    if (listed)
-      among(each_listed);
-    else
-      among(each_in_row);
-  };
-
-  if (by_k || by_p) {
-    const bool sums = by_p && !by_k;
-    row.mine([&](int, float l) {
-      const double y = wt.log2w(l);
-      if (wt.some(y)) {
-        const int i = step(l);
-        if (sums) {
-          const uint64_t w = wt.whole(Weights::weight(y));
-          atomicAdd(&s.mass[i], static_cast<unsigned long long>(w));
-        }
-        atomicAdd(&s.count[i], 1u);
-      }
-    });
-    __syncthreads();
-    uint64_t target = k;
-    if (sums) {
-      uint64_t all = 0;
-      for (int i = tid; i < kSteps; i += kThreads) all += s.mass[i];
-      all = block_sum(s, all);
-      const double x = ceil(static_cast<double>(p) * static_cast<double>(all));
-      target = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
-      target = target < all ? target : all;
-      crossing<true>(s, kSteps, target, 0, 0);
-    } else {
-      crossing<false>(s, kSteps, target, 0, 0);
-    }
-    const int border = s.bin;
-    const uint32_t before_n = s.before_n, in_n = s.in_n;
-    const uint64_t before_m = s.before_m;
-    if (border >= 0) {  // (fewer than k weigh anything: k keeps them all)
-      listed = before_n + in_n <= kList;
-      uint32_t lo = 0xffffffffu, hi = 0;
-      row.mine([&](int i, float l) {
-        if (!wt.some(wt.log2w(l))) return;
-        const int at = step(l);
-        if (at > border) return;
-        const uint32_t key = key_of(l);
-        if (at == border) {
-          lo = key < lo ? key : lo;
-          hi = key > hi ? key : hi;
-        }
-        if (listed) s.list[atomicAdd(&s.listed, 1u)] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(i);
-      });
-      lo = wave_all(lo, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
-      hi = wave_all(hi, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-      if (lane == 0) {
-        atomicMin(&s.lo, lo);
-        atomicMax(&s.hi, hi);
-      }
+      sum = wave_sum(sum);
       __syncthreads();
-      lo = s.lo;
-      hi = s.hi;
-      if (sums)
-        narrow(std::true_type{}, lo, hi, target - before_m);
-      else
-        narrow(std::false_type{}, lo, hi, target - before_n);
+      if (lane == 0) s.wave_m[wave] = sum;
+      __syncthreads();
+      if (first) {
+        for (int w = 0; w < kWaves; ++w) total += s.wave_m[w];
+        at = at_of(total);
+      }
+      int w = 0;
+      while (w < kWaves - 1 && at >= s.wave_m[w]) at -= s.wave_m[w++];
+      v0 += w * per;
+      v1 = v0 + per < v1 ? v0 + per : v1;
     }
-  }
-
-  // top-p of what top-k left
-  if (by_k && by_p) {
-    uint64_t all = 0;
-    auto add = [&](uint32_t key, uint32_t i, float l) {
-      if (cut.keeps(key, i)) all += wt.of(l);
-    };
-    if (listed)
-      each_listed(add);
-    else
-      each_in_row(add);
-    all = block_sum(s, all);
-    const double x = ceil(static_cast<double>(p) * static_cast<double>(all));
-    uint64_t target = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
-    target = target < all ? target : all;
-    narrow(std::true_type{}, cut.key, key_of(m), target);
-  }
-
-  // the draw
-  auto weight_kept = [&](uint32_t key, uint32_t i, float l) -> uint64_t {
-    if (!cut.keeps(key, i)) return 0;
-    const double y = wt.log2w(l);
-    if (!wt.some(y)) return 0;
-    const double w = Weights::weight(y);
-    return w >= least ? wt.whole(w) : 0;
-  };
-  auto want = [&](uint64_t total) {  // running sums over this are behind the draw
-    const double x = u > 0.f ? static_cast<double>(u) * static_cast<double>(total) : 0.0;
-    const uint64_t at = x < static_cast<double>(total) ? static_cast<uint64_t>(x) : total;
-    return at < total ? at : total - 1;
-  };
-  auto done = [&](uint32_t index, float l, uint64_t total) {
-    a.token[b] = index;
-    if (a.logprob)
-      a.logprob[b] = static_cast<float>(wt.log2w(l) * 0.6931471805599453 -
-                                        log(ldexp(static_cast<double>(total), -wt.q)));
-  };
-  if (listed) {
-    uint64_t total = 0;
-    each_listed([&](uint32_t key, uint32_t i, float l) { total += weight_kept(key, i, l); });
-    total = block_sum(s, total);
-    const uint32_t last = a.V - 1;
-    const Found f = select<true>(s, bits_of(last), want(total) + 1, [&](auto g) {
-      each_listed([&](uint32_t key, uint32_t i, float l) {
-        const uint64_t w = weight_kept(key, i, l);
-        if (w) g(last - i, w);
-      });
-    });
-    each_listed([&](uint32_t, uint32_t i, float l) {
-      if (i == last - f.rank) done(i, l, total);
-    });
-    return;
-  }
-  int v0 = 0, v1 = row.n;
-  uint64_t total = 0, at = 0;
-  for (bool first = true; first || v1 - v0 > 64; first = false) {
-    const int per = (v1 - v0 + kWaves - 1) / kWaves;
-    const int w0 = v0 + wave * per, w1 = w0 + per < v1 ? w0 + per : v1;
-    uint64_t sum = 0;
-    row.walk(w0, w1, [&](int i, float l) { sum += weight_kept(key_of(l), static_cast<uint32_t>(i), l); });
-    sum = wave_all(sum, [](uint64_t x, uint64_t y) { return x + y; });
-    __syncthreads();
-    if (lane == 0) s.wave_mass[wave] = sum;
-    __syncthreads();
-    if (first) {
-      for (int w = 0; w < kWaves; ++w) total += s.wave_mass[w];
-      at = want(total);
-    }
-    int w = 0;
-    while (w < kWaves - 1 && at >= s.wave_mass[w]) at -= s.wave_mass[w++];
-    v0 += w * per;
-    v1 = v0 + per < v1 ? v0 + per : v1;
-  }
-  if (wave == 0) {
+    if (wave != 0) return;
     float x[E];
     uint64_t w[E], sum = 0;
     const int v = v0 + lane;
     if (v < v1) row.get(v, x);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      w[j] = v < v1 ? weight_kept(key_of(x[j]), static_cast<uint32_t>(v * E - row.off + j), x[j]) : 0;
+      w[j] = v < v1 ? f(v * E - row.off + j, x[j]) : 0;
       sum += w[j];
     }
     uint64_t run = wave_scan(sum) - sum;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      if (run <= at && at < run + w[j]) done(static_cast<uint32_t>(v * E - row.off + j), x[j], total);
+      if (run <= at && at < run + w[j]) done(v * E - row.off + j, x[j], total);
       run += w[j];
+    }
+  };
+  auto share = [&](uint64_t total, double of) -> uint64_t {  // the place of a draw in [0, total)
+    const double x = u > 0.f ? static_cast<double>(u) * of : 0.0;
+    const uint64_t at = x < of ? static_cast<uint64_t>(x) : total;
+    return at < total ? at : total - 1;
+  };
+  auto part = [&](uint64_t total) -> uint64_t {  // what top-p's run has to reach
+    const double x = ceil(static_cast<double>(p) * static_cast<double>(total));
+    const uint64_t y = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
+    return y < total ? y : total;
+  };
+  const bool by_k = k > 0 && k < a.V, by_p = p < 1.f;
+
+  if (m == INFINITY) {  // its tokens weigh the same, all others nothing
+    uint64_t kept = 0;
+    draw_in_row([&](int, float l) -> uint64_t { return l == INFINITY; },
+                [&](uint64_t total) {
+                  kept = by_k && k < static_cast<int64_t>(total) ? k : total;
+                  if (by_p) kept = part(kept);
+                  return share(kept, static_cast<double>(kept));
+                },
+                [&](int i, float, uint64_t) {
+                  a.token[b] = i;
+                  if (a.logprob) a.logprob[b] = static_cast<float>(-log(static_cast<double>(kept)));
+                });
+    return;
+  }
+
+  Weights wt;
+  wt.c = 1.4426950408889634 / static_cast<double>(t);
+  wt.M = m;
+  wt.q = a.q;
+  wt.lowest = -(a.q + 1.0);
+  wt.unit = ldexp(1.0, 52 - a.q);
+  wt.tab = s.tab;
+  double floor_y = wt.lowest;  // of what can be drawn
+  if (least > 0.f) floor_y = fmax(floor_y, log2(static_cast<double>(least)));
+  const uint32_t key_m = key_of(m);
+
+  auto at_of = [&](uint64_t total) { return share(total, static_cast<double>(total)); };
+  auto done = [&](int index, float l, uint64_t total) {
+    a.token[b] = index;
+    if (a.logprob)
+      a.logprob[b] = static_cast<float>(wt.log2w(l) * 0.6931471805599453 -
+                                        log(ldexp(static_cast<double>(total), -wt.q)));
+  };
+
+  // -- the list ----------------------------------------------------------------------
+  Cut cut{0, 0xffffffffu};  // all
+  uint32_t key[kEach], index[kEach];
+  int n = 0;                // tokens of the list, kEach threads apart
+  auto each_listed = [&](auto f) {  // f(key, index, e)
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (tid + e * NT < n) f(key[e], index[e]);
+  };
+  auto each_in_row = [&](auto f) {
+    row.mine([&](int i, const float(&x)[E]) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (wt.log2w(x[j]) >= wt.lowest) f(key_of(x[j]), static_cast<uint32_t>(i + j));
+    });
+  };
+  // the cut at which the running count or mass of the tokens of the present cut with
+  // keys in [lo, hi] reaches target
+  auto narrow = [&](auto by_mass, auto each, uint32_t lo, uint32_t hi, uint64_t target) {
+    constexpr bool BM = decltype(by_mass)::value;
+    const Found f = select<NT, BM>(s, bits_of(hi - lo), target, [&](auto g) {
+      each([&](uint32_t ky, uint32_t i) {
+        if (ky >= lo && ky <= hi && cut.keeps(ky, i)) g(ky - lo, BM ? wt.of(of_key(ky), wt.lowest) : 0);
+      });
+    });
+    const uint32_t border = lo + f.rank;
+    // equal ones: as many as it takes
+    uint64_t take = target - f.before;
+    if constexpr (BM) {
+      const uint64_t one = f.in_m / f.in_n;
+      take = (take + one - 1) / one;
+    }
+    uint32_t to = cut.key == border ? cut.index : 0xffffffffu;
+    if (take < f.in_n) {
+      const uint32_t last = a.V - 1;
+      const Found g = select<NT, false>(s, bits_of(last), take, [&](auto h) {
+        each([&](uint32_t ky, uint32_t i) {
+          if (ky == border && cut.keeps(ky, i)) h(last - i, 0);
+        });
+      });
+      to = last - g.rank;
+    }
+    cut = Cut{border, to};
+  };
+  // the row's tokens that `wanted` names become the list; whether it holds them
+  auto collect = [&](auto wanted) -> bool {
+    row.mine([&](int i, const float(&x)[E]) {
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < E; ++j) any |= wanted(x[j]);
+      if (!any) return;
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (wanted(x[j])) {
+          const uint32_t at = atomicAdd(&s.listed, 1u);
+          if (at < kList) s.list[at] = static_cast<uint64_t>(key_of(x[j])) << 32 | static_cast<uint32_t>(i + j);
+        }
+    });
+    __syncthreads();
+    n = static_cast<int>(s.listed);
+    const bool fits = n <= kList;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (fits && tid + e * NT < n) {
+        const uint64_t x = s.list[tid + e * NT];
+        key[e] = static_cast<uint32_t>(x >> 32);
+        index[e] = static_cast<uint32_t>(x);
+      }
+    __syncthreads();
+    if (tid == 0) s.listed = 0;
+    __syncthreads();
+    if (!fits) n = 0;
+    return fits;
+  };
+  auto under = [&](double steps) { return float_under(static_cast<double>(m) - steps / (64.0 * wt.c)); };
+
+  bool listed = kWhole;  // all that the cut keeps is in the list
+  if constexpr (kWhole) {
+    n = a.V;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (tid + e * NT < n) {
+        key[e] = key_of(row.one(tid + e * NT));
+        index[e] = tid + e * NT;
+        if (!(wt.log2w(of_key(key[e])) >= wt.lowest)) key[e] = 0;
+      }
+    if (by_k) {
+      uint64_t weigh = 0;
+      each_listed([&](uint32_t ky, uint32_t) { weigh += ky != 0; });
+      weigh = block_sum<NT>(s, weigh);
+      if (k < static_cast<int64_t>(weigh)) narrow(std::false_type{}, each_listed, 1, key_m, k);
+    }
+  } else if (by_k || by_p) {
+    const bool sums = by_p && !by_k;
+    // Top-k of up to NT: where the threads' largest tokens count k, so many lie above.
+    const bool by_threads = by_k && k <= NT;
+    auto count = [&](float l) {
+      const double y = wt.log2w(l);
+      if (y >= wt.lowest) atomicAdd(&s.count[wt.step(y)], 1u);
+    };
+    if (by_threads)
+      count(mine);
+    else
+      row.mine([&](int, const float(&x)[E]) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          if (sums) {
+            const double y = wt.log2w(x[j]);
+            const uint64_t w = wt.whole(y);
+            if (y >= wt.lowest) atomicAdd(&s.mass[wt.step(y)], static_cast<unsigned long long>(w));
+          } else {
+            count(x[j]);
+          }
+        }
+      });
+    __syncthreads();
+    uint64_t target = k;
+    if (sums)
+      crossing<NT, true>(s, [&](uint64_t total) { return target = part(total); });
+    else
+      crossing<NT, false>(s, [&](uint64_t) { return target; });
+    int border = s.bin;
+    if (by_threads && border < 0) border = kSteps - 1;
+    if (border >= 0) {  // (fewer than k weigh anything: k keeps them all)
+      // (half a step more than the border's, for roundings)
+      const float from = border == kSteps - 1 ? under(64.0 * (a.q + 2)) : under(border + 1.0);
+      const uint64_t before = s.before_m;
+      listed = collect([&](float l) { return l >= from; });
+      if (listed) {
+        uint64_t weigh = 0;
+        each_listed([&](uint32_t ky, uint32_t) { weigh += wt.log2w(of_key(ky)) >= wt.lowest; });
+        if (sums) {
+          narrow(std::true_type{}, each_listed, key_of(from), key_m, target);
+        } else {
+          weigh = block_sum<NT>(s, weigh);
+          if (k < static_cast<int64_t>(weigh)) narrow(std::false_type{}, each_listed, key_of(from), key_m, target);
+        }
+      } else if (!by_threads &&
+                 collect([&](float l) {
+                   if (!(l >= from)) return false;
+                   const double y = wt.log2w(l);
+                   return y >= wt.lowest && wt.step(y) == border;
+                 })) {
+        // the border's step alone
+        uint32_t lo = 0xffffffffu, hi = 0;
+        each_listed([&](uint32_t ky, uint32_t) {
+          lo = ky < lo ? ky : lo;
+          hi = ky > hi ? ky : hi;
+        });
+        lo = wave_all(lo, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+        hi = wave_all(hi, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+        if (lane == 0) {
+          atomicMin(&s.lo, lo);
+          atomicMax(&s.hi, hi);
+        }
+        __syncthreads();
+        lo = s.lo;
+        hi = s.hi;
+        if (sums)
+          narrow(std::true_type{}, each_listed, lo, hi, target - before);
+        else
+          narrow(std::false_type{}, each_listed, lo, hi, target - before);
+      } else {
+        uint64_t weigh = 0;
+        each_in_row([&](uint32_t, uint32_t) { ++weigh; });
+        weigh = block_sum<NT>(s, weigh);
+        if (sums)
+          narrow(std::true_type{}, each_in_row, 0, key_m, target);
+        else if (k < static_cast<int64_t>(weigh))
+          narrow(std::false_type{}, each_in_row, 0, key_m, target);
+      }
+    }
+  }
+
+  // top-p of what top-k left, or of a row that is its own list
+  if (by_p && (by_k || kWhole)) {
+    uint64_t all = 0;
+    auto add = [&](uint32_t ky, uint32_t i) {
+      if (cut.keeps(ky, i)) all += wt.of(of_key(ky), wt.lowest);
+    };
+    if (listed) {
+      each_listed(add);
+      all = block_sum<NT>(s, all);
+      narrow(std::true_type{}, each_listed, cut.key, key_m, part(all));
+    } else if constexpr (!kWhole) {
+      each_in_row(add);
+      all = block_sum<NT>(s, all);
+      narrow(std::true_type{}, each_in_row, cut.key, key_m, part(all));
+    }
+  }
+
+  // -- the draw ----------------------------------------------------------------------
+  if (listed) {
+    uint64_t w[kEach], total = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      w[e] = 0;
+      if (tid + e * NT < n && cut.keeps(key[e], index[e])) w[e] = wt.of(of_key(key[e]), floor_y);
+      total += w[e];
+    }
+    total = block_sum<NT>(s, total);
+    const uint32_t last = a.V - 1;
+    const Found f = select<NT, true>(s, bits_of(last), at_of(total) + 1, [&](auto g) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (w[e]) g(last - index[e], w[e]);
+    });
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (w[e] && index[e] == last - f.rank) done(index[e], of_key(key[e]), total);
+  } else if constexpr (!kWhole) {
+    if (cut.key == 0) {
+      draw_in_row([&](int, float l) { return wt.of(l, floor_y); }, at_of, done);
+    } else {
+      const float border = of_key(cut.key);
+      const int to = cut.index > 0x7fffffffu ? 0x7fffffff : static_cast<int>(cut.index);
+      draw_in_row([&](int i, float l) { return l > border || (l == border && i <= to) ? wt.of(l, floor_y) : 0; }, at_of,
+                  done);
     }
   }
 }
@@ -603,9 +753,16 @@ extern "C" srw_status_t srw_sample(const srw_sample_t* d, void* stream) {
   a.logprob = d->logprob;
   (void)hipGetLastError();
   const dim3 grid(static_cast<unsigned>(d->B));
-  if (d->dtype == SRW_F32)
-    hipLaunchKernelGGL((srw::sample_kernel<float>), grid, dim3(srw::kThreads), 0, static_cast<hipStream_t>(stream), a);
-  else
-    hipLaunchKernelGGL((srw::sample_kernel<uint16_t>), grid, dim3(srw::kThreads), 0, static_cast<hipStream_t>(stream), a);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (d->V <= srw::kList) {
+    if (d->dtype == SRW_F32)
+      hipLaunchKernelGGL((srw::sample_kernel<float, 256>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((srw::sample_kernel<uint16_t, 256>), grid, dim3(256), 0, s, a);
+  } else if (d->dtype == SRW_F32) {
+    hipLaunchKernelGGL((srw::sample_kernel<float, 1024>), grid, dim3(1024), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((srw::sample_kernel<uint16_t, 1024>), grid, dim3(1024), 0, s, a);
+  }
   return hipGetLastError() == hipSuccess ? SRW_OK : SRW_EHIP;
 }
