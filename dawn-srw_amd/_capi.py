@@ -61,7 +61,7 @@ EXPORTED_SYMBOLS = (
     "srw_diag_summary", "srw_cast_bf16", "srw_dawn_decode_step",
     "srw_kv_write", "srw_kv_read", "srw_attention_workspace_size", "srw_attention", "srw_attention_plan",
     "srw_kv_copy", "srw_kv_index", "srw_kv_select", "srw_attention_kept_workspace_size", "srw_attention_kept",
-    "srw_sample",
+    "srw_sample_workspace_size", "srw_sample",
 )
 
 # srw_diag_out_t: the result tuple's per-token values and scalars (SRW_DSUM_*)
@@ -268,9 +268,13 @@ def load_library() -> ctypes.CDLL:
         lib.srw_attention_plan.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]
         lib.srw_attention.restype = ctypes.c_int
         lib.srw_attention.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
-        for name in ("srw_kv_copy", "srw_kv_select", "srw_sample"):
+        for name in ("srw_kv_copy", "srw_kv_select"):
             getattr(lib, name).restype = ctypes.c_int
             getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        lib.srw_sample_workspace_size.restype = ctypes.c_int
+        lib.srw_sample_workspace_size.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]
+        lib.srw_sample.restype = ctypes.c_int
+        lib.srw_sample.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.srw_kv_index.restype = ctypes.c_int
         lib.srw_kv_index.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         lib.srw_attention_kept_workspace_size.restype = ctypes.c_int

@@ -6,18 +6,29 @@
 // each keep a first part of that order, and the token drawn is the first, by
 // index, at which the kept weights' running sum passes u times their sum.
 //
-// Weights are whole numbers W = round(2^q w), w from a polynomial in 64 bits (to
-// 2^-46), q as large as V W < 2^62 allows: sums of them are exact, so no order of
-// adding, no atomic and no split of the row changes what a row gives, and a
-// border is where 64 bits put it.  What rounds to zero cannot be drawn and takes
-// no part.
+// With y = l log2 e / t, weights are whole numbers W = round(2^(q + y - R)), from a
+// polynomial in 64 bits (to 2^-40), R a whole number not under M's y and q as large as
+// V W < 2^62 allows: sums of them are exact, so no order of adding and no atomic
+// changes what a row gives, and a border is where 64 bits put it.  What rounds to zero
+// cannot be drawn and takes no part.
 //
-// Nothing is sorted.  One pass finds M.  A threshold that the border of top-k or
-// top-p cannot lie above comes from counts or sums of tokens by how far they lie
-// under M, in steps of 2^(1/64); the tokens down to it, if there are no more than
-// kList, become a list that a workgroup holds in registers, and the rest is done on
-// them: the border by digits of the logits' bits, the draw by digits of the index.
-// Rows that keep more are walked again instead.
+// Nothing is sorted.  A threshold that the border of top-k or top-p cannot lie above
+// is found first; the tokens down to it, if there are no more than kList, become a
+// list in LDS, and the rest is done on them: borders by digits of the logits' bits,
+// the draw by digits of the index.
+//
+// * Top-k of up to 1 024: the threads' largest logits are counted by steps of
+//   2^(1/32); where k of them lie above, so many tokens do.
+// * Top-p, and rows without either: sample_parts_kernel has summed each part of 8 192
+//   logits, for top-p by steps of 2^(1/8), over its own R (sums of parts meet in
+//   float64, 2^-52 of them).  Of top-p rows that keep more than kList the tokens of the
+//   border's step alone become the list; the draw finds its part by the parts' sums and
+//   walks that one.
+//
+// A workgroup of sixteen waves has a CU's vector units to itself, and an instruction
+// of all of them takes it 16 cycles (24 in 64 bits): what is done for the row as a
+// whole is left to one wave, lists are dense so that the waves behind their end have
+// nothing to do, and loops over the row test a vector before they look at its logits.
 
 #include <math.h>
 
@@ -27,156 +38,238 @@
 namespace srw {
 namespace {
 
-constexpr int kSteps = 2048;   // of 2^(1/64) under M
-constexpr int kList = 4096;    // tokens that a workgroup's registers hold
-constexpr int kDigit = 9;      // bits of a select's pass
+constexpr int kSteps = 1024;   // of 2^(1/32) under 2^R
+constexpr int kCoarse = 256;   // of 2^(1/8), what parts are summed by
+constexpr int kList = 4096;    // tokens of a list
+constexpr int kPart = 8192;    // logits of a part
+constexpr int kDigit = 9, kBins = 1 << kDigit;  // bits of a select's pass
+constexpr int kMostParts = (1 << 24) / kPart + 2;
 
 struct SampleArgs {
   const char* logits;
   int64_t stride;  // elements
-  int32_t V, q;
+  int32_t V, q, parts;
   const float *u, *temperature, *top_p, *min_p;
   const int32_t* top_k;
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
   int64_t* token;
   float* logprob;
+  // of every row and part: its largest logit, its sum, and for top-p the steps' sums
+  float* part_max;
+  unsigned long long *part_sum, *part_steps;
+};
+
+// A row's parameters.
+struct Rules {
+  float t, p, least;
+  int k;
+  bool greedy, by_k, by_p;
+  __device__ __forceinline__ Rules(const SampleArgs& a, int64_t b) {
+    t = a.temperature ? a.temperature[b] : a.temperature_all;
+    k = a.top_k ? a.top_k[b] : a.top_k_all;
+    p = a.top_p ? a.top_p[b] : a.top_p_all;
+    least = a.min_p ? a.min_p[b] : a.min_p_all;
+    least = least > 0.f ? (least < 1.f ? least : 1.f) : 0.f;
+    greedy = !(t > 0.f) || k == 1;
+    by_k = k > 0 && k < a.V;
+    by_p = p < 1.f;
+  }
+  // whether the parts' sums are asked for
+  __device__ __forceinline__ bool by_parts() const { return !greedy && !by_k && (by_p || least == 0.f); }
 };
 
 // A number's place among all: larger logits have larger keys, -0 is 0, NaN the
 // smallest.
-__device__ inline uint32_t key_of(float l) {
+__device__ __forceinline__ uint32_t key_of(float l) {
   const uint32_t b = __float_as_uint(l + 0.f);
   if (l != l) return 0;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ inline float of_key(uint32_t k) {
+__device__ __forceinline__ float of_key(uint32_t k) {
   return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
-__device__ inline float float_under(double x) {  // the largest float that is not above x
+__device__ __forceinline__ float float_under(double x) {  // the largest float that is not above x
   const float f = static_cast<float>(x);
   if (!(static_cast<double>(f) > x)) return f;
   return of_key(key_of(f) - 1);
 }
 
-// What a row's weights go by: log2 w = (l - M) c, c = log2 e / t.
+// 2^(j / 128).
+__device__ __forceinline__ void fill_table(double* tab) {
+  if (threadIdx.x < 128) tab[threadIdx.x] = exp2(static_cast<int>(threadIdx.x) / 128.0);
+}
+
+// What the weights of a row, or of a part, go by.  The same roundings wherever a weight
+// is worked out (no contraction): sums of some tokens and of all agree to the last unit.
 struct Weights {
-  double c, M, lowest, unit;  // lowest: what weighs less rounds to zero; unit 2^(52 - q)
-  int q;
-  const double* tab;                // 2^(j / 64)
-  __device__ double log2w(float l) const { return (static_cast<double>(l) - M) * c; }
-  // 64 log2 w to the nearest, in the low bits of a sum (of log2 w above -2^25)
-  static constexpr double kMagic = 0x1.8p46;
-  // round(2^q w): 2^(n / 64) from the table, the rest of the exponent, at most 1 / 128,
-  // by a polynomial that is 1 at 0 and elsewhere 5e-15 off at most.  Garbage below
-  // `lowest`.
-  __device__ uint64_t whole(double y) const {
-    const double t = y + kMagic;
-    const int n = static_cast<int>(__double_as_longlong(t));
+  double c, unit;     // log2 e / t, 2^(52 - q)
+  const double* tab;  // 2^(j / 128)
+  int R;
+  float lowest;       // smaller logits weigh nothing; above -infinity
+
+  // Whether 2^30 and more lies under M's y: the next smaller logit is 2^6 octaves away
+  // and weighs nothing.
+  __device__ __forceinline__ static bool peaked(float m, double c) {
+    return !(fabs(static_cast<double>(m) * c) < 1073741824.0);
+  }
+  __device__ __forceinline__ void set(float m, int q) {
+    R = static_cast<int>(ceil(static_cast<double>(m) * c));
+    lowest = static_cast<float>(fmax((R - q - 1.0) / c, -3.4028234663852886e38));
+  }
+  // 128 y to the nearest, in the low bits of a sum
+  static constexpr double kMagic = 0x1.8p45;
+  __device__ __forceinline__ static int n_of(double t) { return static_cast<int>(__double_as_longlong(t)); }
+  __device__ __forceinline__ double sum_of(float l) const {
+#pragma clang fp contract(off)
+    return static_cast<double>(l) * c + kMagic;
+  }
+  // W, for logits that weigh something (garbage for others): 2^(n / 128) from the
+  // table, the rest of the exponent, at most 1 / 256, by a polynomial that is 1 at 0 and
+  // elsewhere 6e-13 off at most.
+  __device__ __forceinline__ uint64_t whole(float l) const {
+#pragma clang fp contract(off)
+    const double y = static_cast<double>(l) * c, t = y + kMagic;
+    const int n = n_of(t);
     const double r = y - (t - kMagic);
-    double p = 0x1.3b2acb2c36b23p-7;
-    p = fma(p, r, 0x1.c6b0b9214b9aep-5);
-    p = fma(p, r, 0x1.ebfbdff82bb76p-3);
-    p = fma(p, r, 0x1.62e42fefa2417p-1);
-    p = fma(p, r, 1.0);
-    p *= tab[n & 63];
-    p = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
+    double p = fma(0x1.c6b095a17a14dp-5, r, 0x1.ebfbeebe2d1a2p-3);
+    p = fma(p, r, 0x1.62e42fefa39efp-1);
+    p = fma(p, r, 1.0) * tab[n & 127];
+    p = __hiloint2double(__double2hiint(p) + (((n >> 7) - R) << 20), __double2loint(p));
     // the low bits of a sum whose last place is 2^-q
     return static_cast<uint64_t>(__double_as_longlong(p + unit)) & 0xfffffffffffffull;
   }
-  // What a token adds to sums, down to the log2 weight `least` (false for NaN).
-  __device__ uint64_t of(float l, double least) const {
-    const double y = log2w(l);
-    const uint64_t w = whole(y);
-    return y >= least ? w : 0;
+  __device__ __forceinline__ uint64_t of(float l, float least) const {
+    const uint64_t w = whole(l);
+    return l >= least ? w : 0;
   }
-  // steps of 2^(1/64) under M
-  __device__ int step(double y) const {
-    const int n = -static_cast<int>(__double_as_longlong(fmax(y, -40.0) + kMagic));
-    return n < 0 ? 0 : n < kSteps ? n : kSteps - 1;
+  // steps of 2^(1/32) under 2^R
+  __device__ __forceinline__ int step(float l) const {
+    const int n = 128 * R - n_of(sum_of(l));
+    return n < 4 * kSteps ? n >> 2 : kSteps - 1;
   }
 };
 
+// log2 x of x in [2^-30, 2^63]: float32's, mended by what it is off.
+__device__ __forceinline__ double log2_of(double x, const double* tab) {
+  const float l = __builtin_amdgcn_logf(static_cast<float>(x));
+  Weights w;
+  w.tab = tab;
+  const double y = l, t = y + Weights::kMagic;
+  const int n = Weights::n_of(t);
+  const double r = y - (t - Weights::kMagic);
+  double p = fma(0x1.c6b095a17a14dp-5, r, 0x1.ebfbeebe2d1a2p-3);
+  p = fma(p, r, 0x1.62e42fefa39efp-1);
+  p = fma(p, r, 1.0) * tab[n & 127];
+  p = __hiloint2double(__double2hiint(p) + ((n >> 7) << 20), __double2loint(p));  // 2^l
+  const double e = (x - p) / p;                                                   // some 1e-7
+  return y + e * (1.0 - 0.5 * e) * 1.4426950408889634;
+}
+
+// A row: vectors of 16 bytes, the first and the last of them partly outside of it.
 template <typename T, int NT> struct Row {
   static constexpr int E = 16 / sizeof(T);  // logits of a vector
+  static constexpr int kWaves = NT / 64;
   const T* p;
   int V, off, n;  // the row begins off logits behind a 16-byte border; its vectors
-  __device__ Row(const SampleArgs& a, int64_t b) {
+  int v0, v1;     // the wave's
+  __device__ __forceinline__ Row(const SampleArgs& a, int64_t b) {
     p = reinterpret_cast<const T*>(a.logits) + b * a.stride;
     V = a.V;
     off = static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
     n = (off + V + E - 1) / E;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = part();
+    v0 = wave * per < n ? wave * per : n;
+    v1 = v0 + per < n ? v0 + per : n;
   }
-  __device__ float one(int i) const {
+  __device__ __forceinline__ int part() const { return (n + kWaves - 1) / kWaves; }
+  __device__ __forceinline__ float one(int i) const {
     if constexpr (E == 4)
       return p[i];
     else
       return __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
   }
-  // Vector v: logits E v - off ...; those outside the row as NaN.
-  __device__ void get(int v, float (&x)[E]) const {
-    const int i = v * E - off;
-    if (i >= 0 && i + E <= V) {
-      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p + i);
+  // Vector v + lane: logits E (v + lane) - off ...; those outside the row, and those of
+  // vectors from `end` on, as NaN.
+  __device__ __forceinline__ u32x4_t raw(int v, int end) const {
+    const int lane = threadIdx.x & 63, i = (v + lane) * E - off;
+    const u32x4_t* at = reinterpret_cast<const u32x4_t*>(p + i);
+    if (v * E >= off && (v + 64) * E - off <= V && v + 64 <= end) return *at;
+    u32x4_t w;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (E == 4) {
-          x[j] = __uint_as_float(w[j]);
-        } else {
-          x[2 * j] = lo_f32(w[j]);
-          x[2 * j + 1] = hi_f32(w[j]);
-        }
+    for (int j = 0; j < 4; ++j) w[j] = E == 4 ? 0x7fc00000u : 0x7fc07fc0u;
+    if (v + lane >= end) return w;
+    if (i >= 0 && i + E <= V) return *at;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (i + j >= 0 && i + j < V) {
+        if constexpr (E == 4)
+          w[j] = __float_as_uint(p[i + j]);
+        else
+          w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | static_cast<uint32_t>(p[i + j]) << 16 : (w[j / 2] & 0xffff0000u) | p[i + j];
       }
-    } else {
+    return w;
+  }
+  __device__ __forceinline__ static void wide(u32x4_t w, float (&x)[E]) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        x[j] = __uint_as_float(0x7fc00000u);
-        if (i + j >= 0 && i + j < V) x[j] = one(i + j);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (E == 4) {
+        x[j] = __uint_as_float(w[j]);
+      } else {
+        x[2 * j] = lo_f32(w[j]);
+        x[2 * j + 1] = hi_f32(w[j]);
       }
     }
   }
-  // f(index of the first, logits) of the vectors [v0, v1), one a lane, by the whole wave
+  // f(index of the first, logits) of the vectors [from, to), one a lane, by the whole
+  // wave, the next two on their way.
   template <class F>
-  __device__ void walk(int v0, int v1, F f) const {
-    constexpr int U = 4;  // loads in flight
-    int v = v0 + (threadIdx.x & 63);
-    for (; v + 64 * (U - 1) < v1; v += 64 * U) {
-      float x[U][E];
-#pragma unroll
-      for (int k = 0; k < U; ++k) get(v + 64 * k, x[k]);
-#pragma unroll
-      for (int k = 0; k < U; ++k) f((v + 64 * k) * E - off, x[k]);
-    }
-    for (; v < v1; v += 64) {
+  __device__ __forceinline__ void walk(int from, int to, F f) const {
+    if (from >= to) return;
+    u32x4_t a = raw(from, to), b = raw(from + 64, to);
+#pragma unroll 1
+    for (; from < to; from += 64) {
       float x[E];
-      get(v, x);
-      f(v * E - off, x);
+      wide(a, x);
+      a = b;
+      if (from + 128 < to) b = raw(from + 128, to);
+      f((from + static_cast<int>(threadIdx.x & 63)) * E - off, x);
     }
   }
-  // the part of the row that is this wave's
-  template <class F>
-  __device__ void mine(F f) const {
-    constexpr int kWaves = NT / 64;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int per = (n + kWaves - 1) / kWaves;
-    walk(wave * per, (wave + 1) * per < n ? (wave + 1) * per : n, f);
+  __device__ __forceinline__ float largest() const {  // of the thread's part
+    constexpr int U = 4;
+    float m = -INFINITY, x[E];
+    int from = v0;
+#pragma unroll 1
+    for (; from < v1; from += 64 * U) {
+      u32x4_t w[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) w[k] = raw(from + 64 * k, v1);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        wide(w[k], x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) m = fmaxf(m, x[j]);
+      }
+    }
+    return m;
   }
 };
 
 // v of the lane that DPP control C names, 0 where there is none or MASK leaves the
 // row of 16 out.
 template <int C, int MASK>
-__device__ inline uint32_t moved(uint32_t v) {
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), C, MASK, 0xf, false));
 }
 template <int C, int MASK>
-__device__ inline uint64_t moved(uint64_t v) {
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
   return static_cast<uint64_t>(moved<C, MASK>(static_cast<uint32_t>(v >> 32))) << 32 |
          moved<C, MASK>(static_cast<uint32_t>(v));
 }
 // Sums over this lane and those before it: within rows of 16, then the rows.
 template <class N>
-__device__ inline N wave_scan(N v) {
+__device__ __forceinline__ N wave_scan(N v) {
   v += moved<0x111, 0xf>(v);
   v += moved<0x112, 0xf>(v);
   v += moved<0x114, 0xf>(v);
@@ -185,192 +278,272 @@ __device__ inline N wave_scan(N v) {
   v += moved<0x143, 0xc>(v);
   return v;
 }
-__device__ inline uint32_t last_lane(uint32_t v) { return __builtin_amdgcn_readlane(v, 63); }
-__device__ inline uint64_t last_lane(uint64_t v) {
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
   return static_cast<uint64_t>(last_lane(static_cast<uint32_t>(v >> 32))) << 32 | last_lane(static_cast<uint32_t>(v));
 }
 template <class N>
-__device__ inline N wave_sum(N v) {
+__device__ __forceinline__ N wave_sum(N v) {
   return last_lane(wave_scan(v));
 }
 template <class N, class Op>
-__device__ inline N wave_all(N v, Op op) {
+__device__ __forceinline__ N wave_all(N v, Op op) {
 #pragma unroll
   for (int w = 1; w < 64; w <<= 1) v = op(v, __shfl_xor(v, w));
   return v;
 }
 
-struct Shared {
-  double tab[64];
-  unsigned long long mass[kSteps];
+template <int NT> struct Shared {
+  double tab[128];
+  union {
+    unsigned long long list[kList];  // key << 32 | index
+    double steps[4][kCoarse];        // of parts, a quarter of them each
+  };
   uint32_t count[kSteps];
-  unsigned long long list[kList];  // key << 32 | index
+  unsigned long long mass[kBins + 64];
+  unsigned long long kept[NT == 1024 ? kMostParts : 1];  // of each part, in its units
+  unsigned long long few_rank[64], few_mass[64];
   unsigned long long wave_m[16];
-  uint32_t wave_n[16];
   float wave_max[16];
   // a crossing: the bin (-1: none), what lies before it and in it
-  int bin;
-  uint32_t before_n, in_n, listed, lo, hi;
-  unsigned long long before_m, in_m;
+  int bin, part;
+  uint32_t in_n, few, first, listed;
+  unsigned long long before, rank, at;
+  double total, above, guess;
 };
 
+// Every wave's number, on all lanes: each of the first NT / 64 lanes its own.
 template <int NT>
-__device__ inline uint64_t block_sum(Shared& s, uint64_t v) {
-  v = wave_sum(v);
+__device__ __forceinline__ uint64_t of_waves(Shared<NT>& s, uint64_t v) {
   if ((threadIdx.x & 63) == 0) s.wave_m[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) v += s.wave_m[w];
+  const int lane = threadIdx.x & 63;
+  v = lane < NT / 64 ? s.wave_m[lane] : 0;
   __syncthreads();
   return v;
 }
+template <int NT>
+__device__ __forceinline__ uint64_t block_sum(Shared<NT>& s, uint64_t v) {
+  return wave_sum(of_waves<NT>(s, wave_sum(v)));
+}
 
-// The first of kSteps bins (of s.count, or BY_MASS of s.mass) at which the running
-// count (or mass) reaches what target(total) says.
-template <int NT, bool BY_MASS, class Target>
-__device__ inline void crossing(Shared& s, Target target) {
-  const int tid = threadIdx.x, wave = tid >> 6;
-  constexpr int per = kSteps / NT;  // bins a thread
-  uint64_t x[per], sum = 0;
-#pragma unroll
-  for (int k = 0; k < per; ++k) {
-    x[k] = BY_MASS ? s.mass[tid * per + k] : s.count[tid * per + k];
-    sum += x[k];
-  }
-  uint64_t run = wave_scan(sum);
-  if ((tid & 63) == 63) s.wave_m[wave] = run;
-  if (tid == 0) s.bin = -1;
-  __syncthreads();
-  uint64_t total = 0;
-  run -= sum;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) {
-    run += w < wave ? s.wave_m[w] : 0;
-    total += s.wave_m[w];
-  }
-  const uint64_t t = target(total);
-#pragma unroll
-  for (int k = 0; k < per; ++k) {
-    if (run < t && run + x[k] >= t) {
-      s.bin = tid * per + k;
-      s.before_m = run;
-    }
-    run += x[k];
+// The first step at which s.count's running sum reaches target.
+template <int NT>
+__device__ __forceinline__ void crossing(Shared<NT>& s, uint32_t target) {
+  static_assert(NT == kSteps);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t c = s.count[threadIdx.x];
+  uint32_t run = wave_scan(c);
+  if (threadIdx.x == 0) s.bin = -1;
+  const uint32_t waves = wave_scan(static_cast<uint32_t>(of_waves<NT>(s, last_lane(run))));
+  run += (wave > 0 ? __builtin_amdgcn_readlane(waves, wave > 0 ? wave - 1 : 0) : 0) - c;
+  if (run < target && run + c >= target) {
+    s.bin = threadIdx.x;
+    s.before = run;
   }
   __syncthreads();
 }
 
-// Among candidates, the rank (the largest first, of `bits` bits) at which the
-// running count (or mass) reaches target >= 1, with what lies before that rank and
-// in it.  each(f) calls f(rank, mass) for every candidate of this thread.  There
-// must be such a rank.
-struct Found {
-  uint32_t rank, in_n;
-  uint64_t before, in_m;
-};
-template <int NT, bool BY_MASS, class Each>
-__device__ inline Found select(Shared& s, int bits, uint64_t target, Each each) {
-  constexpr int kBins = 1 << kDigit, kEach = kBins / 64;
+// Among candidates of different ranks (of `bits` bits), the one at which the running
+// mass, the largest rank first, reaches target >= 1; there must be one.  each(f) calls
+// f(rank, mass) for every candidate of this thread, of which there are no more than n.
+// A pass takes a digit; where no more than 64 candidates share the digits up to the
+// border's, one wave compares each with each.
+template <int NT, class Each>
+__device__ __forceinline__ uint64_t select(Shared<NT>& s, int bits, uint64_t target, uint32_t n, Each each) {
+  constexpr int kEach = kBins / 64;
   auto place = [](int i) { return i + i / kEach; };  // (a lane's run of bins, over all banks)
-  Found f{0, 0, 0, 0};
+  const int lane = threadIdx.x & 63;
+  uint64_t rank = 0, before = 0;
   int left = bits;
-  while (left > 0) {
+#pragma unroll 1
+  for (;;) {
+    if (threadIdx.x == 0) s.few = 0;
+    if (n <= 64) {
+      __syncthreads();
+      each([&](uint64_t r, uint64_t m) {
+        if (left < 64 && r >> left != rank) return;
+        const uint32_t at = atomicAdd(&s.few, 1u);
+        s.few_rank[at] = r;
+        s.few_mass[at] = m;
+      });
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        const int c = static_cast<int>(s.few);
+        const uint64_t r = lane < c ? s.few_rank[lane] : 0, m = lane < c ? s.few_mass[lane] : 0;
+        uint64_t run = before;
+#pragma unroll 1
+        for (int j = 0; j < c; ++j) {
+          const uint64_t rj = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(r >> 32), j)) << 32 |
+                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(r), j));
+          const uint64_t mj = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(m >> 32), j)) << 32 |
+                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(m), j));
+          run += rj > r ? mj : 0;
+        }
+        if (lane < c && run < target && run + m >= target) s.rank = r;
+      }
+      __syncthreads();
+      return s.rank;
+    }
     const int d = left < kDigit ? left : kDigit, shift = left - d, last = (1 << d) - 1;
     for (int i = threadIdx.x; i < kBins + 64; i += NT) {
       s.count[i] = 0;
-      if constexpr (BY_MASS) s.mass[i] = 0;
+      s.mass[i] = 0;
     }
     __syncthreads();
-    each([&](uint32_t rank, uint64_t m) {
-      if (left < 32 && rank >> left != f.rank) return;
-      const int bin = place(last - static_cast<int>(rank >> shift & static_cast<uint32_t>(last)));  // the largest first
+    each([&](uint64_t r, uint64_t m) {
+      if (r >> left != rank) return;
+      const int bin = place(last - static_cast<int>(static_cast<uint32_t>(r >> shift) & static_cast<uint32_t>(last)));
       atomicAdd(&s.count[bin], 1u);
-      if constexpr (BY_MASS) atomicAdd(&s.mass[bin], static_cast<unsigned long long>(m));
+      atomicAdd(&s.mass[bin], static_cast<unsigned long long>(m));
     });
     __syncthreads();
     if (threadIdx.x < 64) {
-      uint32_t c[kEach];
       uint64_t m[kEach], sum = 0;
 #pragma unroll
       for (int k = 0; k < kEach; ++k) {
-        const int i = place(threadIdx.x * kEach + k);
-        c[k] = s.count[i];
-        m[k] = BY_MASS ? s.mass[i] : c[k];
+        m[k] = s.mass[place(lane * kEach + k)];
         sum += m[k];
       }
-      uint64_t run = f.before + wave_scan(sum) - sum;
+      uint64_t run = before + wave_scan(sum) - sum;
 #pragma unroll
       for (int k = 0; k < kEach; ++k) {
         if (run < target && run + m[k] >= target) {
-          s.bin = threadIdx.x * kEach + k;
-          s.before_m = run;
-          s.in_n = c[k];
-          s.in_m = m[k];
+          s.bin = lane * kEach + k;
+          s.before = run;
+          s.in_n = s.count[place(lane * kEach + k)];
         }
         run += m[k];
       }
     }
     __syncthreads();
-    f.rank = f.rank << d | static_cast<uint32_t>(last - s.bin);
-    f.before = s.before_m;
-    f.in_n = s.in_n;
-    f.in_m = s.in_m;
+    rank = rank << d | static_cast<uint32_t>(last - s.bin);
+    before = s.before;
+    n = s.in_n;
     left = shift;
+    if (left == 0) return rank;
   }
-  return f;
 }
 
-__device__ inline int bits_of(uint32_t most) { return most == 0 ? 1 : 32 - __clz(most); }
+__device__ __forceinline__ int first_of(uint64_t lanes) { return __builtin_ctzll(lanes); }
+__device__ __forceinline__ int last_of(uint64_t lanes) { return 63 - __builtin_clzll(lanes); }
+__device__ __forceinline__ int bits_of(uint32_t most) { return most == 0 ? 1 : 32 - __clz(most); }
 
 // A first part of the order: tokens of larger keys, and those of this key up to an
 // index.
 struct Cut {
   uint32_t key, index;
-  __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= index); }
+  __device__ __forceinline__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= index); }
 };
+
+// The largest logit and the sum of weights of a row's part of kPart logits, and, for
+// top-p, its sums by steps.  A lane holds its 32 logits in registers.  Bound by the
+// memory for whole rows of float32 (512 rows of 100 003: MEASURED1), by the ten
+// operations in 64 bits of a weight and as many others for top-p and bf16.
+template <typename T>
+__global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
+  using R = Row<T, 256>;
+  constexpr int E = R::E, kHeld = kPart / 256 / E;  // vectors of a lane
+  __shared__ double tab[128];
+  __shared__ unsigned long long hist[kSteps], wave_sums[4];
+  __shared__ float wave_max[4];
+  const int64_t b = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  const Rules rules(a, b);
+  if (!rules.by_parts()) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const R row(a, b);
+  const int first = part * (kPart / E) + wave * 64 * kHeld;
+  u32x4_t held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) held[k] = row.raw(first + 64 * k, row.n);
+  fill_table(tab);
+  if (rules.by_p)
+    for (int i = tid; i < kSteps; i += 256) hist[i] = 0;
+  float m = -INFINITY, x[E];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    R::wide(held[k], x);
+#pragma unroll
+    for (int j = 0; j < E; ++j) m = fmaxf(m, x[j]);
+  }
+  m = wave_all(m, [](float u, float v) { return fmaxf(u, v); });
+  if (lane == 0) wave_max[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
+  const int64_t at = b * a.parts + part;
+  Weights wt;
+  wt.c = 1.4426950408889634 / static_cast<double>(rules.t);
+  wt.unit = ldexp(1.0, 52 - a.q);
+  wt.tab = tab;
+  const bool nothing = Weights::peaked(m, wt.c) || m == -INFINITY;  // (the row's draw does not ask)
+  if (!nothing) wt.set(m, a.q);
+  uint64_t sum = 0;
+  if (!nothing) {
+    if (rules.by_p) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        R::wide(held[k], x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const uint64_t w = wt.whole(x[j]);
+          if (x[j] >= wt.lowest) atomicAdd(&hist[wt.step(x[j])], static_cast<unsigned long long>(w));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        R::wide(held[k], x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum += wt.of(x[j], wt.lowest);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      sum = wave_sum(sum);
+      if (lane == 0) wave_sums[wave] = sum;
+    }
+  }
+  if (tid == 0) a.part_max[at] = m;
+  __syncthreads();
+  if (rules.by_p) {
+    a.part_steps[at * kCoarse + tid] = hist[4 * tid] + hist[4 * tid + 1] + hist[4 * tid + 2] + hist[4 * tid + 3];
+  } else if (tid == 0) {
+    a.part_sum[at] = nothing ? 0 : wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
+  }
+}
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
-  constexpr int kWaves = NT / 64, kEach = kList / NT;  // kEach: a thread's tokens of a list
-  constexpr bool kWhole = NT == 256;                   // every row is its own list
+  constexpr int kWaves = NT / 64;
+  constexpr bool kWhole = NT == 256;  // every row is its own list
   using R = Row<T, NT>;
   constexpr int E = R::E;
-  __shared__ Shared s;
+  __shared__ Shared<NT> s;
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const R row(a, b);
-  const float t = a.temperature ? a.temperature[b] : a.temperature_all;
-  const int k = a.top_k ? a.top_k[b] : a.top_k_all;
-  const float p = a.top_p ? a.top_p[b] : a.top_p_all;
-  float least = a.min_p ? a.min_p[b] : a.min_p_all;
-  least = least > 0.f ? (least < 1.f ? least : 1.f) : 0.f;
+  const Rules rules(a, b);
+  const int k = rules.k;
+  const bool by_k = rules.by_k, by_p = rules.by_p, by_parts = !kWhole && rules.by_parts();
   const float u = a.u[b];
+  const float* part_max = a.part_max + b * a.parts;
 
-  if (tid < 64) s.tab[tid] = exp2(tid / 64.0);
+  fill_table(s.tab);
   if (tid == 0) {
+    s.first = 0xffffffffu;
     s.listed = 0;
-    s.lo = 0xffffffffu;
-    s.hi = 0;
   }
-  auto clear = [&] {
-    for (int i = tid; i < kSteps; i += NT) {
-      s.count[i] = 0;
-      s.mass[i] = 0;
-    }
-  };
-  clear();
+  if constexpr (!kWhole) s.count[tid] = 0;
   float mine = -INFINITY;  // the thread's largest
-  row.mine([&](int, const float(&x)[E]) {
-#pragma unroll
-    for (int j = 0; j < E; ++j) mine = fmaxf(mine, x[j]);
-  });
+  if (by_parts) {
+    for (int i = tid; i < a.parts; i += NT) mine = fmaxf(mine, part_max[i]);
+  } else {
+    mine = row.largest();
+  }
   const float wm = wave_all(mine, [](float x, float y) { return fmaxf(x, y); });
   if (lane == 0) s.wave_max[wave] = wm;
   __syncthreads();
-  float m = s.wave_max[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s.wave_max[w]);
+  const float m = wave_all(s.wave_max[lane % kWaves], [](float x, float y) { return fmaxf(x, y); });
   if (m == -INFINITY) {  // nothing to draw
     if (tid == 0) {
       a.token[b] = -1;
@@ -378,333 +551,477 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     }
     return;
   }
-  if (!(t > 0.f) || k == 1) {  // the first of the largest
-    uint32_t first = 0xffffffffu;
-    if (mine == m)
-      row.mine([&](int i, const float(&x)[E]) {
+  if (rules.greedy) {  // the first of the largest
+    if (__ballot(mine == m))
+      row.walk(row.v0, row.v1, [&](int i, const float(&x)[E]) {
 #pragma unroll
-        for (int j = E - 1; j >= 0; --j)
-          if (x[j] == m && static_cast<uint32_t>(i + j) < first) first = i + j;
+        for (int j = 0; j < E; ++j)
+          if (x[j] == m) atomicMin(&s.first, static_cast<uint32_t>(i + j));
       });
-    if (first != 0xffffffffu) atomicMin(&s.lo, first);
     __syncthreads();
     if (tid == 0) {
-      a.token[b] = s.lo;
+      a.token[b] = s.first;
       if (a.logprob) a.logprob[b] = 0.f;
     }
     return;
   }
+  const uint32_t key_m = key_of(m), last = a.V - 1;
+  const int index_bits = bits_of(last);
+  Weights wt;
+  wt.c = 1.4426950408889634 / static_cast<double>(rules.t);
+  wt.unit = ldexp(1.0, 52 - a.q);
+  wt.tab = s.tab;
+  wt.lowest = m;
+  wt.R = 0;
+  const bool peaked = Weights::peaked(m, wt.c);  // the largest weigh the same, all others nothing
+  if (!peaked) wt.set(m, a.q);
+  float floor_l = wt.lowest;  // of what can be drawn
+  if (rules.least > 0.f && !peaked) {
+    const double x = m + log2_of(fmax(static_cast<double>(rules.least), 0x1p-100), s.tab) / wt.c;
+    floor_l = fmaxf(floor_l, -float_under(fmin(-x, 3.4028234663852886e38)));  // (the smallest float that is not below x)
+  }
+  auto part = [&](uint64_t total) -> uint64_t {  // what top-p's run has to reach
+    const double x = ceil(static_cast<double>(rules.p) * static_cast<double>(total));
+    const uint64_t y = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
+    return y < total ? y : total;
+  };
+  auto place = [&](uint64_t total) -> uint64_t {  // of the draw in [0, total)
+    const double of = static_cast<double>(total), x = u > 0.f ? static_cast<double>(u) * of : 0.0;
+    const uint64_t at = x < of ? static_cast<uint64_t>(x) : total;
+    return at < total ? at : total - 1;
+  };
+  // The token and the logarithm of its share: weight and total in one unit, the total
+  // also in units of 2^R.
+  auto done = [&](int i, float l, double weight, double total, double total_r) {
+    a.token[b] = i;
+    if (!a.logprob) return;
+    double log2p = 0.0;
+    if (weight != total)
+      log2p = (peaked ? 0.0 : static_cast<double>(l) * wt.c - wt.R) - log2_of(total_r, s.tab);
+    a.logprob[b] = static_cast<float>(log2p * 0.6931471805599453);
+  };
+  const double per_unit = peaked ? 1.0 : ldexp(1.0, -a.q);
 
-  // The first token, by index, at which the running sum of f(index, logit) passes
-  // at(total): its index goes to done.  Every wave sums a part of the row, then of the
-  // part in which that is, until one wave holds the rest.
-  auto draw_in_row = [&](auto f, auto at_of, auto done) {
+  // -- the list: what the first border is decided on ------------------------------------
+  Cut cut{0, 0xffffffffu};    // all
+  bool listed = kWhole;       // all that the cut keeps are in the list
+  bool first_cut = false, counts = true, from_list = true;
+  int n = 0, border = -1;
+  uint32_t lo = 0;            // keys from here on
+  uint64_t target = k;
+  if constexpr (kWhole) {
+    n = a.V;
+    for (int i = tid; i < n; i += NT) {
+      const float l = row.one(i);
+      s.list[i] = l >= wt.lowest ? static_cast<uint64_t>(key_of(l)) << 32 | static_cast<uint32_t>(i) : 0;
+    }
+    __syncthreads();
+    first_cut = by_k;
+  } else if (!peaked && (by_k || by_p || rules.least > 0.f)) {
+    const bool by_threads = by_k && k <= NT;
+    bool all = true, band = false;  // what the list may be: all from the border's step on, that step alone
+    float from = floor_l, to = INFINITY;
+    int wide = 2;                   // the steps are of 2^wide / 128
+    double before = 0.0;
+    if (by_k) {
+      if (by_threads) {
+        if (mine >= wt.lowest) atomicAdd(&s.count[wt.step(mine)], 1u);
+      } else {
+        row.walk(row.v0, row.v1, [&](int, const float(&x)[E]) {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (x[j] >= wt.lowest) atomicAdd(&s.count[wt.step(x[j])], 1u);
+        });
+      }
+      __syncthreads();
+      crossing<NT>(s, static_cast<uint32_t>(k));
+      border = s.bin;
+      before = static_cast<double>(s.before);
+      if (by_threads && border < 0) border = kSteps - 1;
+      band = !by_threads;
+      all = first_cut = border >= 0;  // (fewer than k weigh anything: k keeps them all)
+    } else if (by_p) {
+      // the parts' sums by steps, over the row's R
+      const int i = tid & (kCoarse - 1);
+      double g = 0.0;
+      for (int p = tid / kCoarse; p < a.parts; p += NT / kCoarse) {
+        const float pm = part_max[p];
+        if (pm == -INFINITY || Weights::peaked(pm, wt.c)) continue;
+        const double under = wt.R - ceil(static_cast<double>(pm) * wt.c);
+        if (!(under < kCoarse)) continue;
+        const int off = 8 * static_cast<int>(under);
+        const unsigned long long* steps = a.part_steps + (b * a.parts + p) * kCoarse;
+        uint64_t w = 0;
+        if (i >= off) w = steps[i - off];
+        if (i == kCoarse - 1)
+          for (int j = off < kCoarse ? kCoarse - off : 0; j < kCoarse; ++j) w += steps[j];
+        g += ldexp(static_cast<double>(w), -static_cast<int>(under));
+      }
+      s.steps[tid / kCoarse][i] = g;
+      if (tid == 0) s.bin = -1;
+      __syncthreads();
+      if (wave == 0) {
+        constexpr int kEach = kCoarse / 64;
+        double x[kEach], sum = 0.0, guess = 0.0, scale = exp2(lane * kEach / 8.0);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const int c = lane * kEach + j;
+          x[j] = s.steps[0][c] + s.steps[1][c] + s.steps[2][c] + s.steps[3][c];
+          sum += x[j];
+        }
+        double run = sum;
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) {
+          const double o = __shfl_up(run, w);
+          if (lane >= w) run += o;
+        }
+        const double total = __shfl(run, 63), goal = fmax(static_cast<double>(rules.p) * total, 1.0);
+        double at = run - sum;
+        // (a token of step c weighs more than 2^(-(c + 1) / 8))
+        guess = sum * scale * 1.4142135623730951 * per_unit;
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) {
+          const double o = __shfl_up(guess, w);
+          if (lane >= w) guess += o;
+        }
+        const bool here = at < goal && run >= goal;
+        const uint64_t lanes = __ballot(here);
+        // (by roundings no lane may reach it: then the last that has anything)
+        const uint64_t any = __ballot(sum > 0.0);
+        const int pick = lanes ? first_of(lanes) : last_of(any);
+        if (lane == pick) {
+          int c = -1;
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) {
+            if (c < 0 && x[j] > 0.0) {
+              if (at + x[j] >= goal)
+                c = j;
+              else
+                at += x[j];
+            }
+          }
+          if (c < 0) {  // roundings again: the last of the lane's
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+              if (x[j] > 0.0) c = j;
+            at -= x[0] * (c == 0) + x[1] * (c == 1) + x[2] * (c == 2) + x[3] * (c == 3);
+          }
+          s.bin = lane * kEach + c;
+          s.above = at;
+          s.total = goal;
+          s.guess = guess;
+        }
+      }
+      __syncthreads();
+      border = s.bin;
+      before = s.above;
+      wide = 4;
+      counts = false;
+      first_cut = true;
+      band = true;
+      all = s.guess < kList;
+      target = static_cast<uint64_t>(ceil(s.total));
+    }
+    if (border >= 0) {
+      // logits of the steps up to the border's, and of the border's, with a little room
+      // for roundings
+      const double low = 1 << wide, first_n = low * border;  // n of its first, under 128 R
+      const bool lowest_step = border == (wide == 2 ? kSteps : kCoarse) - 1;
+      from = lowest_step ? wt.lowest : float_under((wt.R - (first_n + low) / 128.0) / wt.c);
+      to = -float_under(-(wt.R - (first_n - 1.0) / 128.0) / wt.c);
+    }
+    // gathers the tokens from `from` on (first all, then the border's step alone)
+    from_list = false;
+#pragma unroll 1
+    for (int attempt = all ? 0 : 1; attempt < (band ? 2 : 1) && !from_list && (all || band); ++attempt) {
+      const bool alone = attempt == 1;
+      const float most = alone ? to : INFINITY;
+      __syncthreads();
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+      row.walk(row.v0, row.v1, [&](int i, const float(&x)[E]) {
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) top = fmaxf(top, x[j]);
+        if (!__ballot(top >= from)) return;
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) in |= static_cast<uint32_t>(x[j] >= from && x[j] <= most) << j;
+#pragma unroll 1
+        while (__ballot(in != 0)) {  // a token of every lane that has one
+          const int j = __ffs(in) - 1;
+          float l = x[0];
+#pragma unroll
+          for (int c = 1; c < E; ++c) l = j == c ? x[c] : l;
+          bool take = in != 0;
+          if (alone && take) {
+            const int step = wide == 2 ? wt.step(l) : wt.step(l) >> 2;
+            take = l >= wt.lowest && step == border;
+          }
+          const uint64_t mask = __ballot(take);
+          in &= in - 1;
+          if (mask == 0) continue;
+          uint32_t at = 0;
+          if (lane == 0) at = atomicAdd(&s.listed, static_cast<uint32_t>(__popcll(mask)));
+          at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((1ull << lane) - 1));
+          if (take && at < kList) s.list[at] = static_cast<uint64_t>(key_of(l)) << 32 | static_cast<uint32_t>(i + j);
+        }
+      });
+      __syncthreads();
+      n = static_cast<int>(s.listed);
+      if (n <= kList) {
+        from_list = true;
+        listed = !alone;
+        if (alone) {
+          const double x = ceil(target - before);
+          target = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
+        }
+        lo = first_cut && !alone ? key_of(from) : 0;
+      }
+    }
+  }
+
+  // f(key, index) of the list's tokens, or the row's, of the cut, from lo on
+  auto each = [&](bool in_list, auto f) {
+    if (kWhole || in_list) {
+#pragma unroll 1
+      for (int i = tid; i < n; i += NT) {
+        const uint64_t x = s.list[i];
+        const uint32_t ky = static_cast<uint32_t>(x >> 32), at = static_cast<uint32_t>(x);
+        if (ky != 0 && ky >= lo && cut.keeps(ky, at)) f(ky, at);
+      }
+    } else if constexpr (!kWhole) {
+      row.walk(row.v0, row.v1, [&](int i, const float(&x)[E]) {
+#pragma unroll 1
+        for (int j = 0; j < E; ++j) {
+          float l = x[0];
+#pragma unroll
+          for (int c = 1; c < E; ++c) l = j == c ? x[c] : l;
+          const uint32_t ky = key_of(l), at = static_cast<uint32_t>(i + j);
+          if (l >= wt.lowest && ky >= lo && cut.keeps(ky, at)) f(ky, at);
+        }
+      });
+    }
+  };
+  // Three selects, each on what the one before left: top-k's or top-p's border, top-p's
+  // behind top-k's, the draw (of a list; a row's has walks of its own below).
+#pragma unroll 1
+  for (int stage = 0; stage < 3; ++stage) {
+    const bool draw = stage == 2;
+    bool ones = peaked, in_list = listed;
+    if (stage == 0) {
+      if (!first_cut) continue;
+      ones |= counts;
+      in_list = from_list;
+    } else if (stage == 1 ? !by_p || by_parts || (peaked && !kWhole) : !listed) {
+      continue;
+    }
+    const float floor = draw ? floor_l : wt.lowest;
+    auto mass = [&](uint32_t ky) -> uint64_t {
+      const float l = of_key(ky);
+      if (ones) return l >= floor;
+      return wt.of(l, floor);
+    };
+    if (stage > 0) lo = cut.key > lo ? cut.key : lo;
+    uint64_t total = 0;
+    each(in_list, [&](uint32_t ky, uint32_t) { total += mass(ky); });
+    total = block_sum<NT>(s, total);
+    if (stage == 0) {
+      if (counts && target >= total) continue;   // k keeps them all
+      target = target < total ? target : total;  // (a border's step, by roundings)
+    } else {
+      target = draw ? place(total) + 1 : part(total);
+    }
+    const int bits = draw ? index_bits : bits_of(key_m - lo) + index_bits;
+    const uint64_t r = select<NT>(s, bits, target, in_list ? n : a.V, [&](auto g) {
+      each(in_list, [&](uint32_t ky, uint32_t i) {
+        const uint64_t w = mass(ky);
+        if (w) g(static_cast<uint64_t>(draw ? 0 : ky - lo) << index_bits | (last - i), w);
+      });
+    });
+    const uint32_t at = last - (static_cast<uint32_t>(r) & ((1u << index_bits) - 1));
+    if (!draw) {
+      cut = Cut{lo + static_cast<uint32_t>(r >> index_bits), at};
+    } else if (tid == 0) {
+      const float l = row.one(at);
+      done(at, l, static_cast<double>(peaked ? 1 : wt.whole(l)), static_cast<double>(total),
+           static_cast<double>(total) * per_unit);
+    }
+  }
+  if constexpr (!kWhole) {
+    if (listed) return;
+    const float key_l = cut.key ? of_key(cut.key) : -INFINITY;
+    const uint32_t to = cut.index;
     int v0 = 0, v1 = row.n;
-    uint64_t total = 0, at = 0;
-    for (bool first = true; first || v1 - v0 > 64; first = false) {
+    uint64_t at = 0;
+    double total = 0.0, total_r = 0.0;
+    bool need_total = true;
+    if (by_parts && !peaked && (by_p ? from_list && floor_l <= key_l : rules.least == 0.f)) {
+      // The parts' sums of what is kept: of top-p the steps before the border's, and of
+      // its step what the cut keeps.
+      __syncthreads();
+      constexpr int kVectors = kPart / E;
+      auto r_of = [&](float pm) { return static_cast<int>(ceil(static_cast<double>(pm) * wt.c)); };
+      for (int p = wave; p < a.parts; p += kWaves) {
+        const float pm = part_max[p];
+        uint64_t sum = 0;
+        if (pm != -INFINITY && !Weights::peaked(pm, wt.c)) {
+          if (!by_p) {
+            sum = a.part_sum[b * a.parts + p];
+          } else {
+            const double under = wt.R - static_cast<double>(r_of(pm));
+            const int end = under < kCoarse ? border - 8 * static_cast<int>(under) : 0;
+            for (int i = lane; i < end; i += 64) sum += a.part_steps[(b * a.parts + p) * kCoarse + i];
+            sum = wave_sum(sum);
+          }
+        }
+        if (lane == 0) s.kept[p] = sum;
+      }
+      __syncthreads();
+      if (by_p) {
+        for (int i = tid; i < n; i += NT) {
+          const uint64_t x = s.list[i];
+          const uint32_t ky = static_cast<uint32_t>(x >> 32), index = static_cast<uint32_t>(x);
+          if (!cut.keeps(ky, index)) continue;
+          const int p = (static_cast<int>(index) + row.off) / E / kVectors;
+          Weights w = wt;
+          w.set(part_max[p], a.q);
+          atomicAdd(&s.kept[p], static_cast<unsigned long long>(w.of(of_key(ky), w.lowest)));
+        }
+        __syncthreads();
+      }
+      if (wave == 0) {
+        auto kept_of = [&](int p, int& under) -> double {  // in the row's units
+          under = 0;
+          if (p >= a.parts || s.kept[p] == 0) return 0.0;
+          under = wt.R - r_of(part_max[p]);
+          return ldexp(static_cast<double>(s.kept[p]), -under);
+        };
+        auto scan = [&](double v) {
+#pragma unroll
+          for (int w = 1; w < 64; w <<= 1) {
+            const double o = __shfl_up(v, w);
+            if (lane >= w) v += o;
+          }
+          return v;
+        };
+        int under;
+        double sum = 0.0;
+        for (int p0 = 0; p0 < a.parts; p0 += 64) sum += __shfl(scan(kept_of(p0 + lane, under)), 63);
+        const double x = u > 0.f ? fmin(static_cast<double>(u), 0.9999999999999999) * sum : 0.0;
+        double run = 0.0;
+        for (int p0 = 0; p0 < a.parts; p0 += 64) {
+          const double v = kept_of(p0 + lane, under), to_here = run + scan(v);
+          // (the last with anything, should roundings leave none that reaches it)
+          const uint64_t over = __ballot(v > 0.0 && to_here > x), any = __ballot(v > 0.0);
+          const int pick = over ? first_of(over) : any ? last_of(any) : -1;
+          if (lane == pick) {
+            const double in = ldexp(x - (to_here - v), under);
+            const uint64_t most = s.kept[p0 + lane];
+            s.part = p0 + lane;
+            s.at = in > 0.0 ? (in < static_cast<double>(most) ? static_cast<uint64_t>(in) : most - 1) : 0;
+            if (s.at >= most) s.at = most - 1;
+          }
+          if (over) break;
+          run = __shfl(to_here, 63);
+        }
+        if (lane == 0) s.total = sum;
+      }
+      __syncthreads();
+      at = s.at;
+      total = s.total;
+      total_r = total * per_unit;
+      v0 = s.part * kVectors;
+      v1 = v0 + kVectors < row.n ? v0 + kVectors : row.n;
+      need_total = false;
+    }
+    // The draw: every wave sums what its part of the row keeps, then of the part in
+    // which the draw lies, until one step of a wave holds the rest.
+    Weights w = wt;  // in the units of the row, or of its part
+    if (!need_total) w.set(part_max[s.part], a.q);
+    const float low = fmaxf(fmaxf(floor_l, key_l), w.lowest);
+    auto weight = [&](float l, int i) -> uint64_t {
+      uint64_t x = w.whole(l);
+      if (peaked) x = 1;
+      return l >= low && (l != key_l || static_cast<uint32_t>(i) <= to) ? x : 0;
+    };
+#pragma unroll 1
+    while (need_total || v1 - v0 > 64) {
       const int per = (v1 - v0 + kWaves - 1) / kWaves;
       const int w0 = v0 + wave * per, w1 = w0 + per < v1 ? w0 + per : v1;
       uint64_t sum = 0;
       row.walk(w0, w1, [&](int i, const float(&x)[E]) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) sum += f(i + j, x[j]);
+        for (int j = 0; j < E; ++j) sum += weight(x[j], i + j);
       });
-      sum = wave_sum(sum);
-      __syncthreads();
-      if (lane == 0) s.wave_m[wave] = sum;
-      __syncthreads();
-      if (first) {
-        for (int w = 0; w < kWaves; ++w) total += s.wave_m[w];
-        at = at_of(total);
+      const uint64_t sums = of_waves<NT>(s, wave_sum(sum)), run = wave_scan(sums);
+      if (need_total) {
+        uint64_t kept = last_lane(run);
+        if (peaked) {  // (top-k and top-p count, and the first ones by index are kept)
+          if (by_k && k < static_cast<int64_t>(kept)) kept = k;
+          if (by_p) kept = part(kept);
+        }
+        at = place(kept);
+        total = static_cast<double>(kept);
+        total_r = total * per_unit;
+        need_total = false;
       }
-      int w = 0;
-      while (w < kWaves - 1 && at >= s.wave_m[w]) at -= s.wave_m[w++];
-      v0 += w * per;
+      const int pick = first_of(__ballot(run > at) | 1ull << 63) & (kWaves - 1);  // (there is one)
+      const uint64_t to_here = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(run >> 32), pick)) << 32 |
+                               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(run), pick));
+      const uint64_t here = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(sums >> 32), pick)) << 32 |
+                            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(sums), pick));
+      at -= to_here - here;
+      v0 += pick * per;
       v1 = v0 + per < v1 ? v0 + per : v1;
     }
     if (wave != 0) return;
     float x[E];
-    uint64_t w[E], sum = 0;
-    const int v = v0 + lane;
-    if (v < v1) row.get(v, x);
+    uint64_t wx[E], sum = 0;
+    R::wide(row.raw(v0, v1), x);
+    const int i = (v0 + lane) * E - row.off;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      w[j] = v < v1 ? f(v * E - row.off + j, x[j]) : 0;
-      sum += w[j];
+      wx[j] = weight(x[j], i + j);
+      sum += wx[j];
     }
     uint64_t run = wave_scan(sum) - sum;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      if (run <= at && at < run + w[j]) done(v * E - row.off + j, x[j], total);
-      run += w[j];
-    }
-  };
-  auto share = [&](uint64_t total, double of) -> uint64_t {  // the place of a draw in [0, total)
-    const double x = u > 0.f ? static_cast<double>(u) * of : 0.0;
-    const uint64_t at = x < of ? static_cast<uint64_t>(x) : total;
-    return at < total ? at : total - 1;
-  };
-  auto part = [&](uint64_t total) -> uint64_t {  // what top-p's run has to reach
-    const double x = ceil(static_cast<double>(p) * static_cast<double>(total));
-    const uint64_t y = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
-    return y < total ? y : total;
-  };
-  const bool by_k = k > 0 && k < a.V, by_p = p < 1.f;
-
-  if (m == INFINITY) {  // its tokens weigh the same, all others nothing
-    uint64_t kept = 0;
-    draw_in_row([&](int, float l) -> uint64_t { return l == INFINITY; },
-                [&](uint64_t total) {
-                  kept = by_k && k < static_cast<int64_t>(total) ? k : total;
-                  if (by_p) kept = part(kept);
-                  return share(kept, static_cast<double>(kept));
-                },
-                [&](int i, float, uint64_t) {
-                  a.token[b] = i;
-                  if (a.logprob) a.logprob[b] = static_cast<float>(-log(static_cast<double>(kept)));
-                });
-    return;
-  }
-
-  Weights wt;
-  wt.c = 1.4426950408889634 / static_cast<double>(t);
-  wt.M = m;
-  wt.q = a.q;
-  wt.lowest = -(a.q + 1.0);
-  wt.unit = ldexp(1.0, 52 - a.q);
-  wt.tab = s.tab;
-  double floor_y = wt.lowest;  // of what can be drawn
-  if (least > 0.f) floor_y = fmax(floor_y, log2(static_cast<double>(least)));
-  const uint32_t key_m = key_of(m);
-
-  auto at_of = [&](uint64_t total) { return share(total, static_cast<double>(total)); };
-  auto done = [&](int index, float l, uint64_t total) {
-    a.token[b] = index;
-    if (a.logprob)
-      a.logprob[b] = static_cast<float>(wt.log2w(l) * 0.6931471805599453 -
-                                        log(ldexp(static_cast<double>(total), -wt.q)));
-  };
-
-  // -- the list ----------------------------------------------------------------------
-  Cut cut{0, 0xffffffffu};  // all
-  uint32_t key[kEach], index[kEach];
-  int n = 0;                // tokens of the list, kEach threads apart
-  auto each_listed = [&](auto f) {  // f(key, index, e)
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (tid + e * NT < n) f(key[e], index[e]);
-  };
-  auto each_in_row = [&](auto f) {
-    row.mine([&](int i, const float(&x)[E]) {
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (wt.log2w(x[j]) >= wt.lowest) f(key_of(x[j]), static_cast<uint32_t>(i + j));
-    });
-  };
-  // the cut at which the running count or mass of the tokens of the present cut with
-  // keys in [lo, hi] reaches target
-  auto narrow = [&](auto by_mass, auto each, uint32_t lo, uint32_t hi, uint64_t target) {
-    constexpr bool BM = decltype(by_mass)::value;
-    const Found f = select<NT, BM>(s, bits_of(hi - lo), target, [&](auto g) {
-      each([&](uint32_t ky, uint32_t i) {
-        if (ky >= lo && ky <= hi && cut.keeps(ky, i)) g(ky - lo, BM ? wt.of(of_key(ky), wt.lowest) : 0);
-      });
-    });
-    const uint32_t border = lo + f.rank;
-    // equal ones: as many as it takes
-    uint64_t take = target - f.before;
-    if constexpr (BM) {
-      const uint64_t one = f.in_m / f.in_n;
-      take = (take + one - 1) / one;
-    }
-    uint32_t to = cut.key == border ? cut.index : 0xffffffffu;
-    if (take < f.in_n) {
-      const uint32_t last = a.V - 1;
-      const Found g = select<NT, false>(s, bits_of(last), take, [&](auto h) {
-        each([&](uint32_t ky, uint32_t i) {
-          if (ky == border && cut.keeps(ky, i)) h(last - i, 0);
-        });
-      });
-      to = last - g.rank;
-    }
-    cut = Cut{border, to};
-  };
-  // the row's tokens that `wanted` names become the list; whether it holds them
-  auto collect = [&](auto wanted) -> bool {
-    row.mine([&](int i, const float(&x)[E]) {
-      bool any = false;
-#pragma unroll
-      for (int j = 0; j < E; ++j) any |= wanted(x[j]);
-      if (!any) return;
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (wanted(x[j])) {
-          const uint32_t at = atomicAdd(&s.listed, 1u);
-          if (at < kList) s.list[at] = static_cast<uint64_t>(key_of(x[j])) << 32 | static_cast<uint32_t>(i + j);
-        }
-    });
-    __syncthreads();
-    n = static_cast<int>(s.listed);
-    const bool fits = n <= kList;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (fits && tid + e * NT < n) {
-        const uint64_t x = s.list[tid + e * NT];
-        key[e] = static_cast<uint32_t>(x >> 32);
-        index[e] = static_cast<uint32_t>(x);
-      }
-    __syncthreads();
-    if (tid == 0) s.listed = 0;
-    __syncthreads();
-    if (!fits) n = 0;
-    return fits;
-  };
-  auto under = [&](double steps) { return float_under(static_cast<double>(m) - steps / (64.0 * wt.c)); };
-
-  bool listed = kWhole;  // all that the cut keeps is in the list
-  if constexpr (kWhole) {
-    n = a.V;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (tid + e * NT < n) {
-        key[e] = key_of(row.one(tid + e * NT));
-        index[e] = tid + e * NT;
-        if (!(wt.log2w(of_key(key[e])) >= wt.lowest)) key[e] = 0;
-      }
-    if (by_k) {
-      uint64_t weigh = 0;
-      each_listed([&](uint32_t ky, uint32_t) { weigh += ky != 0; });
-      weigh = block_sum<NT>(s, weigh);
-      if (k < static_cast<int64_t>(weigh)) narrow(std::false_type{}, each_listed, 1, key_m, k);
-    }
-  } else if (by_k || by_p) {
-    const bool sums = by_p && !by_k;
-    // Top-k of up to NT: where the threads' largest tokens count k, so many lie above.
-    const bool by_threads = by_k && k <= NT;
-    auto count = [&](float l) {
-      const double y = wt.log2w(l);
-      if (y >= wt.lowest) atomicAdd(&s.count[wt.step(y)], 1u);
-    };
-    if (by_threads)
-      count(mine);
-    else
-      row.mine([&](int, const float(&x)[E]) {
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          if (sums) {
-            const double y = wt.log2w(x[j]);
-            const uint64_t w = wt.whole(y);
-            if (y >= wt.lowest) atomicAdd(&s.mass[wt.step(y)], static_cast<unsigned long long>(w));
-          } else {
-            count(x[j]);
-          }
-        }
-      });
-    __syncthreads();
-    uint64_t target = k;
-    if (sums)
-      crossing<NT, true>(s, [&](uint64_t total) { return target = part(total); });
-    else
-      crossing<NT, false>(s, [&](uint64_t) { return target; });
-    int border = s.bin;
-    if (by_threads && border < 0) border = kSteps - 1;
-    if (border >= 0) {  // (fewer than k weigh anything: k keeps them all)
-      // (half a step more than the border's, for roundings)
-      const float from = border == kSteps - 1 ? under(64.0 * (a.q + 2)) : under(border + 1.0);
-      const uint64_t before = s.before_m;
-      listed = collect([&](float l) { return l >= from; });
-      if (listed) {
-        uint64_t weigh = 0;
-        each_listed([&](uint32_t ky, uint32_t) { weigh += wt.log2w(of_key(ky)) >= wt.lowest; });
-        if (sums) {
-          narrow(std::true_type{}, each_listed, key_of(from), key_m, target);
-        } else {
-          weigh = block_sum<NT>(s, weigh);
-          if (k < static_cast<int64_t>(weigh)) narrow(std::false_type{}, each_listed, key_of(from), key_m, target);
-        }
-      } else if (!by_threads &&
-                 collect([&](float l) {
-                   if (!(l >= from)) return false;
-                   const double y = wt.log2w(l);
-                   return y >= wt.lowest && wt.step(y) == border;
-                 })) {
-        // the border's step alone
-        uint32_t lo = 0xffffffffu, hi = 0;
-        each_listed([&](uint32_t ky, uint32_t) {
-          lo = ky < lo ? ky : lo;
-          hi = ky > hi ? ky : hi;
-        });
-        lo = wave_all(lo, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
-        hi = wave_all(hi, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-        if (lane == 0) {
-          atomicMin(&s.lo, lo);
-          atomicMax(&s.hi, hi);
-        }
-        __syncthreads();
-        lo = s.lo;
-        hi = s.hi;
-        if (sums)
-          narrow(std::true_type{}, each_listed, lo, hi, target - before);
-        else
-          narrow(std::false_type{}, each_listed, lo, hi, target - before);
-      } else {
-        uint64_t weigh = 0;
-        each_in_row([&](uint32_t, uint32_t) { ++weigh; });
-        weigh = block_sum<NT>(s, weigh);
-        if (sums)
-          narrow(std::true_type{}, each_in_row, 0, key_m, target);
-        else if (k < static_cast<int64_t>(weigh))
-          narrow(std::false_type{}, each_in_row, 0, key_m, target);
-      }
+      if (run <= at && at < run + wx[j])
+        done(i + j, x[j], ldexp(static_cast<double>(wx[j]), w.R - wt.R), total, total_r);
+      run += wx[j];
     }
   }
+}
 
-  // top-p of what top-k left, or of a row that is its own list
-  if (by_p && (by_k || kWhole)) {
-    uint64_t all = 0;
-    auto add = [&](uint32_t ky, uint32_t i) {
-      if (cut.keeps(ky, i)) all += wt.of(of_key(ky), wt.lowest);
-    };
-    if (listed) {
-      each_listed(add);
-      all = block_sum<NT>(s, all);
-      narrow(std::true_type{}, each_listed, cut.key, key_m, part(all));
-    } else if constexpr (!kWhole) {
-      each_in_row(add);
-      all = block_sum<NT>(s, all);
-      narrow(std::true_type{}, each_in_row, cut.key, key_m, part(all));
-    }
-  }
-
-  // -- the draw ----------------------------------------------------------------------
-  if (listed) {
-    uint64_t w[kEach], total = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      w[e] = 0;
-      if (tid + e * NT < n && cut.keeps(key[e], index[e])) w[e] = wt.of(of_key(key[e]), floor_y);
-      total += w[e];
-    }
-    total = block_sum<NT>(s, total);
-    const uint32_t last = a.V - 1;
-    const Found f = select<NT, true>(s, bits_of(last), at_of(total) + 1, [&](auto g) {
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (w[e]) g(last - index[e], w[e]);
-    });
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (w[e] && index[e] == last - f.rank) done(index[e], of_key(key[e]), total);
-  } else if constexpr (!kWhole) {
-    if (cut.key == 0) {
-      draw_in_row([&](int, float l) { return wt.of(l, floor_y); }, at_of, done);
-    } else {
-      const float border = of_key(cut.key);
-      const int to = cut.index > 0x7fffffffu ? 0x7fffffff : static_cast<int>(cut.index);
-      draw_in_row([&](int i, float l) { return l > border || (l == border && i <= to) ? wt.of(l, floor_y) : 0; }, at_of,
-                  done);
-    }
-  }
+// Parts of a row (0: it is its own list): its vectors are one more where it begins
+// inside of one.
+int64_t parts_of(const srw_sample_t& d) {
+  if (d.V <= kList) return 0;
+  const int64_t size = d.dtype == SRW_F32 ? 4 : 2, E = 16 / size;
+  const bool whole = (reinterpret_cast<uintptr_t>(d.logits) | (d.B > 1 ? d.row_stride * size : 0)) % 16 == 0;
+  return ((d.V + E - 1) / E + (whole ? 0 : 1) + kPart / E - 1) / (kPart / E);
+}
+// Whether a row may ask for its parts' sums.
+bool by_parts(const srw_sample_t& d) {
+  if (d.V <= kList) return false;
+  if (!d.temperature && !(d.temperature_all > 0.f)) return false;
+  const bool by_p = d.top_p || d.top_p_all < 1.f, whole = d.min_p || d.min_p_all == 0.f;
+  return (d.top_k || d.top_k_all == 0 || d.top_k_all >= d.V) && (by_p || whole);
+}
+struct Workspace {
+  size_t max, sum, steps, bytes;  // offsets, and the whole
+};
+Workspace workspace_of(const srw_sample_t& d) {
+  Workspace w{};
+  if (!by_parts(d)) return w;
+  const size_t n = static_cast<size_t>(d.B) * parts_of(d);
+  const bool by_p = d.top_p || d.top_p_all < 1.f;
+  w.sum = (n * 4 + 255) & ~size_t{255};
+  w.steps = (w.sum + n * 8 + 255) & ~size_t{255};
+  w.bytes = w.steps + (by_p ? n * kCoarse * 8 : 0);
+  return w;
 }
 
 srw_status_t check_sample(const srw_sample_t* d) {
@@ -712,6 +1029,7 @@ srw_status_t check_sample(const srw_sample_t* d) {
   if (d->B < 0 || d->V < 1 || (d->dtype != SRW_F32 && d->dtype != SRW_BF16)) return SRW_EINVAL;
   if (d->B > (1 << 21) || d->V > (1 << 24)) return SRW_EUNSUPPORTED;  // (a launch has under 2^32 threads)
   if (d->B == 0) return SRW_OK;
+  if (d->B * parts_of(*d) >= (1 << 24)) return SRW_EUNSUPPORTED;
   auto array = [](const void* p, size_t size, bool needed) {
     return p ? reinterpret_cast<uintptr_t>(p) % size == 0 : !needed;
   };
@@ -730,16 +1048,30 @@ srw_status_t check_sample(const srw_sample_t* d) {
 }  // namespace
 }  // namespace srw
 
-extern "C" srw_status_t srw_sample(const srw_sample_t* d, void* stream) {
+extern "C" {
+
+srw_status_t srw_sample_workspace_size(const srw_sample_t* d, size_t* bytes) {
+  const srw_status_t st = srw::check_sample(d);
+  if (st != SRW_OK) return st;
+  if (!bytes) return SRW_EINVAL;
+  *bytes = d->B == 0 ? 0 : srw::workspace_of(*d).bytes;
+  return SRW_OK;
+}
+
+srw_status_t srw_sample(const srw_sample_t* d, void* workspace, size_t workspace_bytes, void* stream) {
   const srw_status_t st = srw::check_sample(d);
   if (st != SRW_OK || d->B == 0) return st;
+  const srw::Workspace w = srw::workspace_of(*d);
+  if (w.bytes > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < w.bytes))
+    return SRW_EWORKSPACE;
   srw::SampleArgs a{};
   a.logits = static_cast<const char*>(d->logits);
-  a.stride = d->row_stride;
+  a.stride = d->B > 1 ? d->row_stride : 0;
   a.V = static_cast<int32_t>(d->V);
   int bits = 0;  // V <= 2^bits
   while ((int64_t{1} << bits) < d->V) ++bits;
   a.q = 62 - bits < 51 ? 62 - bits : 51;
+  a.parts = static_cast<int32_t>(srw::parts_of(*d));
   a.u = d->u;
   a.temperature = d->temperature;
   a.top_p = d->top_p;
@@ -751,18 +1083,26 @@ extern "C" srw_status_t srw_sample(const srw_sample_t* d, void* stream) {
   a.top_k_all = d->top_k_all;
   a.token = d->token;
   a.logprob = d->logprob;
+  char* ws = static_cast<char*>(workspace);
+  a.part_max = reinterpret_cast<float*>(ws + w.max);
+  a.part_sum = reinterpret_cast<unsigned long long*>(ws + w.sum);
+  a.part_steps = reinterpret_cast<unsigned long long*>(ws + w.steps);
   (void)hipGetLastError();
-  const dim3 grid(static_cast<unsigned>(d->B));
+  const dim3 grid(static_cast<unsigned>(d->B)), parts(static_cast<unsigned>(d->B * a.parts));
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (d->V <= srw::kList) {
-    if (d->dtype == SRW_F32)
-      hipLaunchKernelGGL((srw::sample_kernel<float, 256>), grid, dim3(256), 0, s, a);
+  auto launch = [&](auto logit) {
+    using T = decltype(logit);
+    if (w.bytes > 0) hipLaunchKernelGGL((srw::sample_parts_kernel<T>), parts, dim3(256), 0, s, a);
+    if (d->V <= srw::kList)
+      hipLaunchKernelGGL((srw::sample_kernel<T, 256>), grid, dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((srw::sample_kernel<uint16_t, 256>), grid, dim3(256), 0, s, a);
-  } else if (d->dtype == SRW_F32) {
-    hipLaunchKernelGGL((srw::sample_kernel<float, 1024>), grid, dim3(1024), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((srw::sample_kernel<uint16_t, 1024>), grid, dim3(1024), 0, s, a);
-  }
+      hipLaunchKernelGGL((srw::sample_kernel<T, 1024>), grid, dim3(1024), 0, s, a);
+  };
+  if (d->dtype == SRW_F32)
+    launch(float{});
+  else
+    launch(uint16_t{});
   return hipGetLastError() == hipSuccess ? SRW_OK : SRW_EHIP;
 }
+
+}  // extern "C"

@@ -5,6 +5,7 @@ graph."""
 
 from __future__ import annotations
 
+import ctypes
 import struct
 
 import torch
@@ -80,5 +81,12 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     logprob = torch.empty(B, dtype=F32, device=dev)
     d = _SAMPLE.pack(logits.data_ptr(), logits.stride(0), B, V, u, *(a for a, _ in given), token.data_ptr(),
                      logprob.data_ptr(), *(x for _, x in given), _DTYPES[logits.dtype], 0)
-    C.check(_call(C.load_library().srw_sample, dev, d))
+    lib = C.load_library()
+    status = _call(lib.srw_sample, dev, d, None, 0)
+    if status == C.SRW_EWORKSPACE:  # sums of the rows' parts, nothing launched yet
+        need = ctypes.c_size_t(0)
+        C.check(lib.srw_sample_workspace_size(d, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        status = _call(lib.srw_sample, dev, d, ws.data_ptr(), need.value)
+    C.check(status)
     return token, logprob

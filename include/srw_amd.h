@@ -599,7 +599,8 @@ typedef struct srw_sample {
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all, dtype, reserved;
 } srw_sample_t;
-srw_status_t srw_sample(const srw_sample_t* s, void* stream);
+srw_status_t srw_sample_workspace_size(const srw_sample_t* s, size_t* bytes);
+srw_status_t srw_sample(const srw_sample_t* s, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Name of the kernel family the last srw_forward on this thread used
  * ("generic", "mfma_bf16", "mfma_ss_bf16", ...), for tests and benchmarks. */
