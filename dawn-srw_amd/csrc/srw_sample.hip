@@ -20,8 +20,8 @@
 // * Top-k of up to 1 024: the threads' largest logits are counted by steps of
 //   2^(1/32); where k of them lie above, so many tokens do.
 // * Top-p, and rows without either: sample_parts_kernel has summed each part of 8 192
-//   logits, for top-p by steps of 2^(1/8), over its own R (sums of parts meet in
-//   float64, 2^-52 of them).  Of top-p rows that keep more than kList the tokens of the
+//   logits, for top-p by steps of 2^(1/16), over its own R (a part's sums are shifted to
+//   the row's R where they meet).  Of top-p rows that keep more than kList the tokens of the
 //   border's step alone become the list; the draw finds its part by the parts' sums and
 //   walks that one.
 //
@@ -39,8 +39,9 @@ namespace srw {
 namespace {
 
 constexpr int kSteps = 1024;   // of 2^(1/32) under 2^R
-constexpr int kCoarse = 256;   // of 2^(1/8), what parts are summed by
+constexpr int kCoarse = 512;   // of 2^(1/16), what parts are summed by
 constexpr int kList = 4096;    // tokens of a list
+constexpr int kFew = 128;      // tokens that are compared each with each
 constexpr int kPart = 8192;    // logits of a part
 constexpr int kDigit = 9, kBins = 1 << kDigit;  // bits of a select's pass
 constexpr int kMostParts = (1 << 24) / kPart + 2;
@@ -103,7 +104,7 @@ __device__ __forceinline__ void fill_table(double* tab) {
 // What the weights of a row, or of a part, go by.  The same roundings wherever a weight
 // is worked out (no contraction): sums of some tokens and of all agree to the last unit.
 struct Weights {
-  double c, unit;     // log2 e / t, 2^(52 - q)
+  double c, per, unit;  // log2 e / t, and its inverse; 2^(52 - q)
   const double* tab;  // 2^(j / 128)
   int R;
   float lowest;       // smaller logits weigh nothing; above -infinity
@@ -113,9 +114,15 @@ struct Weights {
   __device__ __forceinline__ static bool peaked(float m, double c) {
     return !(fabs(static_cast<double>(m) * c) < 1073741824.0);
   }
+  __device__ __forceinline__ void begin(float t, int q, const double* table) {
+    c = 1.4426950408889634 / static_cast<double>(t);
+    per = fmin(static_cast<double>(t) * 0.6931471805599453, 1e300);
+    unit = ldexp(1.0, 52 - q);
+    tab = table;
+  }
   __device__ __forceinline__ void set(float m, int q) {
     R = static_cast<int>(ceil(static_cast<double>(m) * c));
-    lowest = static_cast<float>(fmax((R - q - 1.0) / c, -3.4028234663852886e38));
+    lowest = static_cast<float>(fmax((R - q - 1.0) * per, -3.4028234663852886e38));
   }
   // 128 y to the nearest, in the low bits of a sum
   static constexpr double kMagic = 0x1.8p45;
@@ -169,37 +176,34 @@ __device__ __forceinline__ double log2_of(double x, const double* tab) {
 // A row: vectors of 16 bytes, the first and the last of them partly outside of it.
 template <typename T, int NT> struct Row {
   static constexpr int E = 16 / sizeof(T);  // logits of a vector
-  static constexpr int kWaves = NT / 64;
+  static constexpr int kWaves = NT / 64, kAhead = 8;
   const T* p;
   int V, off, n;  // the row begins off logits behind a 16-byte border; its vectors
-  int v0, v1;     // the wave's
   __device__ __forceinline__ Row(const SampleArgs& a, int64_t b) {
     p = reinterpret_cast<const T*>(a.logits) + b * a.stride;
     V = a.V;
     off = static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
     n = (off + V + E - 1) / E;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = part();
-    v0 = wave * per < n ? wave * per : n;
-    v1 = v0 + per < n ? v0 + per : n;
   }
-  __device__ __forceinline__ int part() const { return (n + kWaves - 1) / kWaves; }
   __device__ __forceinline__ float one(int i) const {
     if constexpr (E == 4)
       return p[i];
     else
       return __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
   }
+  __device__ __forceinline__ const u32x4_t* at(int v) const { return reinterpret_cast<const u32x4_t*>(p + (v * E - off)); }
+  __device__ __forceinline__ static u32x4_t nothing() {
+    constexpr uint32_t nan = E == 4 ? 0x7fc00000u : 0x7fc07fc0u;
+    return u32x4_t{nan, nan, nan, nan};
+  }
   // Vector v + lane: logits E (v + lane) - off ...; those outside the row, and those of
   // vectors from `end` on, as NaN.
   __device__ __forceinline__ u32x4_t raw(int v, int end) const {
     const int lane = threadIdx.x & 63, i = (v + lane) * E - off;
-    const u32x4_t* at = reinterpret_cast<const u32x4_t*>(p + i);
-    if (v * E >= off && (v + 64) * E - off <= V && v + 64 <= end) return *at;
-    u32x4_t w;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = E == 4 ? 0x7fc00000u : 0x7fc07fc0u;
+    if (v * E >= off && (v + 64) * E - off <= V && v + 64 <= end) return *at(v + lane);
+    u32x4_t w = nothing();
     if (v + lane >= end) return w;
-    if (i >= 0 && i + E <= V) return *at;
+    if (i >= 0 && i + E <= V) return *at(v + lane);
 #pragma unroll
     for (int j = 0; j < E; ++j)
       if (i + j >= 0 && i + j < V) {
@@ -221,38 +225,137 @@ template <typename T, int NT> struct Row {
       }
     }
   }
-  // f(index of the first, logits) of the vectors [from, to), one a lane, by the whole
-  // wave, the next two on their way.
+  // f(index of the first, logits) of the vectors [from, to) (n of two and more), one a
+  // lane: the runs of 64 at from, from + 64 step, ..., those of a wave.  Eight loads are on
+  // their way together (one takes about a microsecond where another XCD's kernel, or none,
+  // has read the row before), and f stands once: a vector comes out of the registers by
+  // its number.  The logits of a first or last vector that is partly outside of the row
+  // come one a lane, with NaN beside each, to the wave that asks for that end.
   template <class F>
-  __device__ __forceinline__ void walk(int from, int to, F f) const {
-    if (from >= to) return;
-    u32x4_t a = raw(from, to), b = raw(from + 64, to);
+  __device__ __forceinline__ void walk(int from, int to, int step, bool head, bool tail, F f) const {
+    const int lane = threadIdx.x & 63;
+    int edge = -1;  // its index
+    if (head && off > 0 && lane < E - off) edge = lane;
+    const int behind = (n - 1) * E - off + lane - 32;
+    if (tail && n * E - off > V && lane >= 32 && behind < V) edge = behind;
+    bool more = __ballot(edge >= 0) != 0;
+    const float x0 = edge >= 0 ? one(edge) : __uint_as_float(0x7fc00000u);
+    from = from < first() ? first() : from;
+    to = to > end() ? end() : to;
 #pragma unroll 1
-    for (; from < to; from += 64) {
-      float x[E];
-      wide(a, x);
-      a = b;
-      if (from + 128 < to) b = raw(from + 128, to);
-      f((from + static_cast<int>(threadIdx.x & 63)) * E - off, x);
+    for (; from < to || more; from += 64 * step * kAhead) {
+      typedef uint32_t held_t __attribute__((ext_vector_type(4 * kAhead)));
+      held_t held = {};
+      if (from < to) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int v = from + 64 * step * k + lane;
+          const u32x4_t w = *at(v < to ? v : to - 1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) held[4 * k + j] = w[j];
+        }
+      }
+#pragma unroll 1
+      for (int k = 0; k < kAhead; ++k) {
+        const int v = from + 64 * step * k;
+        float x[E];
+        int i;
+        if (v < to) {
+          wide(u32x4_t{held[4 * k], held[4 * k + 1], held[4 * k + 2], held[4 * k + 3]}, x);
+          i = (v + lane) * E - off;
+          if (v + 64 > to && v + lane >= to) wide(nothing(), x);
+        } else if (more) {
+          wide(nothing(), x);
+          x[0] = x0;
+          i = edge;
+          more = false;
+        } else {
+          break;
+        }
+        f(i, x);
+      }
     }
   }
-  __device__ __forceinline__ float largest() const {  // of the thread's part
-    constexpr int U = 4;
-    float m = -INFINITY, x[E];
-    int from = v0;
+  // vectors that are in the row as a whole
+  __device__ __forceinline__ int first() const { return off > 0 ? 1 : 0; }
+  __device__ __forceinline__ int end() const { return n * E - off > V ? n - 1 : n; }
+  // A wave's part of [from, to), a run of vectors.
+  template <class F>
+  __device__ __forceinline__ void part(int wave, int from, int to, F f) const {
+    const int per = (to - from + kWaves - 1) / kWaves, v0 = from + wave * per, v1 = v0 + per < to ? v0 + per : to;
+    if (v0 < v1) walk(v0, v1, 1, v0 == 0, v1 == n, f);
+  }
+  // The largest logit of the thread's share of the row.
+  __device__ __forceinline__ float largest() const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float m = -INFINITY;
+    if (threadIdx.x < E) {  // those of a first and last vector that are partly outside
+      const int i = threadIdx.x, j = (n - 1) * E - off + i;
+      if (off > 0 && i < E - off) m = one(i);
+      if (n * E - off > V && j < V) m = fmaxf(m, one(j));
+    }
+    const int last = end();
 #pragma unroll 1
-    for (; from < v1; from += 64 * U) {
-      u32x4_t w[U];
+    for (int from = first() + 64 * wave; from < last; from += 64 * kWaves * kAhead) {
+      u32x4_t w[kAhead];
 #pragma unroll
-      for (int k = 0; k < U; ++k) w[k] = raw(from + 64 * k, v1);
+      for (int k = 0; k < kAhead; ++k) {
+        const int v = from + 64 * kWaves * k + lane;
+        w[k] = *at(v < last ? v : last - 1);
+      }
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
+      for (int k = 0; k < kAhead; ++k) {
+        float x[E];
         wide(w[k], x);
+        float top = x[0];
 #pragma unroll
-        for (int j = 0; j < E; ++j) m = fmaxf(m, x[j]);
+        for (int j = 1; j < E; ++j) top = fmaxf(top, x[j]);
+        // (a token is one thread's alone: top-k counts threads)
+        m = fmaxf(m, from + 64 * kWaves * k + lane < last ? top : -INFINITY);
       }
     }
     return m;
+  }
+  // f(index, logit, lanes) for each logit of a vector of the thread's share that lies in
+  // [from, to] on some lanes.  (Two instructions a logit where none does.)
+  template <class F>
+  __device__ __forceinline__ void between(float from, float to, F f) const {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), last = end();
+    if (wave == 0) {  // of a first and last vector that are partly outside, one a lane
+      int edge = -1;
+      if (off > 0 && lane < E - off) edge = lane;
+      const int behind = (n - 1) * E - off + lane - 32;
+      if (n * E - off > V && lane >= 32 && behind < V) edge = behind;
+      const float x = edge >= 0 ? one(edge) : __uint_as_float(0x7fc00000u);
+      const uint64_t hits = __ballot(x >= from && x <= to);
+      if (hits) f(edge, x, hits);
+    }
+#pragma unroll 1
+    for (int v0 = first() + 64 * wave; v0 < last; v0 += 64 * kWaves * kAhead) {
+      u32x4_t w[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int v = v0 + 64 * kWaves * k + lane;
+        w[k] = __builtin_nontemporal_load(at(v < last ? v : last - 1));
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        float x[E];
+        wide(w[k], x);
+        const int v = v0 + 64 * kWaves * k + lane;
+        const uint64_t in = __ballot(v < last);
+        uint64_t hits[E], any = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          hits[j] = __ballot(__builtin_amdgcn_fmed3f(x[j], from, to) == x[j]) & in;
+          any |= hits[j];
+        }
+        if (any)
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (hits[j]) f(v * E - off + j, x[j], hits[j]);
+      }
+    }
   }
 };
 
@@ -282,6 +385,10 @@ __device__ __forceinline__ uint32_t last_lane(uint32_t v) { return __builtin_amd
 __device__ __forceinline__ uint64_t last_lane(uint64_t v) {
   return static_cast<uint64_t>(last_lane(static_cast<uint32_t>(v >> 32))) << 32 | last_lane(static_cast<uint32_t>(v));
 }
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+  return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane)) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane));
+}
 template <class N>
 __device__ __forceinline__ N wave_sum(N v) {
   return last_lane(wave_scan(v));
@@ -297,19 +404,23 @@ template <int NT> struct Shared {
   double tab[128];
   union {
     unsigned long long list[kList];  // key << 32 | index
-    double steps[4][kCoarse];        // of parts, a quarter of them each
+    unsigned long long steps[kCoarse];  // of the row's parts
   };
+  unsigned long long weight[kList];  // of the list's tokens
   uint32_t count[kSteps];
   unsigned long long mass[kBins + 64];
+  float part_max[NT == 1024 ? kMostParts : 1];
+  float under[NT == 1024 ? kMostParts : 1];  // octaves of a part's R under the row's; 1e9: it weighs nothing
   unsigned long long kept[NT == 1024 ? kMostParts : 1];  // of each part, in its units
-  unsigned long long few_rank[64], few_mass[64];
+  unsigned long long few_rank[kFew], few_mass[kFew], few_run[kFew];
   unsigned long long wave_m[16];
   float wave_max[16];
   // a crossing: the bin (-1: none), what lies before it and in it
   int bin, part;
-  uint32_t in_n, few, first, listed;
+  uint32_t in_n, few, first;
   unsigned long long before, rank, at;
-  double total, above, guess;
+  unsigned long long total;
+  float guess;
 };
 
 // Every wave's number, on all lanes: each of the first NT / 64 lanes its own.
@@ -359,6 +470,7 @@ __device__ __forceinline__ uint64_t select(Shared<NT>& s, int bits, uint64_t tar
 #pragma unroll 1
   for (;;) {
     if (threadIdx.x == 0) s.few = 0;
+    if (threadIdx.x < 64) s.few_run[threadIdx.x] = 0;
     if (n <= 64) {
       __syncthreads();
       each([&](uint64_t r, uint64_t m) {
@@ -368,18 +480,16 @@ __device__ __forceinline__ uint64_t select(Shared<NT>& s, int bits, uint64_t tar
         s.few_mass[at] = m;
       });
       __syncthreads();
+      // a lane for each, a wave for some of those that it is compared with
+      const int c = static_cast<int>(s.few), wave = threadIdx.x >> 6;
+      const uint64_t r = s.few_rank[lane], m = s.few_mass[lane];  // (garbage behind the last)
+      uint64_t run = 0;
+#pragma unroll 2
+      for (int j = wave; j < c; j += NT / 64) run += s.few_rank[j] > r ? s.few_mass[j] : 0;
+      if (lane < c && run) atomicAdd(&s.few_run[lane], static_cast<unsigned long long>(run));
+      __syncthreads();
       if (threadIdx.x < 64) {
-        const int c = static_cast<int>(s.few);
-        const uint64_t r = lane < c ? s.few_rank[lane] : 0, m = lane < c ? s.few_mass[lane] : 0;
-        uint64_t run = before;
-#pragma unroll 1
-        for (int j = 0; j < c; ++j) {
-          const uint64_t rj = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(r >> 32), j)) << 32 |
-                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(r), j));
-          const uint64_t mj = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(m >> 32), j)) << 32 |
-                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(m), j));
-          run += rj > r ? mj : 0;
-        }
+        run = before + s.few_run[lane];
         if (lane < c && run < target && run + m >= target) s.rank = r;
       }
       __syncthreads();
@@ -426,7 +536,6 @@ __device__ __forceinline__ uint64_t select(Shared<NT>& s, int bits, uint64_t tar
 }
 
 __device__ __forceinline__ int first_of(uint64_t lanes) { return __builtin_ctzll(lanes); }
-__device__ __forceinline__ int last_of(uint64_t lanes) { return 63 - __builtin_clzll(lanes); }
 __device__ __forceinline__ int bits_of(uint32_t most) { return most == 0 ? 1 : 32 - __clz(most); }
 
 // A first part of the order: tokens of larger keys, and those of this key up to an
@@ -473,9 +582,7 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
   m = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
   const int64_t at = b * a.parts + part;
   Weights wt;
-  wt.c = 1.4426950408889634 / static_cast<double>(rules.t);
-  wt.unit = ldexp(1.0, 52 - a.q);
-  wt.tab = tab;
+  wt.begin(rules.t, a.q, tab);
   const bool nothing = Weights::peaked(m, wt.c) || m == -INFINITY;  // (the row's draw does not ask)
   if (!nothing) wt.set(m, a.q);
   uint64_t sum = 0;
@@ -506,7 +613,7 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
   if (tid == 0) a.part_max[at] = m;
   __syncthreads();
   if (rules.by_p) {
-    a.part_steps[at * kCoarse + tid] = hist[4 * tid] + hist[4 * tid + 1] + hist[4 * tid + 2] + hist[4 * tid + 3];
+    for (int i = tid; i < kCoarse; i += 256) a.part_steps[at * kCoarse + i] = hist[2 * i] + hist[2 * i + 1];
   } else if (tid == 0) {
     a.part_sum[at] = nothing ? 0 : wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
   }
@@ -517,7 +624,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   constexpr int kWaves = NT / 64;
   constexpr bool kWhole = NT == 256;  // every row is its own list
   using R = Row<T, NT>;
-  constexpr int E = R::E;
+  constexpr int E = R::E, kShift = E == 8 ? 16 : 0;  // bits of keys that say nothing
   __shared__ Shared<NT> s;
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -529,14 +636,18 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   const float* part_max = a.part_max + b * a.parts;
 
   fill_table(s.tab);
-  if (tid == 0) {
-    s.first = 0xffffffffu;
-    s.listed = 0;
-  }
+  if (tid == 0) s.first = 0xffffffffu;
   if constexpr (!kWhole) s.count[tid] = 0;
   float mine = -INFINITY;  // the thread's largest
   if (by_parts) {
-    for (int i = tid; i < a.parts; i += NT) mine = fmaxf(mine, part_max[i]);
+    for (int i = tid; i < a.parts; i += NT) {
+      const float x = part_max[i];
+      if (!by_p) s.kept[i] = a.part_sum[b * a.parts + i];
+      s.part_max[i] = x;
+      mine = fmaxf(mine, x);
+    }
+  } else if constexpr (kWhole) {
+    for (int i = tid; i < a.V; i += NT) mine = fmaxf(mine, row.one(i));
   } else {
     mine = row.largest();
   }
@@ -552,12 +663,18 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     return;
   }
   if (rules.greedy) {  // the first of the largest
-    if (__ballot(mine == m))
-      row.walk(row.v0, row.v1, [&](int i, const float(&x)[E]) {
+    {
+      if constexpr (kWhole) {
+        for (int i = tid; i < a.V; i += NT)
+          if (row.one(i) == m) atomicMin(&s.first, static_cast<uint32_t>(i));
+      } else {
+        row.part(wave, 0, row.n, [&](int i, const float(&x)[E]) {
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (x[j] == m) atomicMin(&s.first, static_cast<uint32_t>(i + j));
-      });
+          for (int j = 0; j < E; ++j)
+            if (x[j] == m) atomicMin(&s.first, static_cast<uint32_t>(i + j));
+        });
+      }
+    }
     __syncthreads();
     if (tid == 0) {
       a.token[b] = s.first;
@@ -568,16 +685,14 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   const uint32_t key_m = key_of(m), last = a.V - 1;
   const int index_bits = bits_of(last);
   Weights wt;
-  wt.c = 1.4426950408889634 / static_cast<double>(rules.t);
-  wt.unit = ldexp(1.0, 52 - a.q);
-  wt.tab = s.tab;
+  wt.begin(rules.t, a.q, s.tab);
   wt.lowest = m;
   wt.R = 0;
   const bool peaked = Weights::peaked(m, wt.c);  // the largest weigh the same, all others nothing
   if (!peaked) wt.set(m, a.q);
   float floor_l = wt.lowest;  // of what can be drawn
   if (rules.least > 0.f && !peaked) {
-    const double x = m + log2_of(fmax(static_cast<double>(rules.least), 0x1p-100), s.tab) / wt.c;
+    const double x = m + log2_of(fmax(static_cast<double>(rules.least), 0x1p-100), s.tab) * wt.per;
     floor_l = fmaxf(floor_l, -float_under(fmin(-x, 3.4028234663852886e38)));  // (the smallest float that is not below x)
   }
   auto part = [&](uint64_t total) -> uint64_t {  // what top-p's run has to reach
@@ -600,14 +715,37 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       log2p = (peaked ? 0.0 : static_cast<double>(l) * wt.c - wt.R) - log2_of(total_r, s.tab);
     a.logprob[b] = static_cast<float>(log2p * 0.6931471805599453);
   };
+  auto under_of = [&](float pm) -> float {
+    if (pm == -INFINITY || Weights::peaked(pm, wt.c)) return 1e9f;
+    return static_cast<float>(fmin(wt.R - ceil(static_cast<double>(pm) * wt.c), 1e9));
+  };
+  const uint32_t key_floor = key_of(floor_l);
   const double per_unit = peaked ? 1.0 : ldexp(1.0, -a.q);
+
+  // f(part, step, octaves of the part's R under the row's, sum) of the parts' steps
+  auto each_step = [&](auto f) {
+    constexpr int kSome = 8, kOf = NT / kCoarse > 0 ? NT / kCoarse : 1;  // loads on their way together; threads of a step
+    const int i = tid & (kCoarse - 1);
+#pragma unroll 1
+    for (int p0 = tid / kCoarse; p0 < a.parts; p0 += kSome * kOf) {
+      unsigned long long w[kSome];
+#pragma unroll
+      for (int j = 0; j < kSome; ++j) {
+        const int p = p0 + j * kOf < a.parts ? p0 + j * kOf : p0;
+        w[j] = a.part_steps[(b * a.parts + p) * kCoarse + i];
+      }
+#pragma unroll
+      for (int j = 0; j < kSome; ++j)
+        if (p0 + j * kOf < a.parts) f(p0 + j * kOf, i, s.under[p0 + j * kOf], w[j]);
+    }
+  };
 
   // -- the list: what the first border is decided on ------------------------------------
   Cut cut{0, 0xffffffffu};    // all
   bool listed = kWhole;       // all that the cut keeps are in the list
   bool first_cut = false, counts = true, from_list = true;
   int n = 0, border = -1;
-  uint32_t lo = 0;            // keys from here on
+  uint32_t lo = 0, hi = key_m;  // keys from here on, up to there
   uint64_t target = k;
   if constexpr (kWhole) {
     n = a.V;
@@ -622,12 +760,12 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     bool all = true, band = false;  // what the list may be: all from the border's step on, that step alone
     float from = floor_l, to = INFINITY;
     int wide = 2;                   // the steps are of 2^wide / 128
-    double before = 0.0;
+    uint64_t before = 0;
     if (by_k) {
       if (by_threads) {
         if (mine >= wt.lowest) atomicAdd(&s.count[wt.step(mine)], 1u);
       } else {
-        row.walk(row.v0, row.v1, [&](int, const float(&x)[E]) {
+        row.part(wave, 0, row.n, [&](int, const float(&x)[E]) {
 #pragma unroll
           for (int j = 0; j < E; ++j)
             if (x[j] >= wt.lowest) atomicAdd(&s.count[wt.step(x[j])], 1u);
@@ -636,99 +774,71 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       __syncthreads();
       crossing<NT>(s, static_cast<uint32_t>(k));
       border = s.bin;
-      before = static_cast<double>(s.before);
+      before = s.before;
       if (by_threads && border < 0) border = kSteps - 1;
       band = !by_threads;
       all = first_cut = border >= 0;  // (fewer than k weigh anything: k keeps them all)
     } else if (by_p) {
-      // the parts' sums by steps, over the row's R
-      const int i = tid & (kCoarse - 1);
-      double g = 0.0;
-      for (int p = tid / kCoarse; p < a.parts; p += NT / kCoarse) {
-        const float pm = part_max[p];
-        if (pm == -INFINITY || Weights::peaked(pm, wt.c)) continue;
-        const double under = wt.R - ceil(static_cast<double>(pm) * wt.c);
-        if (!(under < kCoarse)) continue;
-        const int off = 8 * static_cast<int>(under);
-        const unsigned long long* steps = a.part_steps + (b * a.parts + p) * kCoarse;
-        uint64_t w = 0;
-        if (i >= off) w = steps[i - off];
-        if (i == kCoarse - 1)
-          for (int j = off < kCoarse ? kCoarse - off : 0; j < kCoarse; ++j) w += steps[j];
-        g += ldexp(static_cast<double>(w), -static_cast<int>(under));
-      }
-      s.steps[tid / kCoarse][i] = g;
-      if (tid == 0) s.bin = -1;
+      // the parts' sums by steps, shifted to the row's R
+      for (int p = tid; p < a.parts; p += NT) s.under[p] = under_of(s.part_max[p]);
+      if (tid < kCoarse) s.steps[tid] = 0;
+      __syncthreads();
+      each_step([&](int, int i, float under, unsigned long long w) {
+        const int down = static_cast<int>(fminf(under, 63.f));
+        w >>= down;
+        if (w) atomicAdd(&s.steps[i + 16 * down < kCoarse ? i + 16 * down : kCoarse - 1], w);
+      });
       __syncthreads();
       if (wave == 0) {
         constexpr int kEach = kCoarse / 64;
-        double x[kEach], sum = 0.0, guess = 0.0, scale = exp2(lane * kEach / 8.0);
+        uint64_t x[kEach], sum = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-          const int c = lane * kEach + j;
-          x[j] = s.steps[0][c] + s.steps[1][c] + s.steps[2][c] + s.steps[3][c];
+          x[j] = s.steps[lane * kEach + j];
           sum += x[j];
         }
-        double run = sum;
+        const uint64_t to_here = wave_scan(sum), goal = part(last_lane(to_here));
+        uint64_t run = to_here - sum;
+        int c = -1;
 #pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-          const double o = __shfl_up(run, w);
-          if (lane >= w) run += o;
-        }
-        const double total = __shfl(run, 63), goal = fmax(static_cast<double>(rules.p) * total, 1.0);
-        double at = run - sum;
-        // (a token of step c weighs more than 2^(-(c + 1) / 8))
-        guess = sum * scale * 1.4142135623730951 * per_unit;
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-          const double o = __shfl_up(guess, w);
-          if (lane >= w) guess += o;
-        }
-        const bool here = at < goal && run >= goal;
-        const uint64_t lanes = __ballot(here);
-        // (by roundings no lane may reach it: then the last that has anything)
-        const uint64_t any = __ballot(sum > 0.0);
-        const int pick = lanes ? first_of(lanes) : last_of(any);
-        if (lane == pick) {
-          int c = -1;
-#pragma unroll
-          for (int j = 0; j < kEach; ++j) {
-            if (c < 0 && x[j] > 0.0) {
-              if (at + x[j] >= goal)
-                c = j;
-              else
-                at += x[j];
-            }
+        for (int j = 0; j < kEach; ++j) {
+          if (run < goal && run + x[j] >= goal) {
+            c = lane * kEach + j;
+            s.bin = c;
+            s.before = run;
           }
-          if (c < 0) {  // roundings again: the last of the lane's
+          run += x[j];
+        }
+        // how many tokens that are at most: one of step j weighs more than 2^(-(j + 1) / 16)
+        c = __builtin_amdgcn_readlane(c, first_of(__ballot(c >= 0)));
+        float guess = 0.f;
 #pragma unroll
-            for (int j = 0; j < kEach; ++j)
-              if (x[j] > 0.0) c = j;
-            at -= x[0] * (c == 0) + x[1] * (c == 1) + x[2] * (c == 2) + x[3] * (c == 3);
-          }
-          s.bin = lane * kEach + c;
-          s.above = at;
+        for (int j = 0; j < kEach; ++j)
+          if (lane * kEach + j <= c)
+            guess += static_cast<float>(x[j]) * __builtin_amdgcn_exp2f((lane * kEach + j + 1) * 0.0625f - a.q);
+        guess = wave_all(guess, [](float x, float y) { return x + y; });
+        if (lane == 0) {
           s.total = goal;
           s.guess = guess;
         }
       }
       __syncthreads();
       border = s.bin;
-      before = s.above;
-      wide = 4;
+      before = s.before;
+      wide = 3;
       counts = false;
       first_cut = true;
       band = true;
-      all = s.guess < kList;
-      target = static_cast<uint64_t>(ceil(s.total));
+      all = s.guess <= kFew;
+      target = s.total;
     }
     if (border >= 0) {
       // logits of the steps up to the border's, and of the border's, with a little room
       // for roundings
       const double low = 1 << wide, first_n = low * border;  // n of its first, under 128 R
       const bool lowest_step = border == (wide == 2 ? kSteps : kCoarse) - 1;
-      from = lowest_step ? wt.lowest : float_under((wt.R - (first_n + low) / 128.0) / wt.c);
-      to = -float_under(-(wt.R - (first_n - 1.0) / 128.0) / wt.c);
+      from = lowest_step ? wt.lowest : fmaxf(wt.lowest, float_under((wt.R - (first_n + low) * 0.0078125) * wt.per));
+      to = -float_under(-(wt.R - (first_n - 1.0) * 0.0078125) * wt.per);
     }
     // gathers the tokens from `from` on (first all, then the border's step alone)
     from_list = false;
@@ -737,94 +847,151 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       const bool alone = attempt == 1;
       const float most = alone ? to : INFINITY;
       __syncthreads();
-      if (tid == 0) s.listed = 0;
-      __syncthreads();
-      row.walk(row.v0, row.v1, [&](int i, const float(&x)[E]) {
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < E; ++j) top = fmaxf(top, x[j]);
-        if (!__ballot(top >= from)) return;
-        uint32_t in = 0;
-#pragma unroll
-        for (int j = 0; j < E; ++j) in |= static_cast<uint32_t>(x[j] >= from && x[j] <= most) << j;
-#pragma unroll 1
-        while (__ballot(in != 0)) {  // a token of every lane that has one
-          const int j = __ffs(in) - 1;
-          float l = x[0];
-#pragma unroll
-          for (int c = 1; c < E; ++c) l = j == c ? x[c] : l;
-          bool take = in != 0;
-          if (alone && take) {
-            const int step = wide == 2 ? wt.step(l) : wt.step(l) >> 2;
-            take = l >= wt.lowest && step == border;
-          }
-          const uint64_t mask = __ballot(take);
-          in &= in - 1;
-          if (mask == 0) continue;
-          uint32_t at = 0;
-          if (lane == 0) at = atomicAdd(&s.listed, static_cast<uint32_t>(__popcll(mask)));
-          at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((1ull << lane) - 1));
-          if (take && at < kList) s.list[at] = static_cast<uint64_t>(key_of(l)) << 32 | static_cast<uint32_t>(i + j);
-        }
+      // first into places of the wave's own (in s.weight), then together
+      constexpr int kSlots = kList / kWaves;
+      unsigned long long* slots = s.weight + kSlots * wave;
+      int mine_n = 0;
+      row.between(from, most, [&](int i, float l, uint64_t mask) {
+        const int before = mine_n;
+        mine_n += __popcll(mask);
+        if (mine_n > kSlots) return;
+        if (mask >> lane & 1)
+          slots[__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                          __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), before))] =
+              static_cast<uint64_t>(__float_as_uint(l)) << 32 | static_cast<uint32_t>(i);
       });
+      const uint32_t counted = static_cast<uint32_t>(of_waves<NT>(s, static_cast<uint64_t>(mine_n)));
+      const uint32_t places = wave_scan(counted);
+      const bool fits = !__ballot(counted > kSlots);
+      n = static_cast<int>(last_lane(places));
+      if (fits) {
+        const int at = static_cast<int>(__builtin_amdgcn_readlane(places, wave)) - mine_n;
+        for (int i = lane; i < mine_n; i += 64) {
+          const uint64_t x = slots[i];
+          const float l = __uint_as_float(static_cast<uint32_t>(x >> 32));
+          // (what is not of the step that stands alone leaves a hole)
+          const bool of = !alone || (l >= wt.lowest && (wide == 2 ? wt.step(l) : wt.step(l) >> 1) == border);
+          s.list[at + i] = of ? static_cast<uint64_t>(key_of(l)) << 32 | static_cast<uint32_t>(x) : 0;
+        }
+      } else {
+        n = kList + 1;
+      }
       __syncthreads();
-      n = static_cast<int>(s.listed);
       if (n <= kList) {
         from_list = true;
         listed = !alone;
-        if (alone) {
-          const double x = ceil(target - before);
-          target = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
-        }
-        lo = first_cut && !alone ? key_of(from) : 0;
+        if (alone) target -= before;
+        lo = first_cut ? key_of(from) : 0;
+        hi = first_cut && alone && key_of(to) < hi ? key_of(to) : hi;
       }
     }
   }
 
-  // f(key, index) of the list's tokens, or the row's, of the cut, from lo on
+  if (kWhole || from_list) {  // weights, for every look at the list
+    for (int i = tid; i < n; i += NT) {
+      const float l = of_key(static_cast<uint32_t>(s.list[i] >> 32));
+      s.weight[i] = peaked ? l >= wt.lowest : wt.of(l, wt.lowest);
+    }
+  }
+  // f(key, index, weight) of the list's tokens, or the row's, of the cut, from lo on
   auto each = [&](bool in_list, auto f) {
     if (kWhole || in_list) {
 #pragma unroll 1
-      for (int i = tid; i < n; i += NT) {
+      for (int i = tid; i < n; i += NT) {  // (a thread's own)
         const uint64_t x = s.list[i];
         const uint32_t ky = static_cast<uint32_t>(x >> 32), at = static_cast<uint32_t>(x);
-        if (ky != 0 && ky >= lo && cut.keeps(ky, at)) f(ky, at);
+        if (ky != 0 && ky >= lo && cut.keeps(ky, at)) f(ky, at, s.weight[i]);
       }
     } else if constexpr (!kWhole) {
-      row.walk(row.v0, row.v1, [&](int i, const float(&x)[E]) {
+      row.part(wave, 0, row.n, [&](int i, const float(&x)[E]) {
 #pragma unroll 1
         for (int j = 0; j < E; ++j) {
           float l = x[0];
 #pragma unroll
           for (int c = 1; c < E; ++c) l = j == c ? x[c] : l;
           const uint32_t ky = key_of(l), at = static_cast<uint32_t>(i + j);
-          if (l >= wt.lowest && ky >= lo && cut.keeps(ky, at)) f(ky, at);
+          if (l >= wt.lowest && ky >= lo && cut.keeps(ky, at)) f(ky, at, peaked ? 1 : wt.whole(l));
         }
       });
     }
   };
+  // Few tokens: each is compared with each, a lane for each and a pair of waves for some
+  // of those that it is compared with; once in the order, once by index.
+  if (listed && n <= kFew) {
+    if (tid < kFew) s.few_rank[tid] = s.few_run[tid] = s.mass[tid] = 0;
+    __syncthreads();
+    constexpr int kOf = NT / kFew;
+    const int e = tid & (kFew - 1), slice = tid / kFew;
+    const uint64_t x = e < n ? s.list[e] : 0, place_of = x ^ 0xffffffffu;
+    uint64_t rank = 0, before = 0;
+#pragma unroll 2
+    for (int j = slice; j < n; j += kOf) {
+      const bool over = (s.list[j] ^ 0xffffffffu) > place_of;
+      rank += over;
+      before += over ? s.weight[j] : 0;
+    }
+    if (rank) {
+      atomicAdd(&s.few_rank[e], static_cast<unsigned long long>(rank));
+      atomicAdd(&s.few_run[e], static_cast<unsigned long long>(before));
+    }
+    __syncthreads();
+    uint64_t total = 0;
+    if (wave == 0) {
+      constexpr int kEach = kFew / 64;
+      uint64_t w[kEach], sum = 0;
+#pragma unroll
+      for (int h = 0; h < kEach; ++h) {
+        const int i = lane + 64 * h;
+        w[h] = i < n && (!by_k || s.few_rank[i] < static_cast<uint64_t>(k)) ? s.weight[i] : 0;
+        sum += w[h];
+      }
+      if (by_p && !by_parts) target = part(wave_sum(sum));
+      sum = 0;
+#pragma unroll
+      for (int h = 0; h < kEach; ++h) {
+        const int i = lane + 64 * h;
+        if (by_p && s.few_run[i] >= target) w[h] = 0;
+        if (static_cast<uint32_t>(s.list[i] >> 32) < key_floor) w[h] = 0;
+        s.few_mass[i] = w[h];
+        sum += w[h];
+      }
+      total = wave_sum(sum);
+      if (lane == 0) s.total = total;
+    }
+    __syncthreads();
+    const uint32_t index = static_cast<uint32_t>(x);
+    before = 0;
+#pragma unroll 2
+    for (int j = slice; j < n; j += kOf) before += static_cast<uint32_t>(s.list[j]) < index ? s.few_mass[j] : 0;
+    if (before) atomicAdd(&s.mass[e], static_cast<unsigned long long>(before));
+    __syncthreads();
+    if (tid < kFew) {
+      total = s.total;
+      const uint64_t at = place(total), own = s.few_mass[e];
+      before = s.mass[e];
+      if (e < n && before <= at && at < before + own)
+        done(index, of_key(static_cast<uint32_t>(x >> 32)), static_cast<double>(own), static_cast<double>(total),
+             static_cast<double>(total) * per_unit);
+    }
+    return;
+  }
   // Three selects, each on what the one before left: top-k's or top-p's border, top-p's
   // behind top-k's, the draw (of a list; a row's has walks of its own below).
 #pragma unroll 1
   for (int stage = 0; stage < 3; ++stage) {
     const bool draw = stage == 2;
-    bool ones = peaked, in_list = listed;
+    bool ones = false, in_list = listed;
     if (stage == 0) {
       if (!first_cut) continue;
-      ones |= counts;
+      ones = counts;
       in_list = from_list;
     } else if (stage == 1 ? !by_p || by_parts || (peaked && !kWhole) : !listed) {
       continue;
     }
-    const float floor = draw ? floor_l : wt.lowest;
-    auto mass = [&](uint32_t ky) -> uint64_t {
-      const float l = of_key(ky);
-      if (ones) return l >= floor;
-      return wt.of(l, floor);
-    };
     if (stage > 0) lo = cut.key > lo ? cut.key : lo;
+    if (draw) lo = key_floor > lo ? key_floor : lo;
     uint64_t total = 0;
-    each(in_list, [&](uint32_t ky, uint32_t) { total += mass(ky); });
+    each(in_list, [&](uint32_t, uint32_t, uint64_t w) { total += ones ? 1 : w; });
     total = block_sum<NT>(s, total);
     if (stage == 0) {
       if (counts && target >= total) continue;   // k keeps them all
@@ -832,16 +999,20 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     } else {
       target = draw ? place(total) + 1 : part(total);
     }
-    const int bits = draw ? index_bits : bits_of(key_m - lo) + index_bits;
+    const uint32_t lowest = lo >> kShift;
+    const int bits = draw ? index_bits : bits_of((hi >> kShift) - lowest) + index_bits;
     const uint64_t r = select<NT>(s, bits, target, in_list ? n : a.V, [&](auto g) {
-      each(in_list, [&](uint32_t ky, uint32_t i) {
-        const uint64_t w = mass(ky);
-        if (w) g(static_cast<uint64_t>(draw ? 0 : ky - lo) << index_bits | (last - i), w);
+      each(in_list, [&](uint32_t ky, uint32_t i, uint64_t w) {
+        if (ones) w = 1;
+        if (w) g(static_cast<uint64_t>(draw ? 0 : (ky >> kShift) - lowest) << index_bits | (last - i), w);
       });
     });
     const uint32_t at = last - (static_cast<uint32_t>(r) & ((1u << index_bits) - 1));
     if (!draw) {
-      cut = Cut{lo + static_cast<uint32_t>(r >> index_bits), at};
+      uint32_t ky = (lowest + static_cast<uint32_t>(r >> index_bits)) << kShift;
+      if (kShift > 0 && !(ky & 0x80000000u)) ky |= (1u << kShift) - 1;  // (a negative number's)
+      cut = Cut{ky, at};
+      hi = key_m;
     } else if (tid == 0) {
       const float l = row.one(at);
       done(at, l, static_cast<double>(peaked ? 1 : wt.whole(l)), static_cast<double>(total),
@@ -861,75 +1032,53 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       // its step what the cut keeps.
       __syncthreads();
       constexpr int kVectors = kPart / E;
-      auto r_of = [&](float pm) { return static_cast<int>(ceil(static_cast<double>(pm) * wt.c)); };
-      for (int p = wave; p < a.parts; p += kWaves) {
-        const float pm = part_max[p];
-        uint64_t sum = 0;
-        if (pm != -INFINITY && !Weights::peaked(pm, wt.c)) {
-          if (!by_p) {
-            sum = a.part_sum[b * a.parts + p];
-          } else {
-            const double under = wt.R - static_cast<double>(r_of(pm));
-            const int end = under < kCoarse ? border - 8 * static_cast<int>(under) : 0;
-            for (int i = lane; i < end; i += 64) sum += a.part_steps[(b * a.parts + p) * kCoarse + i];
-            sum = wave_sum(sum);
-          }
-        }
-        if (lane == 0) s.kept[p] = sum;
-      }
-      __syncthreads();
       if (by_p) {
+        for (int p = tid; p < a.parts; p += NT) s.kept[p] = 0;
+        __syncthreads();
+        each_step([&](int p, int i, float under, unsigned long long w) {
+          // (a wave's steps are of one part)
+          const uint64_t sum = wave_sum(under < kCoarse && i < border - 16 * static_cast<int>(under) ? static_cast<uint64_t>(w) : 0);
+          if (lane == 0 && sum) atomicAdd(&s.kept[p], static_cast<unsigned long long>(sum));
+        });
         for (int i = tid; i < n; i += NT) {
           const uint64_t x = s.list[i];
           const uint32_t ky = static_cast<uint32_t>(x >> 32), index = static_cast<uint32_t>(x);
-          if (!cut.keeps(ky, index)) continue;
+          if (ky == 0 || !cut.keeps(ky, index)) continue;
           const int p = (static_cast<int>(index) + row.off) / E / kVectors;
           Weights w = wt;
-          w.set(part_max[p], a.q);
+          w.set(s.part_max[p], a.q);
           atomicAdd(&s.kept[p], static_cast<unsigned long long>(w.of(of_key(ky), w.lowest)));
         }
         __syncthreads();
       }
       if (wave == 0) {
-        auto kept_of = [&](int p, int& under) -> double {  // in the row's units
-          under = 0;
-          if (p >= a.parts || s.kept[p] == 0) return 0.0;
-          under = wt.R - r_of(part_max[p]);
-          return ldexp(static_cast<double>(s.kept[p]), -under);
+        int under = 0;
+        auto kept_of = [&](int p) -> uint64_t {  // in the row's units
+          const uint64_t x = p < a.parts ? s.kept[p] : 0;
+          under = x ? static_cast<int>(fminf(under_of(s.part_max[p]), 63.f)) : 0;
+          return x >> under;
         };
-        auto scan = [&](double v) {
-#pragma unroll
-          for (int w = 1; w < 64; w <<= 1) {
-            const double o = __shfl_up(v, w);
-            if (lane >= w) v += o;
-          }
-          return v;
-        };
-        int under;
-        double sum = 0.0;
-        for (int p0 = 0; p0 < a.parts; p0 += 64) sum += __shfl(scan(kept_of(p0 + lane, under)), 63);
-        const double x = u > 0.f ? fmin(static_cast<double>(u), 0.9999999999999999) * sum : 0.0;
-        double run = 0.0;
+        uint64_t sum = 0;
+        for (int p0 = 0; p0 < a.parts; p0 += 64) sum += wave_sum(kept_of(p0 + lane));
+        uint64_t place_in = place(sum);
+#pragma unroll 1
         for (int p0 = 0; p0 < a.parts; p0 += 64) {
-          const double v = kept_of(p0 + lane, under), to_here = run + scan(v);
-          // (the last with anything, should roundings leave none that reaches it)
-          const uint64_t over = __ballot(v > 0.0 && to_here > x), any = __ballot(v > 0.0);
-          const int pick = over ? first_of(over) : any ? last_of(any) : -1;
-          if (lane == pick) {
-            const double in = ldexp(x - (to_here - v), under);
-            const uint64_t most = s.kept[p0 + lane];
-            s.part = p0 + lane;
-            s.at = in > 0.0 ? (in < static_cast<double>(most) ? static_cast<uint64_t>(in) : most - 1) : 0;
-            if (s.at >= most) s.at = most - 1;
+          const uint64_t v = kept_of(p0 + lane), to_here = wave_scan(v);
+          const uint64_t over = __ballot(to_here > place_in);
+          if (over) {
+            if (lane == first_of(over)) {
+              s.part = p0 + lane;
+              s.at = (place_in - (to_here - v)) << under;  // (the first of the part's units that are this one of the row's)
+            }
+            break;
           }
-          if (over) break;
-          run = __shfl(to_here, 63);
+          place_in -= last_lane(to_here);
         }
         if (lane == 0) s.total = sum;
       }
       __syncthreads();
       at = s.at;
-      total = s.total;
+      total = static_cast<double>(s.total);
       total_r = total * per_unit;
       v0 = s.part * kVectors;
       v1 = v0 + kVectors < row.n ? v0 + kVectors : row.n;
@@ -938,22 +1087,15 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     // The draw: every wave sums what its part of the row keeps, then of the part in
     // which the draw lies, until one step of a wave holds the rest.
     Weights w = wt;  // in the units of the row, or of its part
-    if (!need_total) w.set(part_max[s.part], a.q);
+    if (!need_total) w.set(s.part_max[s.part], a.q);
     const float low = fmaxf(fmaxf(floor_l, key_l), w.lowest);
     auto weight = [&](float l, int i) -> uint64_t {
       uint64_t x = w.whole(l);
       if (peaked) x = 1;
       return l >= low && (l != key_l || static_cast<uint32_t>(i) <= to) ? x : 0;
     };
-#pragma unroll 1
-    while (need_total || v1 - v0 > 64) {
-      const int per = (v1 - v0 + kWaves - 1) / kWaves;
-      const int w0 = v0 + wave * per, w1 = w0 + per < v1 ? w0 + per : v1;
-      uint64_t sum = 0;
-      row.walk(w0, w1, [&](int i, const float(&x)[E]) {
-#pragma unroll
-        for (int j = 0; j < E; ++j) sum += weight(x[j], i + j);
-      });
+    // the wave in whose part the draw lies, with the draw's place there
+    auto pick = [&](uint64_t sum) -> int {
       const uint64_t sums = of_waves<NT>(s, wave_sum(sum)), run = wave_scan(sums);
       if (need_total) {
         uint64_t kept = last_lane(run);
@@ -966,31 +1108,55 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
         total_r = total * per_unit;
         need_total = false;
       }
-      const int pick = first_of(__ballot(run > at) | 1ull << 63) & (kWaves - 1);  // (there is one)
-      const uint64_t to_here = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(run >> 32), pick)) << 32 |
-                               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(run), pick));
-      const uint64_t here = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(sums >> 32), pick)) << 32 |
-                            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(sums), pick));
-      at -= to_here - here;
-      v0 += pick * per;
+      const int w = first_of(__ballot(run > at) | 1ull << 63) & (kWaves - 1);  // (there is one)
+      at -= lane_of(run, w) - lane_of(sums, w);
+      return w;
+    };
+    constexpr int kHeld = kPart / E / NT, kMost = kHeld * NT;  // vectors of a lane, of a workgroup
+#pragma unroll 1
+    while (v1 - v0 > kMost) {
+      const int per = (v1 - v0 + kWaves - 1) / kWaves;
+      uint64_t sum = 0;
+      row.part(wave, v0, v1, [&](int i, const float(&x)[E]) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum += weight(x[j], i + j);
+      });
+      v0 += pick(sum) * per;
       v1 = v0 + per < v1 ? v0 + per : v1;
     }
-    if (wave != 0) return;
-    float x[E];
-    uint64_t wx[E], sum = 0;
-    R::wide(row.raw(v0, v1), x);
-    const int i = (v0 + lane) * E - row.off;
+    uint64_t of[kHeld], sum = 0;
+    u32x4_t held[kHeld];
+    const int mine0 = v0 + wave * 64 * kHeld;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      wx[j] = weight(x[j], i + j);
-      sum += wx[j];
+    for (int h = 0; h < kHeld; ++h) held[h] = row.raw(mine0 + 64 * h, v1);
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+      float x[E];
+      R::wide(held[h], x);
+      of[h] = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) of[h] += weight(x[j], (mine0 + 64 * h + lane) * E - row.off + j);
+      sum += of[h];
     }
-    uint64_t run = wave_scan(sum) - sum;
+    if (pick(sum) != wave) return;
+    uint64_t run = 0;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      if (run <= at && at < run + wx[j])
-        done(i + j, x[j], ldexp(static_cast<double>(wx[j]), w.R - wt.R), total, total_r);
-      run += wx[j];
+    for (int h = 0; h < kHeld; ++h) {
+      const uint64_t to_here = run + wave_scan(of[h]);
+      if (to_here - of[h] <= at && at < to_here) {
+        float x[E];
+        R::wide(held[h], x);
+        const int i = (mine0 + 64 * h + lane) * E - row.off;
+        uint64_t before = to_here - of[h];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const uint64_t y = weight(x[j], i + j);
+          if (before <= at && at < before + y)
+            done(i + j, x[j], ldexp(static_cast<double>(y), w.R - wt.R), total, total_r);
+          before += y;
+        }
+      }
+      run = last_lane(to_here);
     }
   }
 }
