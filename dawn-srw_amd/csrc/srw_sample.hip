@@ -56,7 +56,8 @@ struct SampleArgs {
   int32_t top_k_all;
   int64_t* token;
   float* logprob;
-  // of every row and part: its largest logit, its sum, and for top-p the steps' sums
+  // of every row and part: its largest logit, its sum, and for top-p the steps' running
+  // sums
   float* part_max;
   unsigned long long *part_sum, *part_steps;
 };
@@ -330,19 +331,28 @@ template <typename T, int NT> struct Row {
       const uint64_t hits = __ballot(x >= from && x <= to);
       if (hits) f(edge, x, hits);
     }
-#pragma unroll 1
-    for (int v0 = first() + 64 * wave; v0 < last; v0 += 64 * kWaves * kAhead) {
-      u32x4_t w[kAhead];
+    constexpr int kSome = 4;  // and as many on their way behind them
+    u32x4_t w[kSome], next[kSome];
+    auto fetch = [&](int from) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int v = v0 + 64 * kWaves * k + lane;
-        w[k] = __builtin_nontemporal_load(at(v < last ? v : last - 1));
+      for (int k = 0; k < kSome; ++k) {
+        const int v = from + 64 * kWaves * k + lane;
+        next[k] = __builtin_nontemporal_load(at(v < last ? v : last - 1));
       }
+    };
+    int v0 = first() + 64 * wave;
+    if (v0 < last) fetch(v0);
+#pragma unroll 1
+    for (; v0 < last; v0 += 64 * kWaves * kSome) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
+      for (int k = 0; k < kSome; ++k) w[k] = next[k];
+      if (v0 + 64 * kWaves * kSome < last) fetch(v0 + 64 * kWaves * kSome);
+#pragma unroll
+      for (int k = 0; k < kSome; ++k) {
+        const int v = v0 + 64 * kWaves * k + lane;
+        if (v0 + 64 * kWaves * k >= last) break;
         float x[E];
         wide(w[k], x);
-        const int v = v0 + 64 * kWaves * k + lane;
         const uint64_t in = __ballot(v < last);
         uint64_t hits[E], any = 0;
 #pragma unroll
@@ -400,18 +410,22 @@ __device__ __forceinline__ N wave_all(N v, Op op) {
   return v;
 }
 
-template <int NT> struct Shared {
+// WHAT a kernel's rows are: any; each its own list; each drawn from its whole
+// distribution.
+enum { kAnyRow, kListRow, kWholeRow };
+template <int WHAT> struct Shared {
+  static constexpr int kListed = WHAT == kWholeRow ? 1 : kList, kParts = WHAT == kListRow ? 1 : kMostParts;
   double tab[128];
   union {
-    unsigned long long list[kList];  // key << 32 | index
-    unsigned long long steps[kCoarse];  // of the row's parts
+    unsigned long long list[kListed];  // key << 32 | index
+    unsigned long long steps[WHAT == kAnyRow ? 2 : 1][kCoarse];  // of the row's parts, half of them each
   };
-  unsigned long long weight[kList];  // of the list's tokens
+  unsigned long long weight[kListed];  // of the list's tokens
   uint32_t count[kSteps];
   unsigned long long mass[kBins + 64];
-  float part_max[NT == 1024 ? kMostParts : 1];
-  float under[NT == 1024 ? kMostParts : 1];  // octaves of a part's R under the row's; 1e9: it weighs nothing
-  unsigned long long kept[NT == 1024 ? kMostParts : 1];  // of each part, in its units
+  float part_max[kParts];
+  float under[kParts];  // octaves of a part's R under the row's; 1e9: it weighs nothing
+  unsigned long long kept[kParts];  // of each part, in its units
   unsigned long long few_rank[kFew], few_mass[kFew], few_run[kFew];
   unsigned long long wave_m[16];
   float wave_max[16];
@@ -424,8 +438,8 @@ template <int NT> struct Shared {
 };
 
 // Every wave's number, on all lanes: each of the first NT / 64 lanes its own.
-template <int NT>
-__device__ __forceinline__ uint64_t of_waves(Shared<NT>& s, uint64_t v) {
+template <int NT, class S>
+__device__ __forceinline__ uint64_t of_waves(S& s, uint64_t v) {
   if ((threadIdx.x & 63) == 0) s.wave_m[threadIdx.x >> 6] = v;
   __syncthreads();
   const int lane = threadIdx.x & 63;
@@ -433,14 +447,14 @@ __device__ __forceinline__ uint64_t of_waves(Shared<NT>& s, uint64_t v) {
   __syncthreads();
   return v;
 }
-template <int NT>
-__device__ __forceinline__ uint64_t block_sum(Shared<NT>& s, uint64_t v) {
+template <int NT, class S>
+__device__ __forceinline__ uint64_t block_sum(S& s, uint64_t v) {
   return wave_sum(of_waves<NT>(s, wave_sum(v)));
 }
 
 // The first step at which s.count's running sum reaches target.
-template <int NT>
-__device__ __forceinline__ void crossing(Shared<NT>& s, uint32_t target) {
+template <int NT, class S>
+__device__ __forceinline__ void crossing(S& s, uint32_t target) {
   static_assert(NT == kSteps);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t c = s.count[threadIdx.x];
@@ -460,8 +474,8 @@ __device__ __forceinline__ void crossing(Shared<NT>& s, uint32_t target) {
 // f(rank, mass) for every candidate of this thread, of which there are no more than n.
 // A pass takes a digit; where no more than 64 candidates share the digits up to the
 // border's, one wave compares each with each.
-template <int NT, class Each>
-__device__ __forceinline__ uint64_t select(Shared<NT>& s, int bits, uint64_t target, uint32_t n, Each each) {
+template <int NT, class S, class Each>
+__device__ __forceinline__ uint64_t select(S& s, int bits, uint64_t target, uint32_t n, Each each) {
   constexpr int kEach = kBins / 64;
   auto place = [](int i) { return i + i / kEach; };  // (a lane's run of bins, over all banks)
   const int lane = threadIdx.x & 63;
@@ -613,19 +627,25 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
   if (tid == 0) a.part_max[at] = m;
   __syncthreads();
   if (rules.by_p) {
-    for (int i = tid; i < kCoarse; i += 256) a.part_steps[at * kCoarse + i] = hist[2 * i] + hist[2 * i + 1];
+    // running sums: what a border leaves of a part is one number
+    const uint64_t s0 = hist[4 * tid] + hist[4 * tid + 1], s1 = hist[4 * tid + 2] + hist[4 * tid + 3];
+    uint64_t run = wave_scan(s0 + s1);
+    if (lane == 63) wave_sums[wave] = run;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) run += wave_sums[w];
+    *reinterpret_cast<ulonglong2*>(&a.part_steps[at * kCoarse + 2 * tid]) = make_ulonglong2(run - s1, run);
   } else if (tid == 0) {
     a.part_sum[at] = nothing ? 0 : wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
   }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, int WHAT>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   constexpr int kWaves = NT / 64;
-  constexpr bool kWhole = NT == 256;  // every row is its own list
+  constexpr bool kWhole = WHAT == kListRow;
   using R = Row<T, NT>;
   constexpr int E = R::E, kShift = E == 8 ? 16 : 0;  // bits of keys that say nothing
-  __shared__ Shared<NT> s;
+  __shared__ Shared<WHAT> s;
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const R row(a, b);
@@ -637,7 +657,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
 
   fill_table(s.tab);
   if (tid == 0) s.first = 0xffffffffu;
-  if constexpr (!kWhole) s.count[tid] = 0;
+  if constexpr (WHAT == kAnyRow) s.count[tid] = 0;
   float mine = -INFINITY;  // the thread's largest
   if (by_parts) {
     for (int i = tid; i < a.parts; i += NT) {
@@ -722,24 +742,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   const uint32_t key_floor = key_of(floor_l);
   const double per_unit = peaked ? 1.0 : ldexp(1.0, -a.q);
 
-  // f(part, step, octaves of the part's R under the row's, sum) of the parts' steps
-  auto each_step = [&](auto f) {
-    constexpr int kSome = 8, kOf = NT / kCoarse > 0 ? NT / kCoarse : 1;  // loads on their way together; threads of a step
-    const int i = tid & (kCoarse - 1);
-#pragma unroll 1
-    for (int p0 = tid / kCoarse; p0 < a.parts; p0 += kSome * kOf) {
-      unsigned long long w[kSome];
-#pragma unroll
-      for (int j = 0; j < kSome; ++j) {
-        const int p = p0 + j * kOf < a.parts ? p0 + j * kOf : p0;
-        w[j] = a.part_steps[(b * a.parts + p) * kCoarse + i];
-      }
-#pragma unroll
-      for (int j = 0; j < kSome; ++j)
-        if (p0 + j * kOf < a.parts) f(p0 + j * kOf, i, s.under[p0 + j * kOf], w[j]);
-    }
-  };
-
   // -- the list: what the first border is decided on ------------------------------------
   Cut cut{0, 0xffffffffu};    // all
   bool listed = kWhole;       // all that the cut keeps are in the list
@@ -747,7 +749,9 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   int n = 0, border = -1;
   uint32_t lo = 0, hi = key_m;  // keys from here on, up to there
   uint64_t target = k;
-  if constexpr (kWhole) {
+  if constexpr (WHAT == kWholeRow) {
+    from_list = false;
+  } else if constexpr (kWhole) {
     n = a.V;
     for (int i = tid; i < n; i += NT) {
       const float l = row.one(i);
@@ -781,45 +785,37 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     } else if (by_p) {
       // the parts' sums by steps, shifted to the row's R
       for (int p = tid; p < a.parts; p += NT) s.under[p] = under_of(s.part_max[p]);
-      if (tid < kCoarse) s.steps[tid] = 0;
       __syncthreads();
-      each_step([&](int, int i, float under, unsigned long long w) {
-        const int down = static_cast<int>(fminf(under, 63.f));
-        w >>= down;
-        if (w) atomicAdd(&s.steps[i + 16 * down < kCoarse ? i + 16 * down : kCoarse - 1], w);
-      });
+      // the running sums, shifted to the row's R
+      constexpr int kSome = 8, kOf = NT / kCoarse;  // loads on their way together; threads of a step
+      const int i = tid & (kCoarse - 1);
+      uint64_t sum = 0;
+#pragma unroll 1
+      for (int p0 = tid / kCoarse; p0 < a.parts; p0 += kSome * kOf) {
+        unsigned long long w[kSome];
+        int down[kSome];
+#pragma unroll
+        for (int j = 0; j < kSome; ++j) {
+          const int p = p0 + j * kOf < a.parts ? p0 + j * kOf : p0;
+          down[j] = static_cast<int>(fminf(s.under[p], 63.f));
+          // (the last step holds all that lies lower)
+          const int at = i == kCoarse - 1 ? i : i - 16 * down[j];
+          if (at < 0 || p0 + j * kOf >= a.parts) down[j] = 63;
+          w[j] = a.part_steps[(b * a.parts + p) * kCoarse + (at < 0 ? 0 : at)];
+        }
+#pragma unroll
+        for (int j = 0; j < kSome; ++j) sum += w[j] >> down[j];
+      }
+      s.steps[tid / kCoarse][i] = sum;
       __syncthreads();
-      if (wave == 0) {
-        constexpr int kEach = kCoarse / 64;
-        uint64_t x[kEach], sum = 0;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          x[j] = s.steps[lane * kEach + j];
-          sum += x[j];
-        }
-        const uint64_t to_here = wave_scan(sum), goal = part(last_lane(to_here));
-        uint64_t run = to_here - sum;
-        int c = -1;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          if (run < goal && run + x[j] >= goal) {
-            c = lane * kEach + j;
-            s.bin = c;
-            s.before = run;
-          }
-          run += x[j];
-        }
-        // how many tokens that are at most: one of step j weighs more than 2^(-(j + 1) / 16)
-        c = __builtin_amdgcn_readlane(c, first_of(__ballot(c >= 0)));
-        float guess = 0.f;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-          if (lane * kEach + j <= c)
-            guess += static_cast<float>(x[j]) * __builtin_amdgcn_exp2f((lane * kEach + j + 1) * 0.0625f - a.q);
-        guess = wave_all(guess, [](float x, float y) { return x + y; });
-        if (lane == 0) {
-          s.total = goal;
-          s.guess = guess;
+      const uint64_t goal = part(s.steps[0][kCoarse - 1] + s.steps[1][kCoarse - 1]);
+      if (tid < kCoarse) {
+        const uint64_t here = s.steps[0][i] + s.steps[1][i], over = i > 0 ? s.steps[0][i - 1] + s.steps[1][i - 1] : 0;
+        if (here >= goal && over < goal) {
+          s.bin = i;
+          s.before = over;
+          // (about as many tokens, were they half as heavy again as the border's)
+          s.guess = static_cast<float>(here) * __builtin_amdgcn_exp2f((i + 1) * 0.0625f - a.q) * 0.5f;
         }
       }
       __syncthreads();
@@ -830,7 +826,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       first_cut = true;
       band = true;
       all = s.guess <= kFew;
-      target = s.total;
+      target = goal;
     }
     if (border >= 0) {
       // logits of the steps up to the border's, and of the border's, with a little room
@@ -887,6 +883,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     }
   }
 
+  if constexpr (WHAT != kWholeRow) {
   if (kWhole || from_list) {  // weights, for every look at the list
     for (int i = tid; i < n; i += NT) {
       const float l = of_key(static_cast<uint32_t>(s.list[i] >> 32));
@@ -1019,6 +1016,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
            static_cast<double>(total) * per_unit);
     }
   }
+  }
   if constexpr (!kWhole) {
     if (listed) return;
     const float key_l = cut.key ? of_key(cut.key) : -INFINITY;
@@ -1032,14 +1030,12 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       // its step what the cut keeps.
       __syncthreads();
       constexpr int kVectors = kPart / E;
-      if (by_p) {
-        for (int p = tid; p < a.parts; p += NT) s.kept[p] = 0;
+      if (WHAT == kAnyRow && by_p) {
+        for (int p = tid; p < a.parts; p += NT) {
+          const int end = border - 16 * static_cast<int>(fminf(s.under[p], 63.f));
+          s.kept[p] = end > 0 ? a.part_steps[(b * a.parts + p) * kCoarse + end - 1] : 0;
+        }
         __syncthreads();
-        each_step([&](int p, int i, float under, unsigned long long w) {
-          // (a wave's steps are of one part)
-          const uint64_t sum = wave_sum(under < kCoarse && i < border - 16 * static_cast<int>(under) ? static_cast<uint64_t>(w) : 0);
-          if (lane == 0 && sum) atomicAdd(&s.kept[p], static_cast<unsigned long long>(sum));
-        });
         for (int i = tid; i < n; i += NT) {
           const uint64_t x = s.list[i];
           const uint32_t ky = static_cast<uint32_t>(x >> 32), index = static_cast<uint32_t>(x);
@@ -1139,24 +1135,34 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       sum += of[h];
     }
     if (pick(sum) != wave) return;
-    uint64_t run = 0;
+    // of the wave's vectors that with the draw, and the lane's place in front of it
+    uint64_t run = 0, before = 0, in = 0;
+    u32x4_t it = held[0];
+    int first = mine0;
+    bool found = false;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
-      const uint64_t to_here = run + wave_scan(of[h]);
-      if (to_here - of[h] <= at && at < to_here) {
-        float x[E];
-        R::wide(held[h], x);
-        const int i = (mine0 + 64 * h + lane) * E - row.off;
-        uint64_t before = to_here - of[h];
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const uint64_t y = weight(x[j], i + j);
-          if (before <= at && at < before + y)
-            done(i + j, x[j], ldexp(static_cast<double>(y), w.R - wt.R), total, total_r);
-          before += y;
-        }
+      const uint64_t to_here = run + wave_scan(of[h]), all = last_lane(to_here);
+      if (!found && all > at) {
+        found = true;
+        it = held[h];
+        first = mine0 + 64 * h;
+        before = to_here - of[h];
+        in = of[h];
       }
-      run = last_lane(to_here);
+      run = all;
+    }
+    if (found && before <= at && at < before + in) {
+      float x[E];
+      R::wide(it, x);
+      const int i = (first + lane) * E - row.off;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const uint64_t y = weight(x[j], i + j);
+        if (before <= at && at < before + y)
+          done(i + j, x[j], ldexp(static_cast<double>(y), w.R - wt.R), total, total_r);
+        before += y;
+      }
     }
   }
 }
@@ -1175,6 +1181,10 @@ bool by_parts(const srw_sample_t& d) {
   if (!d.temperature && !(d.temperature_all > 0.f)) return false;
   const bool by_p = d.top_p || d.top_p_all < 1.f, whole = d.min_p || d.min_p_all == 0.f;
   return (d.top_k || d.top_k_all == 0 || d.top_k_all >= d.V) && (by_p || whole);
+}
+// Whether no row can do otherwise, and for its sums alone.
+bool only_whole(const srw_sample_t& d) {
+  return by_parts(d) && !d.temperature && !d.top_k && !d.top_p && d.top_p_all >= 1.f && !d.min_p && d.min_p_all == 0.f;
 }
 struct Workspace {
   size_t max, sum, steps, bytes;  // offsets, and the whole
@@ -1260,9 +1270,11 @@ srw_status_t srw_sample(const srw_sample_t* d, void* workspace, size_t workspace
     using T = decltype(logit);
     if (w.bytes > 0) hipLaunchKernelGGL((srw::sample_parts_kernel<T>), parts, dim3(256), 0, s, a);
     if (d->V <= srw::kList)
-      hipLaunchKernelGGL((srw::sample_kernel<T, 256>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((srw::sample_kernel<T, 256, srw::kListRow>), grid, dim3(256), 0, s, a);
+    else if (srw::only_whole(*d))
+      hipLaunchKernelGGL((srw::sample_kernel<T, 256, srw::kWholeRow>), grid, dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((srw::sample_kernel<T, 1024>), grid, dim3(1024), 0, s, a);
+      hipLaunchKernelGGL((srw::sample_kernel<T, 1024, srw::kAnyRow>), grid, dim3(1024), 0, s, a);
   };
   if (d->dtype == SRW_F32)
     launch(float{});
