@@ -1,11 +1,12 @@
-// srw_host.cpp -- the Python side of the paged cache's calls in native code.
+// srw_host.cpp -- the Python side of the paged cache's calls, and of sampling, in
+// native code.
 //
 // For single tokens the kernels take a few microseconds, and checking a call's
 // tensors and describing it from Python takes more than that.  Here a call whose
 // tensors are as the C entry points take them is described and made in about a
 // microsecond beside its launch.  Anything else -- another type, shape, stride or
 // alignment, whether an error or a case that kv.py prepares first -- gives None
-// (False), and kv.py goes through its own checks, which say what is wrong.
+// (False), and kv.py (sampling.py) goes through its own checks, which say what is wrong.
 //
 // Tensors are looked at, nothing is kept of them; the current stream is the
 // caller's last argument.
@@ -15,6 +16,9 @@
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <cfloat>
+#include <cmath>
 
 #include "srw_amd.h"
 
@@ -206,6 +210,210 @@ PyObject* host_attention(PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// The index of pages of c: (codes, scale).
+bool index_of(PyObject* o, const srw_kv_t& c, int device, srw_kv_index_t* x) {
+  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 2) return false;
+  const at::Tensor *codes = tensor(PyTuple_GET_ITEM(o, 0)), *scale = tensor(PyTuple_GET_ITEM(o, 1));
+  if (!plain(codes, at::kChar, 3, device) || !plain(scale, at::kFloat, 2, device) || !codes->is_contiguous() ||
+      !scale->is_contiguous() || wants_grad(scale) || codes->size(0) != c.n_pages || codes->size(1) != c.n_kv_heads ||
+      codes->size(2) != c.head_dim || scale->size(0) != c.n_pages || scale->size(1) != c.n_kv_heads)
+    return false;
+  x->codes = static_cast<int8_t*>(codes->data_ptr());
+  x->scale = static_cast<float*>(scale->data_ptr());
+  return true;
+}
+
+void written(const at::Tensor* t) {
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+// index(pages, index, table, lens, cu, T, stream) -> status, or None
+PyObject* host_index(PyObject* const* a, Py_ssize_t n) {
+  srw_kv_t c{};
+  srw_kv_index_t x{};
+  int device;
+  int64_t T, stream;
+  if (n != 7 || !pages_of(a[0], &c, &device) || !index_of(a[1], c, device, &x) || !i64(a[5], &T) || !i64(a[6], &stream))
+    return none();
+  if (T < 0 || !sequences(a[2], a[3], a[4], T, device, &c)) return none();
+  const int status = srw_kv_index(&c, &x, reinterpret_cast<void*>(stream));
+  written(tensor(PyTuple_GET_ITEM(a[1], 0)));
+  written(tensor(PyTuple_GET_ITEM(a[1], 1)));
+  return PyLong_FromLong(status);
+}
+
+// select(pages, index, q, table, lens, cu, n, first, last, stream) -> keep, or None
+PyObject* host_select(PyObject* const* a, Py_ssize_t n) {
+  srw_kv_select_t s{};
+  int device;
+  int64_t most, first, last, stream;
+  if (n != 10 || !pages_of(a[0], &s.kv, &device) || !index_of(a[1], s.kv, device, &s.index) || !i64(a[6], &most) ||
+      !i64(a[7], &first) || !i64(a[8], &last) || !i64(a[9], &stream))
+    return none();
+  const at::Tensor* q = tensor(a[2]);
+  if (!plain(q, at::kBFloat16, 3, device) || wants_grad(q) || q->size(1) > kMost ||
+      !rows(q, 4, s.kv.head_dim, &s.q_token_stride, &s.q_head_stride))
+    return none();
+  if (most < 1 || most > kMost || first < 0 || first > kMost || last < 0 || last > kMost) return none();
+  const int64_t T = q->size(0);
+  if (!sequences(a[3], a[4], a[5], T, device, &s.kv)) return none();
+  s.q = q->data_ptr();
+  s.n_heads = static_cast<int32_t>(q->size(1));
+  s.n = static_cast<int32_t>(most);
+  s.first = static_cast<int32_t>(first);
+  s.last = static_cast<int32_t>(last);
+  at::Tensor keep = at::empty({T, s.kv.n_kv_heads, most}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
+  s.keep = static_cast<int32_t*>(keep.data_ptr());
+  if (srw_kv_select(&s, reinterpret_cast<void*>(stream)) != SRW_OK) return none();
+  return THPVariable_Wrap(std::move(keep));
+}
+
+// attention_kept(pages, q, table, lens, cu, scale, keep, stream) -> out, or None
+PyObject* host_attention_kept(PyObject* const* a, Py_ssize_t n) {
+  srw_attention_t s{};
+  int device;
+  int64_t stream;
+  if (n != 8 || !pages_of(a[0], &s.kv, &device) || !PyFloat_Check(a[5]) || !i64(a[7], &stream)) return none();
+  const at::Tensor *q = tensor(a[1]), *keep = tensor(a[6]);
+  if (!plain(q, at::kBFloat16, 3, device) || wants_grad(q) || q->size(1) > kMost ||
+      !rows(q, 8, s.kv.head_dim, &s.q_token_stride, &s.q_head_stride))
+    return none();
+  const int64_t T = q->size(0);
+  if (T == 0 || !plain(keep, at::kInt, 3, device) || !keep->is_contiguous() || keep->size(0) != T ||
+      keep->size(1) != s.kv.n_kv_heads || !sequences(a[2], a[3], a[4], T, device, &s.kv))
+    return none();
+  s.q = q->data_ptr();
+  s.n_heads = static_cast<int32_t>(q->size(1));
+  s.scale = static_cast<float>(PyFloat_AS_DOUBLE(a[5]));
+  const int32_t* lists = static_cast<const int32_t*>(keep->data_ptr());
+  size_t need = 0;
+  if (srw_attention_kept_workspace_size(&s, keep->size(2), &need) != SRW_OK) return none();
+  const auto opt = at::TensorOptions().device(at::kCUDA, device);
+  at::Tensor out = at::empty({T, q->size(1), s.kv.head_dim}, opt.dtype(at::kBFloat16)), ws;
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, opt.dtype(at::kByte));
+  s.out = out.data_ptr();
+  if (srw_attention_kept(&s, lists, keep->size(2), need ? ws.data_ptr() : nullptr, need,
+                         reinterpret_cast<void*>(stream)) != SRW_OK)
+    return none();
+  return THPVariable_Wrap(std::move(out));
+}
+
+// The tensors of a copy: [layers, n_pages, ...], a layer's pages contiguous.
+bool copied(PyObject* list, int device, srw_kv_copy_t* c) {
+  if (!PyList_CheckExact(list) && !PyTuple_CheckExact(list)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
+  if (n < 1 || n > SRW_KV_COPY_TENSORS) return false;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor* t = tensor(PySequence_Fast_GET_ITEM(list, i));
+    if (!t || t->dim() < 2 || !t->is_cuda() || t->get_device() != device || !t->is_contiguous() || wants_grad(t)) return false;
+    int64_t bytes = static_cast<int64_t>(t->element_size());
+    for (int64_t d = 2; d < t->dim(); ++d) bytes *= t->size(d);
+    const int64_t pages = t->size(1), stride = pages * bytes;
+    if (i == 0) {
+      c->n_layers = t->size(0);
+      c->n_src_pages = c->n_dst_pages = pages;
+    }
+    if (t->size(0) != c->n_layers || pages != c->n_src_pages) return false;
+    c->src[i] = c->dst[i] = t->data_ptr();
+    c->page_bytes[i] = bytes;
+    c->src_layer_stride[i] = c->dst_layer_stride[i] = stride;
+  }
+  c->n_tensors = static_cast<int32_t>(n);
+  return true;
+}
+
+// copy(tensors, src, dst, device, stream) -> status, or None: within contiguous tensors of the
+// current device; src and dst arrays of C ints
+PyObject* host_copy(PyObject* const* a, Py_ssize_t n) {
+  srw_kv_copy_t c{};
+  int64_t stream, device;
+  if (n != 5 || !i64(a[3], &device) || !i64(a[4], &stream) || !copied(a[0], static_cast<int>(device), &c)) return none();
+  Py_buffer src, dst;
+  if (PyObject_GetBuffer(a[1], &src, PyBUF_SIMPLE)) return none();
+  if (PyObject_GetBuffer(a[2], &dst, PyBUF_SIMPLE)) {
+    PyBuffer_Release(&src);
+    return none();
+  }
+  int status = -1;
+  if (src.len == dst.len) {
+    c.src_page = static_cast<const int32_t*>(src.buf);
+    c.dst_page = static_cast<const int32_t*>(dst.buf);
+    c.n_pairs = static_cast<int64_t>(src.len / 4);
+    status = srw_kv_copy(&c, reinterpret_cast<void*>(stream));
+  }
+  PyBuffer_Release(&src);
+  PyBuffer_Release(&dst);
+  if (status != SRW_OK) return none();  // (the general path says what is wrong)
+  if (c.n_pairs)
+    for (Py_ssize_t i = 0; i < c.n_tensors; ++i) written(tensor(PySequence_Fast_GET_ITEM(a[0], i)));
+  return PyLong_FromLong(status);
+}
+
+// A parameter of sampling: a tensor [B] of this type, or a number that its check takes.
+bool parameter(PyObject* o, at::ScalarType type, int64_t B, int device, const void** array, double* number) {
+  if (const at::Tensor* t = tensor(o)) {
+    if (!plain(t, type, 1, device) || t->size(0) != B || !t->is_contiguous() || wants_grad(t)) return false;
+    *array = t->data_ptr();
+    return true;
+  }
+  if (type == at::kInt) {
+    int64_t v;
+    if (!i64(o, &v) || v < 0 || v > kMost) return false;
+    *number = static_cast<double>(v);
+    return true;
+  }
+  if (!PyFloat_Check(o) && !PyLong_CheckExact(o)) return false;
+  *number = PyFloat_AsDouble(o);
+  return *number >= 0 && (*number <= FLT_MAX || *number == HUGE_VAL);  // (an error gives -1; inf is a temperature)
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p, device, stream) -> (tokens, logprobs), or None
+PyObject* host_sample(PyObject* const* a, Py_ssize_t n) {
+  int64_t device, stream;
+  if (n != 8 || !i64(a[6], &device) || !i64(a[7], &stream)) return none();
+  const at::Tensor *logits = tensor(a[0]), *u = tensor(a[1]);
+  if (!logits || (logits->scalar_type() != at::kFloat && logits->scalar_type() != at::kBFloat16)) return none();
+  if (!plain(logits, logits->scalar_type(), 2, static_cast<int>(device)) || wants_grad(logits)) return none();
+  const int64_t B = logits->size(0), V = logits->size(1);
+  if (V < 1 || (V > 1 && logits->stride(1) != 1)) return none();
+  if (!plain(u, at::kFloat, 1, static_cast<int>(device)) || u->size(0) != B || !u->is_contiguous() || wants_grad(u)) return none();
+  const void *t = nullptr, *k = nullptr, *p = nullptr, *m = nullptr;
+  double number[4] = {0, 0, 0, 0};
+  if (!parameter(a[2], at::kFloat, B, static_cast<int>(device), &t, &number[0]) ||
+      !parameter(a[3], at::kInt, B, static_cast<int>(device), &k, &number[1]) ||
+      !parameter(a[4], at::kFloat, B, static_cast<int>(device), &p, &number[2]) ||
+      !parameter(a[5], at::kFloat, B, static_cast<int>(device), &m, &number[3]))
+    return none();
+  const auto opt = at::TensorOptions().device(at::kCUDA, static_cast<c10::DeviceIndex>(device));
+  at::Tensor token = at::empty({B}, opt.dtype(at::kLong)), logprob = at::empty({B}, opt.dtype(at::kFloat)), ws;
+  srw_sample_t d{};
+  d.logits = logits->data_ptr();
+  d.row_stride = logits->stride(0);
+  d.B = B;
+  d.V = V;
+  d.u = static_cast<const float*>(u->data_ptr());
+  d.temperature = static_cast<const float*>(t);
+  d.top_k = static_cast<const int32_t*>(k);
+  d.top_p = static_cast<const float*>(p);
+  d.min_p = static_cast<const float*>(m);
+  d.temperature_all = static_cast<float>(number[0]);
+  d.top_k_all = static_cast<int32_t>(number[1]);
+  d.top_p_all = static_cast<float>(number[2]);
+  d.min_p_all = static_cast<float>(number[3]);
+  d.token = static_cast<int64_t*>(token.data_ptr());
+  d.logprob = static_cast<float*>(logprob.data_ptr());
+  d.dtype = logits->scalar_type() == at::kFloat ? SRW_F32 : SRW_BF16;
+  size_t need = 0;
+  if (srw_sample_workspace_size(&d, &need) != SRW_OK) return none();
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, opt.dtype(at::kByte));
+  if (srw_sample(&d, need ? ws.data_ptr() : nullptr, need, reinterpret_cast<void*>(stream)) != SRW_OK) return none();
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(token)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(logprob)));
+  return out;
+}
+
 // Nothing thrown leaves through Python's C frames: a tensor without memory of its
 // own, no memory for an output -- the general path meets it again and says so.
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
@@ -222,6 +430,11 @@ PyMethodDef methods[] = {
     {"write", reinterpret_cast<PyCFunction>(caught<host_write>), METH_FASTCALL, nullptr},
     {"read", reinterpret_cast<PyCFunction>(caught<host_read>), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(caught<host_attention>), METH_FASTCALL, nullptr},
+    {"index", reinterpret_cast<PyCFunction>(caught<host_index>), METH_FASTCALL, nullptr},
+    {"select", reinterpret_cast<PyCFunction>(caught<host_select>), METH_FASTCALL, nullptr},
+    {"attention_kept", reinterpret_cast<PyCFunction>(caught<host_attention_kept>), METH_FASTCALL, nullptr},
+    {"copy", reinterpret_cast<PyCFunction>(caught<host_copy>), METH_FASTCALL, nullptr},
+    {"sample", reinterpret_cast<PyCFunction>(caught<host_sample>), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_srw_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -325,6 +325,10 @@ def kv_copy(tensors, src, dst, *, to=None) -> None:
         raise ValueError("src and dst name pages") from None
     if len(src) != len(dst):
         raise ValueError(f"{len(src)} pages to read and {len(dst)} to write")
+    if to is None and isinstance(a[0], torch.Tensor) and a[0].is_cuda:
+        at = _current_device()
+        if (_host or _native()).copy(a, src, dst, at, _raw_stream(at)) is not None:
+            return
     shape = None
     at, size, strides = ([], []), [], ([], [])
     for x, y in zip(a, b):
@@ -380,6 +384,10 @@ def kv_index(pages: KvPages, index: KvIndex, table, lens, cu=None, *, total=None
         T = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() else -1
         if cu is not None and isinstance(table, torch.Tensor) and table.dim() == 2:
             T *= table.shape[1] * pages.page_size
+    if _current_device() == pages.device.index:
+        status = (_host or _native()).index(pages._t, index._t, table, lens, cu, T, _raw_stream(pages.device.index))
+        if status is not None:
+            return C.check(status)
     at = index._at(pages)
     a = _address(pages, table, lens, cu, T)
     C.check(_call(C.load_library().srw_kv_index, pages.device, _KV.pack(*a), _INDEX.pack(*at)))
@@ -395,6 +403,11 @@ def kv_select(q, pages: KvPages, index: KvIndex, table, lens, cu=None, *, n: int
     scores, equal ones from the front.  A page's score is the product of its mean key
     and the sum of the queries of the heads that read the key head, both in 8 bits: a
     whole number times the page's scale.  Pages whose index is NaN come first."""
+    if _current_device() == pages.device.index:
+        got = (_host or _native()).select(pages._t, index._t, q, table, lens, cu, n, first, last,
+                                          _raw_stream(pages.device.index))
+        if got is not None:
+            return got
     for name, x in (("n", n), ("first", first), ("last", last)):
         if not hasattr(x, "__index__"):
             raise TypeError(f"{name} is a whole number; got {x!r}")
@@ -431,9 +444,14 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
     rows, heads and the table's width: a sequence's outputs are the same bit for
     bit in calls that agree in these, and within these roundings in any."""
     scale = pages.head_dim ** -0.5 if scale is None else float(scale)
-    if keep is None and out is None and _current_device() == pages.device.index:
-        got = (_host or _native()).attention(pages._t, q, table, lens, cu, max_new, scale, window, sinks,
-                                             _raw_stream(pages.device.index))
+    if out is None and _current_device() == pages.device.index:
+        stream = _raw_stream(pages.device.index)
+        if keep is None:
+            got = (_host or _native()).attention(pages._t, q, table, lens, cu, max_new, scale, window, sinks, stream)
+        elif type(window) is int is type(sinks) and window == sinks == 0 and max_new >= 0:
+            got = (_host or _native()).attention_kept(pages._t, q, table, lens, cu, scale, keep, stream)
+        else:
+            got = None
         if got is not None:
             return got
     T = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else -1

@@ -11,7 +11,8 @@ import struct
 import torch
 
 from . import _capi as C
-from .kv import _call, _no_grad, _tensor
+from . import kv
+from .kv import _call, _current_device, _no_grad, _raw_stream, _tensor
 
 __all__ = ["sample"]
 
@@ -57,10 +58,17 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     above 0 as off, a min_p above 1 as 1.  u outside of [0, 1) counts as the nearest
     number inside (NaN as 0).
 
-    Weights are summed as whole numbers in units of 2^-51 or, of large vocabularies,
-    2^62 / vocab: a row's token goes by its own numbers alone, not by the batch."""
+    Weights are summed as whole numbers, in units of 2^-51 to 2^-50 of the largest (of
+    more than 2048 logits so that the sum stays below 2^62), and top-p's border and the
+    token are exact in these: a row's token goes by its own numbers alone, not by the
+    batch."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be a tensor [B, vocab]")
+    if logits.is_cuda:
+        at = _current_device()
+        got = (kv._host or kv._native()).sample(logits, u, temperature, top_k, top_p, min_p, at, _raw_stream(at))
+        if got is not None:
+            return got
     dev = logits.device
     if dev.type != "cuda":
         raise ValueError(f"logits live on a HIP device; got {dev}")
