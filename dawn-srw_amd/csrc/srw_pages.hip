@@ -279,9 +279,15 @@ __global__ __launch_bounds__(256) void kv_index_kernel(KvView p, int8_t* codes, 
 //
 // A workgroup takes R tokens of a sequence and one key head; the threads score pages
 // (whole numbers by dot products of four codes, one page a thread and step), as keys
-// that order like the scores, into LDS; 256 / R threads then find each row's border by
-// digits of the keys and write the places that lie before it.  Tables of more pages
-// than LDS holds keys are scored again for each digit.
+// that order like the scores, into LDS; NT / R threads then find each row's border and
+// write the places that lie before it.  The border: a histogram of the scores between
+// their smallest and largest, then, of the bin that it falls into, each key's number of
+// larger ones.  Where that bin holds more than 64 keys (many equal scores), and for
+// tables of more pages than LDS holds keys, which are scored again each time, the border
+// comes by digits of the keys.
+//
+// Bound by the chain of loads (lengths, table, codes), by barriers and, for few rows over
+// many pages, by one CU's share of the codes' reads.
 
 struct SelectArgs {
   KvView kv;
@@ -301,13 +307,26 @@ __device__ inline uint32_t key_of(float score) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <int DH, int R>
-__global__ __launch_bounds__(256) void kv_select_kernel(SelectArgs a) {
-  constexpr int kRow = 256 / R;  // threads of a row
+__device__ inline float score_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+constexpr int kBinKeys = 64;
+constexpr int64_t kKeys = 12288;  // of a workgroup in LDS: 48 KB
+
+// x of the lane that C names within each four (quad_perm), all lanes active.
+template <int C>
+__device__ inline int dpp(int x) {
+  return __builtin_amdgcn_mov_dpp(x, C, 0xf, 0xf, false);
+}
+
+template <int DH, int R, int NT>
+__global__ __launch_bounds__(NT) void kv_select_kernel(SelectArgs a) {
+  constexpr int kRow = NT / R;        // threads of a row
+  constexpr int kWaves = kRow / 64;
   extern __shared__ uint32_t keys[];  // [R][hold]
   __shared__ __align__(16) uint32_t qc[R][DH / 4];
-  __shared__ uint32_t most[R], hist[R][256], found[R][2];  // found: the digit, what lies before it
-  __shared__ uint64_t above[R][kRow / 64], equal[R][kRow / 64];
+  __shared__ uint32_t hist[R][256], bin[R][kBinKeys], binned[R], ends[R][kWaves][2];
   const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
   const KvView& p = a.kv;
   int64_t b, at;
@@ -325,47 +344,6 @@ __global__ __launch_bounds__(256) void kv_select_kernel(SelectArgs a) {
   if (at < 0 || at * R >= sq.n) return;
   const int toks = sq.n - tok0 < R ? sq.n - tok0 : R;
 
-  // the rows' codes
-  if (tid < R) most[tid] = 0;
-  __syncthreads();
-  constexpr int kEach = R * DH / 4 > 256 ? R * DH / 4 / 256 : 1;  // times four dims a thread
-  float x[kEach][4];
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = tid + 256 * e, r = i / (DH / 4), c = i % (DH / 4);
-    if (r < toks) {
-      double s[4] = {0.0, 0.0, 0.0, 0.0};
-      const uint16_t* src = a.q + (sq.row0 + tok0 + r) * a.q_token + static_cast<int64_t>(head) * a.G * a.q_head + 4 * c;
-      for (int g = 0; g < a.G; ++g) {
-        const uint2 w = *reinterpret_cast<const uint2*>(src + g * a.q_head);
-        s[0] += static_cast<double>(lo_f32(w.x));
-        s[1] += static_cast<double>(hi_f32(w.x));
-        s[2] += static_cast<double>(lo_f32(w.y));
-        s[3] += static_cast<double>(hi_f32(w.y));
-      }
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[e][j] = static_cast<float>(s[j]);
-        const uint32_t v = __float_as_uint(x[e][j]) & 0x7fffffffu;
-        m = v > m ? v : m;
-      }
-      atomicMax(&most[r], m);
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = tid + 256 * e, r = i / (DH / 4), c = i % (DH / 4);
-    if (r < toks) {
-      const float inv = code_factor(most[r]);
-      qc[r][c] = code_of(x[e][0], inv) | code_of(x[e][1], inv) << 8 | code_of(x[e][2], inv) << 16 | code_of(x[e][3], inv) << 24;
-    } else if (r < R) {
-      qc[r][c] = 0;
-    }
-  }
-  __syncthreads();
-
   // pages that a row sees: [0, own]
   auto own_of = [&](int r) {
     const int pos = sq.len - sq.n + tok0 + r;
@@ -374,100 +352,254 @@ __global__ __launch_bounds__(256) void kv_select_kernel(SelectArgs a) {
     return pos >> p.logP < most_pages ? pos >> p.logP : most_pages - 1;
   };
   const int pages = own_of(toks - 1) + 1;
+
+  auto id_of = [&](int j) { return j < pages ? kv_page(p, b, j << p.logP) : -1; };
+  // the rows' codes: DH / 4 lanes a row, four dims a lane
+  const int qr = tid / (DH / 4), qd = tid % (DH / 4);
+  double x[4] = {0.0, 0.0, 0.0, 0.0};
+  const bool reads = qr < toks && qr < R;
+  const uint16_t* src =
+      a.q + (sq.row0 + tok0 + (reads ? qr : 0)) * a.q_token + static_cast<int64_t>(head) * a.G * a.q_head + 4 * qd;
+  constexpr int kHeads = 8;  // loads in flight
+  uint2 w[kHeads];
+#pragma unroll
+  for (int g = 0; g < kHeads; ++g) w[g] = reads && g < a.G ? *reinterpret_cast<const uint2*>(src + g * a.q_head) : uint2{0, 0};
+  int id = id_of(tid);
+  if (tid < R) binned[tid] = 0;
+  for (int i = tid; i < R * 256; i += NT) hist[0][i] = 0;
+  for (int g0 = 0;;) {
+#pragma unroll
+    for (int g = 0; g < kHeads; ++g) {
+      x[0] += static_cast<double>(lo_f32(w[g].x));
+      x[1] += static_cast<double>(hi_f32(w[g].x));
+      x[2] += static_cast<double>(lo_f32(w[g].y));
+      x[3] += static_cast<double>(hi_f32(w[g].y));
+    }
+    g0 += kHeads;
+    if (g0 >= a.G) break;
+#pragma unroll
+    for (int g = 0; g < kHeads; ++g)
+      w[g] = reads && g0 + g < a.G ? *reinterpret_cast<const uint2*>(src + (g0 + g) * a.q_head) : uint2{0, 0};
+  }
+  if (qr < R) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t m = __float_as_uint(static_cast<float>(x[j])) & 0x7fffffffu;
+      most = m > most ? m : most;
+    }
+#pragma unroll
+    for (int o = 1; o < DH / 4; o <<= 1) {
+      const uint32_t m = __shfl_xor(most, o);
+      most = m > most ? m : most;
+    }
+    const float inv = code_factor(most);
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c |= code_of(static_cast<float>(x[j]), inv) << 8 * j;
+    qc[qr][qd] = c;
+  }
+  __syncthreads();
+
+  // A wave scores 64 places, four lanes a page (a page a lane would touch each line of its
+  // codes DH / 16 times): lane l of a quad loads 16 of every 64 dims of the quad's four
+  // pages and ends up with the sum of the page of place l.
+  constexpr int C = DH / 64;
+  const int part = lane & 3;
   auto score = [&](int from) {  // keys of places [from, from + hold)
     const int to = pages - from < a.hold ? pages - from : a.hold;
-    for (int i = tid; i < ((to + 63) & ~63); i += 256) {
-      const int j = from + i;
-      const int page = i < to ? kv_page(p, b, j << p.logP) : -1;
-      int dot[R];
+    if (pages > a.hold) id = id_of(from + tid);
+    for (int i = tid; i < ((to + 63) & ~63); i += NT) {
+      const int j = from + i, next = i + NT < to ? id_of(j + NT) : -1;
+      int dot[R][4];
+      float scale = 0.f;
+      if (p.n_pages > 0) {
+        scale = a.scale[static_cast<int64_t>(id > 0 ? id : 0) * p.H + head];
+        u32x4_t w[4][C];
 #pragma unroll
-      for (int r = 0; r < R; ++r) dot[r] = 0;
-      float sc = 0.f;
-      if (page >= 0) {
-        const int64_t ph = static_cast<int64_t>(page) * p.H + head;
-        const u32x4_t* src = reinterpret_cast<const u32x4_t*>(a.codes + ph * DH);
-        u32x4_t w[DH / 16];
+        for (int u = 0; u < 4; ++u) {
+          const int other = u == 0 ? dpp<0x00>(id) : u == 1 ? dpp<0x55>(id) : u == 2 ? dpp<0xaa>(id) : dpp<0xff>(id);
+          const u32x4_t* src = reinterpret_cast<const u32x4_t*>(
+              a.codes + (static_cast<int64_t>(other > 0 ? other : 0) * p.H + head) * DH);
 #pragma unroll
-        for (int c = 0; c < DH / 16; ++c) w[c] = src[c];
-        sc = a.scale[ph];
+          for (int c = 0; c < C; ++c) w[u][c] = src[4 * c + part];
+        }
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
 #pragma unroll
-          for (int c = 0; c < DH / 16; ++c) {
-            const u32x4_t y = *reinterpret_cast<const u32x4_t*>(&qc[r][4 * c]);
+          for (int u = 0; u < 4; ++u) dot[r][u] = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              dot[r] = __builtin_amdgcn_sdot4(static_cast<int>(w[c][e]), static_cast<int>(y[e]), dot[r], false);
+          for (int c = 0; c < C; ++c) {
+            const u32x4_t y = *reinterpret_cast<const u32x4_t*>(&qc[r][16 * c + 4 * part]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                dot[r][u] = __builtin_amdgcn_sdot4(static_cast<int>(w[u][c][e]), static_cast<int>(y[e]), dot[r][u], false);
           }
+        }
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        const bool two = part & 2, one = part & 1;
+        const int d0 = (two ? dot[r][2] : dot[r][0]) + dpp<0x4e>(two ? dot[r][0] : dot[r][2]);
+        const int d1 = (two ? dot[r][3] : dot[r][1]) + dpp<0x4e>(two ? dot[r][1] : dot[r][3]);
+        const int sum = (one ? d1 : d0) + dpp<0xb1>(one ? d0 : d1);
         const int own = own_of(r);
         uint32_t key = 0;
-        if (page >= 0 && j <= own)
-          key = j < a.first || j > own - a.last ? kAlways : key_of(static_cast<float>(dot[r]) * sc);
+        if (id >= 0 && j <= own)
+          key = j < a.first || j > own - a.last ? kAlways : key_of(static_cast<float>(sum) * scale);
         keys[r * a.hold + i] = key;
       }
+      id = next;
     }
   };
 
   const int r = tid / kRow, t = tid % kRow;
   const uint32_t* row = keys + r * a.hold;
+  // the bin of the 256, in order, in which `left` falls, and what lies before it; -1: all
+  // fall short of it
+  auto find = [&](uint32_t left, uint32_t* before, uint32_t* count) {
+    uint32_t c[4], s = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      c[k] = hist[r][4 * lane + k];
+      s += c[k];
+    }
+    uint32_t run = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t v = __shfl_up(run, o);
+      if (lane >= o) run += v;
+    }
+    const uint64_t past = __ballot(run >= left);
+    if (!past) return -1;
+    uint32_t at = run - s, n = c[0];
+    int k = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (k == i && at + c[i] < left) {
+        at += c[i];
+        n = c[i + 1];
+        k = i + 1;
+      }
+    const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+    *before = __builtin_amdgcn_readlane(at, l);
+    *count = __builtin_amdgcn_readlane(n, l);
+    return 4 * l + __builtin_amdgcn_readlane(k, l);
+  };
   // the border: keys above K, and as many equal to it as are left
   uint32_t K = 0, left = a.n;
   const bool held = pages <= a.hold;
-  if (held) score(0);
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = t; i < 256; i += kRow) hist[r][i] = 0;
+  bool digits = !held;
+  if (held) {
+    score(0);
     __syncthreads();
-    for (int from = 0; from < pages; from += a.hold) {
-      if (!held) {
-        score(from);
-        __syncthreads();
+  }
+  if (pages <= a.n) {
+    left = 0;
+    digits = false;
+  } else if (held) {
+    uint32_t lo = kAlways, hi = 0;  // of finite scores
+    for (int i = t; i < pages; i += kRow) {
+      const uint32_t key = row[i];
+      if (key > 0x007fffffu && key < 0xff800000u) {
+        lo = key < lo ? key : lo;
+        hi = key > hi ? key : hi;
       }
-      const int to = pages - from < a.hold ? pages - from : a.hold;
-      for (int i = t; i < to; i += kRow) {
-        const uint32_t key = row[i];
-        if (shift == 24 || key >> (shift + 8) == K >> (shift + 8)) atomicAdd(&hist[r][255 - (key >> shift & 255)], 1u);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t l = __shfl_xor(lo, o), h = __shfl_xor(hi, o);
+      lo = l < lo ? l : lo;
+      hi = h > hi ? h : hi;
+    }
+    if constexpr (kWaves > 1) {
+      if (lane == 0) {
+        ends[r][t >> 6][0] = lo;
+        ends[r][t >> 6][1] = hi;
       }
       __syncthreads();
+      lo = ends[r][lane % kWaves][0];
+      hi = ends[r][lane % kWaves][1];
+#pragma unroll
+      for (int o = 1; o < kWaves; o <<= 1) {
+        const uint32_t l = __shfl_xor(lo, o), h = __shfl_xor(hi, o);
+        lo = l < lo ? l : lo;
+        hi = h > hi ? h : hi;
+      }
     }
-    if (t < 64) {
-      uint32_t c[4], s = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        c[k] = hist[r][4 * lane + k];
-        s += c[k];
-      }
-      uint32_t run = s;
-#pragma unroll
-      for (int w = 1; w < 64; w <<= 1) {
-        const uint32_t o = __shfl_up(run, w);
-        if (lane >= w) run += o;
-      }
-      if (lane == 63 && run < left) {  // fewer than that: all
-        found[r][0] = 255;
-        found[r][1] = run - c[3];
-      }
-      uint32_t before = run - s;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (before < left && before + c[k] >= left) {
-          found[r][0] = 4 * lane + k;
-          found[r][1] = before;
-        }
-        before += c[k];
-      }
+    const float low = 0.5f * score_of(lo), wide = 0.5f * score_of(hi) - low;
+    float to_bin = 253.f / wide;
+    if (!(hi > lo) || !(to_bin < 1e38f)) to_bin = 0.f;
+    // a larger key's bin is no later: each rounding keeps the order
+    auto bin_of = [&](uint32_t key) {
+      if (key >= kAlways - 1) return static_cast<int>(kAlways - key);
+      const float y = (0.5f * score_of(key) - low) * to_bin;
+      return 255 - (y >= 253.f ? 253 : y > 0.f ? static_cast<int>(y) : 0);
+    };
+    for (int i = t; i < pages; i += kRow) {
+      const uint32_t key = row[i];
+      if (key) atomicAdd(&hist[r][bin_of(key)], 1u);
     }
     __syncthreads();
-    K |= (255 - found[r][0]) << shift;
-    left -= found[r][1];
+    uint32_t before = 0, count = 0;
+    const int border = find(left, &before, &count);
+    if (border < 0) {
+      left = 0;
+    } else if (count > kBinKeys) {
+      digits = true;
+    } else {
+      for (int i = t; i < pages; i += kRow) {
+        const uint32_t key = row[i];
+        if (key && bin_of(key) == border) bin[r][atomicAdd(&binned[r], 1u)] = key;
+      }
+    }
+    digits = __syncthreads_or(digits);
+    if (border >= 0 && count <= kBinKeys) {
+      const uint32_t mine = lane < static_cast<int>(count) ? bin[r][lane] : 0;
+      uint32_t more = before, same = 0;
+      for (uint32_t i = 0; i < count; ++i) {
+        const uint32_t o = __builtin_amdgcn_readlane(mine, i);
+        more += o > mine;
+        same += o == mine;
+      }
+      const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(mine && more < left && more + same >= left)));
+      K = __builtin_amdgcn_readlane(mine, l);
+      left -= __builtin_amdgcn_readlane(more, l);
+    }
   }
-  // write: runs of places in order
+  if (digits) {
+    K = 0;
+    left = a.n;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      __syncthreads();
+      for (int i = t; i < 256; i += kRow) hist[r][i] = 0;
+      __syncthreads();
+      for (int from = 0; from < pages; from += a.hold) {
+        if (!held) {
+          score(from);
+          __syncthreads();
+        }
+        const int to = pages - from < a.hold ? pages - from : a.hold;
+        for (int i = t; i < to; i += kRow) {
+          const uint32_t key = row[i];
+          if (shift == 24 || key >> (shift + 8) == K >> (shift + 8)) atomicAdd(&hist[r][255 - (key >> shift & 255)], 1u);
+        }
+        __syncthreads();
+      }
+      // (places without a page count too: there are more pages than are kept)
+      uint32_t before = 0, count = 0;
+      const int digit = find(left, &before, &count);
+      K |= static_cast<uint32_t>(255 - digit) << shift;
+      left -= before;
+    }
+  }
+  // write: a wave the places of a run of its own, in order
   const int tok = tok0 + r;
-  int32_t* out = a.keep + ((sq.row0 + (r < toks ? tok : 0)) * p.H + head) * a.n;
-  int written = 0;
   const bool mine = r < toks;
+  int32_t* out = a.keep + ((sq.row0 + (mine ? tok : 0)) * p.H + head) * a.n;
+  uint32_t more = 0, same = 0;  // before the run
   for (int from = 0; from < pages; from += a.hold) {
     if (!held) {
       __syncthreads();
@@ -475,50 +607,56 @@ __global__ __launch_bounds__(256) void kv_select_kernel(SelectArgs a) {
       __syncthreads();
     }
     const int to = pages - from < a.hold ? pages - from : a.hold;
-    for (int i0 = 0; i0 < to; i0 += kRow) {
-      const uint32_t key = i0 + t < to ? row[i0 + t] : 0;
-      const uint64_t ab = __ballot(key > K), eq = __ballot(key != 0 && key == K);
-      if constexpr (kRow > 64) {
-        if (lane == 0) {
-          above[r][t >> 6] = ab;
-          equal[r][t >> 6] = eq;
-        }
-        __syncthreads();
+    const int run = (to + kRow - 1) / kRow * 64, i0 = t / 64 * run, i1 = i0 + run < to ? i0 + run : to;
+    uint32_t m = 0, e = 0;  // kept for sure, and equal to the border, in the run
+    for (int i = i0; i < i1; i += 64) {
+      const uint32_t key = i + lane < i1 ? row[i + lane] : 0;
+      m += __popcll(__ballot(key > K));
+      e += __popcll(__ballot(key != 0 && key == K));
+    }
+    uint32_t all_m = m, all_e = e;
+    if constexpr (kWaves > 1) {
+      if (lane == 0) {
+        ends[r][t >> 6][0] = m;
+        ends[r][t >> 6][1] = e;
       }
-      int base = written;
-      uint32_t l = left;
-      uint64_t keep = 0;
+      __syncthreads();
+      m = lane < kWaves ? ends[r][lane % kWaves][0] : 0;
+      e = lane < kWaves ? ends[r][lane % kWaves][1] : 0;
+      uint32_t sm = m, se = e;
 #pragma unroll
-      for (int w = 0; w < kRow / 64; ++w) {
-        const uint64_t wa = kRow > 64 ? above[r][w] : ab, we = kRow > 64 ? equal[r][w] : eq;
-        const uint32_t e = static_cast<uint32_t>(__popcll(we));
-        uint64_t k = wa;
-        if (e <= l) {
-          k |= we;
-          l -= e;
-        } else {
-          uint64_t rest = we;
-          for (; l > 0; --l) {
-            k |= rest & -rest;
-            rest &= rest - 1;
-          }
+      for (int o = 1; o < kWaves; o <<= 1) {
+        const uint32_t vm = __shfl_up(sm, o), ve = __shfl_up(se, o);
+        if (lane >= o) {
+          sm += vm;
+          se += ve;
         }
-        if (w == t >> 6) {
-          keep = k;
-          base = written;
-        }
-        written += __popcll(k);
       }
-      left = l;
-      if (mine && (keep >> lane & 1)) {
-        const int o = base + __popcll(keep & ((1ull << lane) - 1));
-        if (o < a.n) out[o] = from + i0 + t;
-      }
-      if constexpr (kRow > 64) __syncthreads();
+      all_m = __shfl(sm, kWaves - 1);
+      all_e = __shfl(se, kWaves - 1);
+      m = __shfl(sm - m, t >> 6);
+      e = __shfl(se - e, t >> 6);
+      __syncthreads();
+    } else {
+      m = e = 0;
+    }
+    m += more;
+    e += same;
+    more += all_m;
+    same += all_e;
+    for (int i = i0; i < i1; i += 64) {
+      const uint32_t key = i + lane < i1 ? row[i + lane] : 0;
+      const uint64_t ab = __ballot(key > K), eq = __ballot(key != 0 && key == K), before = (1ull << lane) - 1;
+      const uint32_t em = e + __popcll(eq & before);
+      const uint32_t o = m + __popcll(ab & before) + (em < left ? em : left);
+      if (mine && o < static_cast<uint32_t>(a.n) && ((ab >> lane & 1) || ((eq >> lane & 1) && em < left)))
+        out[o] = from + i + lane;
+      m += __popcll(ab);
+      e += __popcll(eq);
     }
   }
   if (mine)
-    for (int o = written + t; o < a.n; o += kRow) out[o] = -1;
+    for (int o = static_cast<int>(more + (same < left ? same : left)) + t; o < a.n; o += kRow) out[o] = -1;
 }
 
 template <int DH>
@@ -535,16 +673,25 @@ hipError_t launch_select(const srw_kv_select_t& c, hipStream_t s) {
   a.n = c.n;
   a.first = c.first;
   a.last = c.last;
-  const int R = c.kv.cu ? 4 : 1;
-  const int64_t most = 12288 / R, width = (c.kv.table_width + 63) / 64 * 64;
+  // Four rows share the codes' loads where LDS holds the keys of all four: 5 new tokens of
+  // 32 sequences over 500 pages 18 us (one row a workgroup: five times the 8.1 of a single
+  // token at most), but over 4000, scored anew for each digit, 391 us.
+  const int R = c.kv.cu && c.kv.table_width <= kKeys / 4 ? 4 : 1;
+  // 256 threads, or 512 where a thread would take more than two pages: one row of 8 heads
+  // over 64 | 500 | 1563 | 11000 pages 6.0 | 7.7 | 13.2 | 57 us with 256, 6.2 | 7.3 | 10.8 |
+  // 34 with 512 (1024: 8.3 | 9.0 | 11.6 | 31); 256 rows over 500 | 1000 31 | 72 and 37 | 74.
+  const bool wide = c.kv.table_width > 512;
+  const int64_t most = kKeys / R, width = (c.kv.table_width + 63) / 64 * 64;
   a.hold = static_cast<int>(width < 64 ? 64 : width < most ? width : most);
   const int64_t tiles = c.kv.cu ? c.kv.T / R + c.kv.B : c.kv.B;
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(c.kv.n_kv_heads));
   const unsigned lds = static_cast<unsigned>(a.hold) * R * 4;
-  if (R == 1)
-    hipLaunchKernelGGL((kv_select_kernel<DH, 1>), grid, dim3(256), lds, s, a);
+  if (R == 4)
+    hipLaunchKernelGGL((kv_select_kernel<DH, 4, 256>), grid, dim3(256), lds, s, a);
+  else if (wide)
+    hipLaunchKernelGGL((kv_select_kernel<DH, 1, 512>), grid, dim3(512), lds, s, a);
   else
-    hipLaunchKernelGGL((kv_select_kernel<DH, 4>), grid, dim3(256), lds, s, a);
+    hipLaunchKernelGGL((kv_select_kernel<DH, 1, 256>), grid, dim3(256), lds, s, a);
   return hipGetLastError();
 }
 
@@ -604,7 +751,7 @@ srw_status_t srw_kv_select(const srw_kv_select_t* c, void* stream) {
       static_cast<int64_t>(c->first) + c->last > c->n)
     return SRW_EINVAL;
   if (c->kv.T == 0) return SRW_OK;
-  if (c->kv.T > (1 << 25)) return SRW_EUNSUPPORTED;  // (a launch has under 2^32 threads)
+  if (c->kv.T + c->kv.B > (1 << 22)) return SRW_EUNSUPPORTED;  // (a launch has under 2^32 threads)
   if (!srw::aligned(c->q, 8) || !srw::aligned(c->keep, 4) || c->q_token_stride < 0 || c->q_head_stride < 0 ||
       c->q_token_stride % 4 || c->q_head_stride % 4)
     return SRW_EINVAL;
