@@ -168,6 +168,32 @@ __device__ inline uint32_t code_of(float x, float inv) {
   return static_cast<uint32_t>(static_cast<int>(rintf(inv == 0.f ? 0.f : x * inv))) & 0xffu;
 }
 
+// a's sum over the two halves (W 32; 16: over each half's two rows) in the lower one, b's
+// in the upper one.
+template <int W>
+__device__ inline double traded(double a, double b) {
+  const uint64_t x = __builtin_bit_cast(uint64_t, a), y = __builtin_bit_cast(uint64_t, b);
+  auto trade = [](uint32_t u, uint32_t v) {
+    if constexpr (W == 32)
+      return __builtin_amdgcn_permlane32_swap(u, v, false, false);
+    else
+      return __builtin_amdgcn_permlane16_swap(u, v, false, false);
+  };
+  const auto lo = trade(static_cast<uint32_t>(x), static_cast<uint32_t>(y));
+  const auto hi = trade(static_cast<uint32_t>(x >> 32), static_cast<uint32_t>(y >> 32));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) +
+         __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+}
+// x of the lane W further on in the row of 16, around its end.
+template <int W>
+__device__ inline double turned(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  auto turn = [](uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x120 | W, 0xf, 0xf, false));
+  };
+  return __builtin_bit_cast(double, static_cast<uint64_t>(turn(static_cast<uint32_t>(u >> 32))) << 32 | turn(static_cast<uint32_t>(u)));
+}
+
 // One wave: a page and head.  A lane holds 16 bytes' dims of every (64 / lanes a
 // key)th key and sums them in 64 bits, where sums of up to 256 keys of any 8-bit or
 // bf16 page are exact but for rare exponents far apart, so that the codes do not go by
@@ -245,33 +271,39 @@ __global__ __launch_bounds__(256) void kv_index_kernel(KvView p, int8_t* codes, 
       }
     }
   }
-  float mean[N];
+  // the keys' lanes join: halves, then rows of 16, trade half of their dims, so that a lane
+  // ends with the sums of D of them; lanes of a row that hold the same dims add in turn
+  constexpr int D = N / 4;
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j) sum[j] = traded<32>(sum[j], sum[j + N / 2]);
+#pragma unroll
+  for (int j = 0; j < D; ++j) sum[j] = traded<16>(sum[j], sum[j + D]);
+  float mean[D];
   uint32_t most = 0;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-#pragma unroll
-    for (int w = kLanes; w < 64; w <<= 1) sum[j] += __shfl_xor(sum[j], w);
+  for (int j = 0; j < D; ++j) {
+    if constexpr (kLanes <= 8) sum[j] += turned<8>(sum[j]);
+    if constexpr (kLanes <= 4) sum[j] += turned<4>(sum[j]);
     mean[j] = static_cast<float>(sum[j] / have);
     const uint32_t m = __float_as_uint(mean[j]) & 0x7fffffffu;
     most = m > most ? m : most;
   }
 #pragma unroll
-  for (int w = 1; w < kLanes; w <<= 1) {
+  for (int w = 1; w < 64; w <<= 1) {
+    if (w >= kLanes && w < 16) continue;
     const uint32_t o = __shfl_xor(most, w);
     most = o > most ? o : most;
   }
-  if (lane >= kLanes) return;
+  if ((lane & 15) >= kLanes) return;
   const float inv = code_factor(most), m = __uint_as_float(most);
-  uint32_t c[N / 4];
+  uint32_t c = 0;
 #pragma unroll
-  for (int j = 0; j < N / 4; ++j)
-    c[j] = code_of(mean[4 * j], inv) | code_of(mean[4 * j + 1], inv) << 8 | code_of(mean[4 * j + 2], inv) << 16 |
-           code_of(mean[4 * j + 3], inv) << 24;
-  char* dst = reinterpret_cast<char*>(codes) + ph * DH + lane * N;
-  if constexpr (N == 8)
-    *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
+  for (int j = 0; j < D; ++j) c |= code_of(mean[j], inv) << 8 * j;
+  char* dst = reinterpret_cast<char*>(codes) + ph * DH + (lane & 15) * N + (lane >> 5) * (N / 2) + (lane >> 4 & 1) * D;
+  if constexpr (D == 4)
+    *reinterpret_cast<uint32_t*>(dst) = c;
   else
-    *reinterpret_cast<uint4*>(dst) = make_uint4(c[0], c[1], c[2], c[3]);
+    *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(c);
   if (lane == 0) scale[ph] = not_finite(most) ? __uint_as_float(0x7fc00000u) : inv == 0.f ? 0.f : m / 127.f;
 }
 
