@@ -29,8 +29,9 @@ import torch
 import torch.nn.functional as F
 
 from . import _capi as C
-from .kv import PagedKvCache, _check_window, kv_write, paged_attention
+from .kv import PagedKvCache, _check_window, kv_index, kv_select, kv_write, paged_attention
 from .layer import GateConfig, SrwBatchPlan, SrwPlan
+from .sampling import sample
 from .srw import chunk_plan
 
 __all__ = ["DawnConfig", "init_params", "DawnModel"]
@@ -399,30 +400,38 @@ class DawnModel:
         return x @ self.p["token_emb"]["embedding"].T, cache_K, cache_V, cache_len + 1
 
     # -- serving sequences of different lengths --------------------------------
-    def new_cache(self, n_pages: int, *, page_size: int = 64, dtype=BF16) -> PagedKvCache:
+    def new_cache(self, n_pages: int, *, page_size: int = 64, dtype=BF16, indexed: bool = False) -> PagedKvCache:
         """Pages for the keys and values of all layers (d_head 64 or 128), shared
         by any number of sequences; ``dtype`` bfloat16 holds what the pools
-        give exactly, int8 and float8_e4m3fn half of the bytes."""
+        give exactly, int8 and float8_e4m3fn half of the bytes.  ``indexed``: with
+        the index that ``keep`` of :meth:`extend` chooses pages by."""
         cfg = self.cfg
         return PagedKvCache(cfg.n_layers, n_pages, cfg.n_heads, cfg.d_model // cfg.n_heads, page_size=page_size,
-                            dtype=dtype, device=self.device)
+                            dtype=dtype, device=self.device, indexed=indexed)
 
     @torch.no_grad()
     def extend(self, ids, cache: PagedKvCache, seqs, counts, *, window: int = 0, sinks: int = 0,
-               last_only: bool = False):
+               last_only: bool = False, keep: int = 0, first: int = 1, last: int = 1):
         """counts[i] new tokens of each sequence seqs[i] of the cache -- chunks
         of prompts and single generated tokens in one batch: ``ids`` [sum of
         counts] holds them one sequence after the other.  Logits [T, vocab] of
         the new tokens, or with ``last_only`` [len(seqs), vocab] of each
         sequence's last (every count at least 1).  A token at position i
         attends to positions j <= i of its sequence, with ``window`` to those
-        with j > i - window or j < ``sinks``.  Same model as :meth:`prefill` and
+        with j > i - window or j < ``sinks``, with ``keep`` to those in the pages that
+        :func:`kv_select` chooses for the token and each head of each layer: of at most
+        keep the ``first`` and ``last`` ones and the best others (for few new tokens of
+        long sequences in an indexed cache; every call brings the index up to date).  Same model as :meth:`prefill` and
         :meth:`decode_step` (the SRW layer as ``_srw_inference`` in bf16): the
         cache holds the pools' outputs, the pool scales go into the attention's
         scale and its result.  Whatever it raises, the cache's sequences are as
         before the call."""
         cfg = self.cfg
         _check_window(window, sinks)
+        if keep and (window or not cache.indexed):
+            raise ValueError("keep needs an indexed cache and goes without a window")
+        if keep and not (first >= 0 and last >= 1 and first + last <= keep):
+            raise ValueError("first is not negative, last at least 1, and keep holds both")
         ids = ids.reshape(-1).to(self.device)
         counts = [int(n) for n in counts]
         T = sum(counts)
@@ -438,12 +447,13 @@ class DawnModel:
         place = [cache.length(q) + i for q, n in zip(seqs, counts) for i in range(n)]
         call = cache.extend(seqs, counts)
         try:
-            return self._extend(ids, place, cache, counts, call, window, sinks, last_only)
+            return self._extend(ids, place, cache, counts, call, window, sinks, last_only,
+                                dict(n=keep, first=first, last=last) if keep else None)
         except BaseException:
             cache._take_back(seqs, counts)
             raise
 
-    def _extend(self, ids, place, cache, counts, call, window, sinks, last_only):
+    def _extend(self, ids, place, cache, counts, call, window, sinks, last_only, choice):
         cfg = self.cfg
         D, H = cfg.d_model, cfg.n_heads
         T = len(place)
@@ -462,7 +472,14 @@ class DawnModel:
             qk, v = self._qkv_raw(self._ln(x, bp["norm1"]), "centered")
             q, k, v = (t[:T].view(T, H, -1) for t in (qk[:, 0], qk[:, 1], v[:, 0]))
             kv_write(pages, k, v, table, lens, cu)
-            paged_attention(q, pages, table, lens, cu, max_new=most, scale=scale, window=window, sinks=sinks, out=a[:T])
+            keep = None
+            if cache.indexed:
+                index = cache.index(i)
+                kv_index(pages, index, table, lens, cu, total=T)
+                if choice:
+                    keep = kv_select(q, pages, index, table, lens, cu, **choice)
+            paged_attention(q, pages, table, lens, cu, max_new=most, scale=scale, window=window, sinks=sinks, keep=keep,
+                            out=a[:T])
             x = x + (a.view(Tp, D).float() * self.scale["v"]) @ bp["attn"]["expand_O"]["kernel"]
             x = x + self._know(self._ln(x, bp["norm2"]), "centered")
         x = x[:T]
@@ -473,3 +490,67 @@ class DawnModel:
                 last.append(at - 1)
             x = x[torch.tensor(last, device=self.device)]
         return self._ln(x, self.p["norm"]) @ self.p["token_emb"]["embedding"].T
+
+    @torch.no_grad()
+    def generate(self, prompts, cache: PagedKvCache, n: int, *, samples: int = 1, u=None, temperature=1.0, top_k=0,
+                 top_p=1.0, min_p=0.0, end=None, window: int = 0, sinks: int = 0, keep: int = 0, first: int = 1,
+                 last: int = 1):
+        """``n`` tokens behind each of the ``prompts`` (sequences of ids, none empty),
+        ``samples`` times each: (tokens [B, n] int64, logprobs [B, n] float32), B =
+        len(prompts) * samples, a prompt's samples one after the other.  A prompt is read
+        once, and its samples hold the same pages as far as they agree
+        (``PagedKvCache.fork``).  Tokens come from :func:`sample` with ``u`` [n, B] float32
+        (None: torch's) and these parameters, numbers or tensors [B].  A row that gives
+        ``end`` stops: ``end`` with logprob 0 behind it.  ``window``, ``sinks`` and
+        ``keep``, ``first``, ``last`` as in :meth:`extend`; prompts are read without keep.
+        The sequences are freed at the end."""
+        prompts = [torch.as_tensor(p).reshape(-1) for p in prompts]
+        counts = [p.shape[0] for p in prompts]
+        if not prompts or min(counts) < 1 or n < 1 or samples < 1:
+            raise ValueError("prompts are not empty, n and samples at least 1")
+        for p in prompts:
+            if p.is_floating_point() or int(p.min()) < 0 or int(p.max()) >= self.cfg.vocab_size:
+                raise ValueError(f"prompts hold ids from 0 to {self.cfg.vocab_size - 1}")
+        if max(counts) + n - 1 > self.cfg.max_seq_len:
+            raise ValueError("Sequence length exceeds max_seq_len")
+        B, dev = len(prompts) * samples, self.device
+        if u is None:
+            u = torch.rand(n, B, device=dev)
+        elif tuple(u.shape) != (n, B):
+            raise ValueError(f"u must be [{n}, {B}]")
+        tokens = torch.full((B, n), 0 if end is None else end, dtype=torch.int64, device=dev)
+        logprobs = torch.zeros(B, n, device=dev)
+        seqs = []
+        try:
+            heads = [cache.add() for _ in prompts]
+            seqs += heads
+            logits = self.extend(torch.cat([p.to(dev) for p in prompts]), cache, heads, counts, window=window, sinks=sinks,
+                                 last_only=True)
+            forks = [[cache.fork(s) for _ in range(samples - 1)] for s in heads]
+            seqs = [s for head, more in zip(heads, forks) for s in (head, *more)]
+            logits = logits.repeat_interleave(samples, 0)
+            live = list(range(B))   # rows that go on
+            for i in range(n):
+                at = torch.tensor(live, device=dev)
+                got, share = sample(logits, u[i][at], **{
+                    k: x[at] if isinstance(x, torch.Tensor) else x
+                    for k, x in dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p).items()})
+                tokens[at, i], logprobs[at, i] = got, share
+                ids = got.tolist()
+                if min(ids) < 0:
+                    raise FloatingPointError("a row of logits holds no number above -infinity")
+                go = [j for j, t in enumerate(ids) if t != end]
+                if i + 1 == n or not go:
+                    break
+                if len(go) < len(live):
+                    got, live = got[torch.tensor(go, device=dev)], [live[j] for j in go]
+                rows = [seqs[j] for j in live]
+                if window:
+                    for s in rows:
+                        cache.evict(s, window, sinks)
+                logits = self.extend(got, cache, rows, [1] * len(rows), window=window, sinks=sinks, last_only=True, keep=keep,
+                                     first=first, last=last)
+            return tokens, logprobs
+        finally:
+            for s in seqs:
+                cache.free(s)
