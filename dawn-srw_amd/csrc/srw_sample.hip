@@ -991,7 +991,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     each(in_list, [&](uint32_t, uint32_t, uint64_t w) { total += ones ? 1 : w; });
     total = block_sum<NT>(s, total);
     if (stage == 0) {
-      if (counts && target >= total) continue;   // k keeps them all
+      if (counts && target >= total && in_list == listed) continue;  // k keeps them all
       target = target < total ? target : total;  // (a border's step, by roundings)
     } else {
       target = draw ? place(total) + 1 : part(total);

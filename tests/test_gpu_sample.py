@@ -254,3 +254,35 @@ def test_refusals(pkg, dev):
             pkg.sample(*args, **kw)
     with torch.no_grad():
         pkg.sample(x.clone().requires_grad_(), u)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V,size", [(4500, 450), (20000, 2000), (30001, 1500)])
+def test_top_k_at_the_ends_of_equal_runs(pkg, dev, V, size, dtype):
+    """Runs of equal logits, and k one before, at and one behind each run's end."""
+    print(f"[gpu] sample runs {V} {size} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(V)
+    level = (torch.randperm(V, generator=g) // size).to(F32)
+    k = torch.tensor([size * i + d for i in range(1, V // size + 1) for d in (-1, 0, 1)], dtype=I32)
+    B = len(k)
+    logits = (-0.25 * level)[None].repeat(B, 1).to(dtype)
+    u = torch.rand(B, generator=g)
+    check(pkg, dev, logits, u, top_k=k)
+    check(pkg, dev, logits, u, top_k=k, top_p=0.97)
+    check(pkg, dev, logits, u, top_k=k, top_p=0.9, min_p=0.2, temperature=0.8)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [700, 4097, 4466, 12000, 40001])
+def test_any_parameters(pkg, dev, V, dtype):
+    """Rows with a k of any size, half of them with top-p, some with min-p."""
+    print(f"[gpu] sample any {V} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(V + 1)
+    B = 160
+    logits = (2.5 * torch.randn(B, V, generator=g)).to(dtype)
+    rand = lambda: torch.rand(B, generator=g)  # noqa: E731
+    k = torch.exp(rand() * math.log(V + 1)).to(I32)
+    k[::7] = 0
+    p = torch.where(rand() < 0.5, torch.ones(B), 1 - 10 ** (-3 * rand()))
+    least = torch.where(rand() < 0.7, torch.zeros(B), 10 ** (-4 * rand()))
+    check(pkg, dev, logits, rand(), temperature=0.3 + 1.5 * rand(), top_k=k, top_p=p, min_p=least)
