@@ -563,13 +563,14 @@ struct Cut {
 // top-p, its sums by steps.  A lane holds its 32 logits in registers.  Bound by the
 // memory for whole rows of float32 (512 rows of 100 003: MEASURED1), by the ten
 // operations in 64 bits of a weight and as many others for top-p and bf16.
-template <typename T>
-__global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
-  using R = Row<T, 256>;
-  constexpr int E = R::E, kHeld = kPart / 256 / E;  // vectors of a lane
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_parts_kernel(SampleArgs a) {
+  using R = Row<T, NT>;
+  constexpr int E = R::E, kHeld = kPart / NT / E;  // vectors of a lane
+  constexpr int kWaves = NT / 64;
   __shared__ double tab[128];
-  __shared__ unsigned long long hist[kSteps], wave_sums[4];
-  __shared__ float wave_max[4];
+  __shared__ unsigned long long hist[kSteps], wave_sums[kWaves];
+  __shared__ float wave_max[kWaves];
   const int64_t b = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
   const Rules rules(a, b);
@@ -582,7 +583,7 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
   for (int k = 0; k < kHeld; ++k) held[k] = row.raw(first + 64 * k, row.n);
   fill_table(tab);
   if (rules.by_p)
-    for (int i = tid; i < kSteps; i += 256) hist[i] = 0;
+    for (int i = tid; i < kSteps; i += NT) hist[i] = 0;
   float m = -INFINITY, x[E];
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) {
@@ -593,7 +594,9 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
   m = wave_all(m, [](float u, float v) { return fmaxf(u, v); });
   if (lane == 0) wave_max[wave] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
+  m = wave_max[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_max[w]);
   const int64_t at = b * a.parts + part;
   Weights wt;
   wt.begin(rules.t, a.q, tab);
@@ -627,15 +630,24 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a) {
   if (tid == 0) a.part_max[at] = m;
   __syncthreads();
   if (rules.by_p) {
-    // running sums: what a border leaves of a part is one number
-    const uint64_t s0 = hist[4 * tid] + hist[4 * tid + 1], s1 = hist[4 * tid + 2] + hist[4 * tid + 3];
+    // running sums: what a border leaves of a part is one number; a thread two of the
+    // coarse steps
+    uint64_t s0 = 0, s1 = 0;
+    if (tid < kCoarse / 2) {
+      s0 = hist[4 * tid] + hist[4 * tid + 1];
+      s1 = hist[4 * tid + 2] + hist[4 * tid + 3];
+    }
     uint64_t run = wave_scan(s0 + s1);
     if (lane == 63) wave_sums[wave] = run;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) run += wave_sums[w];
-    *reinterpret_cast<ulonglong2*>(&a.part_steps[at * kCoarse + 2 * tid]) = make_ulonglong2(run - s1, run);
+    if (tid < kCoarse / 2) {
+      for (int w = 0; w < wave; ++w) run += wave_sums[w];
+      *reinterpret_cast<ulonglong2*>(&a.part_steps[at * kCoarse + 2 * tid]) = make_ulonglong2(run - s1, run);
+    }
   } else if (tid == 0) {
-    a.part_sum[at] = nothing ? 0 : wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
+    sum = 0;
+    for (int w = 0; w < kWaves; ++w) sum += wave_sums[w];
+    a.part_sum[at] = nothing ? 0 : sum;
   }
 }
 
@@ -835,6 +847,11 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       const bool lowest_step = border == (wide == 2 ? kSteps : kCoarse) - 1;
       from = lowest_step ? wt.lowest : fmaxf(wt.lowest, float_under((wt.R - (first_n + low) * 0.0078125) * wt.per));
       to = -float_under(-(wt.R - (first_n - 1.0) * 0.0078125) * wt.per);
+      if (by_p && !by_k && floor_l > to) {  // min-p leaves less than top-p: no border of its own
+        from = floor_l;
+        all = true;
+        band = first_cut = false;
+      }
     }
     // gathers the tokens from `from` on (first all, then the border's step alone)
     from_list = false;
@@ -1268,7 +1285,10 @@ srw_status_t srw_sample(const srw_sample_t* d, void* workspace, size_t workspace
   const hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto logit) {
     using T = decltype(logit);
-    if (w.bytes > 0) hipLaunchKernelGGL((srw::sample_parts_kernel<T>), parts, dim3(256), 0, s, a);
+    if (w.bytes > 0 && parts.x <= 512)
+      hipLaunchKernelGGL((srw::sample_parts_kernel<T, 512>), parts, dim3(512), 0, s, a);
+    else if (w.bytes > 0)
+      hipLaunchKernelGGL((srw::sample_parts_kernel<T, 256>), parts, dim3(256), 0, s, a);
     if (d->V <= srw::kList)
       hipLaunchKernelGGL((srw::sample_kernel<T, 256, srw::kListRow>), grid, dim3(256), 0, s, a);
     else if (srw::only_whole(*d))

@@ -286,3 +286,16 @@ def test_any_parameters(pkg, dev, V, dtype):
     p = torch.where(rand() < 0.5, torch.ones(B), 1 - 10 ** (-3 * rand()))
     least = torch.where(rand() < 0.7, torch.zeros(B), 10 ** (-4 * rand()))
     check(pkg, dev, logits, rand(), temperature=0.3 + 1.5 * rand(), top_k=k, top_p=p, min_p=least)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V,B", [(9000, 12), (32001, 40)])
+def test_min_p_above_the_border_of_top_p(pkg, dev, V, B, dtype):
+    """min-p that leaves less than top-p does, far less, about as much and more."""
+    print(f"[gpu] sample p and min_p {V} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(V + 3)
+    logits = (3 * torch.randn(B, V, generator=g)).to(dtype)
+    least = 10 ** (-torch.arange(B, dtype=F32) / 8)
+    for p in (0.999, 0.9, 0.3):
+        check(pkg, dev, logits, torch.rand(B, generator=g), top_p=p, min_p=least)
+    check(pkg, dev, logits, torch.rand(B, generator=g), top_p=0.98, min_p=least, temperature=3.0)
