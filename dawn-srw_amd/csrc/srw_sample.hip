@@ -8,9 +8,9 @@
 //
 // With y = l log2 e / t, weights are whole numbers W = round(2^(q + y - R)), from a
 // polynomial in 64 bits (to 2^-40), R a whole number not under M's y and q as large as
-// V W < 2^62 allows: sums of them are exact, so no order of adding and no atomic
-// changes what a row gives, and a border is where 64 bits put it.  What rounds to zero
-// cannot be drawn and takes no part.
+// V W < 2^62 allows, 51 at most: sums of them are exact, so no order of adding and no
+// atomic changes what a row gives, and a border is where 64 bits put it.  What rounds to
+// zero cannot be drawn and takes no part.
 //
 // Nothing is sorted.  A threshold that the border of top-k or top-p cannot lie above
 // is found first; the tokens down to it, if there are no more than kList, become a
@@ -18,12 +18,18 @@
 // the draw by digits of the index.
 //
 // * Top-k of up to 1 024: the threads' largest logits are counted by steps of
-//   2^(1/32); where k of them lie above, so many tokens do.
+//   2^(1/32); where k of them lie above, so many tokens do.  A larger k: all logits are.
 // * Top-p, and rows without either: sample_parts_kernel has summed each part of 8 192
 //   logits, for top-p by steps of 2^(1/16), over its own R (a part's sums are shifted to
 //   the row's R where they meet).  Of top-p rows that keep more than kList the tokens of the
 //   border's step alone become the list; the draw finds its part by the parts' sums and
-//   walks that one.
+//   walks that one.  Where min-p lies above the border's step its tokens are the list.
+//
+// Measured (kernels alone, us): one row of 30 000 float32, every rule on, 10.6; 64 rows of
+// 32 000 float32 with top-k 11, top-p 27, top-p and min-p 20, from the whole distribution
+// 13, greedy 7.3; 192 rows of 131 073 bf16 with top-p 65 (one read of them: 9.8); 512 rows
+// of 100 003 float32 from the whole distribution 54 (39.7).  A single row is a chain of
+// about twenty steps of a workgroup that each wait for memory or a barrier.
 //
 // A workgroup of sixteen waves has a CU's vector units to itself, and an instruction
 // of all of them takes it 16 cycles (24 in 64 bits): what is done for the row as a
@@ -561,8 +567,11 @@ struct Cut {
 
 // The largest logit and the sum of weights of a row's part of kPart logits, and, for
 // top-p, its sums by steps.  A lane holds its 32 logits in registers.  Bound by the
-// memory for whole rows of float32 (512 rows of 100 003: MEASURED1), by the ten
-// operations in 64 bits of a weight and as many others for top-p and bf16.
+// memory for whole rows of float32 (512 rows of 100 003: 46 us, 4.4 TB/s), by the ten
+// operations in 64 bits of a weight, as many others and an LDS atomic for top-p (192 rows
+// of 131 073 bf16: 29 us, 1.7 TB/s).  256 threads, or 512 where there are too few parts to
+// fill the card with those (64 rows of 32 000: the call 28.8 and 27.5 us; 256 rows 45.0
+// and 45.6).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_parts_kernel(SampleArgs a) {
   using R = Row<T, NT>;
@@ -695,17 +704,15 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     return;
   }
   if (rules.greedy) {  // the first of the largest
-    {
-      if constexpr (kWhole) {
-        for (int i = tid; i < a.V; i += NT)
-          if (row.one(i) == m) atomicMin(&s.first, static_cast<uint32_t>(i));
-      } else {
-        row.part(wave, 0, row.n, [&](int i, const float(&x)[E]) {
+    if constexpr (kWhole) {
+      for (int i = tid; i < a.V; i += NT)
+        if (row.one(i) == m) atomicMin(&s.first, static_cast<uint32_t>(i));
+    } else {
+      row.part(wave, 0, row.n, [&](int i, const float(&x)[E]) {
 #pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (x[j] == m) atomicMin(&s.first, static_cast<uint32_t>(i + j));
-        });
-      }
+        for (int j = 0; j < E; ++j)
+          if (x[j] == m) atomicMin(&s.first, static_cast<uint32_t>(i + j));
+      });
     }
     __syncthreads();
     if (tid == 0) {
@@ -901,138 +908,138 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   }
 
   if constexpr (WHAT != kWholeRow) {
-  if (kWhole || from_list) {  // weights, for every look at the list
-    for (int i = tid; i < n; i += NT) {
-      const float l = of_key(static_cast<uint32_t>(s.list[i] >> 32));
-      s.weight[i] = peaked ? l >= wt.lowest : wt.of(l, wt.lowest);
-    }
-  }
-  // f(key, index, weight) of the list's tokens, or the row's, of the cut, from lo on
-  auto each = [&](bool in_list, auto f) {
-    if (kWhole || in_list) {
-#pragma unroll 1
-      for (int i = tid; i < n; i += NT) {  // (a thread's own)
-        const uint64_t x = s.list[i];
-        const uint32_t ky = static_cast<uint32_t>(x >> 32), at = static_cast<uint32_t>(x);
-        if (ky != 0 && ky >= lo && cut.keeps(ky, at)) f(ky, at, s.weight[i]);
+    if (kWhole || from_list) {  // weights, for every look at the list
+      for (int i = tid; i < n; i += NT) {
+        const float l = of_key(static_cast<uint32_t>(s.list[i] >> 32));
+        s.weight[i] = peaked ? l >= wt.lowest : wt.of(l, wt.lowest);
       }
-    } else if constexpr (!kWhole) {
-      row.part(wave, 0, row.n, [&](int i, const float(&x)[E]) {
+    }
+    // f(key, index, weight) of the list's tokens, or the row's, of the cut, from lo on
+    auto each = [&](bool in_list, auto f) {
+      if (kWhole || in_list) {
 #pragma unroll 1
-        for (int j = 0; j < E; ++j) {
-          float l = x[0];
-#pragma unroll
-          for (int c = 1; c < E; ++c) l = j == c ? x[c] : l;
-          const uint32_t ky = key_of(l), at = static_cast<uint32_t>(i + j);
-          if (l >= wt.lowest && ky >= lo && cut.keeps(ky, at)) f(ky, at, peaked ? 1 : wt.whole(l));
+        for (int i = tid; i < n; i += NT) {  // (a thread's own)
+          const uint64_t x = s.list[i];
+          const uint32_t ky = static_cast<uint32_t>(x >> 32), at = static_cast<uint32_t>(x);
+          if (ky != 0 && ky >= lo && cut.keeps(ky, at)) f(ky, at, s.weight[i]);
         }
-      });
-    }
-  };
-  // Few tokens: each is compared with each, a lane for each and a pair of waves for some
-  // of those that it is compared with; once in the order, once by index.
-  if (listed && n <= kFew) {
-    if (tid < kFew) s.few_rank[tid] = s.few_run[tid] = s.mass[tid] = 0;
-    __syncthreads();
-    constexpr int kOf = NT / kFew;
-    const int e = tid & (kFew - 1), slice = tid / kFew;
-    const uint64_t x = e < n ? s.list[e] : 0, place_of = x ^ 0xffffffffu;
-    uint64_t rank = 0, before = 0;
-#pragma unroll 2
-    for (int j = slice; j < n; j += kOf) {
-      const bool over = (s.list[j] ^ 0xffffffffu) > place_of;
-      rank += over;
-      before += over ? s.weight[j] : 0;
-    }
-    if (rank) {
-      atomicAdd(&s.few_rank[e], static_cast<unsigned long long>(rank));
-      atomicAdd(&s.few_run[e], static_cast<unsigned long long>(before));
-    }
-    __syncthreads();
-    uint64_t total = 0;
-    if (wave == 0) {
-      constexpr int kEach = kFew / 64;
-      uint64_t w[kEach], sum = 0;
-#pragma unroll
-      for (int h = 0; h < kEach; ++h) {
-        const int i = lane + 64 * h;
-        w[h] = i < n && (!by_k || s.few_rank[i] < static_cast<uint64_t>(k)) ? s.weight[i] : 0;
-        sum += w[h];
-      }
-      if (by_p && !by_parts) target = part(wave_sum(sum));
-      sum = 0;
-#pragma unroll
-      for (int h = 0; h < kEach; ++h) {
-        const int i = lane + 64 * h;
-        if (by_p && s.few_run[i] >= target) w[h] = 0;
-        if (static_cast<uint32_t>(s.list[i] >> 32) < key_floor) w[h] = 0;
-        s.few_mass[i] = w[h];
-        sum += w[h];
-      }
-      total = wave_sum(sum);
-      if (lane == 0) s.total = total;
-    }
-    __syncthreads();
-    const uint32_t index = static_cast<uint32_t>(x);
-    before = 0;
-#pragma unroll 2
-    for (int j = slice; j < n; j += kOf) before += static_cast<uint32_t>(s.list[j]) < index ? s.few_mass[j] : 0;
-    if (before) atomicAdd(&s.mass[e], static_cast<unsigned long long>(before));
-    __syncthreads();
-    if (tid < kFew) {
-      total = s.total;
-      const uint64_t at = place(total), own = s.few_mass[e];
-      before = s.mass[e];
-      if (e < n && before <= at && at < before + own)
-        done(index, of_key(static_cast<uint32_t>(x >> 32)), static_cast<double>(own), static_cast<double>(total),
-             static_cast<double>(total) * per_unit);
-    }
-    return;
-  }
-  // Three selects, each on what the one before left: top-k's or top-p's border, top-p's
-  // behind top-k's, the draw (of a list; a row's has walks of its own below).
+      } else if constexpr (!kWhole) {
+        row.part(wave, 0, row.n, [&](int i, const float(&x)[E]) {
 #pragma unroll 1
-  for (int stage = 0; stage < 3; ++stage) {
-    const bool draw = stage == 2;
-    bool ones = false, in_list = listed;
-    if (stage == 0) {
-      if (!first_cut) continue;
-      ones = counts;
-      in_list = from_list;
-    } else if (stage == 1 ? !by_p || by_parts || (peaked && !kWhole) : !listed) {
-      continue;
+          for (int j = 0; j < E; ++j) {
+            float l = x[0];
+#pragma unroll
+            for (int c = 1; c < E; ++c) l = j == c ? x[c] : l;
+            const uint32_t ky = key_of(l), at = static_cast<uint32_t>(i + j);
+            if (l >= wt.lowest && ky >= lo && cut.keeps(ky, at)) f(ky, at, peaked ? 1 : wt.whole(l));
+          }
+        });
+      }
+    };
+    // Few tokens: each is compared with each, a lane for each and a pair of waves for some
+    // of those that it is compared with; once in the order, once by index.
+    if (listed && n <= kFew) {
+      if (tid < kFew) s.few_rank[tid] = s.few_run[tid] = s.mass[tid] = 0;
+      __syncthreads();
+      constexpr int kOf = NT / kFew;
+      const int e = tid & (kFew - 1), slice = tid / kFew;
+      const uint64_t x = e < n ? s.list[e] : 0, place_of = x ^ 0xffffffffu;
+      uint64_t rank = 0, before = 0;
+#pragma unroll 2
+      for (int j = slice; j < n; j += kOf) {
+        const bool over = (s.list[j] ^ 0xffffffffu) > place_of;
+        rank += over;
+        before += over ? s.weight[j] : 0;
+      }
+      if (rank) {
+        atomicAdd(&s.few_rank[e], static_cast<unsigned long long>(rank));
+        atomicAdd(&s.few_run[e], static_cast<unsigned long long>(before));
+      }
+      __syncthreads();
+      uint64_t total = 0;
+      if (wave == 0) {
+        constexpr int kEach = kFew / 64;
+        uint64_t w[kEach], sum = 0;
+#pragma unroll
+        for (int h = 0; h < kEach; ++h) {
+          const int i = lane + 64 * h;
+          w[h] = i < n && (!by_k || s.few_rank[i] < static_cast<uint64_t>(k)) ? s.weight[i] : 0;
+          sum += w[h];
+        }
+        if (by_p && !by_parts) target = part(wave_sum(sum));
+        sum = 0;
+#pragma unroll
+        for (int h = 0; h < kEach; ++h) {
+          const int i = lane + 64 * h;
+          if (by_p && s.few_run[i] >= target) w[h] = 0;
+          if (static_cast<uint32_t>(s.list[i] >> 32) < key_floor) w[h] = 0;
+          s.few_mass[i] = w[h];
+          sum += w[h];
+        }
+        total = wave_sum(sum);
+        if (lane == 0) s.total = total;
+      }
+      __syncthreads();
+      const uint32_t index = static_cast<uint32_t>(x);
+      before = 0;
+#pragma unroll 2
+      for (int j = slice; j < n; j += kOf) before += static_cast<uint32_t>(s.list[j]) < index ? s.few_mass[j] : 0;
+      if (before) atomicAdd(&s.mass[e], static_cast<unsigned long long>(before));
+      __syncthreads();
+      if (tid < kFew) {
+        total = s.total;
+        const uint64_t at = place(total), own = s.few_mass[e];
+        before = s.mass[e];
+        if (e < n && before <= at && at < before + own)
+          done(index, of_key(static_cast<uint32_t>(x >> 32)), static_cast<double>(own), static_cast<double>(total),
+               static_cast<double>(total) * per_unit);
+      }
+      return;
     }
-    if (stage > 0) lo = cut.key > lo ? cut.key : lo;
-    if (draw) lo = key_floor > lo ? key_floor : lo;
-    uint64_t total = 0;
-    each(in_list, [&](uint32_t, uint32_t, uint64_t w) { total += ones ? 1 : w; });
-    total = block_sum<NT>(s, total);
-    if (stage == 0) {
-      if (counts && target >= total && in_list == listed) continue;  // k keeps them all
-      target = target < total ? target : total;  // (a border's step, by roundings)
-    } else {
-      target = draw ? place(total) + 1 : part(total);
-    }
-    const uint32_t lowest = lo >> kShift;
-    const int bits = draw ? index_bits : bits_of((hi >> kShift) - lowest) + index_bits;
-    const uint64_t r = select<NT>(s, bits, target, in_list ? n : a.V, [&](auto g) {
-      each(in_list, [&](uint32_t ky, uint32_t i, uint64_t w) {
-        if (ones) w = 1;
-        if (w) g(static_cast<uint64_t>(draw ? 0 : (ky >> kShift) - lowest) << index_bits | (last - i), w);
+    // Three selects, each on what the one before left: top-k's or top-p's border, top-p's
+    // behind top-k's, the draw (of a list; a row's has walks of its own below).
+#pragma unroll 1
+    for (int stage = 0; stage < 3; ++stage) {
+      const bool draw = stage == 2;
+      bool ones = false, in_list = listed;
+      if (stage == 0) {
+        if (!first_cut) continue;
+        ones = counts;
+        in_list = from_list;
+      } else if (stage == 1 ? !by_p || by_parts || (peaked && !kWhole) : !listed) {
+        continue;
+      }
+      if (stage > 0) lo = cut.key > lo ? cut.key : lo;
+      if (draw) lo = key_floor > lo ? key_floor : lo;
+      uint64_t total = 0;
+      each(in_list, [&](uint32_t, uint32_t, uint64_t w) { total += ones ? 1 : w; });
+      total = block_sum<NT>(s, total);
+      if (stage == 0) {
+        if (counts && target >= total && in_list == listed) continue;  // k keeps them all
+        target = target < total ? target : total;  // (a border's step, by roundings)
+      } else {
+        target = draw ? place(total) + 1 : part(total);
+      }
+      const uint32_t lowest = lo >> kShift;
+      const int bits = draw ? index_bits : bits_of((hi >> kShift) - lowest) + index_bits;
+      const uint64_t r = select<NT>(s, bits, target, in_list ? n : a.V, [&](auto g) {
+        each(in_list, [&](uint32_t ky, uint32_t i, uint64_t w) {
+          if (ones) w = 1;
+          if (w) g(static_cast<uint64_t>(draw ? 0 : (ky >> kShift) - lowest) << index_bits | (last - i), w);
+        });
       });
-    });
-    const uint32_t at = last - (static_cast<uint32_t>(r) & ((1u << index_bits) - 1));
-    if (!draw) {
-      uint32_t ky = (lowest + static_cast<uint32_t>(r >> index_bits)) << kShift;
-      if (kShift > 0 && !(ky & 0x80000000u)) ky |= (1u << kShift) - 1;  // (a negative number's)
-      cut = Cut{ky, at};
-      hi = key_m;
-    } else if (tid == 0) {
-      const float l = row.one(at);
-      done(at, l, static_cast<double>(peaked ? 1 : wt.whole(l)), static_cast<double>(total),
-           static_cast<double>(total) * per_unit);
+      const uint32_t at = last - (static_cast<uint32_t>(r) & ((1u << index_bits) - 1));
+      if (!draw) {
+        uint32_t ky = (lowest + static_cast<uint32_t>(r >> index_bits)) << kShift;
+        if (kShift > 0 && !(ky & 0x80000000u)) ky |= (1u << kShift) - 1;  // (a negative number's)
+        cut = Cut{ky, at};
+        hi = key_m;
+      } else if (tid == 0) {
+        const float l = row.one(at);
+        done(at, l, static_cast<double>(peaked ? 1 : wt.whole(l)), static_cast<double>(total),
+             static_cast<double>(total) * per_unit);
+      }
     }
-  }
   }
   if constexpr (!kWhole) {
     if (listed) return;

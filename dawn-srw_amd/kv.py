@@ -336,7 +336,8 @@ def kv_copy(tensors, src, dst, *, to=None) -> None:
             if not isinstance(t, torch.Tensor) or t.dim() < 2:
                 raise ValueError("tensors must be [layers, n_pages, ...]")
             if shape is None:
-                dev, shape = t.device, (t.shape[0], [t.shape[1], b[0].shape[1] if isinstance(b[0], torch.Tensor) and b[0].dim() > 1 else -1])
+                other = b[0].shape[1] if isinstance(b[0], torch.Tensor) and b[0].dim() > 1 else -1
+                dev, shape = t.device, (t.shape[0], [t.shape[1], other])
                 if dev.type != "cuda":
                     raise ValueError(f"the cache lives on a HIP device; got {dev}")
             if t.device != dev:
@@ -435,8 +436,8 @@ def paged_attention(q, pages: KvPages, table, lens, cu=None, *, max_new: int = 0
     sqrt(head_dim)).  ``max_new``: the most new tokens of one sequence, where
     the caller knows it.  With ``keep`` [T, heads, n] int32 (:func:`kv_select`, or
     any ascending places in the sequence's row of ``table``) a token sees, of these
-    positions, those of the kept pages alone; it goes without a window.  Returns ``out`` [T, n_heads, head_dim] bfloat16; a
-    token that sees nothing gets zeros.
+    positions, those of the kept pages alone; it goes without a window.  Returns
+    ``out`` [T, n_heads, head_dim] bfloat16; a token that sees nothing gets zeros.
 
     Sums and statistics are float32.  The softmax weights enter the second
     product as one bfloat16 in calls of many rows, as two (16 bits) in calls of

@@ -587,8 +587,13 @@ srw_status_t srw_attention_kept(const srw_attention_t* a, const int32_t* keep, i
  * which is checked.  In arrays a temperature that is not above 0 counts as 0, a top_k
  * below 1 as off, a top_p that is not below 1 as off, a min_p that is not above 0 as
  * off and one above 1 as 1; u is taken into [0, 1).  Sums are of whole numbers (weights
- * in units of 2^-q, q = min(51, 62 - log2 V)): results do not go by the batch or the
- * order of adding.  V up to 2^24, B up to 2^21. */
+ * in units of 2^(R - q), 2^R the power of two at or above the largest, q = min(51,
+ * 62 - ceil(log2 V))): results do not go by the batch or the order of adding.
+ *
+ * Rows of more than 4 096 logits that may draw from all of them or by top_p without top_k
+ * need a workspace, 16-byte aligned: without it the call returns SRW_EWORKSPACE and
+ * launches nothing.  V up to 2^24, B up to 2^21, and below 2^24 parts of 8 192 logits in
+ * all rows together. */
 typedef struct srw_sample {
   const void* logits;
   int64_t row_stride, B, V;
