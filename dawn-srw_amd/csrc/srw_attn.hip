@@ -797,6 +797,13 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
   const int c = threadIdx.x % L, first = threadIdx.x / L / W * W, grp = threadIdx.x / L - first;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (N / W) + first / W;
   const int64_t row = at < rows ? at : rows - 1;
+  // (no split wrote rows that no sequence names, and neither is written here; asked for
+  // ahead of the loads below)
+  bool named = at < rows;
+  if (cu) {
+    const int t = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(Hq));  // (rows < 2^31)
+    named = named && t >= cu[0] && t < cu[B];
+  }
   float m = kLowest, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   constexpr int U = 4;
@@ -847,10 +854,7 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(const float* part, const 
       for (int k = 0; k < 4; ++k) o[k] += so[first + g][c][k] * e;
     }
   }
-  if (at >= rows) return;
-  // (no split wrote rows that no sequence names, and neither is written here)
-  const int64_t t = row / Hq;
-  if (cu && (t < cu[0] || t >= cu[B])) return;
+  if (!named) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(out + row * DH + 4 * c) =
       make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
