@@ -223,6 +223,20 @@ bool index_of(PyObject* o, const srw_kv_t& c, int device, srw_kv_index_t* x) {
   return true;
 }
 
+// index_pair((codes, scale)) -> whether they are an index of some pages
+PyObject* host_index_pair(PyObject* const* a, Py_ssize_t n) {
+  if (n != 1 || !PyTuple_CheckExact(a[0]) || PyTuple_GET_SIZE(a[0]) != 2) Py_RETURN_FALSE;
+  const at::Tensor* codes = tensor(PyTuple_GET_ITEM(a[0], 0));
+  if (!codes || !codes->is_cuda() || codes->dim() != 3) Py_RETURN_FALSE;
+  srw_kv_t c{};
+  srw_kv_index_t x{};
+  c.n_pages = codes->size(0);
+  c.n_kv_heads = static_cast<int32_t>(codes->size(1));
+  c.head_dim = static_cast<int32_t>(codes->size(2));
+  if (index_of(a[0], c, static_cast<int>(codes->get_device()), &x)) Py_RETURN_TRUE;
+  Py_RETURN_FALSE;
+}
+
 void written(const at::Tensor* t) {
   if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
@@ -430,6 +444,7 @@ PyMethodDef methods[] = {
     {"write", reinterpret_cast<PyCFunction>(caught<host_write>), METH_FASTCALL, nullptr},
     {"read", reinterpret_cast<PyCFunction>(caught<host_read>), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(caught<host_attention>), METH_FASTCALL, nullptr},
+    {"index_pair", reinterpret_cast<PyCFunction>(caught<host_index_pair>), METH_FASTCALL, nullptr},
     {"index", reinterpret_cast<PyCFunction>(caught<host_index>), METH_FASTCALL, nullptr},
     {"select", reinterpret_cast<PyCFunction>(caught<host_select>), METH_FASTCALL, nullptr},
     {"attention_kept", reinterpret_cast<PyCFunction>(caught<host_attention_kept>), METH_FASTCALL, nullptr},

@@ -149,7 +149,8 @@ class KvIndex:
 
     def __init__(self, codes, scale):
         self._t = (codes, scale)
-        self._at(None)
+        if not (_host or _native()).index_pair(self._t):
+            self._at(None)
 
     codes = property(lambda self: self._t[0])
     scale = property(lambda self: self._t[1])
