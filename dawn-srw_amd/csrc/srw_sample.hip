@@ -25,7 +25,9 @@
 //   border's step alone become the list; the draw finds its part by the parts' sums and
 //   walks that one.  Where min-p lies above the border's step its tokens are the list.
 //
-// Measured (kernels alone, us): one row of 30 000 float32, every rule on, 10.6; 64 rows of
+// A row of up to 2 048 logits (1 024 by top-k) is its own list.
+//
+// Measured (kernels alone, us): 64 rows of 1 000 float32 by top-p 10.4; one row of 30 000 float32, every rule on, 10.6; 64 rows of
 // 32 000 float32 with top-k 11, top-p 27, top-p and min-p 20, from the whole distribution
 // 13, greedy 7.3; 192 rows of 131 073 bf16 with top-p 65 (one read of them: 9.8); 512 rows
 // of 100 003 float32 from the whole distribution 54 (39.7).  A single row is a chain of
@@ -47,6 +49,7 @@ namespace {
 constexpr int kSteps = 1024;   // of 2^(1/32) under 2^R
 constexpr int kCoarse = 512;   // of 2^(1/16), what parts are summed by
 constexpr int kList = 4096;    // tokens of a list
+constexpr int kOwnList = 2048; // logits of a row that is its own list, at most
 constexpr int kFew = 128;      // tokens that are compared each with each
 constexpr int kPart = 8192;    // logits of a part
 constexpr int kDigit = 9, kBins = 1 << kDigit;  // bits of a select's pass
@@ -420,15 +423,17 @@ __device__ __forceinline__ N wave_all(N v, Op op) {
 // distribution.
 enum { kAnyRow, kListRow, kWholeRow };
 template <int WHAT> struct Shared {
-  static constexpr int kListed = WHAT == kWholeRow ? 1 : kList, kParts = WHAT == kListRow ? 1 : kMostParts;
+  static constexpr int kListed = WHAT == kWholeRow ? 1 : WHAT == kListRow ? kOwnList : kList;
+  static constexpr int kParts = WHAT == kListRow ? 1 : kMostParts;
   double tab[128];
   union {
     unsigned long long list[kListed];  // key << 32 | index
     unsigned long long steps[WHAT == kAnyRow ? 2 : 1][kCoarse];  // of the row's parts, half of them each
   };
   unsigned long long weight[kListed];  // of the list's tokens
-  uint32_t count[kSteps];
-  unsigned long long mass[kBins + 64];
+  static constexpr int kMass = WHAT == kListRow ? kSteps : kBins;
+  uint32_t count[kSteps + 64];
+  unsigned long long mass[kMass + 64];
   float part_max[kParts];
   float under[kParts];  // octaves of a part's R under the row's; 1e9: it weighs nothing
   unsigned long long kept[kParts];  // of each part, in its units
@@ -479,14 +484,61 @@ __device__ __forceinline__ void crossing(S& s, uint32_t target) {
 // mass, the largest rank first, reaches target >= 1; there must be one.  each(f) calls
 // f(rank, mass) for every candidate of this thread, of which there are no more than n.
 // A pass takes a digit; where no more than 64 candidates share the digits up to the
-// border's, one wave compares each with each.
-template <int NT, class S, class Each>
-__device__ __forceinline__ uint64_t select(S& s, int bits, uint64_t target, uint32_t n, Each each) {
-  constexpr int kEach = kBins / 64;
-  auto place = [](int i) { return i + i / kEach; };  // (a lane's run of bins, over all banks)
+// border's, one wave compares each with each.  With `coarse` (COARSE: it may be) the first
+// pass goes by step_of(rank), which orders as the ranks do: the first digit of logits of a few octaves
+// has a few values, and atomics on few bins wait for each other (64 rows of 1 000 by
+// top-p 14.3 us without, 13.2 with).
+template <int NT, bool COARSE, class S, class Each, class Step>
+__device__ __forceinline__ uint64_t select(S& s, int bits, uint64_t target, uint32_t n, bool coarse, Step step_of, Each each) {
   const int lane = threadIdx.x & 63;
   uint64_t rank = 0, before = 0;
-  int left = bits;
+  int left = bits, step = -1;
+  auto clear = [&](int bins) {
+    for (int i = threadIdx.x; i < bins + 64; i += NT) {
+      s.count[i] = 0;
+      s.mass[i] = 0;
+    }
+  };
+  // the bin in which the target falls, by wave 0: a lane a run of kEach
+  auto cross = [&](auto each_of, auto place) {
+    constexpr int kEach = decltype(each_of)::value;
+    if (threadIdx.x < 64) {
+      uint64_t m[kEach], sum = 0;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        m[k] = s.mass[place(lane * kEach + k)];
+        sum += m[k];
+      }
+      uint64_t run = before + wave_scan(sum) - sum;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        if (run < target && run + m[k] >= target) {
+          s.bin = lane * kEach + k;
+          s.before = run;
+          s.in_n = s.count[place(lane * kEach + k)];
+        }
+        run += m[k];
+      }
+    }
+    __syncthreads();
+    before = s.before;
+    n = s.in_n;
+  };
+  if (COARSE && coarse && n > 64) {
+    auto place = [](int i) { return i + i / (kSteps / 64); };
+    clear(kSteps);
+    __syncthreads();
+    each([&](uint64_t r, uint64_t m) {
+      const int bin = place(step_of(r));
+      atomicAdd(&s.count[bin], 1u);
+      atomicAdd(&s.mass[bin], static_cast<unsigned long long>(m));
+    });
+    __syncthreads();
+    cross(std::integral_constant<int, kSteps / 64>{}, place);
+    step = s.bin;
+  }
+  constexpr int kEach = kBins / 64;
+  auto place = [](int i) { return i + i / kEach; };  // (a lane's run of bins, over all banks)
 #pragma unroll 1
   for (;;) {
     if (threadIdx.x == 0) s.few = 0;
@@ -494,7 +546,7 @@ __device__ __forceinline__ uint64_t select(S& s, int bits, uint64_t target, uint
     if (n <= 64) {
       __syncthreads();
       each([&](uint64_t r, uint64_t m) {
-        if (left < 64 && r >> left != rank) return;
+        if ((left < 64 && r >> left != rank) || (COARSE && step >= 0 && step_of(r) != step)) return;
         const uint32_t at = atomicAdd(&s.few, 1u);
         s.few_rank[at] = r;
         s.few_mass[at] = m;
@@ -516,40 +568,17 @@ __device__ __forceinline__ uint64_t select(S& s, int bits, uint64_t target, uint
       return s.rank;
     }
     const int d = left < kDigit ? left : kDigit, shift = left - d, last = (1 << d) - 1;
-    for (int i = threadIdx.x; i < kBins + 64; i += NT) {
-      s.count[i] = 0;
-      s.mass[i] = 0;
-    }
+    clear(kBins);
     __syncthreads();
     each([&](uint64_t r, uint64_t m) {
-      if (r >> left != rank) return;
+      if (r >> left != rank || (COARSE && step >= 0 && step_of(r) != step)) return;
       const int bin = place(last - static_cast<int>(static_cast<uint32_t>(r >> shift) & static_cast<uint32_t>(last)));
       atomicAdd(&s.count[bin], 1u);
       atomicAdd(&s.mass[bin], static_cast<unsigned long long>(m));
     });
     __syncthreads();
-    if (threadIdx.x < 64) {
-      uint64_t m[kEach], sum = 0;
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        m[k] = s.mass[place(lane * kEach + k)];
-        sum += m[k];
-      }
-      uint64_t run = before + wave_scan(sum) - sum;
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        if (run < target && run + m[k] >= target) {
-          s.bin = lane * kEach + k;
-          s.before = run;
-          s.in_n = s.count[place(lane * kEach + k)];
-        }
-        run += m[k];
-      }
-    }
-    __syncthreads();
+    cross(std::integral_constant<int, kEach>{}, place);
     rank = rank << d | static_cast<uint32_t>(last - s.bin);
-    before = s.before;
-    n = s.in_n;
     left = shift;
     if (left == 0) return rank;
   }
@@ -1022,7 +1051,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       }
       const uint32_t lowest = lo >> kShift;
       const int bits = draw ? index_bits : bits_of((hi >> kShift) - lowest) + index_bits;
-      const uint64_t r = select<NT>(s, bits, target, in_list ? n : a.V, [&](auto g) {
+      auto step_of = [&](uint64_t r) { return wt.step(of_key((lowest + static_cast<uint32_t>(r >> index_bits)) << kShift)); };
+      const uint64_t r = select<NT, kWhole>(s, bits, target, in_list ? n : a.V, !draw && !peaked, step_of, [&](auto g) {
         each(in_list, [&](uint32_t ky, uint32_t i, uint64_t w) {
           if (ones) w = 1;
           if (w) g(static_cast<uint64_t>(draw ? 0 : (ky >> kShift) - lowest) << index_bits | (last - i), w);
@@ -1191,17 +1221,23 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   }
 }
 
+// Whether rows are their own lists.  Top-k's threshold makes short lists of longer rows:
+// 64 rows of 300 | 1 000 | 2 000 float32 take 8.1 | 10.3 | 13 us by top-k as their own
+// lists and 9.0 | 8.7 | 9.1 by a threshold (512 rows of 1 000: 12.4 and 16.9), by top-p
+// 8.1 | 10.4 | 13 and, of parts, 9 | 24 | 25.  A list of 4 096 leaves room for one
+// workgroup a CU.
+bool own_list(const srw_sample_t& d) { return d.V <= (d.top_k || d.top_k_all > 0 ? kOwnList / 2 : kOwnList); }
 // Parts of a row (0: it is its own list): its vectors are one more where it begins
 // inside of one.
 int64_t parts_of(const srw_sample_t& d) {
-  if (d.V <= kList) return 0;
+  if (own_list(d)) return 0;
   const int64_t size = d.dtype == SRW_F32 ? 4 : 2, E = 16 / size;
   const bool whole = (reinterpret_cast<uintptr_t>(d.logits) | (d.B > 1 ? d.row_stride * size : 0)) % 16 == 0;
   return ((d.V + E - 1) / E + (whole ? 0 : 1) + kPart / E - 1) / (kPart / E);
 }
 // Whether a row may ask for its parts' sums.
 bool by_parts(const srw_sample_t& d) {
-  if (d.V <= kList) return false;
+  if (own_list(d)) return false;
   if (!d.temperature && !(d.temperature_all > 0.f)) return false;
   const bool by_p = d.top_p || d.top_p_all < 1.f, whole = d.min_p || d.min_p_all == 0.f;
   return (d.top_k || d.top_k_all == 0 || d.top_k_all >= d.V) && (by_p || whole);
@@ -1296,8 +1332,8 @@ srw_status_t srw_sample(const srw_sample_t* d, void* workspace, size_t workspace
       hipLaunchKernelGGL((srw::sample_parts_kernel<T, 512>), parts, dim3(512), 0, s, a);
     else if (w.bytes > 0)
       hipLaunchKernelGGL((srw::sample_parts_kernel<T, 256>), parts, dim3(256), 0, s, a);
-    if (d->V <= srw::kList)
-      hipLaunchKernelGGL((srw::sample_kernel<T, 256, srw::kListRow>), grid, dim3(256), 0, s, a);
+    if (srw::own_list(*d))
+      hipLaunchKernelGGL((srw::sample_kernel<T, 512, srw::kListRow>), grid, dim3(512), 0, s, a);
     else if (srw::only_whole(*d))
       hipLaunchKernelGGL((srw::sample_kernel<T, 256, srw::kWholeRow>), grid, dim3(256), 0, s, a);
     else

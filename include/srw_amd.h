@@ -590,7 +590,7 @@ srw_status_t srw_attention_kept(const srw_attention_t* a, const int32_t* keep, i
  * in units of 2^(R - q), 2^R the power of two at or above the largest, q = min(51,
  * 62 - ceil(log2 V))): results do not go by the batch or the order of adding.
  *
- * Rows of more than 4 096 logits that may draw from all of them or by top_p without top_k
+ * Rows of more than 2 048 logits that may draw from all of them or by top_p without top_k
  * need a workspace, 16-byte aligned: without it the call returns SRW_EWORKSPACE and
  * launches nothing.  V up to 2^24, B up to 2^21, and below 2^24 parts of 8 192 logits in
  * all rows together. */

@@ -273,7 +273,7 @@ def test_top_k_at_the_ends_of_equal_runs(pkg, dev, V, size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
-@pytest.mark.parametrize("V", [700, 4097, 4466, 12000, 40001])
+@pytest.mark.parametrize("V", [90, 700, 1025, 2047, 2049, 4097, 4466, 12000, 40001])
 def test_any_parameters(pkg, dev, V, dtype):
     """Rows with a k of any size, half of them with top-p, some with min-p."""
     print(f"[gpu] sample any {V} {dtype}", flush=True)
