@@ -236,12 +236,12 @@ template <typename T, int NT> struct Row {
     }
   }
   // f(index of the first, logits) of the vectors [from, to) (n of two and more), one a
-  // lane: the runs of 64 at from, from + 64 step, ..., those of a wave.  Eight loads are on
+  // lane: the runs of 64 at from, from + 64 step, ..., those of a wave.  AHEAD loads are on
   // their way together (one takes about a microsecond where another XCD's kernel, or none,
   // has read the row before), and f stands once: a vector comes out of the registers by
   // its number.  The logits of a first or last vector that is partly outside of the row
   // come one a lane, with NaN beside each, to the wave that asks for that end.
-  template <class F>
+  template <int AHEAD, class F>
   __device__ __forceinline__ void walk(int from, int to, int step, bool head, bool tail, F f) const {
     const int lane = threadIdx.x & 63;
     int edge = -1;  // its index
@@ -253,12 +253,12 @@ template <typename T, int NT> struct Row {
     from = from < first() ? first() : from;
     to = to > end() ? end() : to;
 #pragma unroll 1
-    for (; from < to || more; from += 64 * step * kAhead) {
-      typedef uint32_t held_t __attribute__((ext_vector_type(4 * kAhead)));
+    for (; from < to || more; from += 64 * step * AHEAD) {
+      typedef uint32_t held_t __attribute__((ext_vector_type(4 * AHEAD)));
       held_t held = {};
       if (from < to) {
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
+        for (int k = 0; k < AHEAD; ++k) {
           const int v = from + 64 * step * k + lane;
           const u32x4_t w = *at(v < to ? v : to - 1);
 #pragma unroll
@@ -266,7 +266,7 @@ template <typename T, int NT> struct Row {
         }
       }
 #pragma unroll 1
-      for (int k = 0; k < kAhead; ++k) {
+      for (int k = 0; k < AHEAD; ++k) {
         const int v = from + 64 * step * k;
         float x[E];
         int i;
@@ -290,10 +290,10 @@ template <typename T, int NT> struct Row {
   __device__ __forceinline__ int first() const { return off > 0 ? 1 : 0; }
   __device__ __forceinline__ int end() const { return n * E - off > V ? n - 1 : n; }
   // A wave's part of [from, to), a run of vectors.
-  template <class F>
+  template <int AHEAD = kAhead, class F>
   __device__ __forceinline__ void part(int wave, int from, int to, F f) const {
     const int per = (to - from + kWaves - 1) / kWaves, v0 = from + wave * per, v1 = v0 + per < to ? v0 + per : to;
-    if (v0 < v1) walk(v0, v1, 1, v0 == 0, v1 == n, f);
+    if (v0 < v1) walk<AHEAD>(v0, v1, 1, v0 == 0, v1 == n, f);
   }
   // The largest logit of the thread's share of the row.
   __device__ __forceinline__ float largest() const {
@@ -952,8 +952,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
           const uint32_t ky = static_cast<uint32_t>(x >> 32), at = static_cast<uint32_t>(x);
           if (ky != 0 && ky >= lo && cut.keeps(ky, at)) f(ky, at, s.weight[i]);
         }
-      } else if constexpr (!kWhole) {
-        row.part(wave, 0, row.n, [&](int i, const float(&x)[E]) {
+      } else if constexpr (!kWhole) {  // (four loads ahead: with eight registers spill)
+        row.template part<4>(wave, 0, row.n, [&](int i, const float(&x)[E]) {
 #pragma unroll 1
           for (int j = 0; j < E; ++j) {
             float l = x[0];
@@ -1162,12 +1162,13 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       at -= lane_of(run, w) - lane_of(sums, w);
       return w;
     };
+    constexpr int kFewer = E == 8 ? 4 : 8;  // loads ahead (eight of bf16: registers spill)
     constexpr int kHeld = kPart / E / NT, kMost = kHeld * NT;  // vectors of a lane, of a workgroup
 #pragma unroll 1
     while (v1 - v0 > kMost) {
       const int per = (v1 - v0 + kWaves - 1) / kWaves;
       uint64_t sum = 0;
-      row.part(wave, v0, v1, [&](int i, const float(&x)[E]) {
+      row.template part<kFewer>(wave, v0, v1, [&](int i, const float(&x)[E]) {
 #pragma unroll
         for (int j = 0; j < E; ++j) sum += weight(x[j], i + j);
       });
