@@ -396,3 +396,42 @@ def test_refusals(pkg, dev):
                     (ValueError, dict(keep=keep[..., ::2])), (ValueError, dict(keep=[1]))):
         with pytest.raises(err):
             pkg.paged_attention(q, c.pages, c.table, c.len_t, **kw)
+
+
+@pytest.mark.parametrize("counts", [None, [3]], ids=str)
+@pytest.mark.parametrize("width", [90, 700, 3500])
+@pytest.mark.parametrize("kind", ["zeros", "levels", "near", "infinite", "nan", "spread", "holes"])
+def test_borders_among_scores_of_any_kind(pkg, dev, kind, width, counts):
+    """Equal scores beyond what is counted one by one, infinities, neighbours in the last
+    bit, scores of sixty orders of magnitude, pages that are missing."""
+    print(f"[gpu] kv_select {kind} {width} {counts}", flush=True)
+    H, dh, P, N = 1, 64, 16, 400
+    g = torch.Generator().manual_seed(width + len(kind))
+    pages = pkg.KvPages(*(torch.zeros(s, dtype=BF, device=dev) for s in ((N, H, P, dh), (N, H, dh, P))))
+    codes = torch.randint(-127, 128, (N, H, dh), generator=g, dtype=torch.int8)
+    scale = 0.5 + torch.rand(N, H, generator=g)
+    rows = [torch.randint(0, N, (width,), generator=g).tolist()]
+    if kind == "zeros":
+        codes.zero_()
+    elif kind == "levels":
+        codes[:] = codes[:1]
+        scale = torch.randint(1, 4, (N, H), generator=g).float()
+    elif kind == "near":
+        codes[:] = codes[:1]
+        scale = torch.nextafter(torch.ones(N, H), torch.full((N, H), 2.0)) + torch.randint(0, 5, (N, H), generator=g) * 2.0 ** -23
+    elif kind == "infinite":
+        scale[::2] = math.inf
+    elif kind == "nan":
+        scale[torch.rand(N, H, generator=g) < 0.6] = NAN
+    elif kind == "spread":
+        scale = 10 ** (60 * torch.rand(N, H, generator=g, dtype=F64) - 30).float().clamp_min(1e-38)
+    else:
+        rows[0] = [r if j % 3 else -1 for j, r in enumerate(rows[0])]
+    index = pkg.KvIndex(codes.to(dev), scale.to(dev))
+    table = torch.tensor(rows, dtype=I32, device=dev)
+    lens = [width * P - 2]
+    q = torch.randn(sum(counts or [1]), 2, dh, generator=g).to(BF)
+    for n, first, last in ((20, 1, 2), (70, 0, 1), (width // 2, 2, 3), (width - 1, 1, 1), (width + 5, 0, 1)):
+        keep = pkg.kv_select(q.to(dev), pages, index, table, torch.tensor(lens, dtype=I32, device=dev),
+                             None if counts is None else _cu(dev, counts), n=n, first=first, last=last)
+        assert torch.equal(keep.cpu(), _select(q, codes, scale, rows, lens, counts or [1], P, n, first, last))
