@@ -1138,7 +1138,10 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     // which the draw lies, until one step of a wave holds the rest.
     Weights w = wt;  // in the units of the row, or of its part
     if (!need_total) w.set(s.part_max[s.part], a.q);
-    const float low = fmaxf(fmaxf(floor_l, key_l), w.lowest);
+    // (the part's sum counts what weighs something in the part's units, under the row's
+    // lowest too: a draw that falls into its part finds a token there.  Of top-p the cut lies
+    // above the row's lowest and min-p's.)
+    const float low = fmaxf(need_total ? fmaxf(floor_l, key_l) : key_l, w.lowest);
     auto weight = [&](float l, int i) -> uint64_t {
       uint64_t x = w.whole(l);
       if (peaked) x = 1;
