@@ -887,6 +887,10 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
         from = floor_l;
         all = true;
         band = first_cut = false;
+      } else if (by_p && !by_k && lowest_step) {
+        // the last step's sums count what lies under the row's lowest and weighs nothing in
+        // the row's units, and a list of it could be empty: the border is found on the row
+        all = band = false;
       }
     }
     // gathers the tokens from `from` on (first all, then the border's step alone)
@@ -1045,7 +1049,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       total = block_sum<NT>(s, total);
       if (stage == 0) {
         if (counts && target >= total && in_list == listed) continue;  // k keeps them all
-        target = target < total ? target : total;  // (a border's step, by roundings)
+        if (!counts && !in_list) target = part(total);  // (top-p on the row: all in its units)
+        target = target < total ? target : total;       // (a border's step, by roundings)
       } else {
         target = draw ? place(total) + 1 : part(total);
       }

@@ -51,7 +51,7 @@ class Numbers:
 
     def weights(self, l, R):
         values, place = np.unique(np.asarray(l, np.float32), return_inverse=True)
-        return np.array([self.weight(float(x), R) for x in values], dtype=object)[place]
+        return np.array([self.weight(float(x), R) for x in values], dtype=np.int64)[place]
 
 
 def place(u, total):
@@ -81,5 +81,25 @@ def draw_whole(logits, u, t=1.0):
             break
         at -= s
     token = i * RUN + first_past(own[i], at << under[i])
-    log2 = float(l[token]) * w.c - R - math.log2(total / 2 ** w.q)
-    return token, 0.0 if int(own[i][token - i * RUN]) == total << under[i] else log2 * math.log(2)
+    return token, _log_share(w, l[token], R, int(own[i][token - i * RUN]) == total << under[i], total)
+
+
+def _log_share(w, l, R, alone, total):
+    return 0.0 if alone else (float(l) * w.c - R - math.log2(total / 2 ** w.q)) * math.log(2)
+
+
+def draw_top_p(logits, u, p, t=1.0):
+    """(token, logprob) by top-p, every weight in the units of the row's largest."""
+    l = np.asarray(logits, np.float32)
+    w = Numbers(f32(t), len(l))
+    R = w.top(l.max())
+    own = w.weights(l, R)
+    order = np.argsort(-l, kind="stable")
+    total = int(own.sum())
+    goal = min(max(1, math.ceil(Fraction(f32(p)) * total)), total)
+    n = int(np.nonzero(np.cumsum(own[order]) >= goal)[0][0]) + 1
+    kept = np.zeros_like(own)
+    kept[order[:n]] = own[order[:n]]
+    total = int(kept.sum())
+    token = first_past(kept, place(u, total))
+    return token, _log_share(w, l[token], R, int(kept[token]) == total, total)

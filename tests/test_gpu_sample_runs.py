@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.sample_numbers import draw_whole
+from tests.sample_numbers import draw_top_p, draw_whole
 
 pytestmark = pytest.mark.gpu
 BF, F32, I32 = torch.bfloat16, torch.float32, torch.int32
@@ -68,3 +68,24 @@ def test_draws_inside_runs_that_weigh_little(pkg, dev, V, dtype):
             want, log = draw_whole(l, u)
             assert tokens[b] == want, (b, u, tokens[b], want)
             assert abs(logs[b] - log) <= 2.0 ** -23 * abs(log) + 1e-7, (b, u, logs[b], log)
+
+
+@pytest.mark.parametrize("V,octaves,p", [(1 << 20, 43.2, 1 - 2.0 ** -24), (1 << 20, 43.6, 1 - 2.0 ** -24),
+                                         (1 << 20, 34, 0.99999), (1 << 20, 31.9, 0.99999), (1 << 20, 32.1, 0.9999),
+                                         (1 << 24, 39.4, 1 - 2.0 ** -16), (1 << 24, 36, 1 - 2.0 ** -13)])
+def test_top_p_whose_border_lies_in_the_far_tail(pkg, dev, V, octaves, p):
+    """A token that weighs nearly all, and a tail that weighs together as much as top-p
+    leaves out: each of its tokens nothing in the row's units, or a few."""
+    print(f"[gpu] sample far tail {V} {octaves} {p}", flush=True)
+    rows = []
+    for at in (0, V // 2 + 3, V - 1):
+        l = np.full(V, -octaves * math.log(2), np.float32)
+        l[at] = 0.0
+        rows.append(l)
+    logits = aligned(rows, F32, dev)
+    for u in (0.0, 0.5, 1 - 2.0 ** -24):
+        token, log = pkg.sample(logits, torch.full((3,), u, device=dev), top_p=p)
+        for b, l in enumerate(rows):
+            want, share = draw_top_p(l, u, p)
+            assert token[b].item() == want, (b, u, token[b].item(), want)
+            assert abs(log[b].item() - share) <= 2.0 ** -23 * abs(share) + 1e-7, (b, u, log[b].item(), share)
