@@ -9,8 +9,10 @@
 // With y = l log2 e / t, weights are whole numbers W = round(2^(q + y - R)), from a
 // polynomial in 64 bits (to 2^-40), R a whole number not under M's y and q as large as
 // V W < 2^62 allows, 51 at most: sums of them are exact, so no order of adding and no
-// atomic changes what a row gives, and a border is where 64 bits put it.  What rounds to
-// zero cannot be drawn and takes no part.
+// atomic changes what a row gives.  What rounds to zero cannot be drawn and takes no part.
+// Rows that need the sum of all logits take it by parts of 8 192 from the first on,
+// wherever the row lies, each part over its own R; a part's sum enters the row's rounded
+// down to the row's units, and a draw that falls into a part finds its token in the part's.
 //
 // Nothing is sorted.  A threshold that the border of top-k or top-p cannot lie above
 // is found first; the tokens down to it, if there are no more than kList, become a
@@ -20,8 +22,7 @@
 // * Top-k of up to 1 024: the threads' largest logits are counted by steps of
 //   2^(1/32); where k of them lie above, so many tokens do.  A larger k: all logits are.
 // * Top-p, and rows without either: sample_parts_kernel has summed each part of 8 192
-//   logits, for top-p by steps of 2^(1/16), over its own R (a part's sums are shifted to
-//   the row's R where they meet).  Of top-p rows that keep more than kList the tokens of the
+//   logits, for top-p by steps of 2^(1/16).  Of top-p rows that keep more than kList the tokens of the
 //   border's step alone become the list; the draw finds its part by the parts' sums and
 //   walks that one.  Where min-p lies above the border's step its tokens are the list.
 //
@@ -53,7 +54,7 @@ constexpr int kOwnList = 2048; // logits of a row that is its own list, at most
 constexpr int kFew = 128;      // tokens that are compared each with each
 constexpr int kPart = 8192;    // logits of a part
 constexpr int kDigit = 9, kBins = 1 << kDigit;  // bits of a select's pass
-constexpr int kMostParts = (1 << 24) / kPart + 2;
+constexpr int kMostParts = (1 << 24) / kPart;
 
 struct SampleArgs {
   const char* logits;
@@ -206,6 +207,13 @@ template <typename T, int NT> struct Row {
     constexpr uint32_t nan = E == 4 ? 0x7fc00000u : 0x7fc07fc0u;
     return u32x4_t{nan, nan, nan, nan};
   }
+  // w with the logit of index i in its place j.
+  __device__ __forceinline__ void put(u32x4_t& w, int j, int i) const {
+    if constexpr (E == 4)
+      w[j] = __float_as_uint(p[i]);
+    else
+      w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | static_cast<uint32_t>(p[i]) << 16 : (w[j / 2] & 0xffff0000u) | p[i];
+  }
   // Vector v + lane: logits E (v + lane) - off ...; those outside the row, and those of
   // vectors from `end` on, as NaN.
   __device__ __forceinline__ u32x4_t raw(int v, int end) const {
@@ -216,13 +224,42 @@ template <typename T, int NT> struct Row {
     if (i >= 0 && i + E <= V) return *at(v + lane);
 #pragma unroll
     for (int j = 0; j < E; ++j)
-      if (i + j >= 0 && i + j < V) {
-        if constexpr (E == 4)
-          w[j] = __float_as_uint(p[i + j]);
-        else
-          w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | static_cast<uint32_t>(p[i + j]) << 16 : (w[j / 2] & 0xffff0000u) | p[i + j];
-      }
+      if (i + j >= 0 && i + j < V) put(w, j, i + j);
     return w;
+  }
+  // a, the first `off` logits of it those of b.
+  __device__ __forceinline__ u32x4_t headed(u32x4_t a, u32x4_t b) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t of_b;
+      if constexpr (E == 4)
+        of_b = k < off ? 0xffffffffu : 0u;
+      else
+        of_b = (2 * k < off ? 0xffffu : 0u) | (2 * k + 1 < off ? 0xffff0000u : 0u);
+      a[k] = (b[k] & of_b) | (a[k] & ~of_b);
+    }
+    return a;
+  }
+  // A lane's share of a part's logits, in any order.  The part's vectors are those from
+  // part kPart / E on; its first holds the last `off` logits of the part before, in whose
+  // places its own last ones are put, which lie in the vector behind.
+  template <int kHeld>
+  __device__ __forceinline__ void share(int part, u32x4_t (&held)[kHeld]) const {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int v0 = part * (kPart / E) + wave * 64 * kHeld, begin = part * kPart;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) held[k] = raw(v0 + 64 * k, n);
+    if (wave > 0 || off == 0) return;
+    u32x4_t last = nothing();
+    const int i = begin + kPart - off;
+    if (i + E <= V) {
+      last = *at(v0 + kPart / E);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (j < off && i + j < V) put(last, j, i + j);
+    }
+    if (lane == 0) held[0] = headed(held[0], last);
   }
   __device__ __forceinline__ static void wide(u32x4_t w, float (&x)[E]) {
 #pragma unroll
@@ -615,10 +652,8 @@ __global__ __launch_bounds__(NT) void sample_parts_kernel(SampleArgs a) {
   if (!rules.by_parts()) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const R row(a, b);
-  const int first = part * (kPart / E) + wave * 64 * kHeld;
   u32x4_t held[kHeld];
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k) held[k] = row.raw(first + 64 * k, row.n);
+  row.share(part, held);
   fill_table(tab);
   if (rules.by_p)
     for (int i = tid; i < kSteps; i += NT) hist[i] = 0;
@@ -899,6 +934,12 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     for (int attempt = all ? 0 : 1; attempt < (band ? 2 : 1) && !from_list && (all || band); ++attempt) {
       const bool alone = attempt == 1;
       const float most = alone ? to : INFINITY;
+      // (what is not of the step that stands alone leaves a hole)
+      auto entry = [&](float l, uint32_t i) -> uint64_t {
+        const bool of = !alone || (l >= wt.lowest && (wide == 2 ? wt.step(l) : wt.step(l) >> 1) == border);
+        return of ? static_cast<uint64_t>(key_of(l)) << 32 | i : 0;
+      };
+      if (tid == 0) s.few = 0;
       __syncthreads();
       // first into places of the wave's own (in s.weight), then together
       constexpr int kSlots = kList / kWaves;
@@ -921,11 +962,16 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
         const int at = static_cast<int>(__builtin_amdgcn_readlane(places, wave)) - mine_n;
         for (int i = lane; i < mine_n; i += 64) {
           const uint64_t x = slots[i];
-          const float l = __uint_as_float(static_cast<uint32_t>(x >> 32));
-          // (what is not of the step that stands alone leaves a hole)
-          const bool of = !alone || (l >= wt.lowest && (wide == 2 ? wt.step(l) : wt.step(l) >> 1) == border);
-          s.list[at + i] = of ? static_cast<uint64_t>(key_of(l)) << 32 | static_cast<uint32_t>(x) : 0;
+          s.list[at + i] = entry(__uint_as_float(static_cast<uint32_t>(x >> 32)), static_cast<uint32_t>(x));
         }
+      } else if (by_parts && n <= kList) {
+        // Which wave meets a token goes by the row's address; whether there is a list must
+        // not: top-p sums a list in the row's units and other tokens in their parts'.
+        row.template part<4>(wave, 0, row.n, [&](int i, const float(&x)[E]) {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (x[j] >= from && x[j] <= most) s.list[atomicAdd(&s.few, 1u)] = entry(x[j], static_cast<uint32_t>(i + j));
+        });
       } else {
         n = kList + 1;
       }
@@ -1080,7 +1126,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     if (listed) return;
     const float key_l = cut.key ? of_key(cut.key) : -INFINITY;
     const uint32_t to = cut.index;
-    int v0 = 0, v1 = row.n;
+    int begin = 0, v0 = 0, v1 = row.n;  // of a part: its first logit, and its vectors
     uint64_t at = 0;
     double total = 0.0, total_r = 0.0;
     bool need_total = true;
@@ -1088,7 +1134,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       // The parts' sums of what is kept: of top-p the steps before the border's, and of
       // its step what the cut keeps.
       __syncthreads();
-      constexpr int kVectors = kPart / E;
       if (WHAT == kAnyRow && by_p) {
         for (int p = tid; p < a.parts; p += NT) {
           const int end = border - 16 * static_cast<int>(fminf(s.under[p], 63.f));
@@ -1099,7 +1144,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
           const uint64_t x = s.list[i];
           const uint32_t ky = static_cast<uint32_t>(x >> 32), index = static_cast<uint32_t>(x);
           if (ky == 0 || !cut.keeps(ky, index)) continue;
-          const int p = (static_cast<int>(index) + row.off) / E / kVectors;
+          const int p = static_cast<int>(index) / kPart;
           Weights w = wt;
           w.set(s.part_max[p], a.q);
           atomicAdd(&s.kept[p], static_cast<unsigned long long>(w.of(of_key(ky), w.lowest)));
@@ -1135,18 +1180,20 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       at = s.at;
       total = static_cast<double>(s.total);
       total_r = total * per_unit;
-      v0 = s.part * kVectors;
-      v1 = v0 + kVectors < row.n ? v0 + kVectors : row.n;
+      begin = s.part * kPart;
+      v0 = begin / E;
+      v1 = v0 + kPart / E < row.n ? v0 + kPart / E : row.n;
       need_total = false;
     }
     // The draw: every wave sums what its part of the row keeps, then of the part in
     // which the draw lies, until one step of a wave holds the rest.
     Weights w = wt;  // in the units of the row, or of its part
-    if (!need_total) w.set(s.part_max[s.part], a.q);
+    const bool by_part = !need_total;
+    if (by_part) w.set(s.part_max[s.part], a.q);
     // (the part's sum counts what weighs something in the part's units, under the row's
     // lowest too: a draw that falls into its part finds a token there.  Of top-p the cut lies
     // above the row's lowest and min-p's.)
-    const float low = fmaxf(need_total ? fmaxf(floor_l, key_l) : key_l, w.lowest);
+    const float low = fmaxf(by_part ? key_l : fmaxf(floor_l, key_l), w.lowest);
     auto weight = [&](float l, int i) -> uint64_t {
       uint64_t x = w.whole(l);
       if (peaked) x = 1;
@@ -1183,11 +1230,18 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       v0 += pick(sum) * per;
       v1 = v0 + per < v1 ? v0 + per : v1;
     }
-    uint64_t of[kHeld], sum = 0;
-    u32x4_t held[kHeld];
+    uint64_t of[kHeld + 1], sum = 0;
+    u32x4_t held[kHeld + 1];
     const int mine0 = v0 + wave * 64 * kHeld;
+    // (where the row begins inside of a vector, a part's last logits lie in the vector behind
+    // its own: the last wave's, one a lane)
+    const int behind = begin + kPart - row.off + lane;
+    const bool has_behind = by_part && wave == kWaves - 1 && lane < row.off && behind < a.V;
+    held[kHeld] = R::nothing();
+    if (has_behind) row.put(held[kHeld], 0, behind);
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) held[h] = row.raw(mine0 + 64 * h, v1);
+    if (wave == 0 && begin > 0 && lane == 0) held[0] = row.headed(held[0], R::nothing());  // (of the part before)
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
       float x[E];
@@ -1197,19 +1251,25 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       for (int j = 0; j < E; ++j) of[h] += weight(x[j], (mine0 + 64 * h + lane) * E - row.off + j);
       sum += of[h];
     }
+    {
+      float x[E];
+      R::wide(held[kHeld], x);
+      of[kHeld] = weight(x[0], behind);
+      sum += of[kHeld];
+    }
     if (pick(sum) != wave) return;
     // of the wave's vectors that with the draw, and the lane's place in front of it
     uint64_t run = 0, before = 0, in = 0;
     u32x4_t it = held[0];
-    int first = mine0;
+    int i = 0;
     bool found = false;
 #pragma unroll
-    for (int h = 0; h < kHeld; ++h) {
+    for (int h = 0; h <= kHeld; ++h) {
       const uint64_t to_here = run + wave_scan(of[h]), all = last_lane(to_here);
       if (!found && all > at) {
         found = true;
         it = held[h];
-        first = mine0 + 64 * h;
+        i = h == kHeld ? behind : (mine0 + 64 * h + lane) * E - row.off;
         before = to_here - of[h];
         in = of[h];
       }
@@ -1218,7 +1278,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     if (found && before <= at && at < before + in) {
       float x[E];
       R::wide(it, x);
-      const int i = (first + lane) * E - row.off;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const uint64_t y = weight(x[j], i + j);
@@ -1236,14 +1295,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
 // 8.1 | 10.4 | 13 and, of parts, 9 | 24 | 25.  A list of 4 096 leaves room for one
 // workgroup a CU.
 bool own_list(const srw_sample_t& d) { return d.V <= (d.top_k || d.top_k_all > 0 ? kOwnList / 2 : kOwnList); }
-// Parts of a row (0: it is its own list): its vectors are one more where it begins
-// inside of one.
-int64_t parts_of(const srw_sample_t& d) {
-  if (own_list(d)) return 0;
-  const int64_t size = d.dtype == SRW_F32 ? 4 : 2, E = 16 / size;
-  const bool whole = (reinterpret_cast<uintptr_t>(d.logits) | (d.B > 1 ? d.row_stride * size : 0)) % 16 == 0;
-  return ((d.V + E - 1) / E + (whole ? 0 : 1) + kPart / E - 1) / (kPart / E);
-}
+// Parts of a row (0: it is its own list).
+int64_t parts_of(const srw_sample_t& d) { return own_list(d) ? 0 : (d.V + kPart - 1) / kPart; }
 // Whether a row may ask for its parts' sums.
 bool by_parts(const srw_sample_t& d) {
   if (own_list(d)) return false;

@@ -59,9 +59,10 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     number inside (NaN as 0).
 
     Weights are summed as whole numbers, in units of 2^-51 to 2^-50 of the largest (of
-    more than 2048 logits so that the sum stays below 2^62), and top-p's border and the
-    token are exact in these: a row's token goes by its own numbers alone, not by the
-    batch."""
+    more than 2048 logits so that the sum stays below 2^62); of more than 8192, where the
+    sum of all is needed, by runs of 8192 in units of each run's largest, rounded down to
+    the row's.  What weighs nothing in these is not drawn.  A row's token goes by its own
+    numbers alone, not by the batch or by where the row lies."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be a tensor [B, vocab]")
     if logits.is_cuda:

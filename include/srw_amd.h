@@ -586,9 +586,13 @@ srw_status_t srw_attention_kept(const srw_attention_t* a, const int32_t* keep, i
  * Parameters are device arrays of B or, where the array is NULL, the number beside it,
  * which is checked.  In arrays a temperature that is not above 0 counts as 0, a top_k
  * below 1 as off, a top_p that is not below 1 as off, a min_p that is not above 0 as
- * off and one above 1 as 1; u is taken into [0, 1).  Sums are of whole numbers (weights
+ * off and one above 1 as 1; u is taken into [0, 1).  Sums are of whole numbers: weights
  * in units of 2^(R - q), 2^R the power of two at or above the largest, q = min(51,
- * 62 - ceil(log2 V))): results do not go by the batch or the order of adding.
+ * 62 - ceil(log2 V)).  A row of more than 8 192 logits whose tokens come from all of them
+ * or by top_p without top_k is summed by runs of 8 192 from the first on, each in units of
+ * its own largest; its sum enters the row's rounded down to the row's units.  A row's
+ * result goes by its logits, u and parameters alone: not by the batch, the row's address
+ * or the order of adding.
  *
  * Rows of more than 2 048 logits that may draw from all of them or by top_p without top_k
  * need a workspace, 16-byte aligned: without it the call returns SRW_EWORKSPACE and

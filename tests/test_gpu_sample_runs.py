@@ -89,3 +89,95 @@ def test_top_p_whose_border_lies_in_the_far_tail(pkg, dev, V, octaves, p):
             want, share = draw_top_p(l, u, p)
             assert token[b].item() == want, (b, u, token[b].item(), want)
             assert abs(log[b].item() - share) <= 2.0 ** -23 * abs(share) + 1e-7, (b, u, log[b].item(), share)
+
+
+RULES = [{}, dict(top_p=0.5), dict(top_p=0.93), dict(top_p=0.9995), dict(top_p=0.9, min_p=0.03), dict(min_p=1e-3),
+         dict(top_k=7), dict(top_k=900), dict(top_k=3000), dict(top_k=200, top_p=0.8), dict(temperature=0.0),
+         dict(temperature=0.31), dict(temperature=2.5, top_p=0.99)]
+
+
+def anywhere(l, dtype, dev, B=9):
+    """B rows that all hold l and begin at every place of a 16-byte vector."""
+    V = len(l)
+    stride = V + 3 if V % 2 == 0 else V + 2
+    held = torch.full((B * stride + 8,), 50.0, dtype=dtype, device=dev)      # (larger than what the rows hold)
+    logits = held[:B * stride].as_strided((B, V), (stride, 1))
+    logits.copy_(torch.as_tensor(l).to(dtype).to(dev).expand(B, -1))
+    return logits, logits[4:5]
+
+
+def same_anywhere(pkg, dev, l, dtype, rules, us):
+    one = aligned([np.asarray(l, np.float32)], dtype, dev)
+    many, other = anywhere(l, dtype, dev)
+    for rule in rules:
+        for u in us:
+            token, log = pkg.sample(one, torch.full((1,), u, device=dev), **rule)
+            for logits in (many, other):
+                got = pkg.sample(logits, torch.full((logits.shape[0],), u, device=dev), **rule)
+                assert (got[0] == token).all(), (rule, u, token.tolist(), got[0].tolist())
+                assert (got[1] == log).all(), (rule, u, log.tolist(), got[1].tolist())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [1500, 2047, 2100, 8192, 8193, 16385, 40001])
+def test_rows_give_the_same_wherever_they_lie(pkg, dev, V, dtype):
+    """Bit for bit, in other batches and from every address."""
+    print(f"[gpu] sample anywhere {V} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(V)
+    l = (3 * torch.randn(V, generator=g)).numpy()
+    us = torch.rand(3, generator=g).tolist() + [0.0, 1 - 2.0 ** -24]
+    same_anywhere(pkg, dev, l, dtype, RULES, us)
+    same_anywhere(pkg, dev, np.sort(l), dtype, RULES[:6], us)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [16385, 40001])
+@pytest.mark.parametrize("at", [8187, 8191, 8192, 8195, 16383, 16384])
+def test_a_large_logit_at_a_runs_border(pkg, dev, V, at, dtype):
+    """Over tails whose tokens weigh nothing beside it, and something in a run without it;
+    the last logits of runs drawn too."""
+    print(f"[gpu] sample border {V} {at} {dtype}", flush=True)
+    for octaves in (47.3, 49, 52):
+        l = np.full(V, float(torch.tensor(-octaves * math.log(2)).to(dtype)), np.float32)
+        l[at] = 0.0
+        for u in (0.0, 0.5, 1 - 2.0 ** -24):
+            want, log = draw_whole(l, u)
+            logits, _ = anywhere(l, dtype, dev)
+            token, share = pkg.sample(logits, torch.full((logits.shape[0],), u, device=dev))
+            assert (token == want).all(), (u, want, token.tolist())
+            assert ((share - log).abs() <= 2.0 ** -23 * abs(log) + 1e-7).all()
+        same_anywhere(pkg, dev, l, dtype, [{}, dict(top_p=0.9), dict(top_k=2), dict(min_p=0.5)], [0.0, 0.7])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [24576, 24583])
+def test_draws_of_a_runs_last_logits(pkg, dev, V, dtype):
+    """Every token alike, u at each of the last and first ones of the runs."""
+    print(f"[gpu] sample last of runs {V} {dtype}", flush=True)
+    logits, _ = anywhere(np.zeros(V, np.float32), dtype, dev)
+    for i in [*range(8182, 8196), *range(16380, 16388), *range(24570, V), V - 1]:
+        u = float(np.float32((i + 0.5) / V))
+        token, log = pkg.sample(logits, torch.full((logits.shape[0],), u, device=dev))
+        assert (token == draw_whole(np.zeros(V, np.float32), u)[0]).all(), (i, token.tolist())
+        assert ((log + math.log(V)).abs() < 1e-6).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+def test_whether_top_p_lists_tokens_goes_by_their_number(pkg, dev, dtype):
+    """512 equal logits, 257 of them a wave's where the row begins inside of a vector, over a run that adds
+    a few units to the sum: top-p of a half keeps one more than a half of them."""
+    print(f"[gpu] sample lists {dtype}", flush=True)
+    E = 4 if dtype == F32 else 8
+    V, q = 70001, 45
+    l = np.full(V, -200.0, np.float32)
+    wave = 64 * E                                    # a wave's next logits, every 16 waves
+    places = [16 * wave * j + i for j in range(2) for i in range(128)] + [wave]
+    rest = iter(range(2 * wave, 16 * wave, 7))
+    while len(places) < 512:
+        places.append(next(rest))
+    l[places] = 0.0
+    low = float(torch.tensor(-50 * math.log(2)).to(dtype))
+    l[65536:65536 + 4000] = low                      # nothing each in the row's units, some 120 together
+    same_anywhere(pkg, dev, l, dtype, [dict(top_p=0.5), dict(top_p=0.25)], [0.0, 0.3, 0.75, 1 - 2.0 ** -24])
+    token, _ = pkg.sample(torch.tensor(l).to(dtype).to(dev)[None], torch.full((1,), 1 - 2.0 ** -24, device=dev), top_p=0.5)
+    assert token.item() == sorted(places)[256]
