@@ -43,6 +43,7 @@
 
 #include "srw_internal.hpp"
 #include "srw_mfma_util.hpp"
+#include "srw_sample.hpp"
 
 namespace srw {
 namespace {
@@ -798,15 +799,13 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     const double x = m + log2_of(fmax(static_cast<double>(rules.least), 0x1p-100), s.tab) * wt.per;
     floor_l = fmaxf(floor_l, -float_under(fmin(-x, 3.4028234663852886e38)));  // (the smallest float that is not below x)
   }
+  // (sums are all lanes': the scalar unit takes their shares)
   auto part = [&](uint64_t total) -> uint64_t {  // what top-p's run has to reach
-    const double x = ceil(static_cast<double>(rules.p) * static_cast<double>(total));
-    const uint64_t y = x >= 1.0 ? static_cast<uint64_t>(x) : 1;
-    return y < total ? y : total;
+    return rules.p > 0.f ? share_of<true>(rules.p, lane_of(total, 0)) : 1;
   };
   auto place = [&](uint64_t total) -> uint64_t {  // of the draw in [0, total)
-    const double of = static_cast<double>(total), x = u > 0.f ? static_cast<double>(u) * of : 0.0;
-    const uint64_t at = x < of ? static_cast<uint64_t>(x) : total;
-    return at < total ? at : total - 1;
+    total = lane_of(total, 0);
+    return !(u > 0.f) ? 0 : u < 1.f ? share_of<false>(u, total) : total - 1;
   };
   // The token and the logarithm of its share: weight and total in one unit, the total
   // also in units of 2^R.
@@ -967,11 +966,10 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       } else if (by_parts && n <= kList) {
         // Which wave meets a token goes by the row's address; whether there is a list must
         // not: top-p sums a list in the row's units and other tokens in their parts'.
-        row.template part<4>(wave, 0, row.n, [&](int i, const float(&x)[E]) {
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (x[j] >= from && x[j] <= most) s.list[atomicAdd(&s.few, 1u)] = entry(x[j], static_cast<uint32_t>(i + j));
-        });
+        for (int i = tid; i < a.V; i += NT) {
+          const float l = row.one(i);
+          if (l >= from && l <= most) s.list[atomicAdd(&s.few, 1u)] = entry(l, static_cast<uint32_t>(i));
+        }
       } else {
         n = kList + 1;
       }
@@ -1230,18 +1228,17 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       v0 += pick(sum) * per;
       v1 = v0 + per < v1 ? v0 + per : v1;
     }
-    uint64_t of[kHeld + 1], sum = 0;
-    u32x4_t held[kHeld + 1];
+    uint64_t of[kHeld], sum = 0;
+    u32x4_t held[kHeld];
     const int mine0 = v0 + wave * 64 * kHeld;
-    // (where the row begins inside of a vector, a part's last logits lie in the vector behind
-    // its own: the last wave's, one a lane)
-    const int behind = begin + kPart - row.off + lane;
-    const bool has_behind = by_part && wave == kWaves - 1 && lane < row.off && behind < a.V;
-    held[kHeld] = R::nothing();
-    if (has_behind) row.put(held[kHeld], 0, behind);
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) held[h] = row.raw(mine0 + 64 * h, v1);
-    if (wave == 0 && begin > 0 && lane == 0) held[0] = row.headed(held[0], R::nothing());  // (of the part before)
+    // (a part that begins inside of a vector: that vector's first logits are of the part
+    // before, and as many of its own lie behind its vectors, one a lane of the last wave)
+    const int behind = begin + kPart - row.off + lane;
+    const bool ends = by_part && row.off > 0 && wave == kWaves - 1;
+    const float x_behind = ends && lane < row.off && behind < a.V ? row.one(behind) : __uint_as_float(0x7fc00000u);
+    if (wave == 0 && begin > 0 && lane == 0) held[0] = row.headed(held[0], R::nothing());
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
       float x[E];
@@ -1251,12 +1248,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
       for (int j = 0; j < E; ++j) of[h] += weight(x[j], (mine0 + 64 * h + lane) * E - row.off + j);
       sum += of[h];
     }
-    {
-      float x[E];
-      R::wide(held[kHeld], x);
-      of[kHeld] = weight(x[0], behind);
-      sum += of[kHeld];
-    }
+    if (ends) sum += weight(x_behind, behind);
     if (pick(sum) != wave) return;
     // of the wave's vectors that with the draw, and the lane's place in front of it
     uint64_t run = 0, before = 0, in = 0;
@@ -1264,25 +1256,35 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
     int i = 0;
     bool found = false;
 #pragma unroll
-    for (int h = 0; h <= kHeld; ++h) {
+    for (int h = 0; h < kHeld; ++h) {
       const uint64_t to_here = run + wave_scan(of[h]), all = last_lane(to_here);
       if (!found && all > at) {
         found = true;
         it = held[h];
-        i = h == kHeld ? behind : (mine0 + 64 * h + lane) * E - row.off;
+        i = (mine0 + 64 * h + lane) * E - row.off;
         before = to_here - of[h];
         in = of[h];
       }
       run = all;
     }
+    if (!found && ends) {  // one of those behind
+      found = true;
+      it = R::nothing();
+      it[0] = E == 8 ? __float_as_uint(x_behind) >> 16 | 0x7fc00000u : __float_as_uint(x_behind);
+      i = behind;
+      in = weight(x_behind, behind);
+      before = run + wave_scan(in) - in;
+    }
     if (found && before <= at && at < before + in) {
-      float x[E];
-      R::wide(it, x);
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const uint64_t y = weight(x[j], i + j);
+#pragma unroll 1
+      for (int j = 0; j < E; ++j) {  // (once in the code: one lane's few logits)
+        const int d = j / (E / 4);
+        uint32_t bits = d < 2 ? (d == 0 ? it[0] : it[1]) : d == 2 ? it[2] : it[3];
+        if (E == 8) bits = j & 1 ? bits & 0xffff0000u : bits << 16;
+        const float l = __uint_as_float(bits);
+        const uint64_t y = weight(l, i + j);
         if (before <= at && at < before + y)
-          done(i + j, x[j], ldexp(static_cast<double>(y), w.R - wt.R), total, total_r);
+          done(i + j, l, ldexp(static_cast<double>(y), w.R - wt.R), total, total_r);
         before += y;
       }
     }

@@ -1,0 +1,26 @@
+// srw_sample.hpp -- the whole-number arithmetic of sampling that host and device share
+// (srw_sample.hip).
+#pragma once
+
+#include <stdint.h>
+
+#include <hip/hip_runtime.h>
+
+namespace srw {
+
+// f times total, 0 < f < 1, rounded to the whole number below or (UP) above: f has 24
+// bits, total 62 at most.
+template <bool UP>
+__host__ __device__ inline uint64_t share_of(float f, uint64_t total) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, f), e = bits >> 23, m = (bits & 0x7fffffu) | (e ? 0x800000u : 0u);
+  const int s = 150 - static_cast<int>(e ? e : 1);  // f = m 2^-s, s at least 24
+  const uint64_t b = static_cast<uint64_t>(m) * static_cast<uint32_t>(total);
+  const uint64_t high = static_cast<uint64_t>(m) * static_cast<uint32_t>(total >> 32) + (b >> 32);  // under 2^55
+  const uint32_t low = static_cast<uint32_t>(b);  // m total = high 2^32 + low
+  const int d = s < 32 ? 0 : s < 95 ? s - 32 : 63, l = s < 32 ? s : 32;
+  const uint64_t whole = (high >> d) << (32 - l) | (static_cast<uint64_t>(low) >> l);
+  const bool rest = (high & ((uint64_t{1} << d) - 1)) != 0 || (low & ((uint64_t{1} << l) - 1)) != 0;
+  return UP ? whole + rest : whole;
+}
+
+}  // namespace srw

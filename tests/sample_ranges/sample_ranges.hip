@@ -1,0 +1,52 @@
+// CPU: the whole-number arithmetic that sampling shares with the host (srw_sample.hpp).
+// Host code only: no kernel is built or launched.
+//   sample_ranges shares    u and p times a sum
+#include <math.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <random>
+
+#include "srw_sample.hpp"
+
+static long long failures = 0, checks = 0;
+static void expect(bool ok, const char* what, double a, unsigned long long b, unsigned long long c) {
+  ++checks;
+  if (!ok && ++failures <= 20) printf("FAIL %s: %.17g %llu %llu\n", what, a, b, c);
+}
+
+// f total in 128 bits: f = m 2^-s.
+static void share(float f, uint64_t total) {
+  int e;
+  const float part = frexpf(f, &e);  // f = part 2^e, part of 24 bits in [1/2, 1)
+  const unsigned __int128 product = static_cast<unsigned __int128>(static_cast<uint32_t>(ldexpf(part, 24))) * total;
+  const int s = 24 - e;
+  const unsigned __int128 whole = s < 128 ? product >> s : 0;
+  const bool rest = (s < 128 ? whole << s : 0) != product;
+  const uint64_t under = srw::share_of<false>(f, total), over = srw::share_of<true>(f, total);
+  expect(under == static_cast<uint64_t>(whole), "under", f, total, under);
+  expect(over == static_cast<uint64_t>(whole) + rest, "over", f, total, over);
+  expect(under < total && over >= 1 && over <= total, "range", f, under, over);
+}
+
+static void shares() {
+  std::mt19937_64 g(1);
+  const float ends[] = {1e-45f, 3e-45f, 1.1754942e-38f, 1.1754944e-38f, 5.9604645e-8f, 0.25f, 0.5f, 0.99999994f, 0.1f,
+                        5.421010862427522e-20f, 2.7105054e-20f, 1.0842022e-19f, 3.2311743e-27f, 6.4623485e-27f};
+  for (int b = 0; b <= 62; ++b)
+    for (const uint64_t t : {uint64_t{1} << b, (uint64_t{1} << b) + 1, (uint64_t{1} << b) - 1 + (b == 0)}) {
+      for (const float f : ends) share(f, t ? t : 1);
+      for (int i = 0; i < 2000; ++i) {
+        const float f = ldexpf(static_cast<float>((g() >> 41) + 1), -24 - static_cast<int>(g() % 90));
+        share(f < 1.f ? f : 0.5f, t ? t : 1);
+      }
+    }
+  for (int i = 0; i < 2000000; ++i) share(static_cast<float>((g() >> 40) | 1) * 5.9604645e-8f, (g() >> (2 + g() % 60)) | 1);
+}
+
+int main(int argc, char** argv) {
+  if (argc < 2) return 2;
+  if (!strcmp(argv[1], "shares")) shares();
+  printf("%lld checks, %lld failures\n", checks, failures);
+  return failures ? 1 : 0;
+}

@@ -181,3 +181,29 @@ def test_whether_top_p_lists_tokens_goes_by_their_number(pkg, dev, dtype):
     same_anywhere(pkg, dev, l, dtype, [dict(top_p=0.5), dict(top_p=0.25)], [0.0, 0.3, 0.75, 1 - 2.0 ** -24])
     token, _ = pkg.sample(torch.tensor(l).to(dtype).to(dev)[None], torch.full((1,), 1 - 2.0 ** -24, device=dev), top_p=0.5)
     assert token.item() == sorted(places)[256]
+
+
+def test_sums_of_more_than_53_bits(pkg, dev):
+    """u and p of a half over sums of 2^61 and a few units: the border lies among tokens of
+    a unit each, or in a run of some hundred units."""
+    print("[gpu] sample halves", flush=True)
+    u = lambda x: torch.full((1,), x, device=dev)  # noqa: E731
+    l = np.zeros(1027, np.float32)
+    l[512:515] = -51 * math.log(2)                    # one unit each, behind 2^60 and before 2^60
+    row = torch.tensor(l, device=dev)[None]
+    # 2^60 + 1 of 2^61 + 3 units: the second of them
+    assert draw_whole(l, 0.5)[0] == 513
+    assert pkg.sample(row, u(0.5))[0].item() == 513
+    # top-p reaches 2^60 + 1.5: 513 of the large ones
+    assert draw_top_p(l, 1 - 2.0 ** -24, 0.5)[0] == 515
+    assert pkg.sample(row, u(1 - 2.0 ** -24), top_p=0.5)[0].item() == 515
+    assert pkg.sample(row, u(1 - 2.0 ** -24), top_p=0.5, top_k=1026)[0].item() == 515
+    for V, far in ((24576, 53.0), (24576, 55.5), (24577, 54.0)):
+        l = np.zeros(V, np.float32)
+        l[8192:16384] = -far * math.log(2)
+        for dtype in (F32, BF):
+            l = torch.tensor(l).to(dtype).float().numpy()
+            for x in (0.5, 0.25, 0.75, 0.3):
+                want, log = draw_whole(l, x)
+                token, share = both(pkg, aligned([l], dtype, dev), u(x))
+                assert token == [want] and abs(share[0] - log) <= 2.0 ** -23 * abs(log) + 1e-7, (V, far, x, token, want)
