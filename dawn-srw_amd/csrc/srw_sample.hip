@@ -154,7 +154,7 @@ struct Weights {
     double p = fma(0x1.c6b095a17a14dp-5, r, 0x1.ebfbeebe2d1a2p-3);
     p = fma(p, r, 0x1.62e42fefa39efp-1);
     p = fma(p, r, 1.0) * tab[n & 127];
-    p = __hiloint2double(__double2hiint(p) + (((n >> 7) - R) << 20), __double2loint(p));
+    p = __hiloint2double(at_octave(__double2hiint(p), n, R), __double2loint(p));
     // the low bits of a sum whose last place is 2^-q
     return static_cast<uint64_t>(__double_as_longlong(p + unit)) & 0xfffffffffffffull;
   }
@@ -164,7 +164,7 @@ struct Weights {
   }
   // steps of 2^(1/32) under 2^R
   __device__ __forceinline__ int step(float l) const {
-    const int n = 128 * R - n_of(sum_of(l));
+    const int n = steps_under(R, n_of(sum_of(l)));
     return n < 4 * kSteps ? n >> 2 : kSteps - 1;
   }
 };
@@ -180,7 +180,7 @@ __device__ __forceinline__ double log2_of(double x, const double* tab) {
   double p = fma(0x1.c6b095a17a14dp-5, r, 0x1.ebfbeebe2d1a2p-3);
   p = fma(p, r, 0x1.62e42fefa39efp-1);
   p = fma(p, r, 1.0) * tab[n & 127];
-  p = __hiloint2double(__double2hiint(p) + ((n >> 7) << 20), __double2loint(p));  // 2^l
+  p = __hiloint2double(at_octave(__double2hiint(p), n, 0), __double2loint(p));  // 2^l
   const double e = (x - p) / p;                                                   // some 1e-7
   return y + e * (1.0 - 0.5 * e) * 1.4426950408889634;
 }

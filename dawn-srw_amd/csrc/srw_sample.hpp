@@ -23,4 +23,15 @@ __host__ __device__ inline uint64_t share_of(float f, uint64_t total) {
   return UP ? whole + rest : whole;
 }
 
+// n: the low 32 bits of 128 y, a whole number; |y| and |R| up to 2^30.  128 (R - y), where
+// y lies under 2^24 from R; and the high word of a double times 2^(y rounded down - R),
+// where that is a double.  (128 R alone can pass 32 bits; what lies above them falls out
+// of the difference.)
+__host__ __device__ inline int steps_under(int R, int n) {
+  return static_cast<int>(128u * static_cast<uint32_t>(R) - static_cast<uint32_t>(n));
+}
+__host__ __device__ inline int at_octave(int high, int n, int R) {
+  return static_cast<int>(static_cast<uint32_t>(high) + (static_cast<uint32_t>((n >> 7) - R) << 20));
+}
+
 }  // namespace srw

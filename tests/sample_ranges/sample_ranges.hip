@@ -1,6 +1,7 @@
 // CPU: the whole-number arithmetic that sampling shares with the host (srw_sample.hpp).
 // Host code only: no kernel is built or launched.
 //   sample_ranges shares    u and p times a sum
+//   sample_ranges octaves   octaves under R, over the range of logits and temperatures
 #include <math.h>
 #include <stdio.h>
 #include <string.h>
@@ -44,9 +45,30 @@ static void shares() {
   for (int i = 0; i < 2000000; ++i) share(static_cast<float>((g() >> 40) | 1) * 5.9604645e-8f, (g() >> (2 + g() % 60)) | 1);
 }
 
+// 128 y = 128 (R - octaves) and up to a step beside it.
+static void octave(int R, int octaves, int beside) {
+  const int64_t y = 128 * (static_cast<int64_t>(R) - octaves) + beside;
+  const int n = static_cast<int>(y);
+  expect(srw::steps_under(R, n) == 128 * octaves - beside, "steps", R, octaves, beside);
+  const uint64_t one = static_cast<uint64_t>(static_cast<uint32_t>(srw::at_octave(0x3ff00000, n, R))) << 32;
+  const int64_t whole = y >= 0 ? y / 128 : -((127 - y) / 128);  // rounded down
+  expect(__builtin_bit_cast(double, one) == ldexp(1.0, static_cast<int>(whole - R)), "high word", R, octaves, beside);
+}
+
+static void octaves() {
+  std::mt19937_64 g(2);
+  for (int b = 0; b <= 30; ++b)
+    for (const int R : {1 << b, -(1 << b), (1 << b) - 1, 1 - (1 << b)})
+      for (int o = 0; o < 1000; o += b < 24 ? 7 : 1)
+        for (const int beside : {0, 1, 63, 64, 127}) octave(R, o, beside);
+  for (int i = 0; i < 1000000; ++i)
+    octave(static_cast<int>(g() % (1u << 31)) - (1 << 30), static_cast<int>(g() % 1000), static_cast<int>(g() % 128));
+}
+
 int main(int argc, char** argv) {
   if (argc < 2) return 2;
   if (!strcmp(argv[1], "shares")) shares();
+  if (!strcmp(argv[1], "octaves")) octaves();
   printf("%lld checks, %lld failures\n", checks, failures);
   return failures ? 1 : 0;
 }

@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from tests.sample_numbers import draw_top_p, draw_whole
+from tests.test_gpu_sample import definition, f32
 
 pytestmark = pytest.mark.gpu
 BF, F32, I32 = torch.bfloat16, torch.float32, torch.int32
@@ -207,3 +208,24 @@ def test_sums_of_more_than_53_bits(pkg, dev):
                 want, log = draw_whole(l, x)
                 token, share = both(pkg, aligned([l], dtype, dev), u(x))
                 assert token == [want] and abs(share[0] - log) <= 2.0 ** -23 * abs(log) + 1e-7, (V, far, x, token, want)
+
+
+@pytest.mark.parametrize("t", [1e-5, 1e-6, 1e-7, 2e-8, 1e-8])
+@pytest.mark.parametrize("V", [60, 1000, 3000, 20001])
+def test_very_low_temperatures(pkg, dev, V, t):
+    """Logits a few roundings apart, up to 2^30 octaves over 0 and under it.  A token's
+    octaves are a product of 53 bits, off by 2^-24 at most: so are weights, sums and the
+    logarithm of a share, 2^-23 ln 2 in all, beside what other rows' logprobs are off."""
+    print(f"[gpu] sample cold {V} {t}", flush=True)
+    g = torch.Generator().manual_seed(V)
+    near = torch.randint(0, 40, (6, V), generator=g).float()
+    base = torch.tensor([12.0, -12.0, 10.25, -9.5, 0.75, -0.03])[:, None]
+    logits = base + near * torch.tensor([2.0 ** -20, 2.0 ** -20, 2.0 ** -20, 2.0 ** -20, 2.0 ** -23, 2.0 ** -28])[:, None]
+    u = torch.rand(6, generator=g)
+    for rule in ({}, dict(top_k=V // 3), dict(top_p=0.8), dict(top_k=30, top_p=0.6), dict(min_p=0.2)):
+        token, log = pkg.sample(logits.to(dev), u.to(dev), temperature=t, **rule)
+        for b in range(6):
+            p = {**dict(top_k=0, top_p=1.0, min_p=0.0), **rule}
+            want, share = definition(logits[b], u[b].item(), f32(t), p["top_k"], f32(p["top_p"]), f32(p["min_p"]))
+            assert token[b].item() == want, (rule, b, token[b].item(), want)
+            assert abs(log[b].item() - share) <= 2.0 ** -23 * abs(share) + 1e-7 + 2.0 ** -23 * math.log(2), (rule, b)

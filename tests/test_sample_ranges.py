@@ -38,3 +38,8 @@ def _run(program, what):
 def test_shares_of_a_sum_are_exact(program):
     """u and p times sums of up to 62 bits, against 128 bits."""
     _run(program, "shares")
+
+
+def test_octaves_of_any_temperature(program):
+    """Where a logit lies under the largest, for logits over temperatures up to 2^30."""
+    _run(program, "octaves")
