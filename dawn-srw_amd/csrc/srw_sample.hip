@@ -92,22 +92,6 @@ struct Rules {
   __device__ __forceinline__ bool by_parts() const { return !greedy && !by_k && (by_p || least == 0.f); }
 };
 
-// A number's place among all: larger logits have larger keys, -0 is 0, NaN the
-// smallest.
-__device__ __forceinline__ uint32_t key_of(float l) {
-  const uint32_t b = __float_as_uint(l + 0.f);
-  if (l != l) return 0;
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float of_key(uint32_t k) {
-  return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
-__device__ __forceinline__ float float_under(double x) {  // the largest float that is not above x
-  const float f = static_cast<float>(x);
-  if (!(static_cast<double>(f) > x)) return f;
-  return of_key(key_of(f) - 1);
-}
-
 // 2^(j / 128).
 __device__ __forceinline__ void fill_table(double* tab) {
   if (threadIdx.x < 128) tab[threadIdx.x] = exp2(static_cast<int>(threadIdx.x) / 128.0);
@@ -169,7 +153,8 @@ struct Weights {
   }
 };
 
-// log2 x of x in [2^-30, 2^63]: float32's, mended by what it is off.
+// log2 x of x in [2^-100, 2^63] (min-p's share, sums in units of 2^R): float32's, mended by
+// what it is off.
 __device__ __forceinline__ double log2_of(double x, const double* tab) {
   const float l = __builtin_amdgcn_logf(static_cast<float>(x));
   Weights w;

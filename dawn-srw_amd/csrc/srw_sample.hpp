@@ -2,11 +2,29 @@
 // (srw_sample.hip).
 #pragma once
 
+#include <math.h>
 #include <stdint.h>
 
 #include <hip/hip_runtime.h>
 
 namespace srw {
+
+// A number's place among all: larger logits have larger keys, -0 is 0, NaN the
+// smallest.
+__host__ __device__ inline uint32_t key_of(float l) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, l + 0.f);
+  if (l != l) return 0;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__host__ __device__ inline float of_key(uint32_t k) {
+  return k == 0 ? -INFINITY : __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// The largest float that is not above x.
+__host__ __device__ inline float float_under(double x) {
+  const float f = static_cast<float>(x);
+  if (!(static_cast<double>(f) > x)) return f;
+  return of_key(key_of(f) - (f == 0.f ? 2 : 1));  // (the key under 0's is -0's, which no number has)
+}
 
 // f times total, 0 < f < 1, rounded to the whole number below or (UP) above: f has 24
 // bits, total 62 at most.

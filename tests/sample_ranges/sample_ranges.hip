@@ -1,6 +1,7 @@
 // CPU: the whole-number arithmetic that sampling shares with the host (srw_sample.hpp).
 // Host code only: no kernel is built or launched.
 //   sample_ranges shares    u and p times a sum
+//   sample_ranges unders    the largest float32 under a number
 //   sample_ranges octaves   octaves under R, over the range of logits and temperatures
 #include <math.h>
 #include <stdio.h>
@@ -45,6 +46,26 @@ static void shares() {
   for (int i = 0; i < 2000000; ++i) share(static_cast<float>((g() >> 40) | 1) * 5.9604645e-8f, (g() >> (2 + g() % 60)) | 1);
 }
 
+// float_under(x): a float that is not above x, and the next one is.
+static void under(double x) {
+  const float f = srw::float_under(x), next = nextafterf(f, INFINITY);
+  expect(static_cast<double>(f) <= x && static_cast<double>(next == 0.f ? 0.f : next) > x, "under", x, 0, 0);
+  expect(f == f && srw::of_key(srw::key_of(f)) == f, "key", x, srw::key_of(f), 0);
+}
+
+static void unders() {
+  std::mt19937_64 g(3);
+  for (const double x : {0.0, -0.0, 1e-60, -1e-60, 1e-46, -1e-46, 7e-46, -7e-46, 1.4e-45, -1.4e-45, 2e-45, -2e-45, 1.1754943e-38,
+                         -1.1754943e-38, 1.0, -1.0, 1.0000000001, -1.0000000001, 0.9999999999, 3.4028234663852886e38,
+                         -3.4028234663852886e38, 3.4e38, 16777217.0, -16777217.0})
+    under(x);
+  for (int i = 0; i < 1000000; ++i) {
+    const double x = ldexp(static_cast<double>(g() >> 11), -180 + static_cast<int>(g() % 250));
+    under(x);
+    under(-x);
+  }
+}
+
 // 128 y = 128 (R - octaves) and up to a step beside it.
 static void octave(int R, int octaves, int beside) {
   const int64_t y = 128 * (static_cast<int64_t>(R) - octaves) + beside;
@@ -69,6 +90,7 @@ int main(int argc, char** argv) {
   if (argc < 2) return 2;
   if (!strcmp(argv[1], "shares")) shares();
   if (!strcmp(argv[1], "octaves")) octaves();
+  if (!strcmp(argv[1], "unders")) unders();
   printf("%lld checks, %lld failures\n", checks, failures);
   return failures ? 1 : 0;
 }

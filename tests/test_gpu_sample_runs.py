@@ -229,3 +229,16 @@ def test_very_low_temperatures(pkg, dev, V, t):
             want, share = definition(logits[b], u[b].item(), f32(t), p["top_k"], f32(p["top_p"]), f32(p["min_p"]))
             assert token[b].item() == want, (rule, b, token[b].item(), want)
             assert abs(log[b].item() - share) <= 2.0 ** -23 * abs(share) + 1e-7 + 2.0 ** -23 * math.log(2), (rule, b)
+
+
+@pytest.mark.parametrize("V", [2, 3000])
+def test_min_p_between_zero_and_the_smallest_number(pkg, dev, V):
+    """min-p's border lies between the logits 0 and 2^-149: 0 weighs less than it asks."""
+    print(f"[gpu] sample smallest {V}", flush=True)
+    tiny = 2.0 ** -149
+    l = torch.zeros(1, V)
+    l[0, V // 3] = tiny
+    for least, u in ((0.6, 0.99), (0.6, 0.0), (0.3, 0.99), (0.3, 0.0)):
+        want, share = definition(l[0], u, tiny, 0, 1.0, f32(least))
+        token, log = pkg.sample(l.to(dev), torch.full((1,), u, device=dev), temperature=tiny, min_p=least)
+        assert token.item() == want and abs(log.item() - share) <= 2.0 ** -23 * abs(share) + 1e-7, (least, u, token, want)

@@ -40,6 +40,11 @@ def test_shares_of_a_sum_are_exact(program):
     _run(program, "shares")
 
 
+def test_the_largest_float_under_a_number(program):
+    """Of numbers that round to a zero of either sign too."""
+    _run(program, "unders")
+
+
 def test_octaves_of_any_temperature(program):
     """Where a logit lies under the largest, for logits over temperatures up to 2^30."""
     _run(program, "octaves")
