@@ -1,5 +1,6 @@
-"""Choosing tokens from logits: one HIP kernel (csrc/srw_sample.hip), torch tensors
-in and out.  :func:`sample` takes its random numbers from the caller, so a program
+"""Choosing tokens from logits: HIP kernels (csrc/srw_sample.hip; one for short rows
+and top-k, two where the sum of a long row is needed), torch tensors in and out.
+:func:`sample` takes its random numbers from the caller, so a program
 that keeps them can repeat a run; it waits for nothing and can be captured in a
 graph."""
 

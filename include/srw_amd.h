@@ -594,9 +594,10 @@ srw_status_t srw_attention_kept(const srw_attention_t* a, const int32_t* keep, i
  * result goes by its logits, u and parameters alone: not by the batch, the row's address
  * or the order of adding.
  *
- * Rows of more than 2 048 logits that may draw from all of them or by top_p without top_k
- * need a workspace, 16-byte aligned: without it the call returns SRW_EWORKSPACE and
- * launches nothing.  V up to 2^24, B up to 2^21, and below 2^24 parts of 8 192 logits in
+ * Rows of more than 2 048 logits (1 024 where top_k is an array or its number above 0) that
+ * may draw from all of them or by top_p without top_k need a workspace, 16-byte aligned:
+ * of srw_sample_workspace_size bytes, 0 where none is needed; without it the call returns
+ * SRW_EWORKSPACE and launches nothing.  V up to 2^24, B up to 2^21, and below 2^24 parts of 8 192 logits in
  * all rows together. */
 typedef struct srw_sample {
   const void* logits;
