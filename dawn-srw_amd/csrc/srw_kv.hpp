@@ -130,6 +130,24 @@ __host__ __device__ inline uint64_t kv_seen(int pos, int key0, int window, int s
   return see;
 }
 
+// A tensor's layers: n blocks of bytes, stride (at least as many) apart.
+struct KvBlocks {
+  uintptr_t at;
+  int64_t bytes, stride, n;
+};
+// Whether some block of a and some block of b hold a byte in common.  (Layers of several
+// tensors may lie between each other.)
+inline bool kv_meet(const KvBlocks& a, const KvBlocks& b) {
+  auto end = [](const KvBlocks& t) { return t.at + static_cast<uintptr_t>((t.n - 1) * t.stride + t.bytes); };
+  if (a.n < 1 || b.n < 1 || a.bytes < 1 || b.bytes < 1 || !(a.at < end(b) && b.at < end(a))) return false;
+  for (int64_t i = 0, j = 0; i < a.n && j < b.n;) {
+    const uintptr_t x = a.at + static_cast<uintptr_t>(i * a.stride), y = b.at + static_cast<uintptr_t>(j * b.stride);
+    if (x < y + static_cast<uintptr_t>(b.bytes) && y < x + static_cast<uintptr_t>(a.bytes)) return true;
+    ++(x < y ? i : j);  // (that block ends before the other begins)
+  }
+  return false;
+}
+
 // The page of position pos of sequence b, or -1: past the table, or an entry
 // that names no page.
 __device__ inline int kv_page(const KvView& p, int64_t b, int pos) {

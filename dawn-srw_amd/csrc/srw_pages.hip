@@ -64,12 +64,6 @@ __global__ __launch_bounds__(kCopyThreads) void kv_copy_kernel(CopyArgs a) {
     copy_piece<uint32_t>(src, dst, bytes);
 }
 
-// Whether [a, a + m) and [b, b + n) meet.
-bool meet(const void* a, int64_t m, const void* b, int64_t n) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + static_cast<uintptr_t>(n) && y < x + static_cast<uintptr_t>(m);
-}
-
 srw_status_t check_copy(const srw_kv_copy_t* c) {
   if (!c || c->n_tensors < 0 || c->n_tensors > SRW_KV_COPY_TENSORS) return SRW_EINVAL;
   if (c->n_layers < 0 || c->n_src_pages < 0 || c->n_dst_pages < 0 || c->n_pairs < 0) return SRW_EINVAL;
@@ -77,30 +71,27 @@ srw_status_t check_copy(const srw_kv_copy_t* c) {
   if (c->n_pairs > c->n_dst_pages) return SRW_EINVAL;  // (some page is written twice)
   if (c->n_pairs == 0 || c->n_layers == 0 || c->n_tensors == 0) return SRW_OK;
   if (!aligned(c->src_page, 4) || !aligned(c->dst_page, 4)) return SRW_EINVAL;
-  int64_t src_bytes[SRW_KV_COPY_TENSORS], dst_bytes[SRW_KV_COPY_TENSORS];
+  KvBlocks src[SRW_KV_COPY_TENSORS], dst[SRW_KV_COPY_TENSORS];
   bool inside = false;  // tensors copied within themselves
   for (int i = 0; i < c->n_tensors; ++i) {
     if (c->page_bytes[i] < 1 || c->page_bytes[i] % 4) return SRW_EINVAL;
     if (c->page_bytes[i] > (int64_t{1} << 30)) return SRW_EUNSUPPORTED;
     if (!aligned(c->src[i], 4) || !aligned(c->dst[i], 4)) return SRW_EINVAL;
-    auto span = [&](int64_t stride, int64_t pages, int64_t* bytes) {
-      const int64_t block = pages * c->page_bytes[i];  // below 2^61
-      if (c->n_layers > 1 && (stride < block || stride % 4 || stride > (int64_t{1} << 46))) return false;
-      *bytes = block + (c->n_layers - 1) * (c->n_layers > 1 ? stride : 0);
-      return true;
+    auto blocks = [&](const void* at, int64_t stride, int64_t pages, KvBlocks* b) {
+      *b = {reinterpret_cast<uintptr_t>(at), pages * c->page_bytes[i], c->n_layers > 1 ? stride : 0, c->n_layers};  // below 2^61
+      return c->n_layers == 1 || (stride >= b->bytes && stride % 4 == 0 && stride <= (int64_t{1} << 46));
     };
-    if (!span(c->src_layer_stride[i], c->n_src_pages, &src_bytes[i]) ||
-        !span(c->dst_layer_stride[i], c->n_dst_pages, &dst_bytes[i]))
+    if (!blocks(c->src[i], c->src_layer_stride[i], c->n_src_pages, &src[i]) ||
+        !blocks(c->dst[i], c->dst_layer_stride[i], c->n_dst_pages, &dst[i]))
       return SRW_EINVAL;
   }
   for (int i = 0; i < c->n_tensors; ++i)
     for (int j = 0; j < c->n_tensors; ++j) {
-      if (i < j && meet(c->dst[i], dst_bytes[i], c->dst[j], dst_bytes[j])) return SRW_EINVAL;
-      if (!meet(c->src[i], src_bytes[i], c->dst[j], dst_bytes[j])) continue;
-      if (i != j || c->src[i] != c->dst[i] || c->n_src_pages != c->n_dst_pages ||
-          (c->n_layers > 1 && c->src_layer_stride[i] != c->dst_layer_stride[i]))
+      if (i < j && kv_meet(dst[i], dst[j])) return SRW_EINVAL;
+      if (i == j && src[i].at == dst[i].at && src[i].bytes == dst[i].bytes && src[i].stride == dst[i].stride)
+        inside = true;
+      else if (kv_meet(src[i], dst[j]))
         return SRW_EINVAL;
-      inside = true;
     }
   for (int64_t j = 0; j < c->n_pairs; ++j)
     if (c->src_page[j] < 0 || c->src_page[j] >= c->n_src_pages || c->dst_page[j] < 0 || c->dst_page[j] >= c->n_dst_pages)

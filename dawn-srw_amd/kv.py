@@ -308,8 +308,8 @@ def _page_tensors(tensors):
 def kv_copy(tensors, src, dst, *, to=None) -> None:
     """Copy pages: page ``dst[i]`` of every tensor and layer gets what page ``src[i]``
     holds.  ``tensors``: a :class:`KvPages`, or up to eight tensors [layers, n_pages,
-    ...] of any types, each layer contiguous -- a cache's keys, values, scales and
-    index; ``to``: tensors of the same layouts, with a number of pages of their own, that
+    ...] of any types, each layer contiguous (tensors' layers may lie between each
+    other's) -- a cache's keys, values, scales and index; ``to``: tensors of the same layouts, with a number of pages of their own, that
     get the pages (None: the same ones).  ``src`` and ``dst`` are sequences of whole
     numbers on the host, of one length; the call waits for nothing, and one captured in
     a graph copies these pages in every replay.  A page may be read several times; one

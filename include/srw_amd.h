@@ -516,7 +516,7 @@ srw_status_t srw_attention_plan(const srw_attention_t* a, int32_t* rows, int32_t
  * src_page[j] of that layer of src holds; src[i] == dst[i]: within a tensor.  src_page
  * and dst_page are host arrays, read before the call returns.  A page that is named
  * twice in dst_page, or that is both read and written, and tensors that overlap in
- * any other way are SRW_EINVAL. */
+ * any other way are SRW_EINVAL (layers of several tensors may lie between each other). */
 #define SRW_KV_COPY_TENSORS 8
 typedef struct srw_kv_copy {
   const void* src[SRW_KV_COPY_TENSORS];
