@@ -720,8 +720,11 @@ class PagedKvCache:
             raise ValueError("n_pages is at least 1")
         if len(held) > n_pages:
             raise MemoryError(f"{len(held)} pages are held")
-        new = self._new(n_pages)
-        kv_copy(self._tensors(), held, range(len(held)), to=[t for t in new if t is not None])
+        new, old = self._new(n_pages), self._tensors()
+        kv_copy(old, held, range(len(held)), to=[t for t in new if t is not None])
+        for t in old:
+            if t.is_cuda:  # (allocated on another stream, maybe: not given out again before the copy has read it)
+                t.record_stream(torch.cuda.current_stream(t.device))
         self._hold(new)
         self._renamed({p: i for i, p in enumerate(held)})
         self.n_pages = n_pages
