@@ -31,7 +31,7 @@ import torch.nn.functional as F
 from . import _capi as C
 from .kv import PagedKvCache, _check_window, kv_index, kv_select, kv_write, paged_attention
 from .layer import GateConfig, SrwBatchPlan, SrwPlan
-from .sampling import sample
+from .sampling import check_parameters, sample
 from .srw import chunk_plan
 
 __all__ = ["DawnConfig", "init_params", "DawnModel"]
@@ -155,6 +155,18 @@ class _BatchCall:
         self.plan.launch(pool_cached=self.launches > 0)
         self.launches += 1
         return [c.plan.out for c in self.calls]
+
+
+def _check_sight(cache, window, sinks, keep, first, last):
+    """What a token is to see: a window, or pages kept of an indexed cache."""
+    _check_window(window, sinks)
+    if not all(hasattr(x, "__index__") for x in (keep, first, last)):
+        raise TypeError(f"keep, first and last are whole numbers; got {keep!r}, {first!r} and {last!r}")
+    if keep and (window or not cache.indexed):
+        raise ValueError("keep needs an indexed cache and goes without a window")
+    if keep and not (first >= 0 and last >= 1 and first + last <= keep):
+        raise ValueError("first is not negative, last at least 1, and keep holds both")
+
 
 
 class DawnModel:
@@ -427,11 +439,7 @@ class DawnModel:
         scale and its result.  Whatever it raises, the cache's sequences are as
         before the call."""
         cfg = self.cfg
-        _check_window(window, sinks)
-        if keep and (window or not cache.indexed):
-            raise ValueError("keep needs an indexed cache and goes without a window")
-        if keep and not (first >= 0 and last >= 1 and first + last <= keep):
-            raise ValueError("first is not negative, last at least 1, and keep holds both")
+        _check_sight(cache, window, sinks, keep, first, last)
         ids = ids.reshape(-1).to(self.device)
         counts = [int(n) for n in counts]
         T = sum(counts)
@@ -503,7 +511,9 @@ class DawnModel:
         (None: torch's) and these parameters, numbers or tensors [B].  A row that gives
         ``end`` stops: ``end`` with logprob 0 behind it.  ``window``, ``sinks`` and
         ``keep``, ``first``, ``last`` as in :meth:`extend`; prompts are read without keep.
-        The sequences are freed at the end."""
+        The sequences are freed at the end.  What the arguments say wrong is raised before
+        a prompt is read."""
+        _check_sight(cache, window, sinks, keep, first, last)
         prompts = [torch.as_tensor(p).reshape(-1) for p in prompts]
         counts = [p.shape[0] for p in prompts]
         if not prompts or min(counts) < 1 or n < 1 or samples < 1:
@@ -516,9 +526,12 @@ class DawnModel:
         B, dev = len(prompts) * samples, self.device
         if u is None:
             u = torch.rand(n, B, device=dev)
-        elif tuple(u.shape) != (n, B):
+        elif not isinstance(u, torch.Tensor) or tuple(u.shape) != (n, B):
             raise ValueError(f"u must be [{n}, {B}]")
         tokens = torch.full((B, n), 0 if end is None else end, dtype=torch.int64, device=dev)
+        if u.dtype != F32 or u.device != tokens.device:
+            raise TypeError(f"u must be float32 on {tokens.device}; got {u.dtype} on {u.device}")
+        check_parameters(B, tokens.device, temperature, top_k, top_p, min_p)
         logprobs = torch.zeros(B, n, device=dev)
         seqs = []
         try:

@@ -39,6 +39,17 @@ def _parameter(name, x, dev, dtype, B):
     return 0, x
 
 
+def _parameters(dev, B, temperature, top_k, top_p, min_p):
+    return [_parameter(n, x, dev, t, B) for n, x, t in (("temperature", temperature, F32), ("top_p", top_p, F32),
+                                                       ("min_p", min_p, F32), ("top_k", top_k, I32))]
+
+
+def check_parameters(B, dev, temperature, top_k, top_p, min_p):
+    """Raises what :func:`sample` would of its parameters for B rows on dev (tensors of any
+    stride)."""
+    _parameters(dev, B, *(x.contiguous() if isinstance(x, torch.Tensor) else x for x in (temperature, top_k, top_p, min_p)))
+
+
 def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """(tokens [B] int64, logprobs [B] float32): one token of every row of ``logits``
     [B, vocab] (float32 or bfloat16, any row stride) from the random numbers ``u`` [B]
@@ -83,8 +94,7 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if isinstance(u, torch.Tensor):
         _no_grad("u", u)
     u = _tensor("u", u, dev, F32, (B,))
-    given = [_parameter(n, x, dev, t, B) for n, x, t in (("temperature", temperature, F32), ("top_p", top_p, F32),
-                                                        ("min_p", min_p, F32), ("top_k", top_k, I32))]
+    given = _parameters(dev, B, temperature, top_k, top_p, min_p)
     if V > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     token = torch.empty(B, dtype=I64, device=dev)
