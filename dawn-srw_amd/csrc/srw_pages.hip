@@ -196,8 +196,11 @@ __device__ inline double turned(double x) {
 // going on with fewer dims (sums of all dims over all lanes took 5 us more).  Bound by the
 // keys' bytes: 65 521 tokens of 8 heads of 128, int8, 17.2 us, 4.1 TB/s (13.6 at a copy's
 // rate); 8 prompts of 512 bf16 4.5 us.
+//
+// `pages` > 0: a unit for every place of every table, which needs no search and goes by no
+// number of tokens; 0: units by the tokens.
 template <int KIND, int DH>
-__global__ __launch_bounds__(256) void kv_index_kernel(KvView p, int8_t* codes, float* scale) {
+__global__ __launch_bounds__(256) void kv_index_kernel(KvView p, uint32_t pages, int8_t* codes, float* scale) {
   constexpr int ES = kv_bytes<KIND>(), N = 16 / ES;     // dims a lane
   constexpr int kLanes = DH / N, kKeys = 64 / kLanes;   // lanes a key, keys a step
   constexpr int U = 4;                                  // steps in flight
@@ -206,7 +209,11 @@ __global__ __launch_bounds__(256) void kv_index_kernel(KvView p, int8_t* codes, 
   // units of a page of sequence b: start(b) = cu[b] / P + 2 b leaves room for both
   // partial ends
   int64_t b = unit, at = 0;
-  if (p.cu) {
+  if (pages > 0) {
+    b = static_cast<uint32_t>(unit) / pages;
+    if (b >= p.B) return;
+    at = static_cast<uint32_t>(unit) % pages;
+  } else if (p.cu) {
     auto start = [&](int64_t i) { return (static_cast<int64_t>(p.cu[i]) >> p.logP) + 2 * i; };
     b = kv_find(p.B, unit, start);
     at = unit - start(b);
@@ -216,7 +223,8 @@ __global__ __launch_bounds__(256) void kv_index_kernel(KvView p, int8_t* codes, 
   const KvSeq sq = kv_seq(p, b);
   if (sq.n <= 0 || at < 0) return;
   const int first = sq.len > sq.n ? (sq.len - sq.n) >> p.logP : 0;  // the first page with a new token
-  const int64_t base = (first + at) << p.logP;
+  if (pages > 0 && at < first) return;
+  const int64_t base = (pages > 0 ? at : first + at) << p.logP;
   if (base >= sq.len) return;
   const int page = kv_page(p, b, static_cast<int>(base));
   if (page < 0) return;
@@ -734,12 +742,16 @@ srw_status_t check_index(const srw_kv_t& c, const srw_kv_index_t& i) {
 template <int KIND>
 hipError_t launch_index(const srw_kv_t& c, const srw_kv_index_t& x, hipStream_t s) {
   const KvView p = kv_view(c);
-  const int64_t units = c.cu ? (c.T >> p.logP) + 2 * c.B : c.B;
+  int64_t units = c.cu ? (c.T >> p.logP) + 2 * c.B : c.B;
+  const bool by_table = c.cu && c.B * c.table_width <= units;
+  if (by_table) units = c.B * c.table_width;
+  if (units == 0) return hipSuccess;  // tables without places
+  const uint32_t pages = by_table ? static_cast<uint32_t>(c.table_width) : 0;
   const dim3 grid(static_cast<unsigned>((units + 3) / 4), static_cast<unsigned>(c.n_kv_heads));
   if (c.head_dim == 64)
-    hipLaunchKernelGGL((kv_index_kernel<KIND, 64>), grid, dim3(256), 0, s, p, x.codes, x.scale);
+    hipLaunchKernelGGL((kv_index_kernel<KIND, 64>), grid, dim3(256), 0, s, p, pages, x.codes, x.scale);
   else
-    hipLaunchKernelGGL((kv_index_kernel<KIND, 128>), grid, dim3(256), 0, s, p, x.codes, x.scale);
+    hipLaunchKernelGGL((kv_index_kernel<KIND, 128>), grid, dim3(256), 0, s, p, pages, x.codes, x.scale);
   return hipGetLastError();
 }
 

@@ -56,6 +56,8 @@ _SELECT = struct.Struct("@7P5q4i4P2q4i")
 _COPY = struct.Struct("@16P24q4q2P2i")
 
 
+_ANY_TOKENS = 1 << 29  # kv_index: more than a call has new tokens, as many as it takes
+
 _host = None
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -378,14 +380,14 @@ def kv_index(pages: KvPages, index: KvIndex, table, lens, cu=None, *, total=None
     as codes round(mean * (127 / m)) with scale m / 127.  Means of at most 2^-100 are
     held as zeros; the scale of a page with an infinite or NaN key is NaN.  Other
     entries keep what they hold.  ``total``: the number of new tokens, where the caller
-    knows it (cu's last entry, which lies on the device; without it the launch has room
-    for new tokens at all of the table's positions)."""
+    knows it (cu's last entry, which lies on the device; without it the launch looks at
+    every place of the table)."""
     if total is not None:
         T = operator.index(total)
     else:
         T = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() else -1
-        if cu is not None and isinstance(table, torch.Tensor) and table.dim() == 2:
-            T *= table.shape[1] * pages.page_size
+        if cu is not None:
+            T = _ANY_TOKENS
     if _current_device() == pages.device.index:
         status = (_host or _native()).index(pages._t, index._t, table, lens, cu, T, _raw_stream(pages.device.index))
         if status is not None:
