@@ -7,6 +7,7 @@ graph."""
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 
 import torch
@@ -19,6 +20,7 @@ __all__ = ["sample"]
 
 F32, I32, I64 = torch.float32, torch.int32, torch.int64
 _DTYPES = {torch.float32: C.SRW_F32, torch.bfloat16: C.SRW_BF16}
+_MOST = torch.finfo(F32).max
 _SAMPLE = struct.Struct("@P3q7P3f3i")
 
 
@@ -36,7 +38,7 @@ def _parameter(name, x, dev, dtype, B):
     x = float(x)
     if not (x >= 0 and (name == "temperature" or x <= 1)):
         raise ValueError(f"{name} is not negative{'' if name == 'temperature' else ' and at most 1'}; got {x!r}")
-    return 0, x
+    return 0, x if x <= _MOST else math.inf  # (a temperature that float32 does not hold)
 
 
 def _parameters(dev, B, temperature, top_k, top_p, min_p):

@@ -3,8 +3,10 @@
 from __future__ import annotations
 
 import ctypes
+import math
 
 import pytest
+import torch
 
 from tests.test_serving_host import _sample
 
@@ -34,3 +36,24 @@ def test_workspaces_of_sampling(C, V, top_p, top_k):
         assert lib.srw_sample_workspace_size(ctypes.byref(d), ctypes.byref(n)) == C.SRW_OK and n.value == want
         if want:
             assert lib.srw_sample(ctypes.byref(d), None, 0, None) == C.SRW_EWORKSPACE
+
+
+def test_temperatures_past_float32_are_infinite(pkg):
+    """As a tensor's would be: every token alike."""
+    from dawn_srw_amd import sampling
+    for x in (1e39, 10 ** 40, 1.7e308, math.inf):
+        at, number = sampling._parameter("temperature", x, torch.device("cpu"), torch.float32, 1)
+        assert (at, number) == (0, math.inf)
+    assert sampling._parameter("temperature", 3.4028234e38, torch.device("cpu"), torch.float32, 1) == (0, 3.4028234e38)
+
+
+@pytest.mark.gpu
+def test_rows_at_such_temperatures(pkg, dev):
+    print("[gpu] sample hot", flush=True)
+    logits = torch.randn(3, 700, generator=torch.Generator().manual_seed(1)).to(dev)
+    u = torch.tensor([0.1, 0.5, 0.9], device=dev)
+    want = pkg.sample(logits, u, temperature=math.inf)
+    for x in (1e39, 10 ** 40):
+        got = pkg.sample(logits, u, temperature=x)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert want[0].tolist() == [70, 350, 629]     # (float32 0.9 lies under 0.9, 0.1 over 0.1)
