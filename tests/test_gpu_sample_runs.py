@@ -242,3 +242,49 @@ def test_min_p_between_zero_and_the_smallest_number(pkg, dev, V):
         want, share = definition(l[0], u, tiny, 0, 1.0, f32(least))
         token, log = pkg.sample(l.to(dev), torch.full((1,), u, device=dev), temperature=tiny, min_p=least)
         assert token.item() == want and abs(log.item() - share) <= 2.0 ** -23 * abs(share) + 1e-7, (least, u, token, want)
+
+
+@pytest.mark.parametrize("V", [900, 1500, 2049, 8192, 9001, 40001])
+def test_arrays_give_what_numbers_do(pkg, dev, V):
+    """Other kernels and other parameters beside a row's own, entries that mean off: the
+    same bits."""
+    print(f"[gpu] sample arrays {V}", flush=True)
+    g = torch.Generator().manual_seed(V)
+    B = 6
+    logits = (3 * torch.randn(B, V, generator=g)).to(dev)
+    logits[1, ::2] = logits[1, 1::2][:1]            # many alike
+    logits[2, V // 3:] -= 30.0                      # later runs far under the first
+    u = torch.rand(B, generator=g).to(dev)
+    off = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+    array = lambda k, x: torch.full((B,), x, device=dev, dtype=I32 if k == "top_k" else F32)  # noqa: E731
+    for rule in RULES:
+        want = pkg.sample(logits, u, **rule)
+        whole = {**off, **rule}
+        for names in (["top_k"], ["top_p"], ["min_p"], ["temperature", "top_p"], list(off)):
+            got = pkg.sample(logits, u, **{**rule, **{k: array(k, whole[k]) for k in names}})
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (rule, names)
+        mixed = {k: array(k, x) for k, x in whole.items()}
+        mixed["top_k"][0], mixed["top_p"][1], mixed["min_p"][2], mixed["temperature"][3] = 3, 0.4, 0.2, 0.0
+        got = pkg.sample(logits, u, **mixed)
+        assert torch.equal(got[0][4:], want[0][4:]) and torch.equal(got[1][4:], want[1][4:]), rule
+
+
+@pytest.mark.parametrize("rule", [{}, dict(top_p=0.9), dict(top_p=0.99, min_p=0.01)], ids=str)
+def test_captured_calls_with_workspaces(pkg, dev, rule):
+    """Two graphs of one pool, replayed in turn with eager calls between."""
+    print(f"[gpu] sample captured {rule}", flush=True)
+    draw = lambda seed: 3 * torch.randn(4, 30011, generator=torch.Generator().manual_seed(seed))  # noqa: E731
+    logits, u = [draw(s).to(dev) for s in (1, 2)], torch.rand(4, generator=torch.Generator().manual_seed(3)).to(dev)
+    pkg.sample(logits[0], u, **rule)
+    torch.cuda.synchronize()
+    graphs, got = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph, l in zip(graphs, logits):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if got else None):
+            got.append(pkg.sample(l, u, **rule))
+    for seed in range(4):
+        for i in (seed % 2, 1 - seed % 2):
+            logits[i].copy_(draw(10 * seed + i))
+            graphs[i].replay()
+            want = pkg.sample(logits[i], u, **rule)
+            torch.cuda.synchronize()
+            assert torch.equal(got[i][0], want[0]) and torch.equal(got[i][1], want[1]), (seed, i)
