@@ -28,10 +28,12 @@
 //
 // A row of up to 2 048 logits (1 024 by top-k) is its own list.
 //
-// Measured (kernels alone, us): 64 rows of 1 000 float32 by top-p 10.4; one row of 30 000 float32, every rule on, 10.6; 64 rows of
-// 32 000 float32 with top-k 11, top-p 27, top-p and min-p 20, from the whole distribution
-// 13, greedy 7.3; 192 rows of 131 073 bf16 with top-p 65 (one read of them: 9.8); 512 rows
-// of 100 003 float32 from the whole distribution 54 (39.7).  A single row is a chain of
+// Measured (calls that follow each other, us): 64 rows of 1 000 float32 by top-p 10.9; one
+// row of 30 000 float32, every rule on, 11.3; 64 rows of 32 000 float32 with top-k 11.6 (34
+// with k of 2 000), top-p 28, top-p and min-p 21, min-p 13.4, from the whole distribution
+// 14, greedy 7.8; 192 rows of 131 073 bf16 with top-p 65 to 67 (one read of them: 9.8); 512
+// rows of 100 003 from the whole distribution 54 to 59 in float32 (39.7), and 51 to 56 in
+// bf16, by the 64-bit operations of the sums.  A single row is a chain of
 // about twenty steps of a workgroup that each wait for memory or a barrier.
 //
 // A workgroup of sixteen waves has a CU's vector units to itself, and an instruction
@@ -510,7 +512,7 @@ __device__ __forceinline__ void crossing(S& s, uint32_t target) {
 // border's, one wave compares each with each.  With `coarse` (COARSE: it may be) the first
 // pass goes by step_of(rank), which orders as the ranks do: the first digit of logits of a few octaves
 // has a few values, and atomics on few bins wait for each other (64 rows of 1 000 by
-// top-p 14.3 us without, 13.2 with).
+// top-p 11.8 us without, 10.9 with; of 2 000 15.8 and 14.0).
 template <int NT, bool COARSE, class S, class Each, class Step>
 __device__ __forceinline__ uint64_t select(S& s, int bits, uint64_t target, uint32_t n, bool coarse, Step step_of, Each each) {
   const int lane = threadIdx.x & 63;
@@ -619,11 +621,12 @@ struct Cut {
 
 // The largest logit and the sum of weights of a row's part of kPart logits, and, for
 // top-p, its sums by steps.  A lane holds its 32 logits in registers.  Bound by the
-// memory for whole rows of float32 (512 rows of 100 003: 46 us, 4.4 TB/s), by the ten
+// memory for whole rows of float32 (512 rows of 100 003: 48.7 us, 4.2 TB/s), by the ten
 // operations in 64 bits of a weight, as many others and an LDS atomic for top-p (192 rows
 // of 131 073 bf16: 29 us, 1.7 TB/s).  256 threads, or 512 where there are too few parts to
-// fill the card with those (64 rows of 32 000: the call 28.8 and 27.5 us; 256 rows 45.0
-// and 45.6).
+// fill the card with those (64 rows of 32 000 by top-p: the call 29.7 and 28.3 us; 256 rows
+// 47.0 and 46.3; 512 rows of 100 003 from the whole distribution 58 and 65, and 80 with
+// 1 024; 192 rows of 131 073 bf16 66, 67 and 75).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_parts_kernel(SampleArgs a) {
   using R = Row<T, NT>;
@@ -1277,9 +1280,9 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
 }
 
 // Whether rows are their own lists.  Top-k's threshold makes short lists of longer rows:
-// 64 rows of 300 | 1 000 | 2 000 float32 take 8.1 | 10.3 | 13 us by top-k as their own
-// lists and 9.0 | 8.7 | 9.1 by a threshold (512 rows of 1 000: 12.4 and 16.9), by top-p
-// 8.1 | 10.4 | 13 and, of parts, 9 | 24 | 25.  A list of 4 096 leaves room for one
+// 64 rows of 300 | 1 000 | 2 000 float32 take 8.3 | 10.6 | 13.5 us by top-k as their own
+// lists and 9.0 | 8.8 | 9.2 by a threshold (512 rows of 1 000: 12.7 and 16.7), by top-p
+// 8.3 | 10.7 | 13.9 and, of parts, 21 | 25 | 25.  A list of 4 096 leaves room for one
 // workgroup a CU.
 bool own_list(const srw_sample_t& d) { return d.V <= (d.top_k || d.top_k_all > 0 ? kOwnList / 2 : kOwnList); }
 // Parts of a row (0: it is its own list).
